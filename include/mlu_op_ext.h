@@ -213,6 +213,37 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtIndiceConvolutionBackwardFilterNoAlloc(
     const int64_t indice_num[], const int64_t inverse, const int64_t subm,
     const mluOpTensorDescriptor_t filters_grad_desc, void *filters_grad);
 
+/* ---- the rest of a training step --------------------------------------------------------------
+ * Operators a network over ragged rows of features needs next to its convolutions: none of them has a counterpart in the
+ * reference.  All pointers are device memory unless said otherwise; types are MLUOP_DTYPE_FLOAT, _HALF or _BFLOAT16 for
+ * features, and every sum is held in fp32 and rounded once.  They enqueue kernels on the handle's queue and return: no
+ * wait, no allocation, nothing that a graph capture refuses.  No float atomics: results repeat bit by bit. */
+
+/* One AdamW step (decoupled weight decay) over many tensors in as few launches as they fit in:
+ *   g = grad_scale * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps)
+ * in fp32.  `tensors` is host memory, read before the call returns.  param_type: of all params; grad_type: the same or
+ * FLOAT.  master: fp32 copies of 16-bit params, from which a step starts and which it updates together with the params;
+ * for all tensors or for none.  state_type FLOAT: exp_avg (m) and exp_avg_sq (v) are fp32 [count], the scales are not looked
+ * at.  UINT8: they are OCP e4m3 codes [count] of m and of sqrt(v), and every block of MLUOP_EXT_ADAMW_BLOCK consecutive
+ * elements has an fp32 scale [ceil(count / block)] that its codes' values are multiplied by (largest magnitude / 448).
+ * step counts from 1; 0 <= beta1, beta2 < 1; eps >= 0.  Tensors of no elements are passed over. */
+#define MLUOP_EXT_ADAMW_BLOCK 256
+typedef struct {
+  void *param;
+  const void *grad;
+  void *exp_avg;
+  void *exp_avg_sq;
+  float *master;
+  float *exp_avg_scale;
+  float *exp_avg_sq_scale;
+  int64_t count;
+} mluOpExtAdamWTensor_t;
+mluOpStatus_t MLUOP_WIN_API mluOpExtAdamWStep(mluOpHandle_t handle, const mluOpExtAdamWTensor_t tensors[],
+                                              int num_tensors, mluOpDataType_t param_type, mluOpDataType_t grad_type,
+                                              mluOpDataType_t state_type, int64_t step, double lr, double beta1,
+                                              double beta2, double eps, double weight_decay, double grad_scale);
+
 #if defined(__cplusplus)
 }
 #endif

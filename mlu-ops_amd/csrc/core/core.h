@@ -94,6 +94,12 @@ struct mluOpContext {
   // An operator of this handle is about to write [out, out + bytes): what was noted about a pair
   // tensor or a number of voxels in there describes memory that was handed out again, and is dropped.
   void forgetNotesIn(const void *out, size_t bytes);
+  // Whether there is anything to forget (for operators that write many tensors).
+  bool hasNotes() const {
+    for (const RulebookNote &n : rulebook_notes)
+      if (n.pairs != nullptr) return true;
+    return voxel_count.voxel_num != nullptr;
+  }
 
   // What the kernel launchers need: the stream, and the timer while it is on.
   mluop::KernelChoices kernel_choices;

@@ -624,3 +624,10 @@ def dynamic_point_to_voxel_backward(handle, grad_voxel_feats, feats, voxel_feats
     return native().dynamic_point_to_voxel_backward(handle.ptr.value, _guarded(), grad_voxel_feats, feats, voxel_feats,
                                                     point2voxel_map, voxel_points_count, voxel_num,
                                                     _REDUCE_MODES[reduce_type])
+
+# the rest of a training step (mlu_op_ext.h)
+from . import training  # noqa: E402
+
+SIGNATURES.update(training.SIGNATURES)
+for _name in training.__all__:
+    globals()[_name] = getattr(training, _name)
