@@ -244,6 +244,36 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtAdamWStep(mluOpHandle_t handle, const mluOpE
                                               mluOpDataType_t state_type, int64_t step, double lr, double beta1,
                                               double beta2, double eps, double weight_decay, double grad_scale);
 
+/* Group norm with an activation over rows [rows, channels] whose channels lie side by side.  Rows belong to samples: sample
+ * s has the rows row_starts[s] to row_starts[s + 1] - 1 (int32 [samples + 1], ascending; NULL: one sample of all rows).
+ * Mean and variance (of the population) are taken over a sample's rows and the channels / groups channels of each group;
+ *   out = activation((x - mean) * rstd * weight + bias),  rstd = 1 / sqrt(variance + eps).
+ * weight and bias [channels] of param_type, FLOAT or `type`; NULL: one and zero.  mean and rstd fp32 [samples, groups] are
+ * results that the backward pass takes (0 and 1 / sqrt(eps) for a sample without rows).  Rows of no sample are zero in
+ * every result.  Backward: input_grad [rows, channels], weight_grad and bias_grad [channels] of param_type (NULL where not
+ * wanted).  One workspace size serves both. */
+typedef enum {
+  MLUOP_EXT_ACTIVATION_NONE = 0,
+  MLUOP_EXT_ACTIVATION_RELU = 1,
+  MLUOP_EXT_ACTIVATION_SILU = 2
+} mluOpExtActivation_t;
+mluOpStatus_t MLUOP_WIN_API mluOpExtGetGroupNormWorkspaceSize(int64_t rows, int64_t channels, int64_t groups,
+                                                              int64_t samples, size_t *size);
+mluOpStatus_t MLUOP_WIN_API mluOpExtGroupNormForward(mluOpHandle_t handle, mluOpDataType_t type, const void *features,
+                                                     int64_t rows, int64_t channels, int64_t groups,
+                                                     const int32_t *row_starts, int64_t samples,
+                                                     mluOpDataType_t param_type, const void *weight, const void *bias,
+                                                     float eps, mluOpExtActivation_t activation, void *workspace,
+                                                     size_t workspace_size, void *out, float *mean, float *rstd);
+mluOpStatus_t MLUOP_WIN_API mluOpExtGroupNormBackward(mluOpHandle_t handle, mluOpDataType_t type,
+                                                      const void *output_grad, const void *features, int64_t rows,
+                                                      int64_t channels, int64_t groups, const int32_t *row_starts,
+                                                      int64_t samples, mluOpDataType_t param_type, const void *weight,
+                                                      const void *bias, const float *mean, const float *rstd,
+                                                      mluOpExtActivation_t activation, void *workspace,
+                                                      size_t workspace_size, void *input_grad, void *weight_grad,
+                                                      void *bias_grad);
+
 #if defined(__cplusplus)
 }
 #endif

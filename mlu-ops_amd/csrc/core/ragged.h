@@ -32,6 +32,26 @@ __device__ __forceinline__ void segmentRows(const int32_t *starts, int rows, int
   *count = hi - lo;
 }
 
+// The same with what lies outside of all segments: 0 the rows in front of the first, segments + 1 those behind the last,
+// s the rows of segment s - 1.
+__device__ __forceinline__ void segmentOrOutside(const int32_t *starts, int rows, int segments, int s, int *first,
+                                                 int *count) {
+  if (s > 0 && s <= segments) {
+    segmentRows(starts, rows, s - 1, first, count);
+    return;
+  }
+  *first = *count = 0;
+  if (starts == nullptr) return;
+  const int edge = starts[s == 0 ? 0 : segments];
+  const int at = edge < 0 ? 0 : (edge > rows ? rows : edge);
+  if (s == 0) {
+    *count = at;
+  } else {
+    *first = at;
+    *count = rows - at;
+  }
+}
+
 // Most tiles of `tile_rows` rows that `rows` rows in `segments` segments can make.
 inline int64_t mostRaggedTiles(int64_t rows, int64_t segments, int64_t tile_rows) {
   const int64_t filled = rows < segments ? rows : segments;
@@ -39,7 +59,8 @@ inline int64_t mostRaggedTiles(int64_t rows, int64_t segments, int64_t tile_rows
 }
 
 // Tile `tile` of all tiles of tile_rows rows, segment after segment.  By whole waves; the answer is the same in all
-// lanes.  64 segments at a time: a load, a scan and a ballot.
+// lanes.  64 segments at a time: a load, a scan and a ballot.  OUTSIDE: the segments are those of segmentOrOutside.
+template <bool OUTSIDE>
 __device__ __forceinline__ RaggedTile findRaggedTile(const int32_t *starts, int rows, int segments, int tile_rows,
                                                      int tile) {
   const int lane = threadIdx.x & 63;
@@ -47,9 +68,15 @@ __device__ __forceinline__ RaggedTile findRaggedTile(const int32_t *starts, int 
   t.segment = -1;
   t.first = t.rows = t.in_segment = t.segment_first = t.segment_rows = 0;
   int before = 0;
-  for (int base = 0; base < segments; base += 64) {
+  const int all = OUTSIDE ? segments + 2 : segments;
+  for (int base = 0; base < all; base += 64) {
     int first = 0, count = 0;
-    if (base + lane < segments) segmentRows(starts, rows, base + lane, &first, &count);
+    if (base + lane < all) {
+      if (OUTSIDE)
+        segmentOrOutside(starts, rows, segments, base + lane, &first, &count);
+      else
+        segmentRows(starts, rows, base + lane, &first, &count);
+    }
     const int tiles = (count + tile_rows - 1) / tile_rows;
     const int upto = before + waveInclusiveScan(tiles);
     const unsigned long long behind = __ballot(tile < upto);

@@ -77,7 +77,10 @@ namespace {
   X(mluOpExtBuildRowMap)                                   \
   X(mluOpExtUseRowMap)                                     \
   X(mluOpExtForgetRowMap)                                  \
-  X(mluOpExtAdamWStep)
+  X(mluOpExtAdamWStep)                                     \
+  X(mluOpExtGetGroupNormWorkspaceSize)                     \
+  X(mluOpExtGroupNormForward)                              \
+  X(mluOpExtGroupNormBackward)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -400,124 +403,6 @@ at::Tensor convBackwardFilter(mluOpHandle_t handle, const Buffers &buffers, cons
   buffers.done("mluOpIndiceConvolutionBackwardFilter");
   return dw;
 }
-
-// ---- the rest of a training step -----------------------------------------------------------
-
-// What these operators take is checked here, since the C API sees addresses and sizes only.
-inline void require(bool met, const char *what) {
-  if (!met) throw py::value_error(what);
-}
-
-inline bool isFeatureType(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
-
-// The tensors of an AdamW step: checked once and kept, so that a step looks at its gradients only.
-class AdamWTensors {
- public:
-  using Tensors = std::vector<at::Tensor>;
-  AdamWTensors(Tensors params, Tensors exp_avgs, Tensors exp_avg_sqs, std::optional<Tensors> masters,
-               std::optional<Tensors> exp_avg_scales, std::optional<Tensors> exp_avg_sq_scales) {
-    const size_t n = params.size();
-    require(exp_avgs.size() == n && exp_avg_sqs.size() == n && (!masters || masters->size() == n),
-            "params, states and masters are lists of one length");
-    require(exp_avg_scales.has_value() == exp_avg_sq_scales.has_value(), "both states have scales or neither");
-    eight_ = exp_avg_scales.has_value();
-    require(!eight_ || (exp_avg_scales->size() == n && exp_avg_sq_scales->size() == n),
-            "scales are lists of the params' length");
-    raw_.resize(n);
-    for (size_t i = 0; i < n; ++i) {
-      const at::Tensor &p = params[i];
-      const int64_t count = p.numel();
-      if (i == 0) {
-        type_ = p.scalar_type();
-        device_ = p.device();
-        require(device_.is_cuda(), "params are on the GPU");
-        require(isFeatureType(type_), "params are float32, float16 or bfloat16");
-        require(!masters || type_ != at::kFloat, "float32 params have no masters");
-      }
-      require(p.scalar_type() == type_, "params have one type");
-      require(p.device() == device_ && p.is_non_overlapping_and_dense(), "params are dense, on one device");
-      auto state = [&](const at::Tensor &t, int64_t length) {
-        require(t.device() == device_ && t.numel() == length, "states have their parameter's device and size");
-        // (an element's state lies where the element does)
-        require(t.strides() == p.strides() || (p.is_contiguous() && t.is_contiguous()),
-                "states lie in memory as their parameter does");
-        if (!eight_) return;
-        require(t.scalar_type() == at::kByte || t.scalar_type() == at::kFloat8_e4m3fn,
-                "8-bit states are float8_e4m3fn or uint8");
-      };
-      state(exp_avgs[i], count);
-      state(exp_avg_sqs[i], count);
-      require(eight_ || (exp_avgs[i].scalar_type() == at::kFloat && exp_avg_sqs[i].scalar_type() == at::kFloat),
-              "states without scales are float32");
-      mluOpExtAdamWTensor_t &r = raw_[i];
-      r = {p.data_ptr(), nullptr, exp_avgs[i].data_ptr(), exp_avg_sqs[i].data_ptr(), nullptr, nullptr, nullptr, count};
-      if (masters) {
-        const at::Tensor &m = (*masters)[i];
-        require(m.scalar_type() == at::kFloat && m.device() == device_ && m.numel() == count &&
-                    (m.strides() == p.strides() || (p.is_contiguous() && m.is_contiguous())),
-                "masters are float32 and lie as their parameter does");
-        r.master = static_cast<float *>(m.data_ptr());
-      }
-      if (eight_) {
-        const int64_t blocks = (count + MLUOP_EXT_ADAMW_BLOCK - 1) / MLUOP_EXT_ADAMW_BLOCK;
-        auto scale = [&](const at::Tensor &t) {
-          require(t.scalar_type() == at::kFloat && t.device() == device_ && t.numel() == blocks && t.is_contiguous(),
-                  "scales are float32, one for each 256 elements");
-          return static_cast<float *>(t.data_ptr());
-        };
-        r.exp_avg_scale = scale((*exp_avg_scales)[i]);
-        r.exp_avg_sq_scale = scale((*exp_avg_sq_scales)[i]);
-      }
-    }
-    params_ = std::move(params);
-    for (auto *list : {&exp_avgs, &exp_avg_sqs}) kept_.insert(kept_.end(), list->begin(), list->end());
-    for (auto *list : {&masters, &exp_avg_scales, &exp_avg_sq_scales})
-      if (*list) kept_.insert(kept_.end(), (*list)->begin(), (*list)->end());
-  }
-
-  // Gradients: one for each param, undefined (None) where a param has none and is left alone.
-  void step(mluOpHandle_t handle, const std::vector<std::optional<at::Tensor>> &grads, int64_t step, double lr,
-            double beta1, double beta2, double eps, double weight_decay, double grad_scale) {
-    require(grads.size() == raw_.size(), "a gradient (or None) for each param");
-    std::vector<mluOpExtAdamWTensor_t> own, wide;  // gradients of the params' type, and float32 ones
-    own.reserve(raw_.size());
-    std::vector<at::Tensor> laid_out;  // alive until the launches are enqueued
-    for (size_t i = 0; i < raw_.size(); ++i) {
-      if (!grads[i] || !grads[i]->defined()) continue;
-      at::Tensor g = *grads[i];
-      const at::Tensor &p = params_[i];
-      require(g.device() == device_ && g.numel() == raw_[i].count, "gradients have their parameter's device and size");
-      require(g.scalar_type() == type_ || g.scalar_type() == at::kFloat,
-              "gradients are of the params' type or float32");
-      if (g.strides() != p.strides() && !(p.is_contiguous() && g.is_contiguous())) {
-        require(g.sizes() == p.sizes(), "gradients have their parameter's shape");
-        at::Tensor same = at::empty_strided(p.sizes(), p.strides(), g.options());
-        same.copy_(g);
-        laid_out.push_back(same);
-        g = same;
-      }
-      mluOpExtAdamWTensor_t r = raw_[i];
-      r.grad = g.data_ptr();
-      (g.scalar_type() == type_ ? own : wide).push_back(r);
-    }
-    auto run = [&](const std::vector<mluOpExtAdamWTensor_t> &list, mluOpDataType_t grad_type) {
-      if (list.empty()) return;
-      check(api.mluOpExtAdamWStep(handle, list.data(), static_cast<int>(list.size()), dtypeCode(type_), grad_type,
-                                  eight_ ? MLUOP_DTYPE_UINT8 : MLUOP_DTYPE_FLOAT, step, lr, beta1, beta2, eps,
-                                  weight_decay, grad_scale),
-            "mluOpExtAdamWStep");
-    };
-    run(own, own.empty() ? MLUOP_DTYPE_FLOAT : dtypeCode(type_));
-    run(wide, MLUOP_DTYPE_FLOAT);
-  }
-
- private:
-  std::vector<mluOpExtAdamWTensor_t> raw_;
-  Tensors params_, kept_;
-  at::ScalarType type_ = at::kFloat;
-  at::Device device_ = at::kCPU;
-  bool eight_ = false;
-};
 
 // ---- handles of the layers -----------------------------------------------------------------
 
@@ -931,6 +816,8 @@ at::Tensor scatterBackward(mluOpHandle_t handle, const Buffers &buffers, const a
 
 inline mluOpHandle_t asHandle(uintptr_t h) { return reinterpret_cast<mluOpHandle_t>(h); }
 
+#include "python/training.h"
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -1052,17 +939,7 @@ PYBIND11_MODULE(_native, m) {
                                  count, num, static_cast<mluOpReduceMode_t>(mode));
         });
 
-  py::class_<AdamWTensors>(m, "AdamWTensors")
-      .def(py::init<AdamWTensors::Tensors, AdamWTensors::Tensors, AdamWTensors::Tensors,
-                    std::optional<AdamWTensors::Tensors>, std::optional<AdamWTensors::Tensors>,
-                    std::optional<AdamWTensors::Tensors>>())
-      .def("step", [](AdamWTensors &tensors, uintptr_t handle, const std::vector<std::optional<at::Tensor>> &grads,
-                      int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay,
-                      double grad_scale) {
-        NoGil released;
-        const OperatorLock lock(asHandle(handle));
-        tensors.step(asHandle(handle), grads, step, lr, beta1, beta2, eps, weight_decay, grad_scale);
-      });
+  defineTraining(m);
 
   py::class_<LayerRulebook, LayerRulebookPtr>(m, "LayerRulebook")
       .def(py::init([](const at::Tensor &pairs, std::optional<Counts> counts, int64_t num_act_out, Counts filter_space,

@@ -17,6 +17,7 @@ import math
 import torch
 
 from . import Handle, _capturing, _guarded, get_indice_pairs, native, regular_output_space, rulebook_counts
+from .training import ACTIVATIONS
 
 _handles = {}
 
@@ -142,6 +143,18 @@ class SparseTensor:
     def replace_features(self, features):
         return SparseTensor(features, self.indices, self.spatial_shape, self.batch_size, self.rulebooks,
                             self.distinct)
+
+    def row_starts(self):
+        """int32 [batch_size + 1]: where every sample's rows begin, for rows that are ordered by sample; None for one
+        sample.  Kept with the rulebooks while the coordinates are these."""
+        if self.batch_size == 1:
+            return None
+        kept = self.rulebooks.get("row_starts")
+        if kept is None or kept[0] is not self.indices:
+            samples = torch.arange(self.batch_size + 1, device=self.indices.device, dtype=torch.int32)
+            kept = (self.indices, torch.searchsorted(self.indices[:, 0].contiguous(), samples, out_int32=True))
+            self.rulebooks["row_starts"] = kept
+        return kept[1]
 
     def dense(self):
         """[N, C, D, H, W] dense tensor (for inspection and tests)."""
@@ -317,6 +330,37 @@ def _relu_in_store(conv, relu):
             _unwatched())
 
 
+def group_norm(features, weight, bias, groups, row_starts=None, eps=1e-5, activation="none"):
+    """Group norm with an activation ("none", "relu" or "silu") over `features` [rows, channels] on the current device, with
+    autograd.  Rows row_starts[s] to row_starts[s + 1] - 1 are sample s (int32 on the device; None: one sample of all
+    rows).  `weight` and `bias` [channels] are of the features' type or float32, or None."""
+    return native().group_norm(features, weight, bias, groups, row_starts, eps, ACTIVATIONS[activation], _guarded())
+
+
+class GroupNormAct(torch.nn.Module):
+    """Group norm over the channels of every sample, with an activation ("none", "relu", "silu") in the same pass.
+
+    Takes a SparseTensor, whose rows have to be ordered by sample (as voxelizers, `sparse_tensor_from_voxels` and strided
+    layers give them; the statistics are those of each sample's rows), or a tensor [rows, channels] with `row_starts`.
+    The parameters may be float32 whatever the features are."""
+
+    def __init__(self, groups, channels, eps=1e-5, activation="none", affine=True):
+        super().__init__()
+        if channels % groups != 0:
+            raise ValueError("channels are a multiple of groups")
+        self.groups, self.channels, self.eps = int(groups), int(channels), float(eps)
+        self.activation = activation
+        ACTIVATIONS[activation]
+        self.weight = torch.nn.Parameter(torch.ones(channels)) if affine else None
+        self.bias = torch.nn.Parameter(torch.zeros(channels)) if affine else None
+
+    def forward(self, x, row_starts=None):
+        if not isinstance(x, SparseTensor):
+            return group_norm(x, self.weight, self.bias, self.groups, row_starts, self.eps, self.activation)
+        return x.replace_features(group_norm(x.features, self.weight, self.bias, self.groups, x.row_starts(), self.eps,
+                                             self.activation))
+
+
 class SparseSequential(torch.nn.Sequential):
     """Layers applied in order to a SparseTensor (spconv's SparseSequential): sparse convolutions
     take and return the tensor, any other module is applied to its features.
@@ -387,7 +431,7 @@ class SparseSequential(torch.nn.Sequential):
                 # a launch and a pass over the result less each: voxelizer and 11-layer encoder 1085 -> 1007 us,
                 # the encoder's training step 3231 -> 3095 us
                 x, stored = m._convolve(x, relu=True), following
-            elif isinstance(m, (_ConvBase, SparseSequential)):
+            elif isinstance(m, (_ConvBase, SparseSequential, GroupNormAct)):
                 x = m(x)
             else:
                 x = x.replace_features(m(x.features))

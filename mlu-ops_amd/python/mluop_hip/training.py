@@ -2,19 +2,32 @@
 call of the C API on a `Handle` and returns new tensors; all are names of the package itself."""
 import ctypes
 
-__all__ = ["AdamWTensors"]
+__all__ = ["AdamWTensors", "group_norm_forward", "group_norm_backward"]
 
 _vp = ctypes.c_void_p
 _int, _i64, _float, _double, _size = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double, ctypes.c_size_t
 
 SIGNATURES = {
     "mluOpExtAdamWStep": (_int, [_vp, _vp, _int, _int, _int, _int, _i64] + [_double] * 6),
+    "mluOpExtGetGroupNormWorkspaceSize": (_int, [_i64, _i64, _i64, _i64, ctypes.POINTER(_size)]),
+    "mluOpExtGroupNormForward": (_int, [_vp, _int, _vp, _i64, _i64, _i64, _vp, _i64, _int, _vp, _vp, _float, _int, _vp,
+                                        _size, _vp, _vp, _vp]),
+    "mluOpExtGroupNormBackward": (_int, [_vp, _int, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _int, _vp, _vp, _vp, _vp, _int,
+                                         _vp, _size, _vp, _vp, _vp]),
 }
+
+# mluOpExtActivation_t
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}
 
 
 def _native():
     from . import native
     return native()
+
+
+def _guarded():
+    from . import _guarded
+    return _guarded()
 
 
 class AdamWTensors:
@@ -32,3 +45,20 @@ class AdamWTensors:
     def step(self, handle, grads, step, lr, betas, eps, weight_decay, grad_scale=1.0):
         """`step` counts from 1.  `grad_scale` multiplies the gradients (the reciprocal of a loss scale)."""
         self._tensors.step(handle.ptr.value, grads, step, lr, betas[0], betas[1], eps, weight_decay, grad_scale)
+
+
+def group_norm_forward(handle, features, weight, bias, groups, row_starts=None, eps=1e-5, activation="none"):
+    """Group norm with an activation over `features` [rows, channels].
+
+    `row_starts` int32 [samples + 1] on the device, ascending: sample s has the rows row_starts[s] to row_starts[s + 1] - 1
+    (None: all rows are one sample).  `weight`, `bias` [channels] of the features' type or float32, or None.
+    Returns (out, mean, rstd), the last two float32 [samples, groups]."""
+    return _native().group_norm_forward(handle.ptr.value, _guarded(), features, weight, bias, groups, row_starts, eps,
+                                        ACTIVATIONS[activation])
+
+
+def group_norm_backward(handle, output_grad, features, weight, bias, mean, rstd, groups, row_starts=None,
+                        activation="none"):
+    """Gradients (features, weight, bias) of `group_norm_forward`, whose mean and rstd it takes."""
+    return _native().group_norm_backward(handle.ptr.value, _guarded(), output_grad, features, weight, bias, mean, rstd,
+                                         groups, row_starts, ACTIVATIONS[activation])
