@@ -274,6 +274,23 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGroupNormBackward(mluOpHandle_t handle, mluO
                                                       size_t workspace_size, void *input_grad, void *weight_grad,
                                                       void *bias_grad);
 
+/* Rows of a table by their numbers: out[t, :] = scale * table[tokens[t], :], for num_tokens tokens (token_type INT32 or
+ * INT64) of a table [rows, channels] whose rows lie row_stride elements apart (at least channels); out [num_tokens,
+ * channels].  A token outside [0, rows) names no row: its result is zero.
+ * The gradient of the table: grad_table[v, :] = scale * sum of output_grad[t, :] over the tokens that name v, added up in
+ * ascending t; zero for a row that none names.  The tokens are sorted in the workspace.  rows, num_tokens below 2^31. */
+mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingForward(mluOpHandle_t handle, mluOpDataType_t type, const void *table,
+                                                     int64_t rows, int64_t channels, int64_t row_stride,
+                                                     mluOpDataType_t token_type, const void *tokens, int64_t num_tokens,
+                                                     float scale, void *out);
+mluOpStatus_t MLUOP_WIN_API mluOpExtGetEmbeddingBackwardWorkspaceSize(int64_t num_tokens, int64_t rows,
+                                                                      int64_t channels, size_t *size);
+mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingBackward(mluOpHandle_t handle, mluOpDataType_t type,
+                                                      const void *output_grad, int64_t row_stride,
+                                                      mluOpDataType_t token_type, const void *tokens, int64_t num_tokens,
+                                                      int64_t rows, int64_t channels, float scale, void *workspace,
+                                                      size_t workspace_size, void *grad_table);
+
 #if defined(__cplusplus)
 }
 #endif

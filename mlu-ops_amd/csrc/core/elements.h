@@ -32,6 +32,21 @@ __device__ __forceinline__ void storeFloats(T *to, const float (&from)[V]) {
   *reinterpret_cast<Vector<T, V> *>(to) = packed;
 }
 
+// How the threads of a workgroup lie over rows of `channels`: V channels each, row after row; a slab of channels where a row
+// has more than they take at once (blockIdx.y).
+template <int V, int THREADS>
+struct RowLanes {
+  int across, row, rows_at_once, channel;  // row < 0: a thread without work
+  __device__ explicit RowLanes(int channels) {
+    const int left = channels / V - (int)blockIdx.y * THREADS;
+    across = left < THREADS ? left : THREADS;
+    rows_at_once = THREADS / across;
+    row = (int)threadIdx.x / across;
+    channel = ((int)blockIdx.y * THREADS + (int)threadIdx.x - row * across) * V;
+    if (row >= rows_at_once) row = -1;
+  }
+};
+
 inline bool isFloating(mluOpDataType_t t) {
   return t == MLUOP_DTYPE_FLOAT || t == MLUOP_DTYPE_HALF || t == MLUOP_DTYPE_BFLOAT16;
 }

@@ -43,20 +43,8 @@ struct Params {
   __device__ __forceinline__ float biasAt(int c) const { return at(bias, c, 0.f); }
 };
 
-// How the threads of a workgroup lie over a tile: V channels each, row after row; a slab of channels where a row has more
-// than they take at once (blockIdx.y).
 template <int V>
-struct Lanes {
-  int across, row, rows_at_once, channel;  // row < 0: a thread without work
-  __device__ explicit Lanes(int channels) {
-    const int left = channels / V - (int)blockIdx.y * kThreads;
-    across = left < kThreads ? left : kThreads;
-    rows_at_once = kThreads / across;
-    row = (int)threadIdx.x / across;
-    channel = ((int)blockIdx.y * kThreads + (int)threadIdx.x - row * across) * V;
-    if (row >= rows_at_once) row = -1;
-  }
-};
+using Lanes = RowLanes<V, kThreads>;
 
 __device__ __forceinline__ float sigmoid(float z) {
   // (an exponential beyond the range is infinite, and its reciprocal zero)

@@ -80,7 +80,10 @@ namespace {
   X(mluOpExtAdamWStep)                                     \
   X(mluOpExtGetGroupNormWorkspaceSize)                     \
   X(mluOpExtGroupNormForward)                              \
-  X(mluOpExtGroupNormBackward)
+  X(mluOpExtGroupNormBackward)                             \
+  X(mluOpExtEmbeddingForward)                              \
+  X(mluOpExtGetEmbeddingBackwardWorkspaceSize)             \
+  X(mluOpExtEmbeddingBackward)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;

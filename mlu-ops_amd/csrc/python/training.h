@@ -266,6 +266,86 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
 
 
 
+// ---- embedding -----------------------------------------------------------------------------
+
+// A tensor [rows, channels] whose channels lie side by side: as it is, or laid out anew.
+inline at::Tensor channelsTogether(const at::Tensor &t) {
+  const bool together = (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+  return together ? t : t.contiguous();
+}
+inline int64_t rowStride(const at::Tensor &t) { return t.size(0) <= 1 ? std::max<int64_t>(t.size(1), 1) : t.stride(0); }
+
+inline mluOpDataType_t tokenType(const at::Tensor &tokens) {
+  require(tokens.scalar_type() == at::kInt || tokens.scalar_type() == at::kLong, "tokens are int32 or int64");
+  return tokens.scalar_type() == at::kInt ? MLUOP_DTYPE_INT32 : MLUOP_DTYPE_INT64;
+}
+
+at::Tensor embeddingForward(mluOpHandle_t handle, bool guarded, const at::Tensor &table, const at::Tensor &tokens,
+                            double scale) {
+  require(table.is_cuda() && table.dim() == 2 && isFeatureType(table.scalar_type()),
+          "a table is [rows, channels] of float32, float16 or bfloat16 on the GPU");
+  require(tokens.device() == table.device(), "tokens lie on the table's GPU");
+  const mluOpDataType_t token_type = tokenType(tokens);
+  const at::Tensor w = channelsTogether(table), t = tokens.contiguous();
+  const Buffers buffers(guarded, w.device());
+  std::vector<int64_t> shape = t.sizes().vec();
+  shape.push_back(w.size(1));
+  const at::Tensor out = buffers.output(shape, w.scalar_type(), "out");
+  check(api.mluOpExtEmbeddingForward(handle, dtypeCode(w.scalar_type()), w.data_ptr(), w.size(0), w.size(1), rowStride(w),
+                                     token_type, t.data_ptr(), t.numel(), static_cast<float>(scale), out.data_ptr()),
+        "mluOpExtEmbeddingForward");
+  buffers.done("mluOpExtEmbeddingForward");
+  return out;
+}
+
+at::Tensor embeddingBackward(mluOpHandle_t handle, bool guarded, const at::Tensor &output_grad, const at::Tensor &tokens,
+                             int64_t rows, double scale) {
+  require(output_grad.is_cuda() && output_grad.dim() >= 1 && isFeatureType(output_grad.scalar_type()),
+          "output_grad is float32, float16 or bfloat16 on the GPU");
+  require(tokens.device() == output_grad.device(), "tokens lie on the gradient's GPU");
+  require(output_grad.sizes().slice(0, output_grad.dim() - 1) == tokens.sizes(), "output_grad is [*tokens.shape, channels]");
+  const mluOpDataType_t token_type = tokenType(tokens);
+  const int64_t channels = output_grad.size(-1), n = tokens.numel();
+  const at::Tensor g = output_grad.dim() == 2 ? channelsTogether(output_grad) : output_grad.contiguous().view({n, channels});
+  const at::Tensor t = tokens.contiguous();
+  const Buffers buffers(guarded, g.device());
+  size_t bytes = 0;
+  check(api.mluOpExtGetEmbeddingBackwardWorkspaceSize(n, rows, channels, &bytes),
+        "mluOpExtGetEmbeddingBackwardWorkspaceSize");
+  const at::Tensor grad_table = buffers.output({rows, channels}, g.scalar_type(), "grad_table");
+  const at::Tensor ws = buffers.workspace(bytes);
+  check(api.mluOpExtEmbeddingBackward(handle, dtypeCode(g.scalar_type()), g.data_ptr(), rowStride(g), token_type,
+                                      t.data_ptr(), n, rows, channels, static_cast<float>(scale), ws.data_ptr(), bytes,
+                                      grad_table.data_ptr()),
+        "mluOpExtEmbeddingBackward");
+  buffers.done("mluOpExtEmbeddingBackward");
+  return grad_table;
+}
+
+struct EmbeddingRows : torch::autograd::Function<EmbeddingRows> {
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &table, const at::Tensor &tokens,
+                            double scale, bool guarded) {
+    StreamHandle &h = handleFor(table);
+    const OperatorLock lock(h);
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["rows"] = table.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["guarded"] = guarded;
+    return embeddingForward(h.handle, guarded, table, tokens, scale);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    torch::autograd::variable_list out(4);
+    if (!grads[0].defined() || !ctx->needs_input_grad(0)) return out;
+    const auto saved = ctx->get_saved_variables();
+    StreamHandle &h = handleFor(grads[0]);
+    const OperatorLock lock(h);
+    out[0] = embeddingBackward(h.handle, ctx->saved_data["guarded"].toBool(), grads[0], saved[0],
+                               ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble());
+    return out;
+  }
+};
+
 void defineTraining(py::module_ &m) {
   using NoGil = py::gil_scoped_release;
   py::class_<AdamWTensors>(m, "AdamWTensors")
@@ -308,5 +388,21 @@ void defineTraining(py::module_ &m) {
     NoGil released;
     return GroupNorm::apply(features, weight ? *weight : at::Tensor(), bias ? *bias : at::Tensor(), groups, row_starts,
                             eps, activation, guarded);
+  });
+  m.def("embedding_forward", [](uintptr_t handle, bool guarded, const at::Tensor &table, const at::Tensor &tokens,
+                                double scale) {
+    NoGil released;
+    const OperatorLock lock(asHandle(handle));
+    return embeddingForward(asHandle(handle), guarded, table, tokens, scale);
+  });
+  m.def("embedding_backward", [](uintptr_t handle, bool guarded, const at::Tensor &output_grad, const at::Tensor &tokens,
+                                 int64_t rows, double scale) {
+    NoGil released;
+    const OperatorLock lock(asHandle(handle));
+    return embeddingBackward(asHandle(handle), guarded, output_grad, tokens, rows, scale);
+  });
+  m.def("embedding", [](const at::Tensor &table, const at::Tensor &tokens, double scale, bool guarded) {
+    NoGil released;
+    return EmbeddingRows::apply(table, tokens, scale, guarded);
   });
 }

@@ -330,6 +330,25 @@ def _relu_in_store(conv, relu):
             _unwatched())
 
 
+def embedding(table, tokens, scale=1.0):
+    """scale * table[tokens] on the current device, with autograd: [*tokens.shape, channels] of the table's type.  A token
+    outside the table (-1, say) gives zeros and no gradient.  With a list of rows as tokens it puts the rows of a tensor
+    into another order, any of them several times or never."""
+    return native().embedding(table, tokens, scale, _guarded())
+
+
+class Embedding(torch.nn.Module):
+    """A table of `rows` learned rows, looked up by int32 or int64 tokens and multiplied with `scale`."""
+
+    def __init__(self, rows, channels, scale=1.0):
+        super().__init__()
+        self.scale = float(scale)
+        self.weight = torch.nn.Parameter(torch.randn(rows, channels))
+
+    def forward(self, tokens):
+        return embedding(self.weight, tokens, self.scale)
+
+
 def group_norm(features, weight, bias, groups, row_starts=None, eps=1e-5, activation="none"):
     """Group norm with an activation ("none", "relu" or "silu") over `features` [rows, channels] on the current device, with
     autograd.  Rows row_starts[s] to row_starts[s + 1] - 1 are sample s (int32 on the device; None: one sample of all

@@ -2,7 +2,7 @@
 call of the C API on a `Handle` and returns new tensors; all are names of the package itself."""
 import ctypes
 
-__all__ = ["AdamWTensors", "group_norm_forward", "group_norm_backward"]
+__all__ = ["AdamWTensors", "embedding_forward", "embedding_backward", "group_norm_forward", "group_norm_backward"]
 
 _vp = ctypes.c_void_p
 _int, _i64, _float, _double, _size = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double, ctypes.c_size_t
@@ -14,6 +14,9 @@ SIGNATURES = {
                                         _size, _vp, _vp, _vp]),
     "mluOpExtGroupNormBackward": (_int, [_vp, _int, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _int, _vp, _vp, _vp, _vp, _int,
                                          _vp, _size, _vp, _vp, _vp]),
+    "mluOpExtEmbeddingForward": (_int, [_vp, _int, _vp, _i64, _i64, _i64, _int, _vp, _i64, _float, _vp]),
+    "mluOpExtGetEmbeddingBackwardWorkspaceSize": (_int, [_i64, _i64, _i64, ctypes.POINTER(_size)]),
+    "mluOpExtEmbeddingBackward": (_int, [_vp, _int, _vp, _i64, _int, _vp, _i64, _i64, _i64, _float, _vp, _size, _vp]),
 }
 
 # mluOpExtActivation_t
@@ -62,3 +65,15 @@ def group_norm_backward(handle, output_grad, features, weight, bias, mean, rstd,
     """Gradients (features, weight, bias) of `group_norm_forward`, whose mean and rstd it takes."""
     return _native().group_norm_backward(handle.ptr.value, _guarded(), output_grad, features, weight, bias, mean, rstd,
                                          groups, row_starts, ACTIVATIONS[activation])
+
+
+def embedding_forward(handle, table, tokens, scale=1.0):
+    """scale * table[tokens]: [*tokens.shape, channels] of the table's type.  `tokens` are int32 or int64; one outside
+    [0, rows) names no row, and its result is zero.  The table's rows may lie apart."""
+    return _native().embedding_forward(handle.ptr.value, _guarded(), table, tokens, scale)
+
+
+def embedding_backward(handle, output_grad, tokens, rows, scale=1.0):
+    """Gradient [rows, channels] of the table of `embedding_forward`: each row adds up the gradients of the tokens that
+    name it, in their order, in fp32."""
+    return _native().embedding_backward(handle.ptr.value, _guarded(), output_grad, tokens, rows, scale)
