@@ -291,6 +291,39 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingBackward(mluOpHandle_t handle, mluO
                                                       int64_t rows, int64_t channels, float scale, void *workspace,
                                                       size_t workspace_size, void *grad_table);
 
+/* Products grouped by expert: rows group_starts[g] to group_starts[g + 1] - 1 (int32 [groups + 1] on the device, ascending,
+ * any of them empty) are multiplied with the filter of group g, filters [groups, ci, co]:
+ *   forward          out[r, :]         = features[r, :] . filters[g]            [rows, co]
+ *   backward data    input_grad[r, :]  = output_grad[r, :] . filters[g]^T       [rows, ci]
+ *   backward filter  filters_grad[g]   = features_g^T . output_grad_g           [groups, ci, co]
+ * features_stride, output_grad_stride: elements from row to row.  Rows of no group are zero in the results, a group without
+ * rows has a gradient of zero, and a filter without rows is not read.  The workspace of the queried size (which may be 0)
+ * belongs to one of the three. */
+typedef enum {
+  MLUOP_EXT_GROUPED_FORWARD = 0,
+  MLUOP_EXT_GROUPED_BACKWARD_DATA = 1,
+  MLUOP_EXT_GROUPED_BACKWARD_FILTER = 2
+} mluOpExtGroupedMatmul_t;
+mluOpStatus_t MLUOP_WIN_API mluOpExtGetGroupedMatmulWorkspaceSize(mluOpHandle_t handle, mluOpExtGroupedMatmul_t which,
+                                                                  mluOpDataType_t type, int64_t rows, int64_t groups,
+                                                                  int64_t ci, int64_t co, size_t *size);
+mluOpStatus_t MLUOP_WIN_API mluOpExtGroupedMatmulForward(mluOpHandle_t handle, mluOpDataType_t type,
+                                                         const void *features, int64_t features_stride, int64_t rows,
+                                                         const int32_t *group_starts, int64_t groups, int64_t ci,
+                                                         int64_t co, const void *filters, void *workspace,
+                                                         size_t workspace_size, void *out);
+mluOpStatus_t MLUOP_WIN_API mluOpExtGroupedMatmulBackwardData(mluOpHandle_t handle, mluOpDataType_t type,
+                                                              const void *output_grad, int64_t output_grad_stride,
+                                                              int64_t rows, const int32_t *group_starts, int64_t groups,
+                                                              int64_t ci, int64_t co, const void *filters,
+                                                              void *workspace, size_t workspace_size, void *input_grad);
+mluOpStatus_t MLUOP_WIN_API mluOpExtGroupedMatmulBackwardFilter(mluOpHandle_t handle, mluOpDataType_t type,
+                                                                const void *features, int64_t features_stride,
+                                                                const void *output_grad, int64_t output_grad_stride,
+                                                                int64_t rows, const int32_t *group_starts,
+                                                                int64_t groups, int64_t ci, int64_t co, void *workspace,
+                                                                size_t workspace_size, void *filters_grad);
+
 #if defined(__cplusplus)
 }
 #endif

@@ -98,8 +98,10 @@ __device__ __forceinline__ RaggedTile findRaggedTile(const int32_t *starts, int 
   return t;
 }
 
-// Tiles of the segments in front of `segment`.
-__device__ __forceinline__ int raggedTilesBefore(const int32_t *starts, int rows, int segment, int tile_rows) {
+// The tiles of segment `segment`: how many, and the number of the first among all tiles.  Inside [0, most], the tiles that
+// mostRaggedTiles says there can be, whatever the starts hold.
+__device__ __forceinline__ int raggedTilesOf(const int32_t *starts, int rows, int segment, int tile_rows, int most,
+                                             int *first_tile, int *segment_rows) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int base = 0; base < segment; base += 64) {
@@ -108,7 +110,11 @@ __device__ __forceinline__ int raggedTilesBefore(const int32_t *starts, int rows
     const int tiles = (count + tile_rows - 1) / tile_rows;
     before += __builtin_amdgcn_readlane(waveInclusiveScan(tiles), 63);
   }
-  return before;
+  int first;
+  segmentRows(starts, rows, segment, &first, segment_rows);
+  const int tiles = (*segment_rows + tile_rows - 1) / tile_rows;
+  *first_tile = before < 0 ? 0 : (before > most ? most : before);
+  return tiles < most - *first_tile ? tiles : most - *first_tile;
 }
 
 }  // namespace mluop

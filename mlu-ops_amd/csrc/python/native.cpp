@@ -83,7 +83,11 @@ namespace {
   X(mluOpExtGroupNormBackward)                             \
   X(mluOpExtEmbeddingForward)                              \
   X(mluOpExtGetEmbeddingBackwardWorkspaceSize)             \
-  X(mluOpExtEmbeddingBackward)
+  X(mluOpExtEmbeddingBackward)                             \
+  X(mluOpExtGetGroupedMatmulWorkspaceSize)                 \
+  X(mluOpExtGroupedMatmulForward)                          \
+  X(mluOpExtGroupedMatmulBackwardData)                     \
+  X(mluOpExtGroupedMatmulBackwardFilter)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;

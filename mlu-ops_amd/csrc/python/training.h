@@ -346,6 +346,96 @@ struct EmbeddingRows : torch::autograd::Function<EmbeddingRows> {
   }
 };
 
+// ---- products grouped by expert ------------------------------------------------------------
+
+inline at::Tensor rowsOfProduct(const at::Tensor &t, const char *what) {
+  require(t.is_cuda() && t.dim() == 2 && isFeatureType(t.scalar_type()), what);
+  return channelsTogether(t);
+}
+
+inline at::Tensor groupedWorkspace(mluOpHandle_t handle, const Buffers &buffers, mluOpExtGroupedMatmul_t which,
+                                   mluOpDataType_t type, int64_t rows, int64_t groups, int64_t ci, int64_t co,
+                                   size_t *bytes) {
+  check(api.mluOpExtGetGroupedMatmulWorkspaceSize(handle, which, type, rows, groups, ci, co, bytes),
+        "mluOpExtGetGroupedMatmulWorkspaceSize");
+  return *bytes > 0 ? buffers.workspace(*bytes) : at::Tensor();
+}
+
+// rows [rows, reduction] times the filters of their groups (or their transposes).
+at::Tensor groupedRows(mluOpHandle_t handle, bool guarded, const at::Tensor &rows_in, const at::Tensor &filters,
+                       const at::Tensor &group_starts, bool forward) {
+  const at::Tensor x = rowsOfProduct(rows_in, "rows are [rows, channels] of float32, float16 or bfloat16 on the GPU");
+  const at::Tensor w = rowsOn(filters, x, 3, "filters are [groups, ci, co] of the rows' type, on their GPU");
+  const at::Tensor starts = startsOn(group_starts, x, "group_starts are int32 [groups + 1] on the rows' GPU");
+  const int64_t groups = w.size(0), ci = w.size(1), co = w.size(2), rows = x.size(0);
+  require(starts.size(0) == groups + 1, "group_starts are one more than the filters");
+  require(x.size(1) == (forward ? ci : co), "rows have the filters' channels");
+  const Buffers buffers(guarded, x.device());
+  const mluOpDataType_t type = dtypeCode(x.scalar_type());
+  const at::Tensor out = buffers.output({rows, forward ? co : ci}, x.scalar_type(), forward ? "out" : "input_grad");
+  size_t bytes = 0;
+  const at::Tensor ws = groupedWorkspace(handle, buffers, forward ? MLUOP_EXT_GROUPED_FORWARD : MLUOP_EXT_GROUPED_BACKWARD_DATA,
+                                         type, rows, groups, ci, co, &bytes);
+  void *at = ws.defined() ? ws.data_ptr() : nullptr;
+  const auto *s = static_cast<const int32_t *>(starts.data_ptr());
+  if (forward)
+    check(api.mluOpExtGroupedMatmulForward(handle, type, x.data_ptr(), rowStride(x), rows, s, groups, ci, co, w.data_ptr(),
+                                           at, bytes, out.data_ptr()),
+          "mluOpExtGroupedMatmulForward");
+  else
+    check(api.mluOpExtGroupedMatmulBackwardData(handle, type, x.data_ptr(), rowStride(x), rows, s, groups, ci, co,
+                                                w.data_ptr(), at, bytes, out.data_ptr()),
+          "mluOpExtGroupedMatmulBackwardData");
+  buffers.done(forward ? "mluOpExtGroupedMatmulForward" : "mluOpExtGroupedMatmulBackwardData");
+  return out;
+}
+
+at::Tensor groupedFilter(mluOpHandle_t handle, bool guarded, const at::Tensor &features, const at::Tensor &output_grad,
+                         const at::Tensor &group_starts) {
+  const at::Tensor x = rowsOfProduct(features, "features are [rows, ci] of float32, float16 or bfloat16 on the GPU");
+  require(output_grad.device() == x.device() && output_grad.dim() == 2 && output_grad.scalar_type() == x.scalar_type() &&
+              output_grad.size(0) == x.size(0),
+          "output_grad is [rows, co] of the features' type, on their GPU");
+  const at::Tensor dy = channelsTogether(output_grad);
+  const at::Tensor starts = startsOn(group_starts, x, "group_starts are int32 [groups + 1] on the features' GPU");
+  const int64_t rows = x.size(0), groups = starts.size(0) - 1, ci = x.size(1), co = dy.size(1);
+  const Buffers buffers(guarded, x.device());
+  const mluOpDataType_t type = dtypeCode(x.scalar_type());
+  const at::Tensor out = buffers.output({groups, ci, co}, x.scalar_type(), "filters_grad");
+  size_t bytes = 0;
+  const at::Tensor ws =
+      groupedWorkspace(handle, buffers, MLUOP_EXT_GROUPED_BACKWARD_FILTER, type, rows, groups, ci, co, &bytes);
+  check(api.mluOpExtGroupedMatmulBackwardFilter(handle, type, x.data_ptr(), rowStride(x), dy.data_ptr(), rowStride(dy),
+                                                rows, static_cast<const int32_t *>(starts.data_ptr()), groups, ci, co,
+                                                ws.defined() ? ws.data_ptr() : nullptr, bytes, out.data_ptr()),
+        "mluOpExtGroupedMatmulBackwardFilter");
+  buffers.done("mluOpExtGroupedMatmulBackwardFilter");
+  return out;
+}
+
+struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &features, const at::Tensor &filters,
+                            const at::Tensor &group_starts, bool guarded) {
+    StreamHandle &h = handleFor(features);
+    const OperatorLock lock(h);
+    ctx->save_for_backward({features, filters, group_starts});
+    ctx->saved_data["guarded"] = guarded;
+    return groupedRows(h.handle, guarded, features, filters, group_starts, true);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    torch::autograd::variable_list out(4);
+    if (!grads[0].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const bool guarded = ctx->saved_data["guarded"].toBool();
+    StreamHandle &h = handleFor(saved[0]);
+    const OperatorLock lock(h);
+    if (ctx->needs_input_grad(0)) out[0] = groupedRows(h.handle, guarded, grads[0], saved[1], saved[2], false);
+    if (ctx->needs_input_grad(1)) out[1] = groupedFilter(h.handle, guarded, saved[0], grads[0], saved[2]);
+    return out;
+  }
+};
+
 void defineTraining(py::module_ &m) {
   using NoGil = py::gil_scoped_release;
   py::class_<AdamWTensors>(m, "AdamWTensors")
@@ -404,5 +494,22 @@ void defineTraining(py::module_ &m) {
   m.def("embedding", [](const at::Tensor &table, const at::Tensor &tokens, double scale, bool guarded) {
     NoGil released;
     return EmbeddingRows::apply(table, tokens, scale, guarded);
+  });
+  m.def("grouped_matmul_rows", [](uintptr_t handle, bool guarded, const at::Tensor &rows, const at::Tensor &filters,
+                                  const at::Tensor &group_starts, bool forward) {
+    NoGil released;
+    const OperatorLock lock(asHandle(handle));
+    return groupedRows(asHandle(handle), guarded, rows, filters, group_starts, forward);
+  });
+  m.def("grouped_matmul_backward_filter", [](uintptr_t handle, bool guarded, const at::Tensor &features,
+                                             const at::Tensor &output_grad, const at::Tensor &group_starts) {
+    NoGil released;
+    const OperatorLock lock(asHandle(handle));
+    return groupedFilter(asHandle(handle), guarded, features, output_grad, group_starts);
+  });
+  m.def("grouped_matmul", [](const at::Tensor &features, const at::Tensor &filters, const at::Tensor &group_starts,
+                             bool guarded) {
+    NoGil released;
+    return GroupedMatmul::apply(features, filters, group_starts, guarded);
   });
 }

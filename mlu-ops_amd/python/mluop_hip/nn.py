@@ -349,6 +349,35 @@ class Embedding(torch.nn.Module):
         return embedding(self.weight, tokens, self.scale)
 
 
+def grouped_matmul(features, filters, group_starts):
+    """Rows of groups times the filters of their groups on the current device, with autograd: features [rows, ci] in
+    group order, filters [groups, ci, co], group_starts int32 [groups + 1] on the device -> [rows, co]."""
+    return native().grouped_matmul(features, filters, group_starts, _guarded())
+
+
+class ExpertLinear(torch.nn.Module):
+    """A linear map for each expert, over rows that are ordered by expert (`expert_order`)."""
+
+    def __init__(self, experts, in_channels, out_channels):
+        super().__init__()
+        bound = 1.0 / math.sqrt(in_channels)
+        self.weight = torch.nn.Parameter(torch.empty(experts, in_channels, out_channels).uniform_(-bound, bound))
+
+    def forward(self, features, group_starts):
+        return grouped_matmul(features, self.weight.to(features.dtype), group_starts)
+
+
+def expert_order(experts_of_rows, experts):
+    """(rows, group_starts) of a routing [rows, choices] of integers in [0, experts): the source row of every place when all
+    choices are ordered by expert (equal experts by row), int32 [rows * choices], and where each expert's places begin,
+    int32 [experts + 1].  `embedding(features, rows)` then puts rows into that order, and its gradient adds the
+    copies of a row up again."""
+    flat = experts_of_rows.reshape(experts_of_rows.shape[0], -1)
+    ordered, place = torch.sort(flat.reshape(-1), stable=True)
+    starts = torch.searchsorted(ordered, torch.arange(experts + 1, device=flat.device, dtype=ordered.dtype), out_int32=True)
+    return torch.div(place, max(flat.shape[1], 1), rounding_mode="floor").to(torch.int32), starts
+
+
 def group_norm(features, weight, bias, groups, row_starts=None, eps=1e-5, activation="none"):
     """Group norm with an activation ("none", "relu" or "silu") over `features` [rows, channels] on the current device, with
     autograd.  Rows row_starts[s] to row_starts[s + 1] - 1 are sample s (int32 on the device; None: one sample of all

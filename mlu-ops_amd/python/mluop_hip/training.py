@@ -2,7 +2,8 @@
 call of the C API on a `Handle` and returns new tensors; all are names of the package itself."""
 import ctypes
 
-__all__ = ["AdamWTensors", "embedding_forward", "embedding_backward", "group_norm_forward", "group_norm_backward"]
+__all__ = ["AdamWTensors", "embedding_forward", "embedding_backward", "group_norm_forward", "group_norm_backward",
+           "grouped_matmul_forward", "grouped_matmul_backward_data", "grouped_matmul_backward_filter"]
 
 _vp = ctypes.c_void_p
 _int, _i64, _float, _double, _size = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double, ctypes.c_size_t
@@ -17,6 +18,11 @@ SIGNATURES = {
     "mluOpExtEmbeddingForward": (_int, [_vp, _int, _vp, _i64, _i64, _i64, _int, _vp, _i64, _float, _vp]),
     "mluOpExtGetEmbeddingBackwardWorkspaceSize": (_int, [_i64, _i64, _i64, ctypes.POINTER(_size)]),
     "mluOpExtEmbeddingBackward": (_int, [_vp, _int, _vp, _i64, _int, _vp, _i64, _i64, _i64, _float, _vp, _size, _vp]),
+    "mluOpExtGetGroupedMatmulWorkspaceSize": (_int, [_vp, _int, _int, _i64, _i64, _i64, _i64, ctypes.POINTER(_size)]),
+    "mluOpExtGroupedMatmulForward": (_int, [_vp, _int, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _size, _vp]),
+    "mluOpExtGroupedMatmulBackwardData": (_int, [_vp, _int, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _size, _vp]),
+    "mluOpExtGroupedMatmulBackwardFilter": (_int, [_vp, _int, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp,
+                                                   _size, _vp]),
 }
 
 # mluOpExtActivation_t
@@ -77,3 +83,20 @@ def embedding_backward(handle, output_grad, tokens, rows, scale=1.0):
     """Gradient [rows, channels] of the table of `embedding_forward`: each row adds up the gradients of the tokens that
     name it, in their order, in fp32."""
     return _native().embedding_backward(handle.ptr.value, _guarded(), output_grad, tokens, rows, scale)
+
+
+def grouped_matmul_forward(handle, features, filters, group_starts):
+    """Rows group_starts[g] to group_starts[g + 1] - 1 of `features` [rows, ci] times filters[g] of [groups, ci, co]:
+    [rows, co].  `group_starts` int32 [groups + 1] on the device, ascending, any group empty; rows of no group give zeros.
+    The features' rows may lie apart."""
+    return _native().grouped_matmul_rows(handle.ptr.value, _guarded(), features, filters, group_starts, True)
+
+
+def grouped_matmul_backward_data(handle, output_grad, filters, group_starts):
+    """Gradient [rows, ci] of the features of `grouped_matmul_forward`."""
+    return _native().grouped_matmul_rows(handle.ptr.value, _guarded(), output_grad, filters, group_starts, False)
+
+
+def grouped_matmul_backward_filter(handle, features, output_grad, group_starts):
+    """Gradient [groups, ci, co] of the filters of `grouped_matmul_forward`; zero for a group without rows."""
+    return _native().grouped_matmul_backward_filter(handle.ptr.value, _guarded(), features, output_grad, group_starts)
