@@ -19,7 +19,7 @@ constexpr int kThreads = 256;
 // The problem as its kernels see it.
 struct Shape {
   int rows, channels, groups, samples;
-  int tile_rows;
+  int tile_rows, most_tiles;
   const int32_t *starts;
 };
 
@@ -150,10 +150,8 @@ __global__ __launch_bounds__(kThreads) void groupNormJoinMoments(const float2 *_
   const int sample = blockIdx.x / s.groups, group = blockIdx.x - sample * s.groups;
   const int per_group = s.channels / s.groups;
   int first, rows;
-  segmentRows(s.starts, s.rows, sample, &first, &rows);
-  const int tiles = (rows + s.tile_rows - 1) / s.tile_rows;
-  const float2 *from = partial + (int64_t)raggedTilesBefore(s.starts, s.rows, sample, s.tile_rows) * s.channels +
-                       group * per_group;
+  const int tiles = raggedTilesOf(s.starts, s.rows, sample, s.tile_rows, s.most_tiles, &first, &rows);
+  const float2 *from = partial + (int64_t)first * s.channels + group * per_group;
   const int entries = tiles * per_group;
   auto rowsOf = [&](int tile) { return (float)min(s.tile_rows, rows - tile * s.tile_rows); };
   float sum = 0.f;
@@ -279,10 +277,8 @@ __global__ __launch_bounds__(kThreads) void groupNormJoinGradSums(const float2 *
     const int sample = blockIdx.x / s.groups, group = blockIdx.x - sample * s.groups;
     const int per_group = s.channels / s.groups;
     int first, rows;
-    segmentRows(s.starts, s.rows, sample, &first, &rows);
-    const int entries = (rows + s.tile_rows - 1) / s.tile_rows * per_group;
-    const float2 *from = partial + (int64_t)raggedTilesBefore(s.starts, s.rows, sample, s.tile_rows) * s.channels +
-                         group * per_group;
+    const int entries = raggedTilesOf(s.starts, s.rows, sample, s.tile_rows, s.most_tiles, &first, &rows) * per_group;
+    const float2 *from = partial + (int64_t)first * s.channels + group * per_group;
     float a = 0.f, b = 0.f;
     for (int e = threadIdx.x; e < entries; e += kThreads) {
       const int tile = e / per_group, c = e - tile * per_group;
@@ -297,7 +293,9 @@ __global__ __launch_bounds__(kThreads) void groupNormJoinGradSums(const float2 *
     if (threadIdx.x == 0) means[blockIdx.x] = make_float2(a * by, b * by);
     return;
   }
-  const int tiles = raggedTilesBefore(s.starts, s.rows, s.samples, s.tile_rows);
+  int last, rows;
+  const int of_last = raggedTilesOf(s.starts, s.rows, s.samples - 1, s.tile_rows, s.most_tiles, &last, &rows);
+  const int tiles = last + of_last;
   const int lane = threadIdx.x % kChannels, share = threadIdx.x / kChannels;
   const int c = ((int)blockIdx.x - pairs) * kChannels + lane;
   __shared__ float2 s_sum[kThreads / kChannels][kChannels];
@@ -474,7 +472,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGroupNormForward(mluOpHandle_t handle, mluOp
     handle->forgetNotesIn(rstd, (size_t)samples * groups * sizeof(float));
     handle->forgetNotesIn(workspace, workspace_size);
   }
-  const Shape s = {(int)rows, (int)channels, (int)groups, (int)samples, tileRows(rows, channels), row_starts};
+  const Shape s = {(int)rows, (int)channels, (int)groups, (int)samples, tileRows(rows, channels),
+                   (int)mostRaggedTiles(rows, samples, tileRows(rows, channels)), row_starts};
   const Params p = {weight, bias, param_type};
   const Workspace w = carve(workspace, rows, channels, samples);
   const mluop::LaunchCtx lc = handle->launchCtx();
@@ -532,7 +531,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGroupNormBackward(mluOpHandle_t handle, mluO
     if (bias_grad) handle->forgetNotesIn(bias_grad, (size_t)channels * elementBytes(param_type));
     handle->forgetNotesIn(workspace, workspace_size);
   }
-  const Shape s = {(int)rows, (int)channels, (int)groups, (int)samples, tileRows(rows, channels), row_starts};
+  const Shape s = {(int)rows, (int)channels, (int)groups, (int)samples, tileRows(rows, channels),
+                   (int)mostRaggedTiles(rows, samples, tileRows(rows, channels)), row_starts};
   const Params p = {weight, bias, param_type};
   const Workspace w = carve(workspace, rows, channels, samples);
   const mluop::LaunchCtx lc = handle->launchCtx();

@@ -172,6 +172,18 @@ def test_no_rows(gpu_handle):
     assert dx.shape == (0, 8) and not bool(dw.any()) and not bool(db.any())
 
 
+def test_starts_that_make_no_sense_stay_in_bounds(gpu_handle):
+    """(their results are undefined; no access leaves a tensor: outputs lie between guard bands)"""
+    import torch
+    import mluop_hip
+    x, w, b, dy = inputs(3000, 16, torch.float16, torch.float32, 2)
+    for starts in ([0, 3000, 0, 3000, 0, 3000], [-7, 1 << 30, 5, 4, 3, 2], [9] * 6, [3000, 0, -1, 3000, 0, 1]):
+        dev = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        out, mean, rstd = mluop_hip.group_norm_forward(gpu_handle, x, w, b, 4, dev)
+        mluop_hip.group_norm_backward(gpu_handle, dy, x, w, b, mean, rstd, 4, dev)
+    torch.cuda.synchronize()
+
+
 def test_rows_apart_and_unaligned(gpu_handle):
     """views: every second row, columns of a wider tensor, an address that no vector load takes"""
     import torch
