@@ -32,6 +32,37 @@ __device__ __forceinline__ void storeFloats(T *to, const float (&from)[V]) {
   *reinterpret_cast<Vector<T, V> *>(to) = packed;
 }
 
+// The same past the caches (16-byte pieces of it): for results that the kernel behind this one does not read at once.
+template <typename T, int V>
+__device__ __forceinline__ void streamFloats(T *to, const float (&from)[V]) {
+  if constexpr (sizeof(T) * V % 16 == 0) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    struct alignas(16) Pieces {
+      u32x4 piece[sizeof(T) * V / 16];
+    };
+    Vector<T, V> packed;
+#pragma unroll
+    for (int i = 0; i < V; ++i) packed.v[i] = (T)from[i];
+    const Pieces pieces = __builtin_bit_cast(Pieces, packed);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) * V / 16); ++i)
+      __builtin_nontemporal_store(pieces.piece[i], reinterpret_cast<u32x4 *>(to) + i);
+  } else {
+    storeFloats<T, V>(to, from);
+  }
+}
+
+// Results of so many bytes are streamed: fewer stay where the next kernel finds them in a cache.
+constexpr size_t kStreamedBytes = (size_t)32 << 20;
+
+template <typename T, int V>
+__device__ __forceinline__ void storeFloats(T *to, const float (&from)[V], bool streamed) {
+  if (streamed)
+    streamFloats<T, V>(to, from);
+  else
+    storeFloats<T, V>(to, from);
+}
+
 // How the threads of a workgroup lie over rows of `channels`: V channels each, row after row; a slab of channels where a row
 // has more than they take at once (blockIdx.y).
 template <int V, int THREADS>
