@@ -278,7 +278,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGroupNormBackward(mluOpHandle_t handle, mluO
  * INT64) of a table [rows, channels] whose rows lie row_stride elements apart (at least channels); out [num_tokens,
  * channels].  A token outside [0, rows) names no row: its result is zero.
  * The gradient of the table: grad_table[v, :] = scale * sum of output_grad[t, :] over the tokens that name v, added up in
- * ascending t; zero for a row that none names.  The tokens are sorted in the workspace.  rows, num_tokens below 2^31. */
+ * an order that the tokens alone decide; zero for a row that none names.  The tokens are sorted in the workspace.  rows, num_tokens below 2^31. */
 mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingForward(mluOpHandle_t handle, mluOpDataType_t type, const void *table,
                                                      int64_t rows, int64_t channels, int64_t row_stride,
                                                      mluOpDataType_t token_type, const void *tokens, int64_t num_tokens,

@@ -163,8 +163,54 @@ __global__ __launch_bounds__(kTileThreads) void countTiles(ITEMS items, int64_t 
   for (int d = threadIdx.x; d < digits; d += kTileThreads) hist[(size_t)blockIdx.x * digits + d] = s_count[d];
 }
 
-// (`starts`, where not null, receives the first place of every digit)
-template <typename ITEMS>
+// Exclusive prefix sums of the digits' totals into s_first, and on top of them the counts of the tiles in front of this
+// one: what scanColumns would have left, from the counters as countTiles left them, where the tiles are few enough for every
+// workgroup to read them all.  By a workgroup of kTileThreads.
+constexpr int kFewTiles = 16;
+__device__ inline void digitStartsOfTile(const uint32_t *__restrict__ hist, int tiles, int digits, uint32_t *s_first,
+                                         uint32_t *s_wave) {
+  constexpr int kPer = kMaxDigits / kTileThreads, kAtOnce = 16;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mine = blockIdx.x;
+  const int per = (digits + kTileThreads - 1) / kTileThreads;
+  uint32_t total[kPer] = {}, before[kPer] = {}, sum = 0;
+  for (int t0 = 0; t0 < tiles; t0 += kAtOnce) {
+    uint32_t v[kAtOnce][kPer];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const uint32_t *row = hist + (size_t)(t0 + j < tiles ? t0 + j : 0) * digits;
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        v[j][u] = 0;
+        if (u < per && tid * per + u < digits) v[j][u] = row[tid * per + u];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j)
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        total[u] += t0 + j < tiles ? v[j][u] : 0u;
+        before[u] += t0 + j < mine ? v[j][u] : 0u;
+      }
+  }
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) sum += total[u];
+  const uint32_t incl = waveInclusiveSum(sum);
+  if (lane == 63) s_wave[wave] = incl;
+  __syncthreads();
+  uint32_t run = incl - sum;
+  for (int w = 0; w < wave; ++w) run += s_wave[w];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    const int d = tid * per + u;
+    if (u >= per || d >= digits) continue;
+    s_first[d] = run + before[u];
+    run += total[u];
+  }
+}
+
+// (`starts`, where not null, receives the first place of every digit.  Not SCANNED: the counters are as countTiles left them,
+// and there are no totals.)
+template <typename ITEMS, bool SCANNED = true>
 __global__ __launch_bounds__(kTileThreads) void partitionTiles(ITEMS items, int64_t n, int digits, int digit_bits,
                                                                int rounds, const uint32_t *__restrict__ hist,
                                                                const uint32_t *__restrict__ totals,
@@ -173,11 +219,15 @@ __global__ __launch_bounds__(kTileThreads) void partitionTiles(ITEMS items, int6
   __shared__ uint32_t s_first[kMaxDigits];              // where the next item of a digit goes
   __shared__ uint32_t s_wave[kTileWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  digitStarts(totals, digits, s_first, s_wave);
-  __syncthreads();
-  if (starts != nullptr && blockIdx.x == 0)
-    for (int d = tid; d < digits; d += kTileThreads) starts[d] = s_first[d];
-  for (int d = tid; d < digits; d += kTileThreads) s_first[d] += hist[(size_t)blockIdx.x * digits + d];
+  if constexpr (!SCANNED) {
+    digitStartsOfTile(hist, gridDim.x, digits, s_first, s_wave);
+  } else {
+    digitStarts(totals, digits, s_first, s_wave);
+    __syncthreads();
+    if (starts != nullptr && blockIdx.x == 0)
+      for (int d = tid; d < digits; d += kTileThreads) starts[d] = s_first[d];
+    for (int d = tid; d < digits; d += kTileThreads) s_first[d] += hist[(size_t)blockIdx.x * digits + d];
+  }
   volatile uint16_t *mine = s_count[wave];
   const u64 below = (1ull << lane) - 1ull;
   for (int round = 0; round < rounds; ++round) {
@@ -239,6 +289,17 @@ __global__ __launch_bounds__(kTileThreads) void partitionTiles(ITEMS items, int6
       if (d < digits) s_first[d] += round_total[u];
     }
   }
+}
+
+// The same in two launches, for up to kFewTiles tiles.
+template <typename ITEMS>
+hipError_t partitionFew(hipStream_t stream, const ITEMS &items, int64_t n, int digits, int digit_bits,
+                        uint32_t *counters) {
+  uint32_t *hist = counters + kMaxDigits;
+  countTiles<ITEMS><<<tilesFor(n), kTileThreads, 0, stream>>>(items, n, digits, 1, hist);
+  partitionTiles<ITEMS, false><<<tilesFor(n), kTileThreads, 0, stream>>>(items, n, digits, digit_bits, 1, hist, nullptr,
+                                                                         nullptr);
+  return hipGetLastError();
 }
 
 template <typename ITEMS>

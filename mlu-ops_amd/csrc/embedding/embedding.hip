@@ -69,11 +69,14 @@ __global__ __launch_bounds__(kThreads) void embeddingRows(const T *__restrict__ 
 // ---- backward ------------------------------------------------------------------------------
 //
 // The places of the tokens are sorted by the row they name (equal rows in ascending place): each row of the table then has
-// its gradients' places side by side, and adds them up in a fixed order, without atomics.  Rows named at most kPiece times
-// are summed by the threads that own them.  Longer ones are cut into pieces at multiples of kPiece of the sorted places;
+// its gradients' places side by side, and adds them up in a fixed order, without atomics.  Rows named no more often
+// than a piece is long are summed by the threads that own them.  Longer ones are cut at multiples of it in the sorted places;
 // each piece is summed by a workgroup of its own, and a last launch adds the pieces.
 
-constexpr int kPiece = 64;
+// Words of a piece.  Where a row has many channels its workgroups have no threads to share a piece's words, but more sums to
+// keep: us of the whole gradient at pieces of 32 / 64 words: 120 000 tokens, 517 x 64 fp32: 47 / 52; 65 536 tokens,
+// 131 072 x 2048 bf16: 222 / 216.
+int pieceOf(int64_t channels) { return channels >= 1024 ? 64 : 32; }
 
 // Sorted words: the row above, the place below.
 struct FirstPass {
@@ -85,6 +88,39 @@ struct FirstPass {
   __device__ uint32_t digit(const Item &t) const { return (uint32_t)(t >> 32) & mask; }
   __device__ void store(size_t to, const Item &t, int64_t) const { out[to] = t; }
 };
+
+// Up to kRankedTokens: the place of a word is the number of words below it, counted by a wave for kRanked words at once.
+// One launch, whose work grows with the square of the tokens (us of the whole sort in three launches a pass / this: see
+// below).
+constexpr int kRanked = 4, kRankedTokens = 4096;
+__global__ __launch_bounds__(kThreads) void embeddingRankWords(Tokens tokens, uint32_t n, u64 *__restrict__ sorted) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t first = (blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kRanked;
+  if (first >= n) return;
+  // (words are compared as pairs of a row and a place: one row beside the others is enough where places decide by themselves)
+  uint32_t row[kRanked], below[kRanked] = {};
+#pragma unroll
+  for (int j = 0; j < kRanked; ++j) row[j] = tokens.row(min(first + j, n - 1));
+  constexpr int kAhead = 8;
+  for (uint32_t i0 = lane; i0 < n; i0 += 64 * kAhead) {
+    uint32_t other[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) other[a] = tokens.row(min(i0 + a * 64, n - 1));
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const uint32_t i = i0 + a * 64;
+#pragma unroll
+      for (int j = 0; j < kRanked; ++j)
+        below[j] += i < n && (other[a] < row[j] || (other[a] == row[j] && i < first + j)) ? 1u : 0u;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kRanked; ++j) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) below[j] += __shfl_xor(below[j], d, 64);
+    if (lane == j && first + j < n) sorted[below[j]] = (u64)row[j] << 32 | (first + j);
+  }
+}
 
 // The place of the first sorted word of every row, and of `rows`, where the words end that name a row.
 __global__ __launch_bounds__(kThreads) void embeddingRowStarts(const u64 *__restrict__ sorted, uint32_t n, uint32_t rows,
@@ -102,94 +138,143 @@ __global__ __launch_bounds__(kThreads) void embeddingRowStarts(const u64 *__rest
   starts[row] = lo;
 }
 
-// Adds the gradients of sorted words [begin, end) to sum, one after the other, a few loads in flight.
+// Adds the gradients of the sorted words begin, begin + step, ... below end to sum, a few loads in flight.
 template <typename T, int V>
 __device__ __forceinline__ void addRows(const T *__restrict__ grad, int64_t row_stride, const u64 *__restrict__ sorted,
-                                        uint32_t begin, uint32_t end, int channel, float (&sum)[V]) {
-  constexpr int kAhead = 4;
-  for (uint32_t i = begin; i < end; i += kAhead) {
-    float v[kAhead][V];
+                                        uint32_t begin, uint32_t end, uint32_t step, int channel, float (&sum)[V]) {
+  constexpr int kAhead = 8;
+  for (uint32_t i = begin; i < end; i += kAhead * step) {
+    Vector<T, V> v[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      // (behind the end the last one again, which is not added)
-      const uint32_t place = (uint32_t)sorted[i + j < end ? i + j : end - 1];
-      loadFloats<T, V>(grad + (int64_t)place * row_stride + channel, v[j]);
+      // (behind the end the first one again, which is not added)
+      const uint32_t place = (uint32_t)sorted[i + j * step < end ? i + j * step : i];
+      v[j] = *reinterpret_cast<const Vector<T, V> *>(grad + (int64_t)place * row_stride + channel);
     }
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-      if (i + j < end) {
+      if (i + j * step < end) {
 #pragma unroll
-        for (int c = 0; c < V; ++c) sum[c] += v[j][c];
+        for (int c = 0; c < V; ++c) sum[c] += (float)v[j].v[c];
       }
+  }
+}
+
+// Sums of V values over the `rows` rows of threads of a workgroup (in `scratch`, THREADS * V floats), in the threads of row 0.
+// By the whole workgroup.
+template <int V>
+__device__ __forceinline__ void sumOverThreadRows(int row, int rows, int across, float *scratch, float (&sum)[V]) {
+  for (int left = rows; left > 1;) {
+    const int half = (left + 1) / 2;
+    if (row >= half && row < left) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) scratch[threadIdx.x * V + v] = sum[v];
+    }
+    __syncthreads();
+    if (row >= 0 && row + half < left) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) sum[v] += scratch[(threadIdx.x + half * across) * V + v];
+    }
+    left = half;
   }
 }
 
 struct Sorted {
   const u64 *words;
   const uint32_t *starts;
-  uint32_t n, rows, pieces;
+  uint32_t n, rows, piece;
+  bool streamed;
 };
 
 // The first row_blocks workgroups own rows of the table.  The others take a piece each: of the rows that are longer than
 // one, at most two reach into it, that of its first word and that of its last.
-template <typename T, int V>
+template <typename T, int V, int kTableRows>
 __global__ __launch_bounds__(kThreads) void embeddingGradRows(const T *__restrict__ grad, int64_t row_stride,
                                                               int channels, Sorted s, float scale, int row_blocks,
                                                               float *__restrict__ partial, T *__restrict__ out) {
+  __shared__ float s_sum[kThreads * V];
   const Lanes<V> l(channels);
   if ((int)blockIdx.x < row_blocks) {
-    const uint32_t row = blockIdx.x * l.rows_at_once + l.row;
-    if (l.row < 0 || row >= s.rows) return;
-    const uint32_t begin = s.starts[row], end = s.starts[row + 1];
-    if (end - begin > (uint32_t)kPiece) return;
-    float sum[V] = {};
-    addRows<T, V>(grad, row_stride, s.words, begin, end, l.channel, sum);
-    if (begin < end) {
+    if (l.row < 0) return;
+    const uint32_t first = blockIdx.x * l.rows_at_once * kTableRows + l.row;
+    uint32_t begin[kTableRows], end[kTableRows];
 #pragma unroll
-      for (int c = 0; c < V; ++c) sum[c] *= scale;
+    for (int j = 0; j < kTableRows; ++j) {
+      const uint32_t row = min(first + j * l.rows_at_once, s.rows - 1);
+      begin[j] = s.starts[row];
+      end[j] = s.starts[row + 1];
     }
-    storeFloats<T, V>(out + (int64_t)row * channels + l.channel, sum);
+#pragma unroll
+    for (int j = 0; j < kTableRows; ++j) {
+      const uint32_t row = first + j * l.rows_at_once;
+      if (row >= s.rows) return;
+      if (end[j] - begin[j] > s.piece) continue;
+      float sum[V] = {};
+      if (begin[j] < end[j]) {
+        addRows<T, V>(grad, row_stride, s.words, begin[j], end[j], 1, l.channel, sum);
+#pragma unroll
+        for (int c = 0; c < V; ++c) sum[c] *= scale;
+      }
+      storeFloats<T, V>(out + (int64_t)row * channels + l.channel, sum, s.streamed);
+    }
     return;
   }
   const uint32_t piece = blockIdx.x - row_blocks;
-  const uint32_t lo = piece * kPiece, hi = min(lo + kPiece, s.n);
-  if (l.row < 0 || l.row > 1) return;
-  // (one row of threads where a row has all of them)
-  for (int side = l.row; side < 2; side += min(l.rows_at_once, 2)) {
+  const uint32_t lo = piece * s.piece, hi = min(lo + s.piece, s.n);
+  for (int side = 0; side < 2; ++side) {
     const uint32_t row = (uint32_t)(s.words[side == 0 ? lo : hi - 1] >> 32);
     if (row >= s.rows) continue;
     const uint32_t begin = s.starts[row], end = s.starts[row + 1];
-    if (end - begin <= (uint32_t)kPiece || (side == 1 && begin <= lo)) continue;
+    if (end - begin <= s.piece || (side == 1 && begin <= lo)) continue;
     float sum[V] = {};
-    addRows<T, V>(grad, row_stride, s.words, max(begin, lo), min(end, hi), l.channel, sum);
-    storeFloats<float, V>(partial + ((int64_t)piece * 2 + side) * channels + l.channel, sum);
+    if (l.row >= 0)
+      addRows<T, V>(grad, row_stride, s.words, max(begin, lo) + l.row, min(end, hi), l.rows_at_once, l.channel, sum);
+    __syncthreads();
+    sumOverThreadRows<V>(l.row, l.rows_at_once, l.across, s_sum, sum);
+    if (l.row == 0) storeFloats<float, V>(partial + ((int64_t)piece * 2 + side) * channels + l.channel, sum);
   }
 }
 
-// Adds up the pieces of the long row that begins in piece blockIdx.x, if one does (only one can reach beyond its end).
+// Adds up the pieces of the long row that begins in piece blockIdx.x, if one does (only one can reach beyond its end).  A
+// wave's width of threads across the channels, so that the workgroup's rows of threads share the pieces.
 template <typename T, int V>
 __global__ __launch_bounds__(kThreads) void embeddingGradJoin(int channels, Sorted s, float scale,
                                                               const float *__restrict__ partial, T *__restrict__ out) {
-  const uint32_t lo = blockIdx.x * kPiece, hi = min(lo + kPiece, s.n);
+  constexpr int kAhead = 4;
+  __shared__ float s_sum[kThreads * V];
+  const uint32_t lo = blockIdx.x * s.piece, hi = min(lo + s.piece, s.n);
   const uint32_t row = (uint32_t)(s.words[hi - 1] >> 32);
   if (row >= s.rows) return;
   const uint32_t begin = s.starts[row], end = s.starts[row + 1];
-  if (end - begin <= (uint32_t)kPiece || begin < lo) return;
-  const Lanes<V> l(channels);
-  if (l.row != 0) return;
+  if (end - begin <= s.piece || begin < lo) return;
+  const int across = min(channels / V - (int)blockIdx.y * 64, 64), rows = kThreads / across;
+  const int my_row = (int)threadIdx.x / across < rows ? (int)threadIdx.x / across : -1;
+  const int channel = ((int)blockIdx.y * 64 + (int)threadIdx.x % across) * V;
   float sum[V] = {};
-  const uint32_t last = (end - 1) / kPiece;
-  for (uint32_t p = blockIdx.x; p <= last; ++p) {
-    // (a row that begins with a piece's first word is that piece's first)
-    const int side = p == blockIdx.x && begin > lo ? 1 : 0;
-    float v[V];
-    loadFloats<float, V>(partial + ((int64_t)p * 2 + side) * channels + l.channel, v);
+  if (my_row >= 0) {
+    const uint32_t last = (end - 1) / s.piece;
+    for (uint32_t p0 = blockIdx.x + my_row; p0 <= last; p0 += kAhead * rows) {
+      Vector<float, V> v[kAhead];
 #pragma unroll
-    for (int c = 0; c < V; ++c) sum[c] += v[c];
+      for (int j = 0; j < kAhead; ++j) {
+        const uint32_t p = min(p0 + j * rows, last);
+        // (a row that begins with a piece's first word is that piece's first)
+        const int side = p == blockIdx.x && begin > lo ? 1 : 0;
+        v[j] = *reinterpret_cast<const Vector<float, V> *>(partial + ((int64_t)p * 2 + side) * channels + channel);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (p0 + j * rows > last) break;
+#pragma unroll
+        for (int c = 0; c < V; ++c) sum[c] += v[j].v[c];
+      }
+    }
   }
+  sumOverThreadRows<V>(my_row, rows, across, s_sum, sum);
+  if (my_row != 0) return;
 #pragma unroll
   for (int c = 0; c < V; ++c) sum[c] *= scale;
-  storeFloats<T, V>(out + (int64_t)row * channels + l.channel, sum);
+  storeFloats<T, V>(out + (int64_t)row * channels + channel, sum);
 }
 
 // ---- host side -----------------------------------------------------------------------------
@@ -208,7 +293,7 @@ Plan planOf(int64_t n, int64_t rows, int64_t channels) {
   p.bits = 1;
   while ((rows >> p.bits) != 0) ++p.bits;  // (up to `rows` itself, of tokens that name no row)
   p.pass_bits = device_sort::sortPassBits(p.bits);
-  p.pieces = (uint32_t)((n + kPiece - 1) / kPiece);
+  p.pieces = (uint32_t)((n + pieceOf(channels) - 1) / pieceOf(channels));
   p.words = rounded((size_t)n * sizeof(u64));
   p.counters = rounded(device_sort::sortCounterWords(n) * sizeof(uint32_t));
   p.starts = rounded((size_t)(rows + 1) * sizeof(uint32_t));
@@ -252,6 +337,10 @@ void byType(mluOpDataType_t type, int64_t channels, int64_t row_stride, uintptr_
     f(0.f, std::integral_constant<int, 1>());
   }
 }
+
+// Rows of the table that a row of threads owns, of `turns` it would own one at a time: several of a large table, most of
+// whose rows nobody names, and a workgroup for each would mostly start and end; one of a small table.
+int tableRows(int64_t turns) { return turns >= 16384 ? 4 : 1; }
 
 int rowsAtOnce(int64_t vectors) { return vectors >= kThreads ? 1 : (int)(kThreads / vectors); }
 unsigned slabsOf(int64_t vectors) { return (unsigned)((vectors + kThreads - 1) / kThreads); }
@@ -334,18 +423,32 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingBackward(mluOpHandle_t handle, mluO
   float *partial = reinterpret_cast<float *>(at + 2 * p.words + p.counters + p.starts);
 
   const mluop::LaunchCtx lc = handle->launchCtx();
+  const Tokens names = {tokens, token_type == MLUOP_DTYPE_INT64, (uint32_t)rows};
   bool in_second = false;
-  if (num_tokens > 0) {
-    const FirstPass first = {{tokens, token_type == MLUOP_DTYPE_INT64, (uint32_t)rows}, words[0], (1u << p.pass_bits) - 1u};
-    lc.begin("embeddingSort");
-    HIP_CHECK_RETURN(api, device_sort::partition(lc.stream, first, num_tokens, device_sort::sortDigits(p.pass_bits),
-                                                 p.pass_bits, counters));
-    HIP_CHECK_RETURN(api, (device_sort::sortPairs<u64, false>(lc.stream, counters, words[0], words[1], nullptr, nullptr,
-                                                              num_tokens, 32 + p.pass_bits, 32 + p.bits, p.pass_bits,
-                                                              &in_second)));
-    lc.end();
+  if (num_tokens > 0) lc.begin("embeddingSort");
+  if (num_tokens > kRankedTokens) {
+    const bool few = device_sort::tilesFor(num_tokens) <= device_sort::kFewTiles;
+    const int digits = device_sort::sortDigits(p.pass_bits);
+    const uint32_t mask = (1u << p.pass_bits) - 1u;
+    auto pass = [&](const auto &items) {
+      return few ? device_sort::partitionFew(lc.stream, items, num_tokens, digits, p.pass_bits, counters)
+                 : device_sort::partition(lc.stream, items, num_tokens, digits, p.pass_bits, counters);
+    };
+    HIP_CHECK_RETURN(api, pass(FirstPass{names, words[0], mask}));
+    for (int shift = 32 + p.pass_bits; shift < 32 + p.bits; shift += p.pass_bits) {
+      const device_sort::KeysAndValues<u64, false> items = {words[in_second ? 1 : 0], nullptr, words[in_second ? 0 : 1],
+                                                            nullptr, shift, mask};
+      HIP_CHECK_RETURN(api, pass(items));
+      in_second = !in_second;
+    }
+  } else if (num_tokens > 0) {
+    constexpr int kEach = kThreads / 64 * kRanked;
+    embeddingRankWords<<<(unsigned)((num_tokens + kEach - 1) / kEach), kThreads, 0, lc.stream>>>(
+        names, (uint32_t)num_tokens, words[0]);
   }
-  const Sorted s = {words[in_second ? 1 : 0], starts, (uint32_t)num_tokens, (uint32_t)rows, p.pieces};
+  if (num_tokens > 0) lc.end();
+  const Sorted s = {words[in_second ? 1 : 0], starts, (uint32_t)num_tokens, (uint32_t)rows, (uint32_t)pieceOf(channels),
+                    (size_t)rows * channels * elementBytes(type) >= kStreamedBytes};
   lc.begin("embeddingRowStarts");
   embeddingRowStarts<<<(unsigned)(rows / kThreads + 1), kThreads, 0, lc.stream>>>(s.words, s.n, s.rows, starts);
   lc.end();
@@ -354,15 +457,18 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingBackward(mluOpHandle_t handle, mluO
            typedef decltype(zero) T;
            constexpr int V = decltype(v)::value;
            const int64_t at_once = rowsAtOnce(channels / V);
-           const int row_blocks = (int)((rows + at_once - 1) / at_once);
+           const int each = tableRows(rows / at_once);
+           const int row_blocks = (int)((rows + at_once * each - 1) / (at_once * each));
+           auto kernel = each == 1 ? embeddingGradRows<T, V, 1> : embeddingGradRows<T, V, 4>;
            lc.begin("embeddingGradRows");
-           embeddingGradRows<T, V><<<dim3((unsigned)row_blocks + p.pieces, slabsOf(channels / V)), kThreads, 0, lc.stream>>>(
+           kernel<<<dim3((unsigned)row_blocks + p.pieces, slabsOf(channels / V)), kThreads, 0, lc.stream>>>(
                static_cast<const T *>(output_grad), row_stride, (int)channels, s, scale, row_blocks, partial,
                static_cast<T *>(grad_table));
            lc.end();
-           if (num_tokens <= kPiece) return;  // (no row can be longer)
+           if (num_tokens <= pieceOf(channels)) return;  // (no row can be longer)
            lc.begin("embeddingGradJoin");
-           embeddingGradJoin<T, V><<<dim3(p.pieces, slabsOf(channels / V)), kThreads, 0, lc.stream>>>(
+           constexpr int W = V < 4 ? V : 4;
+           embeddingGradJoin<T, W><<<dim3(p.pieces, (unsigned)((channels / W + 63) / 64)), kThreads, 0, lc.stream>>>(
                (int)channels, s, scale, partial, static_cast<T *>(grad_table));
            lc.end();
          });

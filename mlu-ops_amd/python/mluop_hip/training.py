@@ -81,7 +81,7 @@ def embedding_forward(handle, table, tokens, scale=1.0):
 
 def embedding_backward(handle, output_grad, tokens, rows, scale=1.0):
     """Gradient [rows, channels] of the table of `embedding_forward`: each row adds up the gradients of the tokens that
-    name it, in their order, in fp32."""
+    name it, in fp32 and in an order that the tokens alone decide."""
     return _native().embedding_backward(handle.ptr.value, _guarded(), output_grad, tokens, rows, scale)
 
 
