@@ -98,6 +98,25 @@ __device__ __forceinline__ RaggedTile findRaggedTile(const int32_t *starts, int 
   return t;
 }
 
+// All tiles of all segments (OUTSIDE: of segmentOrOutside).
+template <bool OUTSIDE>
+__device__ __forceinline__ int raggedTiles(const int32_t *starts, int rows, int segments, int tile_rows) {
+  const int lane = threadIdx.x & 63;
+  const int all = OUTSIDE ? segments + 2 : segments;
+  int sum = 0;
+  for (int base = 0; base < all; base += 64) {
+    int first = 0, count = 0;
+    if (base + lane < all) {
+      if (OUTSIDE)
+        segmentOrOutside(starts, rows, segments, base + lane, &first, &count);
+      else
+        segmentRows(starts, rows, base + lane, &first, &count);
+    }
+    sum += __builtin_amdgcn_readlane(waveInclusiveScan((count + tile_rows - 1) / tile_rows), 63);
+  }
+  return sum;
+}
+
 // The tiles of segment `segment`: how many, and the number of the first among all tiles.  Inside [0, most], the tiles that
 // mostRaggedTiles says there can be, whatever the starts hold.
 __device__ __forceinline__ int raggedTilesOf(const int32_t *starts, int rows, int segment, int tile_rows, int most,

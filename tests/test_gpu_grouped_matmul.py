@@ -96,6 +96,56 @@ def test_larger(gpu_handle, dtype, groups, rows, ci, co):
     compare(products(gpu_handle, x, w, dy, dev), x, w, dy, starts, dtype)
 
 
+def launched(handle, call):
+    """(the call's result, the names of the kernels it launched)"""
+    import mluop_hip
+    handle.set_kernel_timing(True)
+    try:
+        out = call()
+        return out, [name for name, _ in handle.kernel_timings()]
+    finally:
+        handle.set_kernel_timing(False)
+
+
+KINDS = [  # groups, rows, ci, co, the kernels of the three products
+    (3, 40, 512, 1032, ("groupedFew16", "groupedFew16", "groupedTiles")),
+    (2, 700, 1024, 520, ("groupedFew", "groupedFew", "groupedTiles")),
+    (5, 1200, 2048, 2048, ("groupedTiles64", "groupedTiles64", "groupedTiles")),
+    (1, 4100, 2056, 2048, ("groupedTiles128", "groupedTiles128", "groupedTiles")),
+    (7, 16000, 1032, 1024, ("groupedTiles", "groupedTiles", "groupedTiles")),
+    (1, 16000, 2048, 2048, ("groupedTiles256", "groupedTiles256", "groupedTiles256")),
+    (1, 30000, 64, 72, ("groupedTiles", "groupedTiles", "groupedTiles"))]
+
+
+@pytest.mark.parametrize("groups,rows,ci,co,kinds", KINDS)
+def test_every_tile(gpu_handle, groups, rows, ci, co, kinds):
+    """uneven groups at sizes at which each kernel is the one that runs (small whole numbers: sums are exact in fp32)"""
+    import random
+    import torch
+    import mluop_hip
+    print("grouped tiles", groups, rows, ci, co, flush=True)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    rng = random.Random(groups)
+    starts = [0] + sorted(rng.randrange(rows + 1) for _ in range(groups - 1)) + [rows]
+    x = torch.randint(-2, 3, (rows, ci), device="cuda", generator=g).half()
+    w = torch.randint(-1, 2, (groups, ci, co), device="cuda", generator=g).half()
+    dy = torch.randint(-1, 2, (rows, co), device="cuda", generator=g).half()
+    dev = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    want = [torch.empty_like(dy, dtype=torch.float32), torch.empty_like(x, dtype=torch.float32),
+            torch.empty(w.shape, device="cuda")]
+    for k, (a, b) in enumerate(zip(starts, starts[1:])):
+        want[0][a:b] = x[a:b].float() @ w[k].float()
+        want[1][a:b] = dy[a:b].float() @ w[k].float().t().contiguous()
+        want[2][k] = x[a:b].float().t().contiguous() @ dy[a:b].float()
+    calls = (lambda: mluop_hip.grouped_matmul_forward(gpu_handle, x, w, dev),
+             lambda: mluop_hip.grouped_matmul_backward_data(gpu_handle, dy, w, dev),
+             lambda: mluop_hip.grouped_matmul_backward_filter(gpu_handle, x, dy, dev))
+    for call, v, kind in zip(calls, want, kinds):
+        got, names = launched(gpu_handle, call)
+        assert names and names[0].startswith(kind), names
+        assert float(v.abs().max()) < 2 ** 24 and torch.equal(got, v.half())
+
+
 def test_integers_are_exact(gpu_handle):
     """small whole numbers: every sum is exact in fp32, so any wrong element shows"""
     import torch
