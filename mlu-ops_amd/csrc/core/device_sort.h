@@ -221,6 +221,10 @@ __global__ __launch_bounds__(kTileThreads) void partitionTiles(ITEMS items, int6
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if constexpr (!SCANNED) {
     digitStartsOfTile(hist, gridDim.x, digits, s_first, s_wave);
+    if (starts != nullptr && blockIdx.x == 0) {  // (no tile in front of this one)
+      __syncthreads();
+      for (int d = tid; d < digits; d += kTileThreads) starts[d] = s_first[d];
+    }
   } else {
     digitStarts(totals, digits, s_first, s_wave);
     __syncthreads();
@@ -294,23 +298,23 @@ __global__ __launch_bounds__(kTileThreads) void partitionTiles(ITEMS items, int6
 // The same in two launches, for up to kFewTiles tiles.
 template <typename ITEMS>
 hipError_t partitionFew(hipStream_t stream, const ITEMS &items, int64_t n, int digits, int digit_bits,
-                        uint32_t *counters) {
+                        uint32_t *counters, uint32_t *starts = nullptr) {
   uint32_t *hist = counters + kMaxDigits;
   countTiles<ITEMS><<<tilesFor(n), kTileThreads, 0, stream>>>(items, n, digits, 1, hist);
   partitionTiles<ITEMS, false><<<tilesFor(n), kTileThreads, 0, stream>>>(items, n, digits, digit_bits, 1, hist, nullptr,
-                                                                         nullptr);
+                                                                         starts);
   return hipGetLastError();
 }
 
 template <typename ITEMS>
 hipError_t partition(hipStream_t stream, const ITEMS &items, int64_t n, int digits, int digit_bits,
-                     uint32_t *counters) {
+                     uint32_t *counters, uint32_t *starts = nullptr) {
   const int tiles = tilesFor(n), rounds = roundsFor(n);
   uint32_t *totals = counters, *hist = counters + kMaxDigits;
   countTiles<ITEMS><<<tiles, kTileThreads, 0, stream>>>(items, n, digits, rounds, hist);
   scanColumns<<<digits / kColumns, kColumns * kColumnGroups, 0, stream>>>(hist, tiles, digits, totals);
   partitionTiles<ITEMS><<<tiles, kTileThreads, 0, stream>>>(items, n, digits, digit_bits, rounds, hist, totals,
-                                                            nullptr);
+                                                            starts);
   return hipGetLastError();
 }
 

@@ -73,10 +73,17 @@ __global__ __launch_bounds__(kThreads) void embeddingRows(const T *__restrict__ 
 // than a piece is long are summed by the threads that own them.  Longer ones are cut at multiples of it in the sorted places;
 // each piece is summed by a workgroup of its own, and a last launch adds the pieces.
 
-// Words of a piece.  Where a row has many channels its workgroups have no threads to share a piece's words, but more sums to
-// keep: us of the whole gradient at pieces of 32 / 64 words: 120 000 tokens, 517 x 64 fp32: 47 / 52; 65 536 tokens,
+// Whether all rows of threads of a workgroup share a row of the table: one that is named often, as all are in a small table.
+bool rowsShared(int64_t n, int64_t rows, int64_t channels) { return n >= 16 * rows && channels < 1024; }
+
+// Words of a piece: as many as the rows of threads of a workgroup (which V = 4 has) read at once, eight each, where they
+// share rows of the table.  Where one of them sums a row alone, fewer; but where a row has many channels there are no
+// threads to share a piece either, and sums to keep.  us of the whole gradient at pieces of 32 / 64 words, 65 536 tokens,
 // 131 072 x 2048 bf16: 222 / 216.
-int pieceOf(int64_t channels) { return channels >= 1024 ? 64 : 32; }
+int pieceOf(int64_t n, int64_t rows, int64_t channels) {
+  if (rowsShared(n, rows, channels)) return (int)std::max<int64_t>(8 * (kThreads * 4 / std::max<int64_t>(channels, 4)), 64);
+  return channels >= 1024 ? 64 : 32;
+}
 
 // Sorted words: the row above, the place below.
 struct FirstPass {
@@ -89,10 +96,11 @@ struct FirstPass {
   __device__ void store(size_t to, const Item &t, int64_t) const { out[to] = t; }
 };
 
-// Up to kRankedTokens: the place of a word is the number of words below it, counted by a wave for kRanked words at once.
-// One launch, whose work grows with the square of the tokens (us of the whole sort in three launches a pass / this: see
-// below).
-constexpr int kRanked = 4, kRankedTokens = 4096;
+// Few tokens (rankedTokens): the place of a word is the number of words below it, counted by a wave for kRanked words at once.
+// One launch, whose work grows with the square of the tokens.  us of a whole gradient with this: 1024 tokens 16 to 18, 2048 21 to 22,
+// 4096 30 to 32; with one pass of the sort (tables of up to 1023 rows) 17 to 19, with two 33.
+constexpr int kRanked = 4;
+int rankedTokens(int passes) { return passes == 1 ? 1024 : 3000; }
 __global__ __launch_bounds__(kThreads) void embeddingRankWords(Tokens tokens, uint32_t n, u64 *__restrict__ sorted) {
   const int lane = threadIdx.x & 63;
   const uint32_t first = (blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kRanked;
@@ -188,12 +196,27 @@ struct Sorted {
 
 // The first row_blocks workgroups own rows of the table.  The others take a piece each: of the rows that are longer than
 // one, at most two reach into it, that of its first word and that of its last.
-template <typename T, int V, int kTableRows>
+// SHARED: a row of the table a workgroup, whose rows of threads share the words.
+template <typename T, int V, int kTableRows, bool SHARED>
 __global__ __launch_bounds__(kThreads) void embeddingGradRows(const T *__restrict__ grad, int64_t row_stride,
                                                               int channels, Sorted s, float scale, int row_blocks,
                                                               float *__restrict__ partial, T *__restrict__ out) {
   __shared__ float s_sum[kThreads * V];
   const Lanes<V> l(channels);
+  if (SHARED && (int)blockIdx.x < row_blocks) {
+    const uint32_t row = blockIdx.x, begin = s.starts[row], end = s.starts[row + 1];
+    if (end - begin > s.piece) return;
+    float sum[V] = {};
+    if (l.row >= 0) addRows<T, V>(grad, row_stride, s.words, begin + l.row, end, l.rows_at_once, l.channel, sum);
+    sumOverThreadRows<V>(l.row, l.rows_at_once, l.across, s_sum, sum);
+    if (l.row != 0) return;
+    if (begin < end) {
+#pragma unroll
+      for (int c = 0; c < V; ++c) sum[c] *= scale;
+    }
+    storeFloats<T, V>(out + (int64_t)row * channels + l.channel, sum, s.streamed);
+    return;
+  }
   if ((int)blockIdx.x < row_blocks) {
     if (l.row < 0) return;
     const uint32_t first = blockIdx.x * l.rows_at_once * kTableRows + l.row;
@@ -280,7 +303,7 @@ __global__ __launch_bounds__(kThreads) void embeddingGradJoin(int channels, Sort
 // ---- host side -----------------------------------------------------------------------------
 
 struct Plan {
-  int bits, pass_bits;
+  int bits, pass_bits, piece;
   uint32_t pieces;
   size_t words, counters, starts, partial;  // bytes of each part
   size_t all() const { return 256 + 2 * words + counters + starts + partial; }
@@ -293,10 +316,11 @@ Plan planOf(int64_t n, int64_t rows, int64_t channels) {
   p.bits = 1;
   while ((rows >> p.bits) != 0) ++p.bits;  // (up to `rows` itself, of tokens that name no row)
   p.pass_bits = device_sort::sortPassBits(p.bits);
-  p.pieces = (uint32_t)((n + pieceOf(channels) - 1) / pieceOf(channels));
+  p.piece = pieceOf(n, rows, channels);
+  p.pieces = (uint32_t)((n + p.piece - 1) / p.piece);
   p.words = rounded((size_t)n * sizeof(u64));
   p.counters = rounded(device_sort::sortCounterWords(n) * sizeof(uint32_t));
-  p.starts = rounded((size_t)(rows + 1) * sizeof(uint32_t));
+  p.starts = rounded((size_t)std::max<int64_t>(rows + 1, device_sort::kMaxDigits) * sizeof(uint32_t));
   p.partial = rounded((size_t)p.pieces * 2 * channels * sizeof(float));
   return p;
 }
@@ -424,15 +448,18 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingBackward(mluOpHandle_t handle, mluO
 
   const mluop::LaunchCtx lc = handle->launchCtx();
   const Tokens names = {tokens, token_type == MLUOP_DTYPE_INT64, (uint32_t)rows};
-  bool in_second = false;
+  bool in_second = false, started = false;
   if (num_tokens > 0) lc.begin("embeddingSort");
-  if (num_tokens > kRankedTokens) {
+  if (num_tokens > rankedTokens((p.bits + p.pass_bits - 1) / p.pass_bits)) {
     const bool few = device_sort::tilesFor(num_tokens) <= device_sort::kFewTiles;
     const int digits = device_sort::sortDigits(p.pass_bits);
     const uint32_t mask = (1u << p.pass_bits) - 1u;
+    // (where one pass sorts, its digits are the rows)
+    started = p.pass_bits >= p.bits;
+    uint32_t *firsts = started ? starts : nullptr;
     auto pass = [&](const auto &items) {
-      return few ? device_sort::partitionFew(lc.stream, items, num_tokens, digits, p.pass_bits, counters)
-                 : device_sort::partition(lc.stream, items, num_tokens, digits, p.pass_bits, counters);
+      return few ? device_sort::partitionFew(lc.stream, items, num_tokens, digits, p.pass_bits, counters, firsts)
+                 : device_sort::partition(lc.stream, items, num_tokens, digits, p.pass_bits, counters, firsts);
     };
     HIP_CHECK_RETURN(api, pass(FirstPass{names, words[0], mask}));
     for (int shift = 32 + p.pass_bits; shift < 32 + p.bits; shift += p.pass_bits) {
@@ -447,25 +474,30 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingBackward(mluOpHandle_t handle, mluO
         names, (uint32_t)num_tokens, words[0]);
   }
   if (num_tokens > 0) lc.end();
-  const Sorted s = {words[in_second ? 1 : 0], starts, (uint32_t)num_tokens, (uint32_t)rows, (uint32_t)pieceOf(channels),
+  const Sorted s = {words[in_second ? 1 : 0], starts, (uint32_t)num_tokens, (uint32_t)rows, (uint32_t)p.piece,
                     (size_t)rows * channels * elementBytes(type) >= kStreamedBytes};
-  lc.begin("embeddingRowStarts");
-  embeddingRowStarts<<<(unsigned)(rows / kThreads + 1), kThreads, 0, lc.stream>>>(s.words, s.n, s.rows, starts);
-  lc.end();
+  if (!started) {
+    lc.begin("embeddingRowStarts");
+    embeddingRowStarts<<<(unsigned)(rows / kThreads + 1), kThreads, 0, lc.stream>>>(s.words, s.n, s.rows, starts);
+    lc.end();
+  }
   byType(type, channels, row_stride, reinterpret_cast<uintptr_t>(output_grad) | reinterpret_cast<uintptr_t>(grad_table),
          [&](auto zero, auto v) {
            typedef decltype(zero) T;
            constexpr int V = decltype(v)::value;
            const int64_t at_once = rowsAtOnce(channels / V);
+           const bool shared = rowsShared(num_tokens, rows, channels);
            const int each = tableRows(rows / at_once);
-           const int row_blocks = (int)((rows + at_once * each - 1) / (at_once * each));
-           auto kernel = each == 1 ? embeddingGradRows<T, V, 1> : embeddingGradRows<T, V, 4>;
+           const int row_blocks = (int)(shared ? rows : (rows + at_once * each - 1) / (at_once * each));
+           auto kernel = shared      ? embeddingGradRows<T, V, 1, true>
+                         : each == 1 ? embeddingGradRows<T, V, 1, false>
+                                     : embeddingGradRows<T, V, 4, false>;
            lc.begin("embeddingGradRows");
            kernel<<<dim3((unsigned)row_blocks + p.pieces, slabsOf(channels / V)), kThreads, 0, lc.stream>>>(
                static_cast<const T *>(output_grad), row_stride, (int)channels, s, scale, row_blocks, partial,
                static_cast<T *>(grad_table));
            lc.end();
-           if (num_tokens <= pieceOf(channels)) return;  // (no row can be longer)
+           if (num_tokens <= p.piece) return;  // (no row can be longer)
            lc.begin("embeddingGradJoin");
            constexpr int W = V < 4 ? V : 4;
            embeddingGradJoin<T, W><<<dim3(p.pieces, (unsigned)((channels / W + 63) / 64)), kThreads, 0, lc.stream>>>(
