@@ -14,9 +14,9 @@ mluOpStatus_t checkShape(const char *api, mluOpDataType_t type, int64_t rows, in
   PARAM_CHECK(api, groups > 0);
   PARAM_CHECK(api, ci > 0);
   PARAM_CHECK(api, co > 0);
-  if (rows > INT32_MAX - 4096 || groups > (1 << 16) || ci > (1 << 20) || co > (1 << 20) || ci * co > ((int64_t)1 << 30) ||
+  if (rows > INT32_MAX - 4096 || groups > 65535 || ci > (1 << 20) || co > (1 << 20) || ci * co > ((int64_t)1 << 30) ||
       groups * ci * co > ((int64_t)1 << 44)) {
-    MLUOP_LOG(ERROR) << api << " At most 2^31 - 4097 rows, 2^16 groups, 2^20 channels and 2^30 elements of a filter are "
+    MLUOP_LOG(ERROR) << api << " At most 2^31 - 4097 rows, 65 535 groups, 2^20 channels and 2^30 elements of a filter are "
                      << "supported.";
     return MLUOP_STATUS_NOT_SUPPORTED;
   }
