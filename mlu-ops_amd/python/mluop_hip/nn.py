@@ -368,14 +368,38 @@ class ExpertLinear(torch.nn.Module):
 
 
 def expert_order(experts_of_rows, experts):
-    """(rows, group_starts) of a routing [rows, choices] of integers in [0, experts): the source row of every place when all
-    choices are ordered by expert (equal experts by row), int32 [rows * choices], and where each expert's places begin,
-    int32 [experts + 1].  `embedding(features, rows)` then puts rows into that order, and its gradient adds the
-    copies of a row up again."""
+    """(rows, group_starts, places) of a routing [rows, choices] of integers in [0, experts): the source row of every place
+    when all choices are ordered by expert (equal experts by row), int32 [rows * choices]; where each expert's
+    places begin, int32 [experts + 1]; and the place of every row's choices, int32 [rows, choices].
+    `embedding(features, rows)` puts rows into that order, and its gradient adds the copies of a row up again;
+    `embedding(results, places)` brings the results back."""
     flat = experts_of_rows.reshape(experts_of_rows.shape[0], -1)
-    ordered, place = torch.sort(flat.reshape(-1), stable=True)
+    ordered, order = torch.sort(flat.reshape(-1), stable=True)
     starts = torch.searchsorted(ordered, torch.arange(experts + 1, device=flat.device, dtype=ordered.dtype), out_int32=True)
-    return torch.div(place, max(flat.shape[1], 1), rounding_mode="floor").to(torch.int32), starts
+    places = torch.empty_like(order, dtype=torch.int32)
+    places[order] = torch.arange(order.shape[0], device=flat.device, dtype=torch.int32)
+    rows = torch.div(order, max(flat.shape[1], 1), rounding_mode="floor").to(torch.int32)
+    return rows, starts, places.view(flat.shape)
+
+
+class ExpertMLP(torch.nn.Module):
+    """Two expert layers with SiLU in between; every row of features [rows, channels] goes to `choices` of `experts`, the
+    largest of a learned linear map, and its results are added up with the softmax of their scores as weights.  One row (a
+    step of a program that answers) takes the same way as a batch."""
+
+    def __init__(self, channels, hidden, experts, choices):
+        super().__init__()
+        self.experts, self.choices = int(experts), int(choices)
+        self.gate = torch.nn.Linear(channels, experts, bias=False)
+        self.up = ExpertLinear(experts, channels, hidden)
+        self.down = ExpertLinear(experts, hidden, channels)
+
+    def forward(self, features):
+        scores, chosen = torch.topk(self.gate(features.to(self.gate.weight.dtype)), self.choices, dim=1)
+        rows, starts, places = expert_order(chosen, self.experts)
+        hidden = torch.nn.functional.silu(self.up(embedding(features, rows), starts))
+        results = embedding(self.down(hidden, starts), places)
+        return (results * torch.softmax(scores, dim=1).to(results.dtype).unsqueeze(2)).sum(dim=1)
 
 
 def group_norm(features, weight, bias, groups, row_starts=None, eps=1e-5, activation="none"):
