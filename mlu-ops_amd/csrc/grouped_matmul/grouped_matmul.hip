@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "core/elements.h"
 #include "core/ragged.h"
@@ -59,6 +60,8 @@ struct Args {
   int most_slices;
   int blocks;       // backward filter: slices there can be, or groups
   int works;        // numbers of works (some of which may not be there)
+  int wide;         // of tiles of rows: workgroups of an XCD whose last round, filled to a quarter or less, is left for smaller tiles; or 0
+  bool streamed;    // results go past the caches
   float *partial;   // backward filter in slices: sums [slice, ci, co]
 };
 
@@ -386,69 +389,143 @@ struct Work {
   int64_t out;               // element of the result's (or the partial sums') first
 };
 
-// Tile of rows number `number`, and which of the tiles_n tiles of columns.  Workgroups go to the eight XCDs in turn, and so
-// do the numbers; an XCD has a run of tiles that share operands in its L2: four tiles of rows by all columns, then the
-// next four.
-template <int BM>
-__device__ __forceinline__ RaggedTile tileOfRows(int number, const int32_t *starts, const Args &a, int tiles_n, int *column) {
+// Tile number `tile` of total_m by tiles_n: bands of four by all columns, so that tiles side by side in number share operands.
+__device__ __forceinline__ void placeOfTile(int tile, int total_m, int tiles_n, int *row, int *column) {
   constexpr int kBand = 4;
-  const int total_m = raggedTiles<true>(starts, a.rows, a.groups, BM), total = total_m * tiles_n, each = (total + 7) / 8;
-  const int in_xcd = number >> 3, tile = (number & 7) * each + in_xcd;
-  if (in_xcd >= each || tile >= total) {
+  const int band = tile / (kBand * tiles_n), in_band = tile - band * (kBand * tiles_n);
+  const int height = min(total_m - band * kBand, kBand);
+  *column = in_band / height;
+  *row = band * kBand + in_band % height;
+}
+
+// Tiles of rows: workgroups go to the eight XCDs in turn, and so do the numbers; an XCD has a run of tiles that share
+// operands in its L2.
+struct RowTiles {
+  int total_m, tiles_n;
+  int each, kept;  // numbers of an XCD: all, and those in front of a last round that is left for smaller tiles
+};
+template <int BM>
+__device__ __forceinline__ RowTiles rowTilesOf(const int32_t *starts, const Args &a, int tiles_n) {
+  RowTiles all;
+  all.total_m = raggedTiles<true>(starts, a.rows, a.groups, BM);
+  all.tiles_n = tiles_n;
+  all.each = all.kept = (all.total_m * tiles_n + 7) / 8;
+  if (a.wide > 0 && all.each % a.wide <= a.wide / 4) all.kept -= all.each % a.wide;
+  return all;
+}
+// Number `in_xcd` of an XCD, and which of the tiles of columns.
+template <int BM>
+__device__ __forceinline__ RaggedTile tileOfRows(const RowTiles &all, int xcd, int in_xcd, const int32_t *starts, const Args &a,
+                                                 int *column) {
+  const int tile = xcd * all.each + in_xcd;
+  if (in_xcd >= all.each || tile >= all.total_m * all.tiles_n) {
     RaggedTile none = {};
     none.segment = -1;
     return none;
   }
-  const int band = tile / (kBand * tiles_n), in_band = tile - band * (kBand * tiles_n);
-  const int height = min(total_m - band * kBand, kBand);
-  *column = in_band / height;
-  return findRaggedTile<true>(starts, a.rows, a.groups, BM, band * kBand + in_band % height);
+  int row;
+  placeOfTile(tile, all.total_m, all.tiles_n, &row, column);
+  return findRaggedTile<true>(starts, a.rows, a.groups, BM, row);
+}
+
+// In which order a workgroup takes its works (in LDS; NULL: by number).
+struct Order {
+  const uint16_t *longest;  // groups by falling length
+  const uint16_t *taken;    // this workgroup's share of what does not fill a round of its XCD: [place in `longest`, tile of the XCD's]; or NULL
+  int whole;                // rounds that an XCD's tiles of every group make
+};
+// Of `tiles` tiles of a block (a group, or a slice of its rows) every XCD has an eighth, tiles that lie side by side;
+// where eighths are of different sizes, the next block has them turned by one XCD.
+__device__ __forceinline__ int eighthFrom(int tiles, int eighth) { return (int)((int64_t)tiles * eighth >> 3); }
+__device__ __forceinline__ int eighthOf(int xcd, int block) { return (xcd + block) & 7; }
+
+constexpr int kStartsInLds = 2048, kRankedGroups = 256, kSharedGroups = 64, kEndSteps = 3;
+constexpr int kShared = 1024;  // groups x workgroups of an XCD
+
+// Groups are of very different lengths, and rounds of works of different lengths wait for whoever has most of the long ones.
+// So every workgroup works out who takes what: group by group, the longest first, whose tiles go to those workgroups of
+// the XCD that have least.  A lane stands for a workgroup; keys are steps of work so far (a tile's beginning and end take some
+// kEndSteps) above the lane's number, so that no two are the same.
+__device__ __forceinline__ int shareOut(const uint16_t *longest, const int32_t *starts, const Args &a, int step, int tiles,
+                                        int behind, int wide, uint16_t *taken) {
+  const int lane = threadIdx.x & 63, own = blockIdx.x >> 3, xcd = blockIdx.x & 7;
+  int first, rows = 0, count = 0;
+  if (lane < a.groups) segmentRows(starts, a.rows, longest[lane], &first, &rows);
+  const uint32_t cost = (uint32_t)((rows + step - 1) / step + kEndSteps) << 6;
+  uint32_t key = lane < wide ? (uint32_t)lane : ~0u;
+  auto rankAmong = [&](auto n) {
+    int rank = 0;
+#pragma unroll
+    for (int o = 0; o < decltype(n)::value; ++o) rank += (uint32_t)__builtin_amdgcn_readlane((int)key, o) < key ? 1 : 0;
+    return rank;
+  };
+  for (int g = 0; g < a.groups; ++g) {
+    const int rank = wide > 32 ? rankAmong(std::integral_constant<int, 64>()) : rankAmong(std::integral_constant<int, 32>());
+    const int eighth = eighthOf(xcd, g);
+    const bool takes = lane < wide && behind + rank < eighthFrom(tiles, eighth + 1) - eighthFrom(tiles, eighth);
+    if (takes && lane == own) {
+      taken[2 * count] = (uint16_t)g;
+      taken[2 * count + 1] = (uint16_t)(behind + rank);
+    }
+    count += __builtin_amdgcn_readlane(takes ? 1 : 0, own);
+    if (takes) key += (uint32_t)__builtin_amdgcn_readlane((int)cost, g);
+  }
+  return count;
 }
 
 // Work number `number` of args.works, from the starts in LDS.  Workgroups go to the eight XCDs in turn, and so do the
-// numbers; those of an XCD take tiles that share operands in its L2.
-template <typename T, int MODE, int BM, int BN>
-__device__ __forceinline__ Work<T> workOf(int number, const int32_t *starts, const uint16_t *longest, const Args &a,
-                                          const T *left, const T *right) {
+// numbers; those of an XCD take tiles that share operands in its L2.  REST: the last round that is left by the kernel of tiles
+// twice as high and wide, a quarter of such a tile each.
+template <typename T, int MODE, int BM, int BN, bool REST>
+__device__ __forceinline__ Work<T> workOf(int number, int works, const int32_t *starts, const Order &order, const RowTiles &tiles,
+                                          const Args &a, const T *left, const T *right) {
   Work<T> w;
   w.there = false;
   w.extent = w.width = w.depth = 0;
   w.left = left;
   w.right = right;
   w.out = 0;
-  if (number >= a.works) return w;
+  if (number >= works) return w;
   const int columns = MODE == kBackwardData ? a.ci : a.co;
-  const int tiles_n = (columns + BN - 1) / BN;
-  const int xcd = number & 7;
   int in_xcd = number >> 3, n0;
   if (MODE == kBackwardFilter) {
-    // an eighth of every block's tiles (a group, or a slice of its rows) for each XCD: groups have very different lengths
-    const int per_block = (a.ci + BM - 1) / BM * tiles_n;
+    const int tiles_n = (columns + BN - 1) / BN, per_block = (a.ci + BM - 1) / BM * tiles_n;
+    const int xcd = blockIdx.x & 7, wide = gridDim.x >> 3;
     int block, tile;
-    if (per_block >= 8) {
-      // (every second round of the workgroups backwards: who had a long one has a short one next)
-      const int wide = gridDim.x >> 3, round = in_xcd / wide;
-      if (longest != nullptr && (round & 1) != 0)
-        in_xcd = 2 * round * wide + min(wide, (a.works >> 3) - round * wide) - 1 - in_xcd;
-      const int each = (per_block + 7) / 8;
-      block = in_xcd / each;
-      tile = xcd * each + in_xcd - block * each;
-      if (tile >= min(per_block, (xcd + 1) * each)) return w;
+    if (order.taken != nullptr) {
+      const int in_rest = number - a.groups * order.whole;
+      if (in_rest < 0) {
+        block = number / order.whole;
+        tile = (number - block * order.whole) * wide + (blockIdx.x >> 3);
+      } else {
+        block = __builtin_amdgcn_readfirstlane(order.taken[2 * in_rest]);
+        tile = __builtin_amdgcn_readfirstlane(order.taken[2 * in_rest + 1]);
+      }
+      tile += eighthFrom(per_block, eighthOf(xcd, block));
     } else {
-      block = number / per_block;
-      tile = number - block * per_block;
+      // (every second round of the workgroups backwards: who had a long one has a short one next)
+      const int round = in_xcd / wide;
+      if (order.longest != nullptr && (round & 1) != 0)
+        in_xcd = 2 * round * wide + min(wide, (works >> 3) - round * wide) - 1 - in_xcd;
+      // (of eight blocks an XCD has as many tiles as there are of one: from its own eighth on, and around)
+      const int eight = in_xcd / per_block;
+      tile = eighthFrom(per_block, xcd) + in_xcd - eight * per_block;
+      if (tile >= per_block) tile -= per_block;
+      const int eighth = (int)((8 * (int64_t)tile + 7) / per_block);
+      block = 8 * eight + ((eighth - xcd) & 7);
     }
     if (block >= a.blocks) return w;
-    const int m0 = tile / tiles_n * BM;
-    n0 = tile % tiles_n * BN;
-    int first;
+    int m0, first;
+    placeOfTile(tile, (a.ci + BM - 1) / BM, tiles_n, &m0, &n0);
+    m0 *= BM;
+    n0 *= BN;
     if (a.slice_rows > 0) {
       const RaggedTile t = findRaggedTile<false>(starts, a.rows, a.groups, a.slice_rows, block);
       if (t.segment < 0) return w;
       first = t.first;
       w.depth = t.rows;
     } else {
-      if (longest != nullptr) block = __builtin_amdgcn_readfirstlane(longest[block]);
+      if (order.longest != nullptr) block = __builtin_amdgcn_readfirstlane(order.longest[block]);
       segmentRows(starts, a.rows, block, &first, &w.depth);
       first = __builtin_amdgcn_readfirstlane(first);
       w.depth = __builtin_amdgcn_readfirstlane(w.depth);
@@ -458,9 +535,18 @@ __device__ __forceinline__ Work<T> workOf(int number, const int32_t *starts, con
     w.right += first * a.right_stride + n0;
     w.out = ((int64_t)block * a.ci + m0) * columns + n0;
   } else {
-    const RaggedTile t = tileOfRows<BM>(number, starts, a, tiles_n, &n0);
+    constexpr int kWhole = REST ? 2 : 1;
+    if (REST) in_xcd = tiles.kept + in_xcd / 4;
+    RaggedTile t = tileOfRows<BM * kWhole>(tiles, number & 7, in_xcd, starts, a, &n0);
     if (t.segment < 0) return w;
-    n0 *= BN;
+    n0 *= BN * kWhole;
+    if (REST) {
+      const int quarter = number >> 3 & 3, down = (quarter >> 1) * BM;
+      n0 += (quarter & 1) * BN;
+      if (down >= t.rows || n0 >= columns) return w;
+      t.first += down;
+      t.rows = min(t.rows - down, BM);
+    }
     const int group = t.segment - 1;
     const bool inside = group >= 0 && group < a.groups;
     w.depth = inside ? (MODE == kForward ? a.ci : a.co) : 0;
@@ -474,11 +560,18 @@ __device__ __forceinline__ Work<T> workOf(int number, const int32_t *starts, con
   return w;
 }
 
-constexpr int kStartsInLds = 2048, kRankedGroups = 256;
+template <int BM>
+__device__ __forceinline__ void storeResults(u32x4 v, __amdgpu_buffer_rsrc_t to, int at, bool streamed) {
+  constexpr int kPastTheCaches = 2;
+  if (BM == 256 && streamed)
+    __builtin_amdgcn_raw_buffer_store_b128(v, to, at, 0, kPastTheCaches);
+  else
+    __builtin_amdgcn_raw_buffer_store_b128(v, to, at, 0, 0);
+}
 
-// Workgroups stay: each takes the works blockIdx.x, blockIdx.x + gridDim.x, ...  The first loads of the next are under way
-// while the results of this one are stored.
-template <typename T, int MODE, int BM, int BN, int WM, int WN>
+// Workgroups stay: each takes the works blockIdx.x, blockIdx.x + gridDim.x, ... (or those of its order).  The first loads of
+// the next are under way while the results of this one are stored.
+template <typename T, int MODE, int BM, int BN, int WM, int WN, bool REST>
 __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict__ left, const T *__restrict__ right,
                                                             Args a, T *__restrict__ out) {
   constexpr bool kFilter = MODE == kBackwardFilter;
@@ -491,11 +584,14 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
 
   for (int i = threadIdx.x; i <= a.groups; i += kWaves * 64) s_starts[i] = a.starts[i];
   __syncthreads();
-  // groups by falling length (few enough for everybody to rank them): static rounds of works of very different lengths
-  // would wait for whoever has most of the long ones
-  const uint16_t *longest = nullptr;
+  const int columns = MODE == kBackwardData ? a.ci : a.co;
+  Order order = {nullptr, nullptr, 0};
+  RowTiles tiles = {};
+  int number = blockIdx.x, ahead = gridDim.x, works = a.works;
   if (kFilter && a.slice_rows == 0 && a.groups <= kRankedGroups) {
-    __shared__ uint16_t s_longest[kRankedGroups];
+    // groups by falling length (few enough for everybody to rank them)
+    __shared__ uint16_t s_longest[kRankedGroups], s_taken[2 * kSharedGroups];
+    __shared__ int s_count;
     for (int g = threadIdx.x; g < a.groups; g += kWaves * 64) {
       int first, rows, place = 0;
       segmentRows(s_starts, a.rows, g, &first, &rows);
@@ -507,9 +603,28 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
       s_longest[place] = (uint16_t)g;
     }
     __syncthreads();
-    longest = s_longest;
+    order.longest = s_longest;
+    const int per_block = (a.ci + BM - 1) / BM * ((columns + BN - 1) / BN), wide = gridDim.x >> 3;
+    if (a.groups * (int64_t)per_block > gridDim.x && wide <= 64 && a.groups <= kSharedGroups && a.groups * wide <= kShared) {
+      order.whole = per_block / 8 / wide;
+      if (threadIdx.x < 64) {
+        const int count = per_block % (8 * wide) == 0
+                              ? 0
+                              : shareOut(s_longest, s_starts, a, kDepth<T>, per_block, order.whole * wide, wide, s_taken);
+        if (threadIdx.x == 0) s_count = count;
+      }
+      __syncthreads();
+      order.taken = s_taken;
+      number = 0;
+      ahead = 1;
+      works = a.groups * order.whole + __builtin_amdgcn_readfirstlane(s_count);
+    }
   }
-  const int columns = MODE == kBackwardData ? a.ci : a.co;
+  if (!kFilter) {
+    constexpr int kWhole = REST ? 2 : 1;
+    tiles = rowTilesOf<BM * kWhole>(s_starts, a, (columns + BN * kWhole - 1) / (BN * kWhole));
+    works = min(works, 8 * (REST ? 4 * (tiles.each - tiles.kept) : tiles.kept));
+  }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   const char *x_tile = s_tiles, *y_tile = s_tiles + 2 * Left::kBytes;
@@ -548,13 +663,12 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
     return Right::fragment(y_tile + buffer * Right::kBytes + Right::place(wn + j * 16, half));
   };
 
-  int number = blockIdx.x;
   bool stored = false;  // behind the loads of the work's first step there are kStores stores
-  Work<T> work = workOf<T, MODE, BM, BN>(number, s_starts, longest, a, left, right);
+  Work<T> work = workOf<T, MODE, BM, BN, REST>(number, works, s_starts, order, tiles, a, left, right);
   begin(work);
-  while (number < a.works) {
-    number += gridDim.x;
-    const Work<T> following = workOf<T, MODE, BM, BN>(number, s_starts, longest, a, left, right);
+  while (work.there) {
+    number += ahead;
+    const Work<T> following = workOf<T, MODE, BM, BN, REST>(number, works, s_starts, order, tiles, a, left, right);
     float4v acc[TM][TN] = {};
     const int steps = (work.depth + kDepth<T> - 1) / kDepth<T>;
     if (steps > 0) {
@@ -572,15 +686,15 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
       }
 #pragma unroll
       for (int j = 0; j < TN; ++j) ys[0][j] = right_fragment(j, 0, 0);
-      int buffer = 0, ahead = work.depth - kDepth<T>;
+      int buffer = 0, left_over = work.depth - kDepth<T>;
       for (int step = 0; step < steps; ++step) {
 #pragma unroll
         for (int n = 0; n < kSlots; ++n) {
           if (n == kSlots - 2) {
             stepBarrier();
-            ahead -= kDepth<T>;
-            x.next(ahead);
-            y.next(ahead);
+            left_over -= kDepth<T>;
+            x.next(left_over);
+            y.next(left_over);
           }
           if (n < kSlots - 2) {
             request(n + 2, buffer ^ 1);
@@ -625,28 +739,29 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
         for (int j = 0; j < TN; ++j) {
           const int n = wn + j * 16 + quarter * 4;
           const int at = m < work.extent && n < work.width ? (m * columns + n) * 4 : (int)kNowhere;
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[i][j]), to, at, 0, 0);
+          storeResults<BM>(__builtin_bit_cast(u32x4, acc[i][j]), to, at, a.streamed);
         }
         continue;
       }
-      if constexpr (sizeof(T) == 2)
-      // Two blocks of columns at once: the odd quarters of the first change places with the even ones of the second, and a
-      // lane has eight columns side by side.
+      if constexpr (sizeof(T) == 2) {
+        // Two blocks of columns at once: the odd quarters of the first change places with the even ones of the second, and a
+        // lane has eight columns side by side.
 #pragma unroll
-      for (int j = 0; j < TN; j += 2) {
-        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-        Vector<T, 4> v[2];
+        for (int j = 0; j < TN; j += 2) {
+          typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+          Vector<T, 4> v[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[0].v[e] = (T)acc[i][j][e];
-          v[1].v[e] = (T)acc[i][j + 1][e];
+          for (int e = 0; e < 4; ++e) {
+            v[0].v[e] = (T)acc[i][j][e];
+            v[1].v[e] = (T)acc[i][j + 1][e];
+          }
+          const u32x2 one = __builtin_bit_cast(u32x2, v[0]), two = __builtin_bit_cast(u32x2, v[1]);
+          const u32x2 lo = __builtin_amdgcn_permlane16_swap(one.x, two.x, false, false);
+          const u32x2 hi = __builtin_amdgcn_permlane16_swap(one.y, two.y, false, false);
+          const int n = wn + (j + (quarter & 1)) * 16 + (quarter >> 1) * 8;
+          const int at = m < work.extent && n < work.width ? (m * columns + n) * 2 : (int)kNowhere;
+          storeResults<BM>(u32x4{lo.x, hi.x, lo.y, hi.y}, to, at, a.streamed);
         }
-        const u32x2 one = __builtin_bit_cast(u32x2, v[0]), two = __builtin_bit_cast(u32x2, v[1]);
-        const u32x2 lo = __builtin_amdgcn_permlane16_swap(one.x, two.x, false, false);
-        const u32x2 hi = __builtin_amdgcn_permlane16_swap(one.y, two.y, false, false);
-        const int n = wn + (j + (quarter & 1)) * 16 + (quarter >> 1) * 8;
-        const int at = m < work.extent && n < work.width ? (m * columns + n) * 2 : (int)kNowhere;
-        __builtin_amdgcn_raw_buffer_store_b128(u32x4{lo.x, hi.x, lo.y, hi.y}, to, at, 0, 0);
       }
     }
     stored = true;
@@ -672,7 +787,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void groupedFew(const T *__restrict
 
   const int columns = MODE == kBackwardData ? a.ci : a.co;
   int n0;
-  const RaggedTile t = tileOfRows<BM>(blockIdx.x, a.starts, a, (columns + kFewColumns - 1) / kFewColumns, &n0);
+  const RowTiles tiles = rowTilesOf<BM>(a.starts, a, (columns + kFewColumns - 1) / kFewColumns);
+  const RaggedTile t = tileOfRows<BM>(tiles, blockIdx.x & 7, blockIdx.x >> 3, a.starts, a, &n0);
   if (t.segment < 0) return;
   n0 *= kFewColumns;
   const int group = t.segment - 1, width = columns - n0;
@@ -775,6 +891,8 @@ struct Tile {
 // 16 rows of a 2048 x 2048 filter 39 / 19 / 14 / 9 / 8.5, 1000 rows 43 / 24 / 21 / 27 / 43, 4000 rows 47 / 36 / 48 / 95 / 158, 40 000
 // rows 288 / 365 / 524 / 895 / 1480.
 constexpr int kTileKinds = 3;
+constexpr int kRestSteps = 16;
+constexpr double kStreamedResults = 64e6;
 // 64 filters of 2048 x 2048 for a row each: 121 / 95 / 97 / 119 / 119, and backward data, which reads their rows, 136 / 125 / 122 /
 // 102 / 102.
 constexpr Tile kTiles[] = {{"groupedTiles256", 256, 256, 1, 1.25, 1.65, 5.0, 4.4, 3.9},
@@ -912,20 +1030,28 @@ hipError_t launchAny(const LaunchCtx &lc, const Problem &p, const Args &a) {
   return hipGetLastError();
 }
 
+// Whether tiles of m rows, as many as the groups' lengths make of them, may fill a quarter or less of an XCD's last round.
+bool restMayBe(const Problem &p, int m, int64_t tiles_n, int wide) {
+  const int64_t least = ((p.rows + m - 1) / m * tiles_n + 7) / 8, most = (mostRaggedTiles(p.rows, p.groups, m) * tiles_n + 7) / 8;
+  const int64_t last = most / wide;  // round that may begin
+  for (int64_t round = std::max<int64_t>(last - 1, 1); round <= last; ++round)
+    if (std::max(least, round * wide + 1) <= std::min(most, round * wide + wide / 4)) return true;
+  return false;
+}
+
 template <typename T, int MODE, int TILE, int WM, int WN>
 hipError_t launchTiles(const LaunchCtx &lc, const Problem &p, Args a, int cu_count) {
   constexpr int BM = kTiles[TILE].m, BN = kTiles[TILE].n;
   constexpr size_t kLds = (size_t)2 * (BM + BN) * 128;
   static_assert((kLds + kStartsInLds * 4 + kRankedGroups * 2) * kTiles[TILE].per_cu <= 160 * 1024, "LDS of a CU");
-  auto kernel = groupedTiles<T, MODE, BM, BN, WM, WN>;
+  auto kernel = groupedTiles<T, MODE, BM, BN, WM, WN, false>;
   const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
   if (allowed != hipSuccess) return allowed;
   const int64_t tiles_n = tilesOf(MODE == kBackwardData ? p.ci : p.co, BN);
   int64_t works;
   if (MODE == kBackwardFilter) {
-    const int64_t per_block = tilesOf(p.ci, BM) * tiles_n;
-    works = per_block >= 8 ? (per_block + 7) / 8 * 8 * a.blocks : per_block * a.blocks;
+    works = tilesOf(p.ci, BM) * tiles_n * ((a.blocks + 7) / 8 * 8);
   } else {
     works = (mostRaggedTiles(p.rows, p.groups + 2, BM) * tiles_n + 7) / 8 * 8;
   }
@@ -933,10 +1059,32 @@ hipError_t launchTiles(const LaunchCtx &lc, const Problem &p, Args a, int cu_cou
   a.works = (int)works;
   // as many workgroups as the GPU holds at once, in whole rounds of the XCDs
   const int64_t stay = std::max<int64_t>((int64_t)kTiles[TILE].per_cu * cu_count / 8, 1) * 8;
+  const int grid = (int)std::min(works, stay);
+  const double results = MODE == kBackwardFilter ? (double)p.groups * p.ci * p.co
+                                                 : (double)p.rows * (MODE == kForward ? p.co : p.ci);
+  a.streamed = TILE == 0 && a.slice_rows == 0 && results * sizeof(T) >= kStreamedResults;
+  if constexpr (MODE != kBackwardFilter && TILE == 0) {
+    const int depth = MODE == kForward ? p.ci : p.co, wide = (int)(stay / 8);
+    if (depth >= kRestSteps * kDepth<T> && restMayBe(p, BM, tiles_n, wide)) a.wide = wide;
+  }
   lc.begin(kTiles[TILE].name);
-  kernel<<<(unsigned)std::min((works + 7) / 8 * 8, stay), WM * WN * 64, kLds, lc.stream>>>(
-      static_cast<const T *>(p.left), static_cast<const T *>(p.right), a, static_cast<T *>(p.out));
+  kernel<<<grid, WM * WN * 64, kLds, lc.stream>>>(static_cast<const T *>(p.left), static_cast<const T *>(p.right), a,
+                                                  static_cast<T *>(p.out));
   lc.end();
+  if constexpr (MODE != kBackwardFilter && TILE == 0) {
+    if (a.wide > 0) {
+      constexpr size_t kRestLds = kLds / 2;
+      auto rest = groupedTiles<T, MODE, BM / 2, BN / 2, 2, 2, true>;
+      const hipError_t fits = hipFuncSetAttribute(reinterpret_cast<const void *>(rest),
+                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)kRestLds);
+      if (fits != hipSuccess) return fits;
+      a.works = (int)std::min<int64_t>(4 * works, 8 * 4 * (a.wide / 4));
+      lc.begin("groupedTilesRest");
+      rest<<<a.works, 256, kRestLds, lc.stream>>>(static_cast<const T *>(p.left), static_cast<const T *>(p.right), a,
+                                                  static_cast<T *>(p.out));
+      lc.end();
+    }
+  }
   if (MODE == kBackwardFilter && a.slice_rows > 0) return sumSlices<T>(lc, p, a);
   return hipGetLastError();
 }
@@ -997,7 +1145,7 @@ size_t workspaceBytes(const Problem &p, int cu_count) {
 }
 
 hipError_t launch(const LaunchCtx &lc, const Problem &p, int cu_count, void *workspace) {
-  Args a = {p.rows, p.groups, p.ci, p.co, p.starts, p.left_stride, p.right_stride, 0, 0, 0, 0, nullptr};
+  Args a = {p.rows, p.groups, p.ci, p.co, p.starts, p.left_stride, p.right_stride, 0, 0, 0, 0, 0, false, nullptr};
   if (p.which == MLUOP_EXT_GROUPED_BACKWARD_FILTER) {
     a.slice_rows = planFilter(p, cu_count).slice_rows;
     a.most_slices = a.slice_rows > 0 ? (int)mostRaggedTiles(p.rows, p.groups, a.slice_rows) : 0;
