@@ -56,14 +56,63 @@ struct Args {
   int rows, groups, ci, co;
   const int32_t *starts;
   int64_t left_stride, right_stride;
-  int slice_rows;   // backward filter: rows of a slice; 0: a group's rows are one slice, and its sums the result
-  int most_slices;
-  int blocks;       // backward filter: slices there can be, or groups
+  int slice_rows;   // backward filter: rows of a slice; 0: a group's rows are one slice
+  int blocks;       // backward filter: slices there can be,
+  int slots;        // and how many there can be of groups of more than one, whose sums go to `partial`
   int works;        // numbers of works (some of which may not be there)
   int wide;         // of tiles of rows: workgroups of an XCD whose last round, filled to a quarter or less, is left for smaller tiles; or 0
   bool streamed;    // results go past the caches
-  float *partial;   // backward filter in slices: sums [slice, ci, co]
+  float *partial;   // backward filter: sums [slot, ci, co]
 };
+
+// A slice of a group's rows.  A group of few rows, or none, is one slice, whose sums are its result; the slices of the others
+// have slots of partial sums, side by side, which groupedSumSlices adds up.
+struct Slice {
+  int group;  // -1: there is no such slice
+  int first, rows;
+  int slot;   // -1: the result
+};
+__device__ __forceinline__ int slicesOf(int rows, int slice_rows) {
+  return rows <= slice_rows ? 1 : (rows - 1) / slice_rows + 1;
+}
+// By whole waves; the answer is the same in all lanes.
+__device__ __forceinline__ Slice findSlice(const int32_t *starts, const Args &a, int number) {
+  Slice s = {-1, 0, 0, -1};
+  if (a.slice_rows == 0) {
+    if (number >= a.groups) return s;
+    s.group = number;
+    segmentRows(starts, a.rows, number, &s.first, &s.rows);
+    return s;
+  }
+  const int lane = threadIdx.x & 63;
+  int before = 0, slots_before = 0;
+  for (int base = 0; base < a.groups; base += 64) {
+    int first = 0, count = 0, slices = 0;
+    if (base + lane < a.groups) {
+      segmentRows(starts, a.rows, base + lane, &first, &count);
+      slices = slicesOf(count, a.slice_rows);
+    }
+    const int slots = slices > 1 ? slices : 0;
+    const int upto = before + waveInclusiveScan(slices), slots_upto = slots_before + waveInclusiveScan(slots);
+    const unsigned long long behind = __ballot(number < upto);
+    if (behind != 0) {
+      const int l = __ffsll((long long)behind) - 1;
+      const int own = __builtin_amdgcn_readlane(slices, l), in_group = number - (__builtin_amdgcn_readlane(upto, l) - own);
+      const int slot = __builtin_amdgcn_readlane(slots_upto, l) - own + in_group;
+      // (starts that overlap can add up to more than an int holds, or than there are slots)
+      if ((uint32_t)in_group >= (uint32_t)own || (own > 1 && (uint32_t)slot >= (uint32_t)a.slots)) return s;
+      s.group = base + l;
+      s.first = __builtin_amdgcn_readlane(first, l) + in_group * a.slice_rows;
+      s.rows = __builtin_amdgcn_readlane(count, l) - in_group * a.slice_rows;
+      if (s.rows > a.slice_rows) s.rows = a.slice_rows;
+      if (own > 1) s.slot = slot;
+      return s;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+    slots_before = __builtin_amdgcn_readlane(slots_upto, 63);
+  }
+  return s;
+}
 
 // ---- any shape, stride and alignment -------------------------------------------------------
 //
@@ -151,27 +200,18 @@ __global__ __launch_bounds__(kAnyThreads) void groupedAny(const T *__restrict__ 
   int group, m0 = 0, extent, depth;
   const T *l, *r;
   int64_t out_row;     // of result row 0
-  bool result = true;  // sums are the result, and not a slice's
+  bool result = true;  // and not partial sums
   if (kFilter) {
-    int first, count;
     m0 = blockIdx.z * kAnyTile;
     extent = a.ci - m0;
-    if (a.slice_rows > 0) {
-      const RaggedTile t = findRaggedTile<false>(a.starts, a.rows, a.groups, a.slice_rows, blockIdx.x);
-      if (t.segment < 0) return;
-      group = t.segment;
-      first = t.first;
-      count = t.rows;
-      out_row = (int64_t)blockIdx.x * a.ci + m0;
-      result = false;
-    } else {
-      group = blockIdx.x;
-      segmentRows(a.starts, a.rows, group, &first, &count);
-      out_row = (int64_t)group * a.ci + m0;
-    }
-    depth = count;
-    l = left + first * a.left_stride + m0;
-    r = right + first * a.right_stride + n0;
+    const Slice slice = findSlice(a.starts, a, blockIdx.x);
+    if (slice.group < 0) return;
+    group = slice.group;
+    result = slice.slot < 0;
+    out_row = (int64_t)(result ? group : slice.slot) * a.ci + m0;
+    depth = slice.rows;
+    l = left + slice.first * a.left_stride + m0;
+    r = right + slice.first * a.right_stride + n0;
   } else {
     const RaggedTile t = findRaggedTile<true>(a.starts, a.rows, a.groups, kAnyTile, blockIdx.x);
     if (t.segment < 0) return;
@@ -383,7 +423,7 @@ struct Operand {
 // What a workgroup multiplies next.
 template <typename T>
 struct Work {
-  bool there;
+  bool there, partial;       // partial: sums of a slice
   int extent, width, depth;  // results of the tile that there are, and the reduction
   const T *left, *right;
   int64_t out;               // element of the result's (or the partial sums') first
@@ -430,27 +470,26 @@ __device__ __forceinline__ RaggedTile tileOfRows(const RowTiles &all, int xcd, i
 
 // In which order a workgroup takes its works (in LDS; NULL: by number).
 struct Order {
-  const uint16_t *longest;  // groups by falling length
+  const uint16_t *longest;  // blocks (groups, or slices of their rows) by falling length
   const uint16_t *taken;    // this workgroup's share of what does not fill a round of its XCD: [place in `longest`, tile of the XCD's]; or NULL
-  int whole;                // rounds that an XCD's tiles of every group make
+  int whole;                // rounds that an XCD's tiles of every block make
+  int blocks;               // that there are
 };
-// Of `tiles` tiles of a block (a group, or a slice of its rows) every XCD has an eighth, tiles that lie side by side;
+// Of `tiles` tiles of a block every XCD has an eighth, tiles that lie side by side;
 // where eighths are of different sizes, the next block has them turned by one XCD.
 __device__ __forceinline__ int eighthFrom(int tiles, int eighth) { return (int)((int64_t)tiles * eighth >> 3); }
 __device__ __forceinline__ int eighthOf(int xcd, int block) { return (xcd + block) & 7; }
 
-constexpr int kStartsInLds = 2048, kRankedGroups = 256, kSharedGroups = 64, kEndSteps = 3;
-constexpr int kShared = 1024;  // groups x workgroups of an XCD
+constexpr int kStartsInLds = 2048, kRanked = 256, kSharedBlocks = 64, kEndSteps = 3;
+constexpr int kShared = 1024;  // blocks x workgroups of an XCD
 
 // Groups are of very different lengths, and rounds of works of different lengths wait for whoever has most of the long ones.
-// So every workgroup works out who takes what: group by group, the longest first, whose tiles go to those workgroups of
+// So every workgroup works out who takes what: block by block, the longest first, whose tiles go to those workgroups of
 // the XCD that have least.  A lane stands for a workgroup; keys are steps of work so far (a tile's beginning and end take some
-// kEndSteps) above the lane's number, so that no two are the same.
-__device__ __forceinline__ int shareOut(const uint16_t *longest, const int32_t *starts, const Args &a, int step, int tiles,
-                                        int behind, int wide, uint16_t *taken) {
-  const int lane = threadIdx.x & 63, own = blockIdx.x >> 3, xcd = blockIdx.x & 7;
-  int first, rows = 0, count = 0;
-  if (lane < a.groups) segmentRows(starts, a.rows, longest[lane], &first, &rows);
+// kEndSteps) above the lane's number, so that no two are the same.  To `taken`; returns how many.
+__device__ __forceinline__ int shareOut(const Order &order, const int *lengths, int step, int tiles, int wide, uint16_t *taken) {
+  const int lane = threadIdx.x & 63, own = blockIdx.x >> 3, xcd = blockIdx.x & 7, behind = order.whole * wide;
+  const int rows = lane < order.blocks ? lengths[order.longest[lane]] : 0;
   const uint32_t cost = (uint32_t)((rows + step - 1) / step + kEndSteps) << 6;
   uint32_t key = lane < wide ? (uint32_t)lane : ~0u;
   auto rankAmong = [&](auto n) {
@@ -459,16 +498,17 @@ __device__ __forceinline__ int shareOut(const uint16_t *longest, const int32_t *
     for (int o = 0; o < decltype(n)::value; ++o) rank += (uint32_t)__builtin_amdgcn_readlane((int)key, o) < key ? 1 : 0;
     return rank;
   };
-  for (int g = 0; g < a.groups; ++g) {
+  int count = 0;
+  for (int b = 0; b < order.blocks; ++b) {
     const int rank = wide > 32 ? rankAmong(std::integral_constant<int, 64>()) : rankAmong(std::integral_constant<int, 32>());
-    const int eighth = eighthOf(xcd, g);
+    const int eighth = eighthOf(xcd, b);
     const bool takes = lane < wide && behind + rank < eighthFrom(tiles, eighth + 1) - eighthFrom(tiles, eighth);
     if (takes && lane == own) {
-      taken[2 * count] = (uint16_t)g;
+      taken[2 * count] = (uint16_t)b;
       taken[2 * count + 1] = (uint16_t)(behind + rank);
     }
     count += __builtin_amdgcn_readlane(takes ? 1 : 0, own);
-    if (takes) key += (uint32_t)__builtin_amdgcn_readlane((int)cost, g);
+    if (takes) key += (uint32_t)__builtin_amdgcn_readlane((int)cost, b);
   }
   return count;
 }
@@ -480,7 +520,7 @@ template <typename T, int MODE, int BM, int BN, bool REST>
 __device__ __forceinline__ Work<T> workOf(int number, int works, const int32_t *starts, const Order &order, const RowTiles &tiles,
                                           const Args &a, const T *left, const T *right) {
   Work<T> w;
-  w.there = false;
+  w.there = w.partial = false;
   w.extent = w.width = w.depth = 0;
   w.left = left;
   w.right = right;
@@ -493,7 +533,7 @@ __device__ __forceinline__ Work<T> workOf(int number, int works, const int32_t *
     const int xcd = blockIdx.x & 7, wide = gridDim.x >> 3;
     int block, tile;
     if (order.taken != nullptr) {
-      const int in_rest = number - a.groups * order.whole;
+      const int in_rest = number - order.blocks * order.whole;
       if (in_rest < 0) {
         block = number / order.whole;
         tile = (number - block * order.whole) * wide + (blockIdx.x >> 3);
@@ -515,25 +555,23 @@ __device__ __forceinline__ Work<T> workOf(int number, int works, const int32_t *
       block = 8 * eight + ((eighth - xcd) & 7);
     }
     if (block >= a.blocks) return w;
-    int m0, first;
+    if (order.longest != nullptr) block = __builtin_amdgcn_readfirstlane(order.longest[block]);
+    Slice slice = findSlice(starts, a, block);
+    if (slice.group < 0) return w;
+    if (a.slice_rows == 0) {  // (read from LDS, and the same in all lanes)
+      slice.first = __builtin_amdgcn_readfirstlane(slice.first);
+      slice.rows = __builtin_amdgcn_readfirstlane(slice.rows);
+    }
+    int m0;
     placeOfTile(tile, (a.ci + BM - 1) / BM, tiles_n, &m0, &n0);
     m0 *= BM;
     n0 *= BN;
-    if (a.slice_rows > 0) {
-      const RaggedTile t = findRaggedTile<false>(starts, a.rows, a.groups, a.slice_rows, block);
-      if (t.segment < 0) return w;
-      first = t.first;
-      w.depth = t.rows;
-    } else {
-      if (order.longest != nullptr) block = __builtin_amdgcn_readfirstlane(order.longest[block]);
-      segmentRows(starts, a.rows, block, &first, &w.depth);
-      first = __builtin_amdgcn_readfirstlane(first);
-      w.depth = __builtin_amdgcn_readfirstlane(w.depth);
-    }
+    w.depth = slice.rows;
     w.extent = a.ci - m0;
-    w.left += first * a.left_stride + m0;
-    w.right += first * a.right_stride + n0;
-    w.out = ((int64_t)block * a.ci + m0) * columns + n0;
+    w.left += slice.first * a.left_stride + m0;
+    w.right += slice.first * a.right_stride + n0;
+    w.partial = slice.slot >= 0;
+    w.out = ((int64_t)(w.partial ? slice.slot : slice.group) * a.ci + m0) * columns + n0;
   } else {
     constexpr int kWhole = REST ? 2 : 1;
     if (REST) in_xcd = tiles.kept + in_xcd / 4;
@@ -585,39 +623,47 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
   for (int i = threadIdx.x; i <= a.groups; i += kWaves * 64) s_starts[i] = a.starts[i];
   __syncthreads();
   const int columns = MODE == kBackwardData ? a.ci : a.co;
-  Order order = {nullptr, nullptr, 0};
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Order order = {nullptr, nullptr, 0, 0};
   RowTiles tiles = {};
   int number = blockIdx.x, ahead = gridDim.x, works = a.works;
-  if (kFilter && a.slice_rows == 0 && a.groups <= kRankedGroups) {
-    // groups by falling length (few enough for everybody to rank them)
-    __shared__ uint16_t s_longest[kRankedGroups], s_taken[2 * kSharedGroups];
-    __shared__ int s_count;
-    for (int g = threadIdx.x; g < a.groups; g += kWaves * 64) {
-      int first, rows, place = 0;
-      segmentRows(s_starts, a.rows, g, &first, &rows);
-      for (int o = 0; o < a.groups; ++o) {
-        int others;
-        segmentRows(s_starts, a.rows, o, &first, &others);
-        place += others > rows || (others == rows && o < g) ? 1 : 0;
+  const int per_block = (a.ci + BM - 1) / BM * ((columns + BN - 1) / BN), wide = gridDim.x >> 3;
+  if (kFilter && a.blocks * (int64_t)per_block > gridDim.x && a.blocks <= (a.slice_rows == 0 ? kRanked : kSharedBlocks)) {
+    // more than one round, and few enough blocks for everybody to rank them
+    __shared__ int s_lengths[kRanked], s_count;
+    __shared__ uint16_t s_longest[kRanked], s_taken[2 * kSharedBlocks];
+    for (int b = wave; b < a.blocks; b += kWaves) {
+      const Slice slice = findSlice(s_starts, a, b);
+      if (lane == 0) s_lengths[b] = slice.group >= 0 ? slice.rows : -1;
+    }
+    __syncthreads();
+    int there = 0;
+    for (int base = 0; base < a.blocks; base += kWaves * 64) {
+      const int b = base + threadIdx.x;
+      const int length = b < a.blocks ? s_lengths[b] : -1;
+      int place = 0;
+      there = 0;
+      for (int o = 0; o < a.blocks; ++o) {
+        const int other = s_lengths[o];
+        place += other > length || (other == length && o < b) ? 1 : 0;
+        there += other >= 0 ? 1 : 0;
       }
-      s_longest[place] = (uint16_t)g;
+      if (b < a.blocks) s_longest[place] = (uint16_t)b;
     }
     __syncthreads();
     order.longest = s_longest;
-    const int per_block = (a.ci + BM - 1) / BM * ((columns + BN - 1) / BN), wide = gridDim.x >> 3;
-    if (a.groups * (int64_t)per_block > gridDim.x && wide <= 64 && a.groups <= kSharedGroups && a.groups * wide <= kShared) {
+    order.blocks = __builtin_amdgcn_readfirstlane(there);
+    if (wide <= 64 && a.blocks <= kSharedBlocks && a.blocks * wide <= kShared) {
       order.whole = per_block / 8 / wide;
       if (threadIdx.x < 64) {
-        const int count = per_block % (8 * wide) == 0
-                              ? 0
-                              : shareOut(s_longest, s_starts, a, kDepth<T>, per_block, order.whole * wide, wide, s_taken);
+        const int count = per_block % (8 * wide) == 0 ? 0 : shareOut(order, s_lengths, kDepth<T>, per_block, wide, s_taken);
         if (threadIdx.x == 0) s_count = count;
       }
       __syncthreads();
       order.taken = s_taken;
       number = 0;
       ahead = 1;
-      works = a.groups * order.whole + __builtin_amdgcn_readfirstlane(s_count);
+      works = order.blocks * order.whole + __builtin_amdgcn_readfirstlane(s_count);
     }
   }
   if (!kFilter) {
@@ -625,7 +671,6 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
     tiles = rowTilesOf<BM * kWhole>(s_starts, a, (columns + BN * kWhole - 1) / (BN * kWhole));
     works = min(works, 8 * (REST ? 4 * (tiles.each - tiles.kept) : tiles.kept));
   }
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   const char *x_tile = s_tiles, *y_tile = s_tiles + 2 * Left::kBytes;
 
@@ -724,7 +769,7 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
     // ended)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     begin(following);
-    const bool partial = kFilter && a.slice_rows > 0;
+    const bool partial = kFilter && work.partial;
     const int size = partial ? 4 : (int)sizeof(T);
     // (stores outside of the results go nowhere: the same number of them for every work)
     const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
@@ -739,7 +784,7 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
         for (int j = 0; j < TN; ++j) {
           const int n = wn + j * 16 + quarter * 4;
           const int at = m < work.extent && n < work.width ? (m * columns + n) * 4 : (int)kNowhere;
-          storeResults<BM>(__builtin_bit_cast(u32x4, acc[i][j]), to, at, a.streamed);
+          storeResults<BM>(__builtin_bit_cast(u32x4, acc[i][j]), to, at, a.streamed && !partial);
         }
         continue;
       }
@@ -838,15 +883,24 @@ __global__ __launch_bounds__(kFewWaves * 64) void groupedFew(const T *__restrict
   }
 }
 
-// Adds up the slices of every group: a workgroup has 64 V results, whose slices its four waves share.
+// Adds up the slices of every group that has several: a workgroup has 64 V results, whose slices its four waves share.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void groupedSumSlices(Args a, T *__restrict__ out) {
   constexpr int kShares = 4, kAhead = 4;
   __shared__ float s_sum[kShares][64 * V];
   const int64_t filter = (int64_t)a.ci * a.co;
   const int group = blockIdx.y, lane = threadIdx.x & 63, share = threadIdx.x >> 6;
-  int first, count;
-  const int slices = raggedTilesOf(a.starts, a.rows, group, a.slice_rows, a.most_slices, &first, &count);
+  int in_group, rows, first = 0;
+  segmentRows(a.starts, a.rows, group, &in_group, &rows);
+  if (rows <= a.slice_rows) return;
+  for (int base = 0; base < group; base += 64) {
+    int other_first, other_rows = 0;
+    if (base + lane < group) segmentRows(a.starts, a.rows, base + lane, &other_first, &other_rows);
+    first += __builtin_amdgcn_readlane(waveInclusiveScan(other_rows <= a.slice_rows ? 0 : slicesOf(other_rows, a.slice_rows)), 63);
+  }
+  // (inside the slots, whatever the starts hold)
+  first = first < 0 || first > a.slots ? a.slots : first;
+  const int slices = min(slicesOf(rows, a.slice_rows), a.slots - first);
   const int64_t at = ((int64_t)blockIdx.x * 64 + lane) * V;
   const bool there = at < filter;
   float sum[V] = {};
@@ -950,20 +1004,33 @@ int planRows(const Problem &p, const Tile *tiles, int kinds, int cu_count) {
   return best;
 }
 
-// Tile and slices of the backward filter: more slices fill the GPU, and cost their partial sums a way to memory and back.
+// Slots that groups of more than slice_rows rows can have: fewer than twice as many as slices that their rows fill.
+int64_t mostSlots(const Problem &p, int64_t slice_rows) { return 2 * (int64_t)p.rows / slice_rows; }
+
+// Tile and slices of the backward filter.  How long the groups are is not known here, but as a rule some are several times as
+// long as the mean: a group of kLongest times that is counted with, whose tiles the end waits for.  Shorter slices take less time, and
+// the sums of groups of several a way to memory and back.
 double planSlices(const Problem &p, const Tile &t, int cu_count, int *slice_rows) {
-  const double tiles = (double)tilesOf(p.ci, t.m) * tilesOf(p.co, t.n);
-  const double mean = (double)p.rows / p.groups;
+  constexpr double kLongest = 3.0;
+  const double tiles = (double)tilesOf(p.ci, t.m) * tilesOf(p.co, t.n), filter = (double)p.ci * p.co;
+  const double filled = std::max(std::min(p.rows, p.groups), 1), mean = p.rows / filled;
+  const double longest = p.groups > 1 ? std::min(kLongest * mean, (double)p.rows) : p.rows;
   const int step = 128 / elementBytes(p.type);
-  double least = timeOf(t, tiles * p.groups, mean / step + 0.5, cu_count);
+  auto micros = [&](double rows) {
+    const double blocks = 0.5 * filled + std::max(0.5 * filled, p.rows / rows);
+    const double rate = tiles * blocks > t.per_cu * 0.5 * cu_count ? t.full : t.few;
+    return std::max(timeOf(t, tiles * blocks, p.rows / blocks / step + 0.5, cu_count),
+                    std::min(rows, longest) / step * rate + t.end);
+  };
+  double least = micros(p.rows);
   *slice_rows = 0;
-  for (int64_t slices = 2; slices <= 1024; slices *= 2) {
-    const int64_t rows = (p.rows / slices + step) / step * step;
-    if (rows < 2 * step || rows >= p.rows) break;
-    const double all = (double)mostRaggedTiles(p.rows, p.groups, rows);
-    const double bytes = all * p.ci * p.co * 8.0;
-    if (bytes > 2.5e9) break;
-    const double us = timeOf(t, tiles * all, (double)rows / step, cu_count) + bytes / 4.0e6 + 5.0;
+  for (double slices = 1.0 / 4; slices <= 1024; slices *= 2) {  // of a group of the mean length
+    const int64_t rows = ((int64_t)(mean / slices) + step) / step * step;
+    if (rows < 2 * step) break;
+    if (rows >= p.rows) continue;
+    if (mostSlots(p, rows) * filter * 4.0 > 1.5e9) break;
+    const double slots = p.rows / (double)rows * std::min(1.0, mean / rows);
+    const double us = micros((double)rows) + slots * filter * 8.0 / 4.0e6 + 5.0;
     if (us < least) {
       least = us;
       *slice_rows = (int)rows;
@@ -1043,7 +1110,7 @@ template <typename T, int MODE, int TILE, int WM, int WN>
 hipError_t launchTiles(const LaunchCtx &lc, const Problem &p, Args a, int cu_count) {
   constexpr int BM = kTiles[TILE].m, BN = kTiles[TILE].n;
   constexpr size_t kLds = (size_t)2 * (BM + BN) * 128;
-  static_assert((kLds + kStartsInLds * 4 + kRankedGroups * 2) * kTiles[TILE].per_cu <= 160 * 1024, "LDS of a CU");
+  static_assert((kLds + kStartsInLds * 4 + kRanked * 6 + kSharedBlocks * 4 + 4) * kTiles[TILE].per_cu <= 160 * 1024, "LDS of a CU");
   auto kernel = groupedTiles<T, MODE, BM, BN, WM, WN, false>;
   const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
@@ -1062,7 +1129,7 @@ hipError_t launchTiles(const LaunchCtx &lc, const Problem &p, Args a, int cu_cou
   const int grid = (int)std::min(works, stay);
   const double results = MODE == kBackwardFilter ? (double)p.groups * p.ci * p.co
                                                  : (double)p.rows * (MODE == kForward ? p.co : p.ci);
-  a.streamed = TILE == 0 && a.slice_rows == 0 && results * sizeof(T) >= kStreamedResults;
+  a.streamed = TILE == 0 && results * sizeof(T) >= kStreamedResults;
   if constexpr (MODE != kBackwardFilter && TILE == 0) {
     const int depth = MODE == kForward ? p.ci : p.co, wide = (int)(stay / 8);
     if (depth >= kRestSteps * kDepth<T> && restMayBe(p, BM, tiles_n, wide)) a.wide = wide;
@@ -1141,15 +1208,15 @@ size_t workspaceBytes(const Problem &p, int cu_count) {
   if (p.which != MLUOP_EXT_GROUPED_BACKWARD_FILTER) return 0;
   const int slice = planFilter(p, cu_count).slice_rows;
   if (slice == 0) return 0;
-  return (size_t)mostRaggedTiles(p.rows, p.groups, slice) * p.ci * p.co * sizeof(float);
+  return (size_t)mostSlots(p, slice) * p.ci * p.co * sizeof(float);
 }
 
 hipError_t launch(const LaunchCtx &lc, const Problem &p, int cu_count, void *workspace) {
   Args a = {p.rows, p.groups, p.ci, p.co, p.starts, p.left_stride, p.right_stride, 0, 0, 0, 0, 0, false, nullptr};
   if (p.which == MLUOP_EXT_GROUPED_BACKWARD_FILTER) {
     a.slice_rows = planFilter(p, cu_count).slice_rows;
-    a.most_slices = a.slice_rows > 0 ? (int)mostRaggedTiles(p.rows, p.groups, a.slice_rows) : 0;
-    a.blocks = a.slice_rows > 0 ? a.most_slices : p.groups;
+    a.blocks = p.groups + (a.slice_rows > 0 ? p.rows / a.slice_rows : 0);
+    a.slots = a.slice_rows > 0 ? (int)mostSlots(p, a.slice_rows) : 0;
     a.partial = static_cast<float *>(workspace);
   }
   if (p.type == MLUOP_DTYPE_HALF) return launchOf<_Float16>(lc, p, a, cu_count);
