@@ -929,6 +929,68 @@ __global__ __launch_bounds__(256) void groupedSumSlices(Args a, T *__restrict__ 
   storeFloats<T, V>(out + group * filter + at, sum);
 }
 
+// ---- rows of other lengths, padded ---------------------------------------------------------
+//
+// Matrices of rows that are no whole 16-byte pieces, copied to such that are: blocks of from_rows x from_width elements to
+// blocks of to_rows x to_width, zeros where there is nothing to copy.  A thread has 16 bytes of the destination.
+
+struct Copy {
+  const char *from;
+  char *to;
+  int64_t from_stride;       // bytes
+  int from_rows, to_rows;    // of a block
+  int from_bytes, to_bytes;  // of a row
+  uint32_t pieces;           // 16 bytes each, of all the destination's rows
+  bool of_groups;            // blocks are groups' filters, and those of groups without rows are not looked at
+};
+
+// `bytes` of sixteen from `from` to `to`, by the widest accesses that both are aligned for.
+template <typename T>
+__device__ __forceinline__ void copyBytes(char *to, const char *from, int bytes) {
+  const uintptr_t all = reinterpret_cast<uintptr_t>(to) | reinterpret_cast<uintptr_t>(from);
+  if (bytes >= 16 && (all & 7) == 0) {
+    reinterpret_cast<uint2 *>(to)[0] = reinterpret_cast<const uint2 *>(from)[0];
+    reinterpret_cast<uint2 *>(to)[1] = reinterpret_cast<const uint2 *>(from)[1];
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 16 / (int)sizeof(T); ++i)
+    if (i * (int)sizeof(T) < bytes) reinterpret_cast<T *>(to)[i] = reinterpret_cast<const T *>(from)[i];
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void groupedPad(Copy one, Copy two, uint32_t one_blocks, const int32_t *starts, int rows) {
+  const bool second = blockIdx.x >= one_blocks;
+  const Copy &c = second ? two : one;
+  const uint32_t piece = (blockIdx.x - (second ? one_blocks : 0u)) * 256u + threadIdx.x, per_row = (uint32_t)c.to_bytes / 16;
+  if (piece >= c.pieces) return;
+  const uint32_t row = piece / per_row, at = (piece - row * per_row) * 16, block = row / (uint32_t)c.to_rows,
+                 in_block = row - block * (uint32_t)c.to_rows;
+  if (c.of_groups) {
+    int first, count;
+    segmentRows(starts, rows, (int)block, &first, &count);
+    if (count == 0) return;
+  }
+  Vector<T, 16 / (int)sizeof(T)> v = {};
+  if (in_block < (uint32_t)c.from_rows && at < (uint32_t)c.from_bytes)
+    copyBytes<T>(reinterpret_cast<char *>(&v), c.from + ((int64_t)block * c.from_rows + in_block) * c.from_stride + at,
+                 c.from_bytes - (int)at);
+  *reinterpret_cast<Vector<T, 16 / (int)sizeof(T)> *>(c.to + (int64_t)piece * 16) = v;
+}
+
+// The results without what was padded; from and to as above, the other way round.
+template <typename T>
+__global__ __launch_bounds__(256) void groupedUnpad(Copy c) {
+  const uint32_t piece = blockIdx.x * 256u + threadIdx.x, per_row = (uint32_t)c.to_bytes / 16;
+  if (piece >= c.pieces) return;
+  const uint32_t row = piece / per_row, at = (piece - row * per_row) * 16, block = row / (uint32_t)c.to_rows,
+                 in_block = row - block * (uint32_t)c.to_rows;
+  if (in_block >= (uint32_t)c.from_rows || at >= (uint32_t)c.from_bytes) return;
+  const Vector<T, 16 / (int)sizeof(T)> v = *reinterpret_cast<const Vector<T, 16 / (int)sizeof(T)> *>(c.to + (int64_t)piece * 16);
+  copyBytes<T>(const_cast<char *>(c.from) + ((int64_t)block * c.from_rows + in_block) * c.from_stride + at,
+               reinterpret_cast<const char *>(&v), c.from_bytes - (int)at);
+}
+
 // ---- host side -----------------------------------------------------------------------------
 
 int tilesOf(int64_t n, int tile) { return (int)((n + tile - 1) / tile); }
@@ -947,6 +1009,8 @@ struct Tile {
 constexpr int kTileKinds = 3;
 constexpr int kRestSteps = 16;
 constexpr double kStreamedResults = 64e6;
+// Bytes a us of padded copies, and a launch of them.
+constexpr double kCopied = 3.0e6, kCopyLaunch = 4.0;
 // 64 filters of 2048 x 2048 for a row each: 121 / 95 / 97 / 119 / 119, and backward data, which reads their rows, 136 / 125 / 122 /
 // 102 / 102.
 constexpr Tile kTiles[] = {{"groupedTiles256", 256, 256, 1, 1.25, 1.65, 5.0, 4.4, 3.9},
@@ -964,7 +1028,7 @@ constexpr Tile kFloatTiles[] = {{"groupedTiles256", 256, 256, 1, 7.2, 7.0, 5.0, 
                                 {"groupedFew16", 16, kFewColumns, 2, 0.29, 0.39, 1.5, 5.2, 5.2}};
 constexpr int kAllKinds = sizeof(kTiles) / sizeof(kTiles[0]);
 // the kernel of any shape
-constexpr Tile kAny = {"groupedAny", kAnyTile, kAnyTile, 4, 1.6, 2.2, 2.0, 3.0, 3.0};
+constexpr Tile kAny = {"groupedAny", kAnyTile, kAnyTile, 4, 2.0, 3.3, 2.0, 3.0, 3.0};
 
 // (how many tiles there are is known nearly: a last round that they fill a little is counted by its chance)
 double timeOf(const Tile &t, double tiles, double steps, int cu_count) {
@@ -984,7 +1048,7 @@ double rowTiles(const Problem &p, int m) {
 }
 
 // The tile of `kinds` that takes least, forward or for backward data.
-int planRows(const Problem &p, const Tile *tiles, int kinds, int cu_count) {
+int planRows(const Problem &p, const Tile *tiles, int kinds, int cu_count, double *us_of_best = nullptr) {
   const bool forward = p.which == MLUOP_EXT_GROUPED_FORWARD;
   const int depth = forward ? p.ci : p.co, columns = forward ? p.co : p.ci;
   const double bytes = (double)std::min(p.rows, p.groups) * p.ci * p.co * elementBytes(p.type);
@@ -1001,6 +1065,7 @@ int planRows(const Problem &p, const Tile *tiles, int kinds, int cu_count) {
       best = i;
     }
   }
+  if (us_of_best != nullptr) *us_of_best = least;
   return best;
 }
 
@@ -1039,7 +1104,7 @@ double planSlices(const Problem &p, const Tile &t, int cu_count, int *slice_rows
   return least;
 }
 
-Plan planFilter(const Problem &p, const Tile *tiles, int kinds, int cu_count) {
+Plan planFilter(const Problem &p, const Tile *tiles, int kinds, int cu_count, double *us_of_best = nullptr) {
   Plan best = {0, 0};
   double least = 0;
   for (int i = 0; i < kinds; ++i) {
@@ -1050,6 +1115,7 @@ Plan planFilter(const Problem &p, const Tile *tiles, int kinds, int cu_count) {
       best = {i, slice};
     }
   }
+  if (us_of_best != nullptr) *us_of_best = least;
   return best;
 }
 
@@ -1202,26 +1268,153 @@ hipError_t launchOf(const LaunchCtx &lc, const Problem &p, const Args &a, int cu
   }
 }
 
-}  // namespace
+// The problem with both numbers of channels in whole pieces: which of its matrices are copies, and how large.
+struct Padded {
+  bool takes;  // it takes less time
+  Problem q;
+  bool left, right, out;
+  size_t left_bytes, right_bytes, out_bytes;  // in multiples of 256
+};
 
-size_t workspaceBytes(const Problem &p, int cu_count) {
+Padded padded(const Problem &p, int cu_count) {
+  Padded d = {};
+  const int piece = pieceOf(p), size = elementBytes(p.type);
+  d.q = p;
+  d.q.ci = (p.ci + piece - 1) / piece * piece;
+  d.q.co = (p.co + piece - 1) / piece * piece;
+  const bool ci = d.q.ci != p.ci, co = d.q.co != p.co;
+  if (wholeSizes(p) || !wholeSizes(d.q) || p.rows == 0) return d;
+  const bool filter = p.which == MLUOP_EXT_GROUPED_BACKWARD_FILTER, forward = p.which == MLUOP_EXT_GROUPED_FORWARD;
+  const size_t x = (size_t)p.rows * d.q.ci * size, y = (size_t)p.rows * d.q.co * size, w = (size_t)p.groups * d.q.ci * d.q.co * size;
+  auto bytes = [](bool there, size_t n) { return there ? (n + 255) / 256 * 256 : 0; };
+  d.left = filter || forward ? ci : co;
+  d.right = filter ? co : true;
+  d.out = filter ? true : (forward ? co : ci);
+  d.left_bytes = bytes(d.left, filter || forward ? x : y);
+  d.right_bytes = bytes(d.right, filter ? y : w);
+  d.out_bytes = bytes(d.out, filter ? w : (forward ? y : x));
+  const double moved = (double)d.left_bytes + d.out_bytes +
+                       (filter ? d.right_bytes : (double)d.right_bytes * std::min(p.rows, p.groups) / p.groups);
+  if (moved > 4e9 || (double)d.right_bytes > 4e9) return d;
+  const Tile *tiles = p.type == MLUOP_DTYPE_FLOAT ? kFloatTiles : kTiles;
+  double any, whole;
+  if (filter) {
+    planFilter(p, &kAny, 1, cu_count, &any);
+    planFilter(d.q, tiles, kTileKinds, cu_count, &whole);
+  } else {
+    planRows(p, &kAny, 1, cu_count, &any);
+    planRows(d.q, tiles, kAllKinds, cu_count, &whole);
+  }
+  // (read and written, and a launch for what is copied in front and behind)
+  d.takes = whole + 2.0 * moved / kCopied + kCopyLaunch * ((d.left || d.right ? 1 : 0) + (d.out ? 1 : 0)) < any;
+  return d;
+}
+
+// `blocks` blocks of rows x width elements at `at` and their padded copy.
+Copy copyOf(const void *at, void *copy, int64_t stride, int64_t blocks, int rows, int padded_rows, int width, int padded_width, int size,
+            bool of_groups) {
+  Copy c = {};
+  c.from = static_cast<const char *>(at);
+  c.to = static_cast<char *>(copy);
+  c.from_stride = stride * size;
+  c.from_rows = rows;
+  c.to_rows = padded_rows;
+  c.from_bytes = width * size;
+  c.to_bytes = padded_width * size;
+  c.pieces = (uint32_t)(blocks * padded_rows * (c.to_bytes / 16));
+  c.of_groups = of_groups;
+  return c;
+}
+
+Args argsOf(const Problem &p, int cu_count, void *partial) {
+  Args a = {p.rows, p.groups, p.ci, p.co, p.starts, p.left_stride, p.right_stride, 0, 0, 0, 0, 0, false, nullptr};
+  if (p.which == MLUOP_EXT_GROUPED_BACKWARD_FILTER) {
+    a.slice_rows = planFilter(p, cu_count).slice_rows;
+    a.blocks = p.groups + (a.slice_rows > 0 ? p.rows / a.slice_rows : 0);
+    a.slots = a.slice_rows > 0 ? (int)mostSlots(p, a.slice_rows) : 0;
+    a.partial = static_cast<float *>(partial);
+  }
+  return a;
+}
+
+template <typename T>
+hipError_t launchPadded(const LaunchCtx &lc, const Problem &p, Padded d, int cu_count, char *workspace) {
+  constexpr int kSize = (int)sizeof(T);
+  const bool filter = p.which == MLUOP_EXT_GROUPED_BACKWARD_FILTER, forward = p.which == MLUOP_EXT_GROUPED_FORWARD;
+  Problem &q = d.q;
+  Copy copies[2] = {};
+  int count = 0;
+  if (d.left) {
+    const bool x = filter || forward;
+    q.left = workspace;
+    q.left_stride = x ? q.ci : q.co;
+    copies[count++] = copyOf(p.left, workspace, p.left_stride, 1, p.rows, p.rows, x ? p.ci : p.co, (int)q.left_stride, kSize, false);
+    workspace += d.left_bytes;
+  }
+  if (d.right) {
+    q.right = workspace;
+    q.right_stride = q.co;
+    copies[count++] = filter ? copyOf(p.right, workspace, p.right_stride, 1, p.rows, p.rows, p.co, q.co, kSize, false)
+                             : copyOf(p.right, workspace, p.right_stride, p.groups, p.ci, q.ci, p.co, q.co, kSize, true);
+    workspace += d.right_bytes;
+  }
+  Copy back = {};
+  if (d.out) {
+    back = filter ? copyOf(p.out, workspace, p.co, p.groups, p.ci, q.ci, p.co, q.co, kSize, false)
+                  : copyOf(p.out, workspace, forward ? p.co : p.ci, 1, p.rows, p.rows, forward ? p.co : p.ci, forward ? q.co : q.ci, kSize,
+                           false);
+    q.out = workspace;
+    workspace += d.out_bytes;
+  }
+  if (count > 0) {
+    const uint32_t one = (copies[0].pieces + 255) / 256, two = (copies[1].pieces + 255) / 256;
+    lc.begin("groupedPad");
+    groupedPad<T><<<one + two, 256, 0, lc.stream>>>(copies[0], copies[1], one, p.starts, p.rows);
+    lc.end();
+  }
+  const hipError_t status = launchOf<T>(lc, q, argsOf(q, cu_count, workspace), cu_count);
+  if (status != hipSuccess) return status;
+  if (d.out) {
+    lc.begin("groupedUnpad");
+    groupedUnpad<T><<<(back.pieces + 255) / 256, 256, 0, lc.stream>>>(back);
+    lc.end();
+  }
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launchAs(const LaunchCtx &lc, const Problem &p, int cu_count, void *workspace) {
+  const Padded d = padded(p, cu_count);
+  // (the matrices that are no copies have to be whole pieces as they are)
+  auto whole = [&](const void *at, int64_t stride) {
+    return alignedTo(at, 16) && stride % pieceOf(p) == 0 && stride < ((int64_t)1 << 20);
+  };
+  if (d.takes && (d.left || whole(p.left, p.left_stride)) && (d.right || whole(p.right, p.right_stride)) &&
+      (d.out || alignedTo(p.out, 16)))
+    return launchPadded<T>(lc, p, d, cu_count, static_cast<char *>(workspace));
+  return launchOf<T>(lc, p, argsOf(p, cu_count, workspace), cu_count);
+}
+
+size_t partialBytes(const Problem &p, int cu_count) {
   if (p.which != MLUOP_EXT_GROUPED_BACKWARD_FILTER) return 0;
   const int slice = planFilter(p, cu_count).slice_rows;
   if (slice == 0) return 0;
   return (size_t)mostSlots(p, slice) * p.ci * p.co * sizeof(float);
 }
 
+}  // namespace
+
+size_t workspaceBytes(const Problem &p, int cu_count) {
+  const Padded d = padded(p, cu_count);
+  const size_t as_it_is = partialBytes(p, cu_count);
+  if (!d.takes) return as_it_is;
+  return std::max(as_it_is, d.left_bytes + d.right_bytes + d.out_bytes + partialBytes(d.q, cu_count));
+}
+
 hipError_t launch(const LaunchCtx &lc, const Problem &p, int cu_count, void *workspace) {
-  Args a = {p.rows, p.groups, p.ci, p.co, p.starts, p.left_stride, p.right_stride, 0, 0, 0, 0, 0, false, nullptr};
-  if (p.which == MLUOP_EXT_GROUPED_BACKWARD_FILTER) {
-    a.slice_rows = planFilter(p, cu_count).slice_rows;
-    a.blocks = p.groups + (a.slice_rows > 0 ? p.rows / a.slice_rows : 0);
-    a.slots = a.slice_rows > 0 ? (int)mostSlots(p, a.slice_rows) : 0;
-    a.partial = static_cast<float *>(workspace);
-  }
-  if (p.type == MLUOP_DTYPE_HALF) return launchOf<_Float16>(lc, p, a, cu_count);
-  if (p.type == MLUOP_DTYPE_BFLOAT16) return launchOf<__bf16>(lc, p, a, cu_count);
-  return launchOf<float>(lc, p, a, cu_count);
+  if (p.type == MLUOP_DTYPE_HALF) return launchAs<_Float16>(lc, p, cu_count, workspace);
+  if (p.type == MLUOP_DTYPE_BFLOAT16) return launchAs<__bf16>(lc, p, cu_count, workspace);
+  return launchAs<float>(lc, p, cu_count, workspace);
 }
 
 }  // namespace grouped_matmul
