@@ -21,25 +21,23 @@ constexpr int kChunk = kRound;                       // elements of a workgroup
 constexpr int kStateBlock = MLUOP_EXT_ADAMW_BLOCK;   // elements that share a scale: 32 lanes
 constexpr int kLanesPerBlock = kStateBlock / kPerThread;
 constexpr float kMostCode = 448.f, kLeastCode = 0x1p-9f;  // of e4m3
-// Tensors of a launch: what 4 KB of kernel arguments hold.  A table in device memory would have to be copied there in
-// front of every step, since gradients are new tensors each time.
-constexpr int kTensors = 56;
-
-struct Tensors {
-  void *param[kTensors];
-  const void *grad[kTensors];
-  void *m[kTensors];
-  void *v[kTensors];
-  float *master[kTensors];
-  float *m_scale[kTensors];
-  float *v_scale[kTensors];
-  int64_t count[kTensors];
-  uint32_t first[kTensors];  // chunk of the launch; 0xffffffff behind the last tensor
-};
 struct Hyper {
   float beta1, one_minus_beta1, beta2, one_minus_beta2, decay, step_size, inv_root2, eps, grad_scale;
 };
-static_assert(sizeof(Tensors) + sizeof(Hyper) <= 4096, "kernel arguments");
+
+// Tensors of a launch: as many as 4 KB of kernel arguments hold, 65 to 106, so that only the addresses that there are have a
+// place and a length is its number of chunks and what the last of them has.  (A launch of small tensors takes some 7 us: 288
+// bf16 tensors of 85 000 elements in all 42 us at 56 a launch, 23 now.  A table in device memory would have to be copied
+// there in front of every step, since gradients are new tensors each time.)
+template <bool MASTER, bool EIGHT>
+struct Tensors {
+  enum { kParam, kGrad, kM, kV, kMaster, kMScale = kMaster + (MASTER ? 1 : 0), kVScale, kAddresses = kMScale + (EIGHT ? 2 : 0) };
+  static constexpr int kTensors = (4096 - (int)sizeof(Hyper) - 16) / (kAddresses * 8 + 6);
+  static_assert(kTensors <= 128, "two to a lane");
+  void *address[kAddresses][kTensors];
+  uint32_t first[kTensors + 1];  // chunk of the launch; behind the last tensor's: the number of chunks
+  uint16_t last[kTensors];       // elements of the last chunk
+};
 
 template <typename T>
 __device__ __forceinline__ void loadEight(const T *from, int64_t at, int n, bool whole, float (&to)[kPerThread]) {
@@ -127,22 +125,30 @@ __device__ __forceinline__ float blockMost(float v) {
 // caches (nobody reads a state before the next step): 130 M bf16 parameters with masters 757 -> 676 us (5.4 TB/s, where
 // a copy has 5.1), 250 M with 8-bit states 472 -> 458 us (5.5 TB/s), 33 fp32 tensors of 1.9 M elements in all 12.3 -> 10.8.
 template <typename P, typename G, bool MASTER, bool EIGHT>
-__global__ __launch_bounds__(kThreads) void adamwStep(Tensors t, Hyper h) {
-  static_assert(kTensors <= 64, "a lane a tensor");
+__global__ __launch_bounds__(kThreads) void adamwStep(Tensors<MASTER, EIGHT> t, Hyper h) {
+  typedef Tensors<MASTER, EIGHT> Table;
   const int lane = threadIdx.x & 63;
-  const uint32_t first = lane < kTensors ? t.first[lane] : 0xffffffffu;
-  const int which = __builtin_amdgcn_readfirstlane(__popcll(__ballot(first <= blockIdx.x)) - 1);
-  const int64_t count = t.count[which];
-  P *param = static_cast<P *>(t.param[which]);
-  const G *grad = static_cast<const G *>(t.grad[which]);
-  float *master = t.master[which];
+  const uint32_t one = t.first[lane], two = lane + 64 < Table::kTensors ? t.first[lane + 64] : 0xffffffffu;
+  const int which =
+      __builtin_amdgcn_readfirstlane(__popcll(__ballot(one <= blockIdx.x)) + __popcll(__ballot(two <= blockIdx.x)) - 1);
+  const uint32_t begin = t.first[which], chunk = blockIdx.x - begin;
+  const int in_chunk = chunk + 1 == t.first[which + 1] - begin ? t.last[which] : kChunk;
+  P *param = static_cast<P *>(t.address[Table::kParam][which]);
+  const G *grad = static_cast<const G *>(t.address[Table::kGrad][which]);
+  void *const m_at = t.address[Table::kM][which], *const v_at = t.address[Table::kV][which];
+  float *master = nullptr, *m_scales = nullptr, *v_scales = nullptr;
+  if constexpr (MASTER) master = static_cast<float *>(t.address[Table::kMaster][which]);
+  if constexpr (EIGHT) {
+    m_scales = static_cast<float *>(t.address[Table::kMScale][which]);
+    v_scales = static_cast<float *>(t.address[Table::kVScale][which]);
+  }
   const uintptr_t wide = reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad) |
                          (MASTER ? reinterpret_cast<uintptr_t>(master) : 0);
-  const uintptr_t states = reinterpret_cast<uintptr_t>(t.m[which]) | reinterpret_cast<uintptr_t>(t.v[which]);
+  const uintptr_t states = reinterpret_cast<uintptr_t>(m_at) | reinterpret_cast<uintptr_t>(v_at);
   const bool aligned = (wide & 15) == 0 && (states & (EIGHT ? 7 : 15)) == 0;
-  const int64_t at = (int64_t)(blockIdx.x - t.first[which]) * kChunk + threadIdx.x * kPerThread;
-  const int64_t left = count - at;
-  const int n = left >= kPerThread ? kPerThread : (left > 0 ? (int)left : 0);
+  const int64_t at = (int64_t)chunk * kChunk + threadIdx.x * kPerThread;
+  const int left = in_chunk - (int)threadIdx.x * kPerThread;
+  const int n = left >= kPerThread ? kPerThread : (left > 0 ? left : 0);
   const bool whole = aligned && n == kPerThread;
 
   float g[kPerThread], p[kPerThread], m[kPerThread], r[kPerThread];
@@ -154,17 +160,17 @@ __global__ __launch_bounds__(kThreads) void adamwStep(Tensors t, Hyper h) {
   else
     loadEight(param, at, n, whole, p);
   if constexpr (EIGHT) {
-    m_codes = loadCodes(static_cast<const uint8_t *>(t.m[which]), at, n, whole);
-    v_codes = loadCodes(static_cast<const uint8_t *>(t.v[which]), at, n, whole);
+    m_codes = loadCodes(static_cast<const uint8_t *>(m_at), at, n, whole);
+    v_codes = loadCodes(static_cast<const uint8_t *>(v_at), at, n, whole);
     if (n > 0) {
-      m_scale = t.m_scale[which][at / kStateBlock];
-      v_scale = t.v_scale[which][at / kStateBlock];
+      m_scale = m_scales[at / kStateBlock];
+      v_scale = v_scales[at / kStateBlock];
     }
     decode(m_codes, m_scale, m);
     decode(v_codes, v_scale, r);
   } else {
-    loadEight(static_cast<const float *>(t.m[which]), at, n, whole, m);
-    loadEight(static_cast<const float *>(t.v[which]), at, n, whole, r);
+    loadEight(static_cast<const float *>(m_at), at, n, whole, m);
+    loadEight(static_cast<const float *>(v_at), at, n, whole, r);
   }
   float v[kPerThread];
 #pragma unroll
@@ -195,35 +201,100 @@ __global__ __launch_bounds__(kThreads) void adamwStep(Tensors t, Hyper h) {
       m[i] = m[i] * by_m;
       r[i] = r[i] > 0.f ? fmaxf(r[i] * by_r, kLeastCode) : 0.f;
     }
-    storeCodes(static_cast<uint8_t *>(t.m[which]), at, n, whole, encode(m));
-    storeCodes(static_cast<uint8_t *>(t.v[which]), at, n, whole, encode(r));
+    storeCodes(static_cast<uint8_t *>(m_at), at, n, whole, encode(m));
+    storeCodes(static_cast<uint8_t *>(v_at), at, n, whole, encode(r));
     if (n > 0 && lane % kLanesPerBlock == 0) {
-      t.m_scale[which][at / kStateBlock] = most_m * (1.f / kMostCode);
-      t.v_scale[which][at / kStateBlock] = most_r * (1.f / kMostCode);
+      m_scales[at / kStateBlock] = most_m * (1.f / kMostCode);
+      v_scales[at / kStateBlock] = most_r * (1.f / kMostCode);
     }
   } else {
-    storeEight(static_cast<float *>(t.m[which]), at, n, whole, m);
-    storeEight(static_cast<float *>(t.v[which]), at, n, whole, v);
+    storeEight(static_cast<float *>(m_at), at, n, whole, m);
+    storeEight(static_cast<float *>(v_at), at, n, whole, v);
   }
 }
 
-typedef void (*Kernel)(Tensors, Hyper);
+struct Step {
+  const char *api;
+  mluOpHandle_t handle;
+  const mluOpExtAdamWTensor_t *tensors;
+  int count;
+  Hyper h;
+};
+constexpr int64_t kMostChunks = 1 << 30;
+
+template <typename P, typename G, bool MASTER, bool EIGHT>
+mluOpStatus_t launchStep(const Step &step) {
+  typedef Tensors<MASTER, EIGHT> Table;
+  static_assert(sizeof(Table) + sizeof(Hyper) <= 4096, "kernel arguments");
+  const LaunchCtx lc = step.handle->launchCtx();
+  const bool notes = step.handle->hasNotes();
+  Table t;
+  int held = 0;
+  uint32_t chunks = 0;
+  auto launch = [&]() -> hipError_t {
+    if (held == 0) return hipSuccess;
+    t.first[held] = chunks;
+    for (int i = held; i < Table::kTensors; ++i) {
+      for (auto &of : t.address) of[i] = nullptr;
+      t.first[i + 1] = 0xffffffffu;
+      t.last[i] = 0;
+    }
+    lc.begin("adamwStep");
+    adamwStep<P, G, MASTER, EIGHT><<<chunks, kThreads, 0, lc.stream>>>(t, step.h);
+    lc.end();
+    held = 0;
+    chunks = 0;
+    return hipGetLastError();
+  };
+  for (int i = 0; i < step.count; ++i) {
+    const mluOpExtAdamWTensor_t &x = step.tensors[i];
+    if (x.count == 0) continue;
+    const int64_t own = (x.count + kChunk - 1) / kChunk;
+    if (held == Table::kTensors || chunks + own > kMostChunks) HIP_CHECK_RETURN(step.api, launch());
+    if (notes) {
+      const int64_t blocks = (x.count + kStateBlock - 1) / kStateBlock;
+      step.handle->forgetNotesIn(x.param, (size_t)x.count * sizeof(P));
+      step.handle->forgetNotesIn(x.exp_avg, (size_t)x.count * (EIGHT ? 1 : 4));
+      step.handle->forgetNotesIn(x.exp_avg_sq, (size_t)x.count * (EIGHT ? 1 : 4));
+      if (MASTER) step.handle->forgetNotesIn(x.master, (size_t)x.count * 4);
+      if (EIGHT) {
+        step.handle->forgetNotesIn(x.exp_avg_scale, (size_t)blocks * 4);
+        step.handle->forgetNotesIn(x.exp_avg_sq_scale, (size_t)blocks * 4);
+      }
+    }
+    t.address[Table::kParam][held] = x.param;
+    t.address[Table::kGrad][held] = const_cast<void *>(x.grad);  // (only read)
+    t.address[Table::kM][held] = x.exp_avg;
+    t.address[Table::kV][held] = x.exp_avg_sq;
+    if constexpr (MASTER) t.address[Table::kMaster][held] = x.master;
+    if constexpr (EIGHT) {
+      t.address[Table::kMScale][held] = x.exp_avg_scale;
+      t.address[Table::kVScale][held] = x.exp_avg_sq_scale;
+    }
+    t.first[held] = chunks;
+    t.last[held] = (uint16_t)(x.count - (own - 1) * kChunk);
+    chunks += (uint32_t)own;
+    ++held;
+  }
+  HIP_CHECK_RETURN(step.api, launch());
+  return MLUOP_STATUS_SUCCESS;
+}
 
 template <typename P, typename G, bool MASTER>
-Kernel ofStates(bool eight) {
-  return eight ? adamwStep<P, G, MASTER, true> : adamwStep<P, G, MASTER, false>;
+mluOpStatus_t ofStates(const Step &step, bool eight) {
+  return eight ? launchStep<P, G, MASTER, true>(step) : launchStep<P, G, MASTER, false>(step);
 }
 
 template <typename P>
-Kernel ofSixteen(bool float_grads, bool masters, bool eight) {
-  if (float_grads) return masters ? ofStates<P, float, true>(eight) : ofStates<P, float, false>(eight);
-  return masters ? ofStates<P, P, true>(eight) : ofStates<P, P, false>(eight);
+mluOpStatus_t ofSixteen(const Step &step, bool float_grads, bool masters, bool eight) {
+  if (float_grads) return masters ? ofStates<P, float, true>(step, eight) : ofStates<P, float, false>(step, eight);
+  return masters ? ofStates<P, P, true>(step, eight) : ofStates<P, P, false>(step, eight);
 }
 
-Kernel kernelFor(mluOpDataType_t param_type, bool float_grads, bool masters, bool eight) {
-  if (param_type == MLUOP_DTYPE_FLOAT) return ofStates<float, float, false>(eight);
-  return param_type == MLUOP_DTYPE_HALF ? ofSixteen<_Float16>(float_grads, masters, eight)
-                                        : ofSixteen<__bf16>(float_grads, masters, eight);
+mluOpStatus_t launchOf(const Step &step, mluOpDataType_t param_type, bool float_grads, bool masters, bool eight) {
+  if (param_type == MLUOP_DTYPE_FLOAT) return ofStates<float, float, false>(step, eight);
+  return param_type == MLUOP_DTYPE_HALF ? ofSixteen<_Float16>(step, float_grads, masters, eight)
+                                        : ofSixteen<__bf16>(step, float_grads, masters, eight);
 }
 
 }  // namespace
@@ -255,12 +326,17 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtAdamWStep(mluOpHandle_t handle, const mluOpE
     PARAM_CHECK(api, masters == (t.master != NULL));
     PARAM_CHECK(api, t.param != NULL && t.grad != NULL && t.exp_avg != NULL && t.exp_avg_sq != NULL);
     PARAM_CHECK(api, !eight || (t.exp_avg_scale != NULL && t.exp_avg_sq_scale != NULL));
+    if ((t.count - 1) / kChunk >= kMostChunks) {
+      MLUOP_LOG(ERROR) << api << " At most " << kMostChunks * kChunk << " elements of a tensor are supported.";
+      return MLUOP_STATUS_NOT_SUPPORTED;
+    }
   }
   PARAM_CHECK(api, !masters || param_type != MLUOP_DTYPE_FLOAT);
   DEVICE_HANDLE_CHECK(api, handle);
   HIP_CHECK_RETURN(api, hipSetDevice(handle->device));
 
-  Hyper h;
+  Step all = {api, handle, tensors, num_tensors, {}};
+  Hyper &h = all.h;
   h.beta1 = (float)beta1;
   h.one_minus_beta1 = (float)(1.0 - beta1);
   h.beta2 = (float)beta2;
@@ -271,61 +347,5 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtAdamWStep(mluOpHandle_t handle, const mluOpE
   h.eps = (float)eps;
   h.grad_scale = (float)grad_scale;
 
-  const Kernel kernel = kernelFor(param_type, grad_type == MLUOP_DTYPE_FLOAT, masters, eight);
-  const mluop::LaunchCtx lc = handle->launchCtx();
-  const bool notes = handle->hasNotes();
-  Tensors t;
-  int held = 0;
-  uint32_t chunks = 0;
-  auto launch = [&]() -> hipError_t {
-    if (held == 0) return hipSuccess;
-    for (int i = held; i < kTensors; ++i) {
-      t.param[i] = t.m[i] = t.v[i] = nullptr;
-      t.grad[i] = nullptr;
-      t.master[i] = t.m_scale[i] = t.v_scale[i] = nullptr;
-      t.count[i] = 0;
-      t.first[i] = 0xffffffffu;
-    }
-    lc.begin("adamwStep");
-    kernel<<<chunks, kThreads, 0, lc.stream>>>(t, h);
-    lc.end();
-    held = 0;
-    chunks = 0;
-    return hipGetLastError();
-  };
-  constexpr int64_t kMostChunks = 1 << 30;
-  for (int i = 0; i < num_tensors; ++i) {
-    const mluOpExtAdamWTensor_t &x = tensors[i];
-    if (x.count == 0) continue;
-    const int64_t own = (x.count + kChunk - 1) / kChunk;
-    if (own > kMostChunks) {
-      MLUOP_LOG(ERROR) << api << " At most " << kMostChunks * kChunk << " elements of a tensor are supported.";
-      return MLUOP_STATUS_NOT_SUPPORTED;
-    }
-    if (held == kTensors || chunks + own > kMostChunks) HIP_CHECK_RETURN(api, launch());
-    if (notes) {
-      const int64_t blocks = (x.count + kStateBlock - 1) / kStateBlock;
-      handle->forgetNotesIn(x.param, (size_t)x.count * elementBytes(param_type));
-      handle->forgetNotesIn(x.exp_avg, (size_t)x.count * (eight ? 1 : 4));
-      handle->forgetNotesIn(x.exp_avg_sq, (size_t)x.count * (eight ? 1 : 4));
-      if (masters) handle->forgetNotesIn(x.master, (size_t)x.count * 4);
-      if (eight) {
-        handle->forgetNotesIn(x.exp_avg_scale, (size_t)blocks * 4);
-        handle->forgetNotesIn(x.exp_avg_sq_scale, (size_t)blocks * 4);
-      }
-    }
-    t.param[held] = x.param;
-    t.grad[held] = x.grad;
-    t.m[held] = x.exp_avg;
-    t.v[held] = x.exp_avg_sq;
-    t.master[held] = x.master;
-    t.m_scale[held] = x.exp_avg_scale;
-    t.v_scale[held] = x.exp_avg_sq_scale;
-    t.count[held] = x.count;
-    t.first[held] = chunks;
-    chunks += (uint32_t)own;
-    ++held;
-  }
-  HIP_CHECK_RETURN(api, launch());
-  return MLUOP_STATUS_SUCCESS;
+  return launchOf(all, param_type, grad_type == MLUOP_DTYPE_FLOAT, masters, eight);
 }
