@@ -19,15 +19,21 @@ constexpr int kThreads = 256;
 template <int V>
 using Lanes = RowLanes<V, kThreads>;
 
-// Tokens of either type.
+// Tokens of either type, read without a branch: one between loads would make each wait for the one before.
 struct Tokens {
-  const void *at;
-  bool wide;
+  const uint32_t *at;
   uint32_t rows;
+  int step, high;  // words of a token, and where its upper half is (32 bits: the token again, of which nothing counts)
+  uint32_t upper;
+  Tokens(const void *tokens, mluOpDataType_t type, int64_t table_rows)
+      : at(static_cast<const uint32_t *>(tokens)), rows((uint32_t)table_rows), step(type == MLUOP_DTYPE_INT64 ? 2 : 1), high(step - 1),
+        upper(high != 0 ? ~0u : 0u) {}
   // The row that token i names; `rows` where it names none.
   __device__ __forceinline__ uint32_t row(int64_t i) const {
-    const int64_t t = wide ? static_cast<const int64_t *>(at)[i] : (int64_t) static_cast<const int32_t *>(at)[i];
-    return (u64)t < rows ? (uint32_t)t : rows;
+    const uint32_t *word = at + i * step;
+    const uint32_t lo = word[0], hi = word[high];
+    const uint32_t none = (hi & upper) | (lo < rows ? 0u : 1u);
+    return none == 0 ? lo : rows;
   }
 };
 
@@ -96,38 +102,61 @@ struct FirstPass {
   __device__ void store(size_t to, const Item &t, int64_t) const { out[to] = t; }
 };
 
-// Few tokens (rankedTokens): the place of a word is the number of words below it, counted by a wave for kRanked words at once.
-// One launch, whose work grows with the square of the tokens.  us of a whole gradient with this: 1024 tokens 16 to 18, 2048 21 to 22,
-// 4096 30 to 32; with one pass of the sort (tables of up to 1023 rows) 17 to 19, with two 33.
-constexpr int kRanked = 4;
-int rankedTokens(int passes) { return passes == 1 ? 1024 : 3000; }
+// Few tokens (rankedTokens): the place of a word is the number of words below it, counted for kRanked words by a workgroup whose
+// waves share the others.  One launch, whose work grows with the square of the tokens.  us of a whole gradient of 64 bf16
+// channels with this / with the sort: one pass of it (500 rows) 1024 tokens 13.2 / 15.9, 4096 18.4 / 19.4, 6000 22.0 / 19.4; two
+// (91 000 rows) 1024 15.3 / 30.0, 8192 25.7 / 35.5, 12 288 34.9 / 36.4, 16 384 46.0 / 37.7.
+constexpr int kRanked = 16;
+int rankedTokens(int passes) { return passes == 1 ? 4096 : 12288; }
 __global__ __launch_bounds__(kThreads) void embeddingRankWords(Tokens tokens, uint32_t n, u64 *__restrict__ sorted) {
-  const int lane = threadIdx.x & 63;
-  const uint32_t first = (blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kRanked;
-  if (first >= n) return;
-  // (words are compared as pairs of a row and a place: one row beside the others is enough where places decide by themselves)
+  constexpr int kAhead = 4;
+  __shared__ uint32_t s_below[kRanked][kThreads];
+  const uint32_t first = blockIdx.x * kRanked, wave = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63u), lane = threadIdx.x & 63;
   uint32_t row[kRanked], below[kRanked] = {};
 #pragma unroll
-  for (int j = 0; j < kRanked; ++j) row[j] = tokens.row(min(first + j, n - 1));
-  constexpr int kAhead = 8;
-  for (uint32_t i0 = lane; i0 < n; i0 += 64 * kAhead) {
-    uint32_t other[kAhead];
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a) other[a] = tokens.row(min(i0 + a * 64, n - 1));
+  for (int j = 0; j < kRanked; ++j) row[j] = __builtin_amdgcn_readfirstlane(tokens.row(min(first + j, n - 1))) + 1;
+  uint32_t next[kAhead];
+  auto request = [&](uint32_t i0) {
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
-      const uint32_t i = i0 + a * 64;
+      const uint32_t i = i0 + a * kThreads + lane;
+      const uint32_t row = tokens.row(min(i, n - 1));
+      next[a] = i < n ? row + 1 : 0x80000000u;  // (below nothing)
+    }
+  };
+  request(wave);
+  for (uint32_t i0 = wave; i0 < n; i0 += kThreads * kAhead) {
+    uint32_t other[kAhead];
 #pragma unroll
-      for (int j = 0; j < kRanked; ++j)
-        below[j] += i < n && (other[a] < row[j] || (other[a] == row[j] && i < first + j)) ? 1u : 0u;
+    for (int a = 0; a < kAhead; ++a) other[a] = next[a];
+    request(i0 + kThreads * kAhead);
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const uint32_t from = i0 + a * kThreads;
+      // (of equal rows those of the places in front are below: all of these 64 or none, mostly)
+      if (from + 63 < first || from >= first + kRanked) {
+        const uint32_t as = other[a] - (from < first ? 1 : 0);
+#pragma unroll
+        for (int j = 0; j < kRanked; ++j) below[j] += as < row[j] ? 1u : 0u;
+      } else {
+#pragma unroll
+        for (int j = 0; j < kRanked; ++j)
+          below[j] += other[a] < row[j] + (from + lane < first + j ? 1u : 0u) ? 1u : 0u;
+      }
     }
   }
 #pragma unroll
-  for (int j = 0; j < kRanked; ++j) {
+  for (int j = 0; j < kRanked; ++j) s_below[j][threadIdx.x] = below[j];
+  __syncthreads();
+  // sixteen threads a word, lines of them
+  constexpr int kShare = kThreads / kRanked;
+  const uint32_t word = threadIdx.x / kShare, share = threadIdx.x % kShare;
+  uint32_t sum = 0;
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) below[j] += __shfl_xor(below[j], d, 64);
-    if (lane == j && first + j < n) sorted[below[j]] = (u64)row[j] << 32 | (first + j);
-  }
+  for (int k = 0; k < kThreads / kShare; ++k) sum += s_below[word][k * kShare + share];
+#pragma unroll
+  for (int d = kShare / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
+  if (share == 0 && first + word < n) sorted[sum] = (u64)tokens.row(first + word) << 32 | (first + word);
 }
 
 // The place of the first sorted word of every row, and of `rows`, where the words end that name a row.
@@ -389,7 +418,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingForward(mluOpHandle_t handle, mluOp
   if (num_tokens == 0) return MLUOP_STATUS_SUCCESS;
   HIP_CHECK_RETURN(api, hipSetDevice(handle->device));
   handle->forgetNotesIn(out, (size_t)num_tokens * channels * elementBytes(type));
-  const Tokens t = {tokens, token_type == MLUOP_DTYPE_INT64, (uint32_t)rows};
+  const Tokens t(tokens, token_type, rows);
   const mluop::LaunchCtx lc = handle->launchCtx();
   byType(type, channels, row_stride, reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(out), [&](auto zero, auto v) {
     typedef decltype(zero) T;
@@ -447,7 +476,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingBackward(mluOpHandle_t handle, mluO
   float *partial = reinterpret_cast<float *>(at + 2 * p.words + p.counters + p.starts);
 
   const mluop::LaunchCtx lc = handle->launchCtx();
-  const Tokens names = {tokens, token_type == MLUOP_DTYPE_INT64, (uint32_t)rows};
+  const Tokens names(tokens, token_type, rows);
   bool in_second = false, started = false;
   if (num_tokens > 0) lc.begin("embeddingSort");
   if (num_tokens > rankedTokens((p.bits + p.pass_bits - 1) / p.pass_bits)) {
@@ -469,9 +498,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingBackward(mluOpHandle_t handle, mluO
       in_second = !in_second;
     }
   } else if (num_tokens > 0) {
-    constexpr int kEach = kThreads / 64 * kRanked;
-    embeddingRankWords<<<(unsigned)((num_tokens + kEach - 1) / kEach), kThreads, 0, lc.stream>>>(
-        names, (uint32_t)num_tokens, words[0]);
+    embeddingRankWords<<<(unsigned)((num_tokens + kRanked - 1) / kRanked), kThreads, 0, lc.stream>>>(names, (uint32_t)num_tokens,
+                                                                                                     words[0]);
   }
   if (num_tokens > 0) lc.end();
   const Sorted s = {words[in_second ? 1 : 0], starts, (uint32_t)num_tokens, (uint32_t)rows, (uint32_t)p.piece,
