@@ -39,6 +39,8 @@ struct Tokens {
 
 // ---- forward -------------------------------------------------------------------------------
 
+// out[t] = scale * table[token t], in one pass; bound by memory, or by the launch where there is little: 240 612 rows of 512 fp16 (247 MB)
+// 36 us, seven tokens 5.
 constexpr int kRowsAThread = 4;  // whose loads are in flight together
 
 template <typename T, int V>
@@ -80,7 +82,9 @@ __global__ __launch_bounds__(kThreads) void embeddingRows(const T *__restrict__ 
 // each piece is summed by a workgroup of its own, and a last launch adds the pieces.
 
 // Whether all rows of threads of a workgroup share a row of the table: one that is named often, as all are in a small table.
-bool rowsShared(int64_t n, int64_t rows, int64_t channels) { return n >= 16 * rows && channels < 1024; }
+// us of the gradient of 5000 x 64 bf16 without / with this: named 8 times on average 38 / 42, 16 times 41 / 44, 32 times 55 / 47, 64 times
+// 75 / 52; 517 x 64 fp32, 232 times, 47 / 31.
+bool rowsShared(int64_t n, int64_t rows, int64_t channels) { return n >= 24 * rows && channels < 1024; }
 
 // Words of a piece: as many as the rows of threads of a workgroup (which V = 4 has) read at once, eight each, where they
 // share rows of the table.  Where one of them sums a row alone, fewer; but where a row has many channels there are no
@@ -223,6 +227,8 @@ struct Sorted {
   bool streamed;
 };
 
+// out[row] = scale * (the gradients of the row's words, in ascending place, in fp32).  Bound by memory: 131 072 x 2048 bf16 from 65 536
+// tokens (805 MB) 140 us, 5.7 TB/s.
 // The first row_blocks workgroups own rows of the table.  The others take a piece each: of the rows that are longer than
 // one, at most two reach into it, that of its first word and that of its last.
 // SHARED: a row of the table a workgroup, whose rows of threads share the words.
@@ -392,7 +398,8 @@ void byType(mluOpDataType_t type, int64_t channels, int64_t row_stride, uintptr_
 }
 
 // Rows of the table that a row of threads owns, of `turns` it would own one at a time: several of a large table, most of
-// whose rows nobody names, and a workgroup for each would mostly start and end; one of a small table.
+// whose rows nobody names, and a workgroup for each would mostly start and end; one of a small table.  us of a gradient with one /
+// with four: 131 072 x 2048 bf16 from 65 536 tokens 202 / 186, 600 000 x 64 from 30 000 55 / 52; 500 x 512 from 4000 18 / 23.
 int tableRows(int64_t turns) { return turns >= 16384 ? 4 : 1; }
 
 int rowsAtOnce(int64_t vectors) { return vectors >= kThreads ? 1 : (int)(kThreads / vectors); }

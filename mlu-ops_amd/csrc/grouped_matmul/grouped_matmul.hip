@@ -1,4 +1,11 @@
-// Kernels of the products grouped by expert.
+// Kernels of the products grouped by expert: y_r = x_r W_g, dx_r = dy_r W_g^T and dW_g = sum over the rows r of a group of x_r^T dy_r,
+// on matrix cores with fp32 sums and one rounding.  A tile of rows never crosses a group's end.
+//   groupedTiles  rows in whole 16-byte pieces; bound by the matrix cores and, long and large, by the power they draw (the same
+//                 product of zeros is faster).  32 768 rows, 8 x 2048 x 8192 bf16: forward 1.00 ms (1.10 PFLOP/s), backward data
+//                 0.95 (1.16), filter gradient 0.87 (1.26), where a large library product has 1.24.
+//   groupedFew    the same with few rows a group; bound by the filters' way from memory: 12 rows of ten of 32 experts, 1024 x 2048
+//                 bf16 (42 MB) 11.0 us, 3.8 TB/s with what a launch costs.
+//   groupedAny    any shape and stride; bound by the step from load to LDS to multiply, some 2 us of 64.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -607,6 +614,8 @@ __device__ __forceinline__ void storeResults(u32x4 v, __amdgpu_buffer_rsrc_t to,
     __builtin_amdgcn_raw_buffer_store_b128(v, to, at, 0, 0);
 }
 
+// A workgroup has one tile and its two steps in LDS (256 x 256: 128 KB, one a CU): operands are read once for 256 results a side, which
+// leaves L2 at 10 TB/s in all; 128 x 128 tiles of the same product need twice that and reach 0.8 of the rate.
 // Workgroups stay: each takes the works blockIdx.x, blockIdx.x + gridDim.x, ... (or those of its order).  The first loads of
 // the next are under way while the results of this one are stored.
 template <typename T, int MODE, int BM, int BN, int WM, int WN, bool REST>
@@ -1007,8 +1016,16 @@ struct Tile {
 // 16 rows of a 2048 x 2048 filter 39 / 19 / 14 / 9 / 8.5, 1000 rows 43 / 24 / 21 / 27 / 43, 4000 rows 47 / 36 / 48 / 95 / 158, 40 000
 // rows 288 / 365 / 524 / 895 / 1480.
 constexpr int kTileKinds = 3;
+// Steps of the reduction from which on a last round that 256 x 256 tiles fill to a quarter or less is left for 128 x 128 ones.  Its
+// tiles take a whole round's time otherwise; an empty launch takes 2 us.  2048 columns of fp16, us of 33 / 40 / 48 tiles an XCD
+// (32 workgroups) without and with this: 8 steps 37 / 36 / 38 either way, 16 steps 58 / 57 / 59 and 51 / 53 / 59, 64 steps 180 / 180 / 182
+// and 152 / 156 / 182.
 constexpr int kRestSteps = 16;
+// Bytes of results from which on 256 x 256 tiles are stored past the caches, which then keep the operands: 82 MB 177 -> 158 us, 134 MB
+// 268 -> 250; 31 MB 34 -> 38.
 constexpr double kStreamedResults = 64e6;
+// Padded copies, us without and with them: 25 973 rows of 2048 x 100 fp16 112 / 35, 229 rows of 64 x 2048 x 100 99 / 32; one row of
+// 16 x 1024 x 100 32 / 12, where the filter is all there is to copy; twelve rows of 32 x 100 x 2048 stay at 6.6, which two launches take.
 // Bytes a us of padded copies, and a launch of them.
 constexpr double kCopied = 3.0e6, kCopyLaunch = 4.0;
 // 64 filters of 2048 x 2048 for a row each: 121 / 95 / 97 / 119 / 119, and backward data, which reads their rows, 136 / 125 / 122 /
@@ -1018,7 +1035,6 @@ constexpr Tile kTiles[] = {{"groupedTiles256", 256, 256, 1, 1.25, 1.65, 5.0, 4.4
                            {"groupedTiles64", 64, 128, 2, 0.43, 0.76, 2.0, 5.6, 4.3},
                            {"groupedFew32", 32, kFewColumns, 2, 0.25, 0.40, 1.5, 5.2, 5.2},
                            {"groupedFew16", 16, kFewColumns, 2, 0.22, 0.36, 1.5, 5.2, 5.2}};
-// the kernel of any shape: a step of 64 is two of its own
 // fp32, whose steps are 32 deep: bound by the multiplies.  Forward of 2048 x 2048, us as above: 1000 rows 464 / 155 / 82 / 85 / 104,
 // 4000 rows 469 / 292 / 269 / 323 / 401, 16 000 rows 949 / 1077 / 1060 / 1258 / 1558 (141 TFLOP/s; a large library product has 154).
 constexpr Tile kFloatTiles[] = {{"groupedTiles256", 256, 256, 1, 7.2, 7.0, 5.0, 4.4, 3.9},
@@ -1037,7 +1053,7 @@ double timeOf(const Tile &t, double tiles, double steps, int cu_count) {
 }
 
 struct Plan {
-  int tile;        // of kTiles, or of kAnyTiles
+  int tile;        // of the tiles that were asked for
   int slice_rows;  // backward filter; 0: whole groups
 };
 
