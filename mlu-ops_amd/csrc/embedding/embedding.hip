@@ -40,7 +40,7 @@ struct Tokens {
 // ---- forward -------------------------------------------------------------------------------
 
 // out[t] = scale * table[token t], in one pass; bound by memory, or by the launch where there is little: 240 612 rows of 512 fp16 (247 MB)
-// 36 us, seven tokens 5.
+// 36 us, 64 rows of 1024 bf16 5.6.
 constexpr int kRowsAThread = 4;  // whose loads are in flight together
 
 template <typename T, int V>

@@ -521,9 +521,8 @@ __device__ __forceinline__ int shareOut(const Order &order, const int *lengths, 
 }
 
 // Work number `number` of args.works, from the starts in LDS.  Workgroups go to the eight XCDs in turn, and so do the
-// numbers; those of an XCD take tiles that share operands in its L2.  REST: the last round that is left by the kernel of tiles
-// twice as high and wide, a quarter of such a tile each.
-template <typename T, int MODE, int BM, int BN, bool REST>
+// numbers; those of an XCD take tiles that share operands in its L2.
+template <typename T, int MODE, int BM, int BN>
 __device__ __forceinline__ Work<T> workOf(int number, int works, const int32_t *starts, const Order &order, const RowTiles &tiles,
                                           const Args &a, const T *left, const T *right) {
   Work<T> w;
@@ -580,18 +579,9 @@ __device__ __forceinline__ Work<T> workOf(int number, int works, const int32_t *
     w.partial = slice.slot >= 0;
     w.out = ((int64_t)(w.partial ? slice.slot : slice.group) * a.ci + m0) * columns + n0;
   } else {
-    constexpr int kWhole = REST ? 2 : 1;
-    if (REST) in_xcd = tiles.kept + in_xcd / 4;
-    RaggedTile t = tileOfRows<BM * kWhole>(tiles, number & 7, in_xcd, starts, a, &n0);
+    const RaggedTile t = tileOfRows<BM>(tiles, number & 7, in_xcd, starts, a, &n0);
     if (t.segment < 0) return w;
-    n0 *= BN * kWhole;
-    if (REST) {
-      const int quarter = number >> 3 & 3, down = (quarter >> 1) * BM;
-      n0 += (quarter & 1) * BN;
-      if (down >= t.rows || n0 >= columns) return w;
-      t.first += down;
-      t.rows = min(t.rows - down, BM);
-    }
+    n0 *= BN;
     const int group = t.segment - 1;
     const bool inside = group >= 0 && group < a.groups;
     w.depth = inside ? (MODE == kForward ? a.ci : a.co) : 0;
@@ -618,7 +608,7 @@ __device__ __forceinline__ void storeResults(u32x4 v, __amdgpu_buffer_rsrc_t to,
 // leaves L2 at 10 TB/s in all; 128 x 128 tiles of the same product need twice that and reach 0.8 of the rate.
 // Workgroups stay: each takes the works blockIdx.x, blockIdx.x + gridDim.x, ... (or those of its order).  The first loads of
 // the next are under way while the results of this one are stored.
-template <typename T, int MODE, int BM, int BN, int WM, int WN, bool REST>
+template <typename T, int MODE, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict__ left, const T *__restrict__ right,
                                                             Args a, T *__restrict__ out) {
   constexpr bool kFilter = MODE == kBackwardFilter;
@@ -676,9 +666,8 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
     }
   }
   if (!kFilter) {
-    constexpr int kWhole = REST ? 2 : 1;
-    tiles = rowTilesOf<BM * kWhole>(s_starts, a, (columns + BN * kWhole - 1) / (BN * kWhole));
-    works = min(works, 8 * (REST ? 4 * (tiles.each - tiles.kept) : tiles.kept));
+    tiles = rowTilesOf<BM>(s_starts, a, (columns + BN - 1) / BN);
+    works = min(works, 8 * tiles.kept);
   }
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   const char *x_tile = s_tiles, *y_tile = s_tiles + 2 * Left::kBytes;
@@ -718,11 +707,11 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
   };
 
   bool stored = false;  // behind the loads of the work's first step there are kStores stores
-  Work<T> work = workOf<T, MODE, BM, BN, REST>(number, works, s_starts, order, tiles, a, left, right);
+  Work<T> work = workOf<T, MODE, BM, BN>(number, works, s_starts, order, tiles, a, left, right);
   begin(work);
   while (work.there) {
     number += ahead;
-    const Work<T> following = workOf<T, MODE, BM, BN, REST>(number, works, s_starts, order, tiles, a, left, right);
+    const Work<T> following = workOf<T, MODE, BM, BN>(number, works, s_starts, order, tiles, a, left, right);
     float4v acc[TM][TN] = {};
     const int steps = (work.depth + kDepth<T> - 1) / kDepth<T>;
     if (steps > 0) {
@@ -824,33 +813,43 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// Few rows a group: the filters are what is read, and every workgroup keeps kFewStages steps of its 64 columns on their way.
-// Four waves have 16 columns each.  (The kernel above has one step under way, which a product of a few steps waits for
-// again and again.)
-constexpr int kFewColumns = 64, kFewStages = 6, kFewWaves = 4;
+// One tile a workgroup, and STAGES steps of both sides on their way: for few rows a group, where the filters are what is read, and
+// for the last round that 256 x 256 tiles leave (REST: a quarter of such a tile each).  The kernel above has one step under
+// way, which a product that takes less than a way from memory for a step waits for again and again: 48 tiles of 64 steps left
+// over took 60 us in tiles of 128 x 128 of its own.
+constexpr int kFewColumns = 64, kFewStages = 6, kRestStages = 4, kFewWaves = 4;
 
-template <typename T, int MODE, int BM>
+template <typename T, int MODE, int BM, int BN, int WM, int WN, int STAGES, bool REST>
 __global__ __launch_bounds__(kFewWaves * 64) void groupedFew(const T *__restrict__ left, const T *__restrict__ right, Args a,
                                                              T *__restrict__ out) {
+  static_assert(WM * WN == kFewWaves, "waves");
   typedef Operand<T, true, BM, kFewWaves> Left;
-  typedef Operand<T, MODE == kBackwardData, kFewColumns, kFewWaves> Right;
+  typedef Operand<T, MODE == kBackwardData, BN, kFewWaves> Right;
   typedef typename Fragment<T>::type fragment;
-  constexpr int TM = BM / 16, kLoads = Left::kLoads + Right::kLoads;
-  static_assert((kFewStages - 2) * kLoads <= 63, "what a wait can count");
+  constexpr int TM = BM / WM / 16, TN = BN / WN / 16, kLoads = Left::kLoads + Right::kLoads, kWhole = REST ? 2 : 1;
+  static_assert((STAGES - 2) * kLoads <= 63, "what a wait can count");
   extern __shared__ __attribute__((aligned(1024))) char s_tiles[];
 
   const int columns = MODE == kBackwardData ? a.ci : a.co;
-  int n0;
-  const RowTiles tiles = rowTilesOf<BM>(a.starts, a, (columns + kFewColumns - 1) / kFewColumns);
-  const RaggedTile t = tileOfRows<BM>(tiles, blockIdx.x & 7, blockIdx.x >> 3, a.starts, a, &n0);
+  int n0, in_xcd = blockIdx.x >> 3;
+  const RowTiles tiles = rowTilesOf<BM * kWhole>(a.starts, a, (columns + BN * kWhole - 1) / (BN * kWhole));
+  if (REST) in_xcd = tiles.kept + in_xcd / 4;
+  RaggedTile t = tileOfRows<BM * kWhole>(tiles, blockIdx.x & 7, in_xcd, a.starts, a, &n0);
   if (t.segment < 0) return;
-  n0 *= kFewColumns;
+  n0 *= BN * kWhole;
+  if (REST) {
+    const int quarter = blockIdx.x >> 3 & 3, down = (quarter >> 1) * BM;
+    n0 += (quarter & 1) * BN;
+    if (down >= t.rows || n0 >= columns) return;
+    t.first += down;
+    t.rows = min(t.rows - down, BM);
+  }
   const int group = t.segment - 1, width = columns - n0;
   const bool inside = group >= 0 && group < a.groups;
   const int depth = inside ? (MODE == kForward ? a.ci : a.co) : 0;
   Left x(left + t.first * a.left_stride, a.left_stride, t.rows, s_tiles);
   Right y(right + (int64_t)(inside ? group : 0) * a.ci * a.co + (MODE == kForward ? (int64_t)n0 : (int64_t)n0 * a.co),
-          a.right_stride, width, s_tiles + kFewStages * Left::kBytes);
+          a.right_stride, width, s_tiles + STAGES * Left::kBytes);
   auto request = [&](int left_over, int buffer) {
     x.next(left_over);
     y.next(left_over);
@@ -860,35 +859,43 @@ __global__ __launch_bounds__(kFewWaves * 64) void groupedFew(const T *__restrict
     for (int u = 0; u < Right::kLoads; ++u) y.request(u, buffer);
   };
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float4v acc[TM] = {};
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  float4v acc[TM][TN] = {};
   if (depth > 0) {
 #pragma unroll
-    for (int s = 0; s < kFewStages - 1; ++s) request(depth - s * kDepth<T>, s);
-    int buffer = 0, fill = kFewStages - 1;
+    for (int s = 0; s < STAGES - 1; ++s) request(depth - s * kDepth<T>, s);
+    int buffer = 0, fill = STAGES - 1;
     for (int k0 = 0; k0 < depth; k0 += kDepth<T>) {
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kFewStages - 2) * kLoads) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * kLoads) : "memory");
       // (past the end the loads give zeros, so that their number stays what is waited for)
-      request(depth - k0 - (kFewStages - 1) * kDepth<T>, fill);
-      const char *x_tile = s_tiles + buffer * Left::kBytes, *y_tile = s_tiles + kFewStages * Left::kBytes + buffer * Right::kBytes;
+      request(depth - k0 - (STAGES - 1) * kDepth<T>, fill);
+      const char *x_tile = s_tiles + buffer * Left::kBytes, *y_tile = s_tiles + STAGES * Left::kBytes + buffer * Right::kBytes;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const fragment ys = Right::fragment(y_tile + Right::place(wave * 16, half));
+        fragment ys[TN];
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
-          acc[i] = Fragment<T>::mma(ys, Left::fragment(x_tile + Left::place(i * 16, half)), acc[i]);
+        for (int j = 0; j < TN; ++j) ys[j] = Right::fragment(y_tile + Right::place(wn + j * 16, half));
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const fragment xs = Left::fragment(x_tile + Left::place(wm + i * 16, half));
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] = Fragment<T>::mma(ys[j], xs, acc[i][j]);
+        }
       }
-      buffer = buffer + 1 == kFewStages ? 0 : buffer + 1;
-      fill = fill + 1 == kFewStages ? 0 : fill + 1;
+      buffer = buffer + 1 == STAGES ? 0 : buffer + 1;
+      fill = fill + 1 == STAGES ? 0 : fill + 1;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
-  const int n = wave * 16 + (lane >> 4) * 4;
-  if (n >= width) return;
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    const int m = i * 16 + (lane & 15);
-    const float v[4] = {acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
-    if (m < t.rows) storeFloats<T, 4>(out + (int64_t)(t.first + m) * columns + n0 + n, v);
+    const int m = wm + i * 16 + (lane & 15);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = wn + j * 16 + (lane >> 4) * 4;
+      const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+      if (m < t.rows && n < width) storeFloats<T, 4>(out + (int64_t)(t.first + m) * columns + n0 + n, v);
+    }
   }
 }
 
@@ -1018,8 +1025,8 @@ struct Tile {
 constexpr int kTileKinds = 3;
 // Steps of the reduction from which on a last round that 256 x 256 tiles fill to a quarter or less is left for 128 x 128 ones.  Its
 // tiles take a whole round's time otherwise; an empty launch takes 2 us.  2048 columns of fp16, us of 33 / 40 / 48 tiles an XCD
-// (32 workgroups) without and with this: 8 steps 37 / 36 / 38 either way, 16 steps 58 / 57 / 59 and 51 / 53 / 59, 64 steps 180 / 180 / 182
-// and 152 / 156 / 182.
+// (32 workgroups) without and with this: 8 steps 37 / 36 / 38 either way, 16 steps 58 / 57 / 59 and 52 / 54 / 58, 64 steps 180 / 180 / 182
+// and 153 / 156 / 183.
 constexpr int kRestSteps = 16;
 // Bytes of results from which on 256 x 256 tiles are stored past the caches, which then keep the operands: 82 MB 177 -> 158 us, 134 MB
 // 268 -> 250; 31 MB 34 -> 38.
@@ -1193,7 +1200,7 @@ hipError_t launchTiles(const LaunchCtx &lc, const Problem &p, Args a, int cu_cou
   constexpr int BM = kTiles[TILE].m, BN = kTiles[TILE].n;
   constexpr size_t kLds = (size_t)2 * (BM + BN) * 128;
   static_assert((kLds + kStartsInLds * 4 + kRanked * 6 + kSharedBlocks * 4 + 4) * kTiles[TILE].per_cu <= 160 * 1024, "LDS of a CU");
-  auto kernel = groupedTiles<T, MODE, BM, BN, WM, WN, false>;
+  auto kernel = groupedTiles<T, MODE, BM, BN, WM, WN>;
   const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
   if (allowed != hipSuccess) return allowed;
@@ -1222,14 +1229,14 @@ hipError_t launchTiles(const LaunchCtx &lc, const Problem &p, Args a, int cu_cou
   lc.end();
   if constexpr (MODE != kBackwardFilter && TILE == 0) {
     if (a.wide > 0) {
-      constexpr size_t kRestLds = kLds / 2;
-      auto rest = groupedTiles<T, MODE, BM / 2, BN / 2, 2, 2, true>;
+      constexpr size_t kRestLds = (size_t)kRestStages * (BM + BN) / 2 * 128;
+      auto rest = groupedFew<T, MODE, BM / 2, BN / 2, 2, 2, kRestStages, true>;
       const hipError_t fits = hipFuncSetAttribute(reinterpret_cast<const void *>(rest),
                                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)kRestLds);
       if (fits != hipSuccess) return fits;
       a.works = (int)std::min<int64_t>(4 * works, 8 * 4 * (a.wide / 4));
-      lc.begin("groupedTilesRest");
-      rest<<<a.works, 256, kRestLds, lc.stream>>>(static_cast<const T *>(p.left), static_cast<const T *>(p.right), a,
+      lc.begin("groupedRest");
+      rest<<<a.works, kFewWaves * 64, kRestLds, lc.stream>>>(static_cast<const T *>(p.left), static_cast<const T *>(p.right), a,
                                                   static_cast<T *>(p.out));
       lc.end();
     }
@@ -1241,7 +1248,7 @@ hipError_t launchTiles(const LaunchCtx &lc, const Problem &p, Args a, int cu_cou
 template <typename T, int MODE, int BM>
 hipError_t launchFew(const LaunchCtx &lc, const Problem &p, const Args &a) {
   constexpr size_t kLds = (size_t)kFewStages * (BM + kFewColumns) * 128;
-  auto kernel = groupedFew<T, MODE, BM>;
+  auto kernel = groupedFew<T, MODE, BM, kFewColumns, 1, kFewWaves, kFewStages, false>;
   const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
   if (allowed != hipSuccess) return allowed;

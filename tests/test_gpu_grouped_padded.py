@@ -124,3 +124,26 @@ def test_starts_that_make_no_sense(gpu_handle, rows, ci, co):
     want = products(x, w, dy, good.tolist())
     assert torch.equal(mluop_hip.grouped_matmul_forward(gpu_handle, x, w, good), want[0])
     assert torch.equal(mluop_hip.grouped_matmul_backward_filter(gpu_handle, x, dy, good), want[2])
+
+
+@pytest.mark.parametrize("sizes,behind", [([8448], 0), ([8192], 0), ([9000, 1], 0), ([4000, 300, 0, 4100], 100), ([8300, 900], 3)])
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+def test_a_last_round_that_is_nearly_empty(gpu_handle, dtype, sizes, behind):
+    """tiles of 256 x 256 fill 256 CUs once and a little of a second time"""
+    import torch
+    import mluop_hip
+    print("grouped rest", dtype, sizes, flush=True)
+    t = getattr(torch, dtype)
+    starts = [0]
+    for n in sizes:
+        starts.append(starts[-1] + n)
+    rows, ci, co = starts[-1] + behind, 1032, 2048
+    x, w, dy = (whole_numbers((rows, ci), -2, 2, t, 9), whole_numbers((len(sizes), ci, co), -1, 1, t, 10),
+                whole_numbers((rows, co), -1, 1, t, 11))
+    dev = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    want = products(x, w, dy, starts)
+    got, names = launched(gpu_handle, lambda: mluop_hip.grouped_matmul_forward(gpu_handle, x, w, dev))
+    if dtype == "float16" and sizes == [8448]:
+        assert names == ["groupedTiles256", "groupedRest"]
+    assert torch.equal(got, want[0])
+    assert torch.equal(mluop_hip.grouped_matmul_backward_data(gpu_handle, dy, w, dev), want[1])
