@@ -227,7 +227,7 @@ struct Sorted {
   bool streamed;
 };
 
-// out[row] = scale * (the gradients of the row's words, in ascending place, in fp32).  Bound by memory: 131 072 x 2048 bf16 from 65 536
+// out[row] = scale * (the gradients of the row's words, added up in fp32 in an order that the words decide).  Bound by memory: 131 072 x 2048 bf16 from 65 536
 // tokens (805 MB) 140 us, 5.7 TB/s.
 // The first row_blocks workgroups own rows of the table.  The others take a piece each: of the rows that are longer than
 // one, at most two reach into it, that of its first word and that of its last.
