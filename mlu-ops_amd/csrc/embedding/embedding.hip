@@ -39,8 +39,8 @@ struct Tokens {
 
 // ---- forward -------------------------------------------------------------------------------
 
-// out[t] = scale * table[token t], in one pass; bound by memory, or by the launch where there is little: 240 612 rows of 512 fp16 (247 MB)
-// 36 us, 64 rows of 1024 bf16 5.6.
+// out[t] = scale * table[token t], in one pass; bound by memory, or by the launch where there is little: 240 612 rows of 512
+// fp16 (247 MB) 36 us, 64 rows of 1024 bf16 5.6.
 constexpr int kRowsAThread = 4;  // whose loads are in flight together
 
 template <typename T, int V>
@@ -82,8 +82,8 @@ __global__ __launch_bounds__(kThreads) void embeddingRows(const T *__restrict__ 
 // each piece is summed by a workgroup of its own, and a last launch adds the pieces.
 
 // Whether all rows of threads of a workgroup share a row of the table: one that is named often, as all are in a small table.
-// us of the gradient of 5000 x 64 bf16 without / with this: named 8 times on average 38 / 42, 16 times 41 / 44, 32 times 55 / 47, 64 times
-// 75 / 52; 517 x 64 fp32, 232 times, 47 / 31.
+// us of the gradient of 5000 x 64 bf16 without / with this: named 8 times on average 38 / 42, 16 times 41 / 44, 32 times 55 / 47,
+// 64 times 75 / 52; 517 x 64 fp32, 232 times, 47 / 31.
 bool rowsShared(int64_t n, int64_t rows, int64_t channels) { return n >= 24 * rows && channels < 1024; }
 
 // Words of a piece: as many as the rows of threads of a workgroup (which V = 4 has) read at once, eight each, where they
@@ -227,8 +227,8 @@ struct Sorted {
   bool streamed;
 };
 
-// out[row] = scale * (the gradients of the row's words, added up in fp32 in an order that the words decide).  Bound by memory: 131 072 x 2048 bf16 from 65 536
-// tokens (805 MB) 140 us, 5.7 TB/s.
+// out[row] = scale * (the gradients of the row's words, added up in fp32 in an order that the words decide).  Bound by memory:
+// 131 072 x 2048 bf16 from 65 536 tokens (805 MB) 140 us, 5.7 TB/s.
 // The first row_blocks workgroups own rows of the table.  The others take a piece each: of the rows that are longer than
 // one, at most two reach into it, that of its first word and that of its last.
 // SHARED: a row of the table a workgroup, whose rows of threads share the words.

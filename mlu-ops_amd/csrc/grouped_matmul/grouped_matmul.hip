@@ -67,7 +67,8 @@ struct Args {
   int blocks;       // backward filter: slices there can be,
   int slots;        // and how many there can be of groups of more than one, whose sums go to `partial`
   int works;        // numbers of works (some of which may not be there)
-  int wide;         // of tiles of rows: workgroups of an XCD whose last round, filled to a quarter or less, is left for smaller tiles; or 0
+  int wide;         // of tiles of rows: an XCD's workgroups, whose last round is left for smaller tiles where they fill a quarter
+                    // of it or less; or 0
   bool streamed;    // results go past the caches
   float *partial;   // backward filter: sums [slot, ci, co]
 };
@@ -305,8 +306,8 @@ __global__ __launch_bounds__(kAnyThreads) void groupedAny(const T *__restrict__ 
 // of fp32), which loads fill directly, 16 bytes a lane.  An operand that memory has along the reduction lies in LDS as
 // [result][step], and a fragment is one 16-byte read.  One that memory has along the results lies as [step][results]:
 // 2-byte elements are transposed by `ds_read_b64_tr_b16` (within 16 lanes, lane i gives the address of four results of the
-// reduction's part i / 4, and lane j receives result j of the four parts), fp32 ones are read one by one.  Either way rows are a multiple of the banks apart,
-// and their 16-byte pieces are permuted by row so that the lanes of a read meet all banks; the loads permute, since a
+// reduction's part i / 4, and lane j receives result j of the four parts), fp32 ones are read one by one.  Either way rows are a
+// multiple of the banks apart, and their 16-byte pieces are permuted by row so that the lanes of a read meet all banks; the loads permute, since a
 // lane's place in LDS is fixed.
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -478,7 +479,8 @@ __device__ __forceinline__ RaggedTile tileOfRows(const RowTiles &all, int xcd, i
 // In which order a workgroup takes its works (in LDS; NULL: by number).
 struct Order {
   const uint16_t *longest;  // blocks (groups, or slices of their rows) by falling length
-  const uint16_t *taken;    // this workgroup's share of what does not fill a round of its XCD: [place in `longest`, tile of the XCD's]; or NULL
+  const uint16_t *taken;    // or NULL: this workgroup's share of what does not fill a round of its XCD, pairs of a place in `longest`
+                            // and a tile of the XCD's
   int whole;                // rounds that an XCD's tiles of every block make
   int blocks;               // that there are
 };
@@ -679,7 +681,8 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
   constexpr int kSlots = 2 * TM, kLoads = Left::kLoads + Right::kLoads, kAtOnce = (2 * kLoads + kSlots - 1) / kSlots;
   static_assert(TM >= 2 && kAtOnce * (kSlots - 2) >= kLoads, "all loads are requested in front of the slots that wait for them");
   static_assert(TN % 2 == 0, "columns are stored two blocks at once");
-  constexpr int kStores = sizeof(T) == 2 ? TM * TN / 2 : TM * TN;  // (partial sums of 2-byte types take twice as many: the wait is for some of them too)
+  // (partial sums of 2-byte types take twice as many: the wait is for some of them too)
+  constexpr int kStores = sizeof(T) == 2 ? TM * TN / 2 : TM * TN;
   Left x(left, 0, 1, s_tiles);
   Right y(right, 0, 1, s_tiles + 2 * Left::kBytes);
   auto request = [&](int slot, int buffer) {  // slot: since the wait
@@ -1025,8 +1028,8 @@ struct Tile {
 constexpr int kTileKinds = 3;
 // Steps of the reduction from which on a last round that 256 x 256 tiles fill to a quarter or less is left for 128 x 128 ones.  Its
 // tiles take a whole round's time otherwise; an empty launch takes 2 us.  2048 columns of fp16, us of 33 / 40 / 48 tiles an XCD
-// (32 workgroups) without and with this: 8 steps 37 / 36 / 38 either way, 16 steps 58 / 57 / 59 and 52 / 54 / 58, 64 steps 180 / 180 / 182
-// and 153 / 156 / 183.
+// (32 workgroups) without and with this: 8 steps 37 / 36 / 38 either way, 16 steps 58 / 57 / 59 and 52 / 54 / 58, 64 steps
+// 180 / 180 / 182 and 153 / 156 / 183.
 constexpr int kRestSteps = 16;
 // Bytes of results from which on 256 x 256 tiles are stored past the caches, which then keep the operands: 82 MB 177 -> 158 us, 134 MB
 // 268 -> 250; 31 MB 34 -> 38.
@@ -1384,8 +1387,8 @@ hipError_t launchPadded(const LaunchCtx &lc, const Problem &p, Padded d, int cu_
   Copy back = {};
   if (d.out) {
     back = filter ? copyOf(p.out, workspace, p.co, p.groups, p.ci, q.ci, p.co, q.co, kSize, false)
-                  : copyOf(p.out, workspace, forward ? p.co : p.ci, 1, p.rows, p.rows, forward ? p.co : p.ci, forward ? q.co : q.ci, kSize,
-                           false);
+                  : copyOf(p.out, workspace, forward ? p.co : p.ci, 1, p.rows, p.rows, forward ? p.co : p.ci,
+                           forward ? q.co : q.ci, kSize, false);
     q.out = workspace;
     workspace += d.out_bytes;
   }
