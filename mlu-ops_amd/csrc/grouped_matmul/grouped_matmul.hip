@@ -3,8 +3,8 @@
 //   groupedTiles  rows in whole 16-byte pieces; bound by the matrix cores and, long and large, by the power they draw (the same
 //                 product of zeros is faster).  32 768 rows, 8 x 2048 x 8192 bf16: forward 1.00 ms (1.10 PFLOP/s), backward data
 //                 0.95 (1.16), filter gradient 0.87 (1.26), where a large library product has 1.24.
-//   groupedFew    the same with few rows a group; bound by the filters' way from memory: 12 rows of ten of 32 experts, 1024 x 2048
-//                 bf16 (42 MB) 11.0 us, 3.8 TB/s with what a launch costs.
+//   groupedFew    the same with few rows a group or few tiles; bound by the filters' way from memory: 12 rows of ten of 32 experts,
+//                 1024 x 2048 bf16 (42 MB) 9.6 us, 4.4 TB/s with what a launch costs.
 //   groupedAny    any shape and stride; bound by the step from load to LDS to multiply, some 2 us of 64.
 #include <hip/hip_runtime.h>
 
@@ -816,11 +816,11 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// One tile a workgroup, and STAGES steps of both sides on their way: for few rows a group, where the filters are what is read, and
+// One tile a workgroup, and STAGES steps of both sides on their way: for few rows or tiles, where the filters are what is read, and
 // for the last round that 256 x 256 tiles leave (REST: a quarter of such a tile each).  The kernel above has one step under
 // way, which a product that takes less than a way from memory for a step waits for again and again: 48 tiles of 64 steps left
 // over took 60 us in tiles of 128 x 128 of its own.
-constexpr int kFewColumns = 64, kFewStages = 6, kRestStages = 4, kFewWaves = 4;
+constexpr int kRestStages = 4, kFewWaves = 4;
 
 template <typename T, int MODE, int BM, int BN, int WM, int WN, int STAGES, bool REST>
 __global__ __launch_bounds__(kFewWaves * 64) void groupedFew(const T *__restrict__ left, const T *__restrict__ right, Args a,
@@ -1022,9 +1022,10 @@ struct Tile {
   double few, full, end;
   double forward, data;  // TB/s at which filters come in, forward and for backward data
 };
-// The first three are groupedTiles, the others groupedFew.  Measured (bf16, us at 256 x 256 / 128 x 128 / 64 x 128 / 32 x 64 / 16 x 64):
-// 16 rows of a 2048 x 2048 filter 39 / 19 / 14 / 9 / 8.5, 1000 rows 43 / 24 / 21 / 27 / 43, 4000 rows 47 / 36 / 48 / 95 / 158, 40 000
-// rows 288 / 365 / 524 / 895 / 1480.
+// The first two are groupedTiles, the others groupedFew; filter gradients take the first three, all of them groupedTiles.  Measured (fp16
+// forward of a 2048 x 2048 filter, us in this order): 16 rows 39 / 18 / 15 / 12 / 12 / 8.7 / 8.5, 500 rows 42 / 19 / 17 / 12.5 / 13 /
+// 15 / 24, 1000 rows 43 / 22 / 17.6 / 18.5 / 22 / 27 / 42, 4000 rows 50 / 38 / 51 / 68 / 70 / 89 / 148; bf16 40 000 rows 288 / 365 / 524
+// / - / - / 895 / 1480.
 constexpr int kTileKinds = 3;
 // Steps of the reduction from which on a last round that 256 x 256 tiles fill to a quarter or less is left for 128 x 128 ones.  Its
 // tiles take a whole round's time otherwise; an empty launch takes 2 us.  2048 columns of fp16, us of 33 / 40 / 48 tiles an XCD
@@ -1038,20 +1039,26 @@ constexpr double kStreamedResults = 64e6;
 // 16 x 1024 x 100 32 / 12, where the filter is all there is to copy; twelve rows of 32 x 100 x 2048 stay at 6.6, which two launches take.
 // Bytes a us of padded copies, and a launch of them.
 constexpr double kCopied = 3.0e6, kCopyLaunch = 4.0;
-// 64 filters of 2048 x 2048 for a row each: 121 / 95 / 97 / 119 / 119, and backward data, which reads their rows, 136 / 125 / 122 /
-// 102 / 102.
+// 64 filters of 2048 x 2048 for a row each: 122 / 95 / 100 / 122 / 103 / 119 / 119, and backward data, which reads their rows, 136 /
+// 125 / 116 / 111 / 104 / 102 / 101.
 constexpr Tile kTiles[] = {{"groupedTiles256", 256, 256, 1, 1.25, 1.65, 5.0, 4.4, 3.9},
                            {"groupedTiles128", 128, 128, 2, 0.59, 1.06, 2.5, 5.6, 4.3},
-                           {"groupedTiles64", 64, 128, 2, 0.43, 0.76, 2.0, 5.6, 4.3},
-                           {"groupedFew32", 32, kFewColumns, 2, 0.25, 0.40, 1.5, 5.2, 5.2},
-                           {"groupedFew16", 16, kFewColumns, 2, 0.22, 0.36, 1.5, 5.2, 5.2}};
-// fp32, whose steps are 32 deep: bound by the multiplies.  Forward of 2048 x 2048, us as above: 1000 rows 464 / 155 / 82 / 85 / 104,
-// 4000 rows 469 / 292 / 269 / 323 / 401, 16 000 rows 949 / 1077 / 1060 / 1258 / 1558 (141 TFLOP/s; a large library product has 154).
+                           {"groupedTiles64", 64, 128, 2, 0.43, 0.76, 2.0, 5.4, 4.6},
+                           {"groupedFew64x64", 64, 64, 2, 0.25, 0.55, 1.5, 4.4, 4.8},
+                           {"groupedFew32x128", 32, 128, 2, 0.28, 0.64, 1.5, 5.2, 5.1},
+                           {"groupedFew32", 32, 64, 2, 0.25, 0.40, 1.5, 4.5, 5.25},
+                           {"groupedFew16", 16, 64, 2, 0.22, 0.36, 1.5, 4.5, 5.3}};
+// fp32, whose steps are 32 deep: bound by the multiplies.  Forward of 2048 x 2048, us as above: 16 rows 460 / 149 / 74 / 45 / 44 / 27 /
+// 19, 1000 rows 461 / 149 / 81 / 79 / 78 / 83 / 103, 4000 rows 469 / 269 / 271 / 289 / 293 / 320 / 403; 16 000 rows 949 in the first
+// (141 TFLOP/s; a large library product has 154), 1077 in the second.  64 filters for a row each 931 / 527 / 277 / 295 / 207 / 233 / 216,
+// backward data 927 / 519 / 269 / 285 / 220 / 239 / 216.
 constexpr Tile kFloatTiles[] = {{"groupedTiles256", 256, 256, 1, 7.2, 7.0, 5.0, 4.4, 3.9},
                                 {"groupedTiles128", 128, 128, 2, 2.3, 4.3, 2.5, 5.6, 4.3},
-                                {"groupedTiles64", 64, 128, 2, 1.17, 2.1, 2.0, 5.6, 4.3},
-                                {"groupedFew32", 32, kFewColumns, 2, 0.42, 0.63, 1.5, 5.2, 5.2},
-                                {"groupedFew16", 16, kFewColumns, 2, 0.29, 0.39, 1.5, 5.2, 5.2}};
+                                {"groupedTiles64", 64, 128, 2, 1.17, 2.1, 2.0, 5.4, 4.6},
+                                {"groupedFew64x64", 64, 64, 2, 0.6, 1.1, 1.5, 4.4, 4.8},
+                                {"groupedFew32x128", 32, 128, 2, 0.7, 1.2, 1.5, 5.1, 4.9},
+                                {"groupedFew32", 32, 64, 2, 0.42, 0.63, 1.5, 4.6, 4.5},
+                                {"groupedFew16", 16, 64, 2, 0.29, 0.39, 1.5, 5.0, 5.0}};
 constexpr int kAllKinds = sizeof(kTiles) / sizeof(kTiles[0]);
 // the kernel of any shape
 constexpr Tile kAny = {"groupedAny", kAnyTile, kAnyTile, 4, 2.0, 3.3, 2.0, 3.0, 3.0};
@@ -1248,15 +1255,16 @@ hipError_t launchTiles(const LaunchCtx &lc, const Problem &p, Args a, int cu_cou
   return hipGetLastError();
 }
 
-template <typename T, int MODE, int BM>
-hipError_t launchFew(const LaunchCtx &lc, const Problem &p, const Args &a) {
-  constexpr size_t kLds = (size_t)kFewStages * (BM + kFewColumns) * 128;
-  auto kernel = groupedFew<T, MODE, BM, kFewColumns, 1, kFewWaves, kFewStages, false>;
+template <typename T, int MODE, int BM, int BN, int WM, int WN, int STAGES>
+hipError_t launchFew(const LaunchCtx &lc, const char *name, const Problem &p, const Args &a) {
+  constexpr size_t kLds = (size_t)STAGES * (BM + BN) * 128;
+  static_assert(kLds * 2 <= 160 * 1024, "two a CU");
+  auto kernel = groupedFew<T, MODE, BM, BN, WM, WN, STAGES, false>;
   const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
   if (allowed != hipSuccess) return allowed;
-  const int64_t tiles_n = tilesOf(MODE == kBackwardData ? p.ci : p.co, kFewColumns);
-  lc.begin(BM == 32 ? kTiles[3].name : kTiles[4].name);
+  const int64_t tiles_n = tilesOf(MODE == kBackwardData ? p.ci : p.co, BN);
+  lc.begin(name);
   const int64_t works = (mostRaggedTiles(p.rows, p.groups + 2, BM) * tiles_n + 7) / 8 * 8;
   if (works > INT32_MAX / 2) return hipErrorInvalidValue;
   kernel<<<(unsigned)works, kFewWaves * 64, kLds, lc.stream>>>(
@@ -1269,14 +1277,18 @@ template <typename T, int MODE>
 hipError_t launchPieces(const LaunchCtx &lc, const Problem &p, const Args &a, int cu_count) {
   const int tile = MODE == kBackwardFilter ? planFilter(p, cu_count).tile
                                            : planRows(p, sizeof(T) == 4 ? kFloatTiles : kTiles, kAllKinds, cu_count);
-  if constexpr (MODE != kBackwardFilter) {
-    if (tile == 3) return launchFew<T, MODE, 32>(lc, p, a);
-    if (tile == 4) return launchFew<T, MODE, 16>(lc, p, a);
-  }
-  switch (tile) {
-    case 0: return launchTiles<T, MODE, 0, 2, 4>(lc, p, a, cu_count);
-    case 1: return launchTiles<T, MODE, 1, 2, 2>(lc, p, a, cu_count);
-    default: return launchTiles<T, MODE, 2, 2, 2>(lc, p, a, cu_count);
+  if (tile == 0) return launchTiles<T, MODE, 0, 2, 4>(lc, p, a, cu_count);
+  if (tile == 1) return launchTiles<T, MODE, 1, 2, 2>(lc, p, a, cu_count);
+  if constexpr (MODE == kBackwardFilter) {
+    return launchTiles<T, MODE, 2, 2, 2>(lc, p, a, cu_count);
+  } else {
+    switch (tile) {
+      case 2: return launchFew<T, MODE, 64, 128, 2, 2, 3>(lc, "groupedFew64x128", p, a);
+      case 3: return launchFew<T, MODE, 64, 64, 2, 2, 4>(lc, kTiles[3].name, p, a);
+      case 4: return launchFew<T, MODE, 32, 128, 1, 4, 4>(lc, kTiles[4].name, p, a);
+      case 5: return launchFew<T, MODE, 32, 64, 1, 4, 6>(lc, kTiles[5].name, p, a);
+      default: return launchFew<T, MODE, 16, 64, 1, 4, 6>(lc, kTiles[6].name, p, a);
+    }
   }
 }
 

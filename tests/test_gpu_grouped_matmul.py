@@ -110,11 +110,11 @@ def launched(handle, call):
 KINDS = [  # groups, rows, ci, co, the kernels of the three products
     (3, 40, 512, 1032, ("groupedFew16", "groupedFew16", "groupedTiles")),
     (2, 700, 1024, 520, ("groupedFew", "groupedFew", "groupedTiles")),
-    (5, 1200, 2048, 2048, ("groupedTiles64", "groupedTiles64", "groupedTiles")),
+    (5, 1200, 2048, 2048, ("groupedFew64x128", "groupedFew64x128", "groupedTiles")),
     (1, 4100, 2056, 2048, ("groupedTiles128", "groupedTiles128", "groupedTiles")),
     (7, 16000, 1032, 1024, ("groupedTiles", "groupedTiles", "groupedTiles")),
     (1, 16000, 2048, 2048, ("groupedTiles256", "groupedTiles256", "groupedTiles256")),
-    (1, 30000, 64, 72, ("groupedTiles", "groupedTiles", "groupedTiles"))]
+    (1, 30000, 64, 72, ("groupedFew64", "groupedFew64", "groupedTiles"))]
 
 
 @pytest.mark.parametrize("groups,rows,ci,co,kinds", KINDS)
