@@ -123,7 +123,7 @@ __device__ __forceinline__ float blockMost(float v) {
 // zero it would leave eps alone in the denominator of the next step.  The parameters take the values in front of this rounding.
 // Bound by memory: 28 bytes an element with fp32 parameters, 10 with 16-bit parameters and 8-bit states.  Results go past the
 // caches (nobody reads a state before the next step): 130 M bf16 parameters with masters 757 -> 676 us (5.4 TB/s, where
-// a copy has 5.1), 250 M with 8-bit states 472 -> 458 us (5.5 TB/s), 33 fp32 tensors of 1.9 M elements in all 12.3 -> 10.8.
+// a copy has 5.1), 250 M with 8-bit states 472 -> 450 us (5.6 TB/s), 33 fp32 tensors of 1.9 M elements in all 12.3 -> 10.8.
 template <typename P, typename G, bool MASTER, bool EIGHT>
 __global__ __launch_bounds__(kThreads) void adamwStep(Tensors<MASTER, EIGHT> t, Hyper h) {
   typedef Tensors<MASTER, EIGHT> Table;
@@ -178,8 +178,9 @@ __global__ __launch_bounds__(kThreads) void adamwStep(Tensors<MASTER, EIGHT> t, 
     const float gi = g[i] * h.grad_scale;
     m[i] = m[i] * h.beta1 + gi * h.one_minus_beta1;
     v[i] = (EIGHT ? r[i] * r[i] : r[i]) * h.beta2 + gi * gi * h.one_minus_beta2;
-    // (the hardware's own root and reciprocal, one unit in the last place each)
-    r[i] = __builtin_amdgcn_sqrtf(v[i]);
+    // (the hardware's own reciprocal, one unit in the last place; and its own root too, but where codes are made of it: half a code
+    // on from there a unit decides between two of them, and the next step starts from it)
+    r[i] = EIGHT ? sqrtf(v[i]) : __builtin_amdgcn_sqrtf(v[i]);
     p[i] = p[i] * h.decay - h.step_size * (m[i] * __builtin_amdgcn_rcpf(r[i] * h.inv_root2 + h.eps));
   }
   if constexpr (MASTER) storeEight(master, at, n, whole, p);
@@ -194,8 +195,8 @@ __global__ __launch_bounds__(kThreads) void adamwStep(Tensors<MASTER, EIGHT> t, 
     }
     most_m = blockMost(most_m);
     most_r = blockMost(most_r);
-    const float by_m = most_m > 1e-30f ? kMostCode / most_m : 0.f;
-    const float by_r = most_r > 1e-30f ? kMostCode / most_r : 0.f;
+    const float by_m = most_m > 1e-30f ? 1.f / most_m * kMostCode : 0.f;
+    const float by_r = most_r > 1e-30f ? 1.f / most_r * kMostCode : 0.f;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
       m[i] = m[i] * by_m;

@@ -263,3 +263,43 @@ def test_refusals(gpu_handle):
     for more in (dict(step=0), dict(step=1, betas=(1.0, 0.9)), dict(step=1, eps=-1.0), dict(step=1, lr=math.nan)):
         with pytest.raises(mluop_hip.MluOpError):
             plan.step(gpu_handle, [t(4)], **{**HYPER, **more})
+
+
+def test_codes_are_those_of_plain_operations(gpu_handle):
+    """half a code on, one unit in the last place decides between two of them: codes and scales of two steps are the same as
+    of torch's operations, one after the other, in fp32"""
+    import torch
+    import mluop_hip
+    n, beta1, beta2, lr, eps = 8_000_000, 0.9, 0.95, 1e-3, 1e-8
+    g = torch.Generator(device="cuda").manual_seed(77)
+    master = torch.randn(n, device="cuda", generator=g) * 0.05
+    param, want = master.bfloat16(), master.clone()
+    m, v = (torch.zeros(n, dtype=torch.uint8, device="cuda") for _ in range(2))
+    ms, vs = (torch.zeros(n // 256, device="cuda") for _ in range(2))
+    plan = mluop_hip.AdamWTensors([param], [m], [v], [master], [ms], [vs])
+
+    def codes(x, root):
+        x = x.view(-1, 256)
+        most = x.abs().amax(dim=1, keepdim=True)
+        q = (x * (most.reciprocal() * 448.0)).to(torch.float8_e4m3fn)
+        if root:
+            f = q.float()
+            q = torch.where((f == 0) & (x > 0), torch.full_like(f, 2.0 ** -9), f).to(torch.float8_e4m3fn)
+        return q.view(-1), most.view(-1) * (1.0 / 448.0)
+
+    def values(q, scale):
+        return (q.float().view(-1, 256) * scale.unsqueeze(1)).view(-1)
+
+    mine = [torch.zeros(n, device="cuda").to(torch.float8_e4m3fn) for _ in range(2)]
+    scales = [torch.zeros(n // 256, device="cuda") for _ in range(2)]
+    for step in (1, 2):
+        grad = (torch.randn(n, device="cuda", generator=g) * 1e-2).bfloat16()
+        plan.step(gpu_handle, [grad], step, lr, (beta1, beta2), eps, 0.0)
+        d = grad.float()
+        a = values(mine[0], scales[0]) * beta1 + d * (1.0 - beta1)
+        r = torch.sqrt(values(mine[1], scales[1]).square() * beta2 + d * d * (1.0 - beta2))
+        want = want - lr / (1.0 - beta1 ** step) * (a / (r * (1.0 / (1.0 - beta2 ** step) ** 0.5) + eps))
+        (mine[0], scales[0]), (mine[1], scales[1]) = codes(a, False), codes(r, True)
+        for got, scale, q, s in ((m, ms, mine[0], scales[0]), (v, vs, mine[1], scales[1])):
+            assert torch.equal(got.view(torch.float8_e4m3fn).float(), q.float()) and torch.equal(scale, s)
+        assert float((master - want).abs().max()) < 1e-6 * step
