@@ -1,6 +1,7 @@
 // mluOpExtAdamWStep (no counterpart in the reference): one AdamW step over many tensors.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "core/core.h"
@@ -221,7 +222,7 @@ struct Step {
   int count;
   Hyper h;
 };
-constexpr int64_t kMostChunks = 1 << 30;
+constexpr int64_t kMostChunks = mostBlocks(kThreads);  // of a launch
 
 template <typename P, typename G, bool MASTER, bool EIGHT>
 mluOpStatus_t launchStep(const Step &step) {
@@ -250,8 +251,6 @@ mluOpStatus_t launchStep(const Step &step) {
   for (int i = 0; i < step.count; ++i) {
     const mluOpExtAdamWTensor_t &x = step.tensors[i];
     if (x.count == 0) continue;
-    const int64_t own = (x.count + kChunk - 1) / kChunk;
-    if (held == Table::kTensors || chunks + own > kMostChunks) HIP_CHECK_RETURN(step.api, launch());
     if (notes) {
       const int64_t blocks = (x.count + kStateBlock - 1) / kStateBlock;
       step.handle->forgetNotesIn(x.param, (size_t)x.count * sizeof(P));
@@ -263,19 +262,25 @@ mluOpStatus_t launchStep(const Step &step) {
         step.handle->forgetNotesIn(x.exp_avg_sq_scale, (size_t)blocks * 4);
       }
     }
-    t.address[Table::kParam][held] = x.param;
-    t.address[Table::kGrad][held] = const_cast<void *>(x.grad);  // (only read)
-    t.address[Table::kM][held] = x.exp_avg;
-    t.address[Table::kV][held] = x.exp_avg_sq;
-    if constexpr (MASTER) t.address[Table::kMaster][held] = x.master;
-    if constexpr (EIGHT) {
-      t.address[Table::kMScale][held] = x.exp_avg_scale;
-      t.address[Table::kVScale][held] = x.exp_avg_sq_scale;
+    // (a tensor of more chunks than a launch takes goes in several)
+    for (int64_t from = 0; from < x.count; from += kMostChunks * kChunk) {
+      const int64_t count = std::min(x.count - from, kMostChunks * kChunk), own = (count + kChunk - 1) / kChunk;
+      if (held == Table::kTensors || chunks + own > kMostChunks) HIP_CHECK_RETURN(step.api, launch());
+      auto at = [&](const void *p, size_t size) { return static_cast<char *>(const_cast<void *>(p)) + from * size; };
+      t.address[Table::kParam][held] = at(x.param, sizeof(P));
+      t.address[Table::kGrad][held] = at(x.grad, sizeof(G));  // (only read)
+      t.address[Table::kM][held] = at(x.exp_avg, EIGHT ? 1 : 4);
+      t.address[Table::kV][held] = at(x.exp_avg_sq, EIGHT ? 1 : 4);
+      if constexpr (MASTER) t.address[Table::kMaster][held] = at(x.master, 4);
+      if constexpr (EIGHT) {
+        t.address[Table::kMScale][held] = x.exp_avg_scale + from / kStateBlock;
+        t.address[Table::kVScale][held] = x.exp_avg_sq_scale + from / kStateBlock;
+      }
+      t.first[held] = chunks;
+      t.last[held] = (uint16_t)(count - (own - 1) * kChunk);
+      chunks += (uint32_t)own;
+      ++held;
     }
-    t.first[held] = chunks;
-    t.last[held] = (uint16_t)(x.count - (own - 1) * kChunk);
-    chunks += (uint32_t)own;
-    ++held;
   }
   HIP_CHECK_RETURN(step.api, launch());
   return MLUOP_STATUS_SUCCESS;
@@ -327,8 +332,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtAdamWStep(mluOpHandle_t handle, const mluOpE
     PARAM_CHECK(api, masters == (t.master != NULL));
     PARAM_CHECK(api, t.param != NULL && t.grad != NULL && t.exp_avg != NULL && t.exp_avg_sq != NULL);
     PARAM_CHECK(api, !eight || (t.exp_avg_scale != NULL && t.exp_avg_sq_scale != NULL));
-    if ((t.count - 1) / kChunk >= kMostChunks) {
-      MLUOP_LOG(ERROR) << api << " At most " << kMostChunks * kChunk << " elements of a tensor are supported.";
+    if (t.count > ((int64_t)1 << 46)) {
+      MLUOP_LOG(ERROR) << api << " At most 2^46 elements of a tensor are supported.";
       return MLUOP_STATUS_NOT_SUPPORTED;
     }
   }

@@ -5,9 +5,22 @@
 
 #include <hip/hip_runtime_api.h>
 
+#include <algorithm>
+#include <cstdint>
 #include <vector>
 
 namespace mluop {
+
+// Most workgroups of `threads` threads that a launch has along x: the threads are counted in 32 bits, and what goes beyond
+// is dropped without an error.  (In whole rounds of the eight XCDs.)
+constexpr int64_t mostBlocks(int threads) { return ((((int64_t)1 << 32) - 1) / threads) & ~(int64_t)7; }
+
+// Workgroups [0, blocks) in as many launches as they need: f(first, count) makes one.
+template <typename F>
+void inLaunches(int64_t blocks, int threads, F f) {
+  for (int64_t first = 0; first < blocks; first += mostBlocks(threads))
+    f(first, (unsigned)std::min(mostBlocks(threads), blocks - first));
+}
 
 struct KernelTimingRecord {
   const char *name;
