@@ -45,10 +45,11 @@ constexpr int kRowsAThread = 4;  // whose loads are in flight together
 
 template <typename T, int V>
 __global__ __launch_bounds__(kThreads) void embeddingRows(const T *__restrict__ table, int64_t row_stride, int channels,
-                                                          Tokens tokens, int64_t n, float scale, T *__restrict__ out) {
+                                                          Tokens tokens, int64_t n, float scale, int64_t first_block,
+                                                          T *__restrict__ out) {
   const Lanes<V> l(channels);
   if (l.row < 0) return;
-  const int64_t first = (int64_t)blockIdx.x * l.rows_at_once * kRowsAThread + l.row;
+  const int64_t first = (first_block + blockIdx.x) * l.rows_at_once * kRowsAThread + l.row;
   uint32_t row[kRowsAThread];
 #pragma unroll
   for (int j = 0; j < kRowsAThread; ++j) {
@@ -224,6 +225,7 @@ struct Sorted {
   const u64 *words;
   const uint32_t *starts;
   uint32_t n, rows, piece;
+  uint32_t first_block;  // of the launch, of all that its kernel has
   bool streamed;
 };
 
@@ -234,12 +236,13 @@ struct Sorted {
 // SHARED: a row of the table a workgroup, whose rows of threads share the words.
 template <typename T, int V, int kTableRows, bool SHARED>
 __global__ __launch_bounds__(kThreads) void embeddingGradRows(const T *__restrict__ grad, int64_t row_stride,
-                                                              int channels, Sorted s, float scale, int row_blocks,
+                                                              int channels, Sorted s, float scale, uint32_t row_blocks,
                                                               float *__restrict__ partial, T *__restrict__ out) {
   __shared__ float s_sum[kThreads * V];
+  const uint32_t block = s.first_block + blockIdx.x;
   const Lanes<V> l(channels);
-  if (SHARED && (int)blockIdx.x < row_blocks) {
-    const uint32_t row = blockIdx.x, begin = s.starts[row], end = s.starts[row + 1];
+  if (SHARED && block < row_blocks) {
+    const uint32_t row = block, begin = s.starts[row], end = s.starts[row + 1];
     if (end - begin > s.piece) return;
     float sum[V] = {};
     if (l.row >= 0) addRows<T, V>(grad, row_stride, s.words, begin + l.row, end, l.rows_at_once, l.channel, sum);
@@ -252,9 +255,9 @@ __global__ __launch_bounds__(kThreads) void embeddingGradRows(const T *__restric
     storeFloats<T, V>(out + (int64_t)row * channels + l.channel, sum, s.streamed);
     return;
   }
-  if ((int)blockIdx.x < row_blocks) {
+  if (block < row_blocks) {
     if (l.row < 0) return;
-    const uint32_t first = blockIdx.x * l.rows_at_once * kTableRows + l.row;
+    const uint32_t first = block * l.rows_at_once * kTableRows + l.row;
     uint32_t begin[kTableRows], end[kTableRows];
 #pragma unroll
     for (int j = 0; j < kTableRows; ++j) {
@@ -277,7 +280,7 @@ __global__ __launch_bounds__(kThreads) void embeddingGradRows(const T *__restric
     }
     return;
   }
-  const uint32_t piece = blockIdx.x - row_blocks;
+  const uint32_t piece = block - row_blocks;
   const uint32_t lo = piece * s.piece, hi = min(lo + s.piece, s.n);
   for (int side = 0; side < 2; ++side) {
     const uint32_t row = (uint32_t)(s.words[side == 0 ? lo : hi - 1] >> 32);
@@ -293,14 +296,14 @@ __global__ __launch_bounds__(kThreads) void embeddingGradRows(const T *__restric
   }
 }
 
-// Adds up the pieces of the long row that begins in piece blockIdx.x, if one does (only one can reach beyond its end).  A
+// Adds up the pieces of the long row that begins in a workgroup's own piece, if one does (only one can reach beyond its end).  A
 // wave's width of threads across the channels, so that the workgroup's rows of threads share the pieces.
 template <typename T, int V>
 __global__ __launch_bounds__(kThreads) void embeddingGradJoin(int channels, Sorted s, float scale,
                                                               const float *__restrict__ partial, T *__restrict__ out) {
   constexpr int kAhead = 4;
   __shared__ float s_sum[kThreads * V];
-  const uint32_t lo = blockIdx.x * s.piece, hi = min(lo + s.piece, s.n);
+  const uint32_t own = s.first_block + blockIdx.x, lo = own * s.piece, hi = min(lo + s.piece, s.n);
   const uint32_t row = (uint32_t)(s.words[hi - 1] >> 32);
   if (row >= s.rows) return;
   const uint32_t begin = s.starts[row], end = s.starts[row + 1];
@@ -311,13 +314,13 @@ __global__ __launch_bounds__(kThreads) void embeddingGradJoin(int channels, Sort
   float sum[V] = {};
   if (my_row >= 0) {
     const uint32_t last = (end - 1) / s.piece;
-    for (uint32_t p0 = blockIdx.x + my_row; p0 <= last; p0 += kAhead * rows) {
+    for (uint32_t p0 = own + my_row; p0 <= last; p0 += kAhead * rows) {
       Vector<float, V> v[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         const uint32_t p = min(p0 + j * rows, last);
         // (a row that begins with a piece's first word is that piece's first)
-        const int side = p == blockIdx.x && begin > lo ? 1 : 0;
+        const int side = p == own && begin > lo ? 1 : 0;
         v[j] = *reinterpret_cast<const Vector<float, V> *>(partial + ((int64_t)p * 2 + side) * channels + channel);
       }
 #pragma unroll
@@ -432,10 +435,12 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingForward(mluOpHandle_t handle, mluOp
     constexpr int V = decltype(v)::value;
     // (the last slab has fewer channels and more rows at once: its surplus workgroups find nothing)
     const int64_t per_block = (int64_t)rowsAtOnce(channels / V) * kRowsAThread;
-    lc.begin("embeddingRows");
-    embeddingRows<T, V><<<dim3((unsigned)((num_tokens + per_block - 1) / per_block), slabsOf(channels / V)), kThreads, 0, lc.stream>>>(
-        static_cast<const T *>(table), row_stride, (int)channels, t, num_tokens, scale, static_cast<T *>(out));
-    lc.end();
+    inLaunches((num_tokens + per_block - 1) / per_block, kThreads, [&](int64_t first, unsigned blocks) {
+      lc.begin("embeddingRows");
+      embeddingRows<T, V><<<dim3(blocks, slabsOf(channels / V)), kThreads, 0, lc.stream>>>(
+          static_cast<const T *>(table), row_stride, (int)channels, t, num_tokens, scale, first, static_cast<T *>(out));
+      lc.end();
+    });
   });
   HIP_CHECK_RETURN(api, hipGetLastError());
   return MLUOP_STATUS_SUCCESS;
@@ -509,8 +514,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingBackward(mluOpHandle_t handle, mluO
                                                                                                      words[0]);
   }
   if (num_tokens > 0) lc.end();
-  const Sorted s = {words[in_second ? 1 : 0], starts, (uint32_t)num_tokens, (uint32_t)rows, (uint32_t)p.piece,
-                    (size_t)rows * channels * elementBytes(type) >= kStreamedBytes};
+  Sorted s = {words[in_second ? 1 : 0], starts, (uint32_t)num_tokens, (uint32_t)rows, (uint32_t)p.piece, 0,
+              (size_t)rows * channels * elementBytes(type) >= kStreamedBytes};
   if (!started) {
     lc.begin("embeddingRowStarts");
     embeddingRowStarts<<<(unsigned)(rows / kThreads + 1), kThreads, 0, lc.stream>>>(s.words, s.n, s.rows, starts);
@@ -523,21 +528,27 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingBackward(mluOpHandle_t handle, mluO
            const int64_t at_once = rowsAtOnce(channels / V);
            const bool shared = rowsShared(num_tokens, rows, channels);
            const int each = tableRows(rows / at_once);
-           const int row_blocks = (int)(shared ? rows : (rows + at_once * each - 1) / (at_once * each));
+           const int64_t row_blocks = shared ? rows : (rows + at_once * each - 1) / (at_once * each);
            auto kernel = shared      ? embeddingGradRows<T, V, 1, true>
                          : each == 1 ? embeddingGradRows<T, V, 1, false>
                                      : embeddingGradRows<T, V, 4, false>;
-           lc.begin("embeddingGradRows");
-           kernel<<<dim3((unsigned)row_blocks + p.pieces, slabsOf(channels / V)), kThreads, 0, lc.stream>>>(
-               static_cast<const T *>(output_grad), row_stride, (int)channels, s, scale, row_blocks, partial,
-               static_cast<T *>(grad_table));
-           lc.end();
+           inLaunches(row_blocks + p.pieces, kThreads, [&](int64_t first, unsigned blocks) {
+             s.first_block = (uint32_t)first;
+             lc.begin("embeddingGradRows");
+             kernel<<<dim3(blocks, slabsOf(channels / V)), kThreads, 0, lc.stream>>>(
+                 static_cast<const T *>(output_grad), row_stride, (int)channels, s, scale, (uint32_t)row_blocks, partial,
+                 static_cast<T *>(grad_table));
+             lc.end();
+           });
            if (num_tokens <= p.piece) return;  // (no row can be longer)
-           lc.begin("embeddingGradJoin");
-           constexpr int W = V < 4 ? V : 4;
-           embeddingGradJoin<T, W><<<dim3(p.pieces, (unsigned)((channels / W + 63) / 64)), kThreads, 0, lc.stream>>>(
-               (int)channels, s, scale, partial, static_cast<T *>(grad_table));
-           lc.end();
+           inLaunches(p.pieces, kThreads, [&](int64_t first, unsigned blocks) {
+             constexpr int W = V < 4 ? V : 4;
+             s.first_block = (uint32_t)first;
+             lc.begin("embeddingGradJoin");
+             embeddingGradJoin<T, W><<<dim3(blocks, (unsigned)((channels / W + 63) / 64)), kThreads, 0, lc.stream>>>(
+                 (int)channels, s, scale, partial, static_cast<T *>(grad_table));
+             lc.end();
+           });
          });
   HIP_CHECK_RETURN(api, hipGetLastError());
   return MLUOP_STATUS_SUCCESS;

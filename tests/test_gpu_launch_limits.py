@@ -47,3 +47,37 @@ def test_adamw_of_a_tensor_longer_than_a_launch(handle):
         assert all_are(m, 0x7e) and all_are(r, 0x7e)
         want = float(torch.tensor(0.5) * torch.tensor(1.0 / 448.0))
         assert all_are(ms, want) and all_are(rs, want)
+
+
+def test_lookup_of_more_rows_than_a_launch(handle):
+    """four tokens a workgroup: 2^26 of them"""
+    import torch
+    import mluop_hip
+    room_for(24)
+    n, channels = (1 << 26) + 1003, 129
+    g = torch.Generator(device="cuda").manual_seed(3)
+    table = torch.randn(50, channels, device="cuda", generator=g).to(torch.bfloat16)
+    tokens = torch.randint(-1, 50, (n,), device="cuda", generator=g, dtype=torch.int32)
+    out = mluop_hip.embedding_forward(handle, table, tokens)
+    padded = torch.cat([table, torch.zeros_like(table[:1])])   # (-1: the last row)
+    same = all(torch.equal(out[at:at + (1 << 22)], padded[tokens[at:at + (1 << 22)].long()]) for at in range(0, n, 1 << 22))
+    assert same
+
+
+@pytest.mark.parametrize("rows,tokens", [((1 << 24) + 77, 24 * ((1 << 24) + 77)),   # a row of the table a workgroup
+                                         (30_000_000, (1 << 29) + 1001)])           # 2^24 pieces of 32 words
+def test_gradient_of_more_rows_than_a_launch(handle, rows, tokens):
+    import torch
+    import mluop_hip
+    room_for(40)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    t = torch.randint(0, rows, (tokens,), device="cuda", generator=g, dtype=torch.int32)
+    t[-5000:-1000], t[-1000:] = rows - 1, rows - 2   # rows longer than a piece, in the last pieces
+    t[:3000] = 1
+    grad = torch.randint(-2, 3, (tokens, 1), device="cuda", generator=g, dtype=torch.int8).to(torch.bfloat16)
+    got = mluop_hip.embedding_backward(handle, grad, t, rows)
+    want = torch.zeros(rows, device="cuda")
+    for at in range(0, tokens, 1 << 27):
+        want.index_add_(0, t[at:at + (1 << 27)], grad[at:at + (1 << 27), 0].float())
+    same = torch.equal(got[:, 0], want.to(torch.bfloat16))
+    assert same
