@@ -67,6 +67,7 @@ struct Args {
   int blocks;       // backward filter: slices there can be,
   int slots;        // and how many there can be of groups of more than one, whose sums go to `partial`
   int works;        // numbers of works (some of which may not be there)
+  int first_block;  // of the launch, of all that its kernel has
   int wide;         // of tiles of rows: an XCD's workgroups, whose last round is left for smaller tiles where they fill a quarter
                     // of it or less; or 0
   bool streamed;    // results go past the caches
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(kAnyThreads) void groupedAny(const T *__restrict__ 
   if (kFilter) {
     m0 = blockIdx.z * kAnyTile;
     extent = a.ci - m0;
-    const Slice slice = findSlice(a.starts, a, blockIdx.x);
+    const Slice slice = findSlice(a.starts, a, a.first_block + (int)blockIdx.x);
     if (slice.group < 0) return;
     group = slice.group;
     result = slice.slot < 0;
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(kAnyThreads) void groupedAny(const T *__restrict__ 
     l = left + slice.first * a.left_stride + m0;
     r = right + slice.first * a.right_stride + n0;
   } else {
-    const RaggedTile t = findRaggedTile<true>(a.starts, a.rows, a.groups, kAnyTile, blockIdx.x);
+    const RaggedTile t = findRaggedTile<true>(a.starts, a.rows, a.groups, kAnyTile, a.first_block + (int)blockIdx.x);
     if (t.segment < 0) return;
     group = t.segment - 1;
     extent = t.rows;
@@ -834,14 +835,15 @@ __global__ __launch_bounds__(kFewWaves * 64) void groupedFew(const T *__restrict
   extern __shared__ __attribute__((aligned(1024))) char s_tiles[];
 
   const int columns = MODE == kBackwardData ? a.ci : a.co;
-  int n0, in_xcd = blockIdx.x >> 3;
+  const int block = a.first_block + (int)blockIdx.x;  // (of an XCD as blockIdx.x is: launches begin at multiples of eight)
+  int n0, in_xcd = block >> 3;
   const RowTiles tiles = rowTilesOf<BM * kWhole>(a.starts, a, (columns + BN * kWhole - 1) / (BN * kWhole));
   if (REST) in_xcd = tiles.kept + in_xcd / 4;
-  RaggedTile t = tileOfRows<BM * kWhole>(tiles, blockIdx.x & 7, in_xcd, a.starts, a, &n0);
+  RaggedTile t = tileOfRows<BM * kWhole>(tiles, block & 7, in_xcd, a.starts, a, &n0);
   if (t.segment < 0) return;
   n0 *= BN * kWhole;
   if (REST) {
-    const int quarter = blockIdx.x >> 3 & 3, down = (quarter >> 1) * BM;
+    const int quarter = block >> 3 & 3, down = (quarter >> 1) * BM;
     n0 += (quarter & 1) * BN;
     if (down >= t.rows || n0 >= columns) return;
     t.first += down;
@@ -1186,12 +1188,16 @@ hipError_t sumSlices(const LaunchCtx &lc, const Problem &p, const Args &a) {
 template <typename T, int MODE>
 hipError_t launchAny(const LaunchCtx &lc, const Problem &p, const Args &a) {
   const unsigned across = tilesOf(MODE == kBackwardData ? p.ci : p.co, kAnyTile);
-  const dim3 grid = MODE == kBackwardFilter ? dim3((unsigned)a.blocks, across, tilesOf(p.ci, kAnyTile))
-                                            : dim3((unsigned)mostRaggedTiles(p.rows, p.groups + 2, kAnyTile), across, 1);
-  lc.begin(kAny.name);
-  groupedAny<T, MODE><<<grid, kAnyThreads, 0, lc.stream>>>(static_cast<const T *>(p.left), static_cast<const T *>(p.right), a,
-                                                           static_cast<T *>(p.out));
-  lc.end();
+  const int64_t blocks = MODE == kBackwardFilter ? a.blocks : mostRaggedTiles(p.rows, p.groups + 2, kAnyTile);
+  const unsigned down = MODE == kBackwardFilter ? tilesOf(p.ci, kAnyTile) : 1;
+  inLaunches(blocks, kAnyThreads, [&](int64_t first, unsigned count) {
+    Args part = a;
+    part.first_block = (int)first;
+    lc.begin(kAny.name);
+    groupedAny<T, MODE><<<dim3(count, across, down), kAnyThreads, 0, lc.stream>>>(
+        static_cast<const T *>(p.left), static_cast<const T *>(p.right), part, static_cast<T *>(p.out));
+    lc.end();
+  });
   if (MODE == kBackwardFilter && a.slice_rows > 0) return sumSlices<T>(lc, p, a);
   return hipGetLastError();
 }
@@ -1264,12 +1270,16 @@ hipError_t launchFew(const LaunchCtx &lc, const char *name, const Problem &p, co
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
   if (allowed != hipSuccess) return allowed;
   const int64_t tiles_n = tilesOf(MODE == kBackwardData ? p.ci : p.co, BN);
-  lc.begin(name);
   const int64_t works = (mostRaggedTiles(p.rows, p.groups + 2, BM) * tiles_n + 7) / 8 * 8;
   if (works > INT32_MAX / 2) return hipErrorInvalidValue;
-  kernel<<<(unsigned)works, kFewWaves * 64, kLds, lc.stream>>>(
-      static_cast<const T *>(p.left), static_cast<const T *>(p.right), a, static_cast<T *>(p.out));
-  lc.end();
+  inLaunches(works, kFewWaves * 64, [&](int64_t first, unsigned count) {
+    Args part = a;
+    part.first_block = (int)first;
+    lc.begin(name);
+    kernel<<<count, kFewWaves * 64, kLds, lc.stream>>>(
+        static_cast<const T *>(p.left), static_cast<const T *>(p.right), part, static_cast<T *>(p.out));
+    lc.end();
+  });
   return hipGetLastError();
 }
 
@@ -1365,7 +1375,7 @@ Copy copyOf(const void *at, void *copy, int64_t stride, int64_t blocks, int rows
 }
 
 Args argsOf(const Problem &p, int cu_count, void *partial) {
-  Args a = {p.rows, p.groups, p.ci, p.co, p.starts, p.left_stride, p.right_stride, 0, 0, 0, 0, 0, false, nullptr};
+  Args a = {p.rows, p.groups, p.ci, p.co, p.starts, p.left_stride, p.right_stride, 0, 0, 0, 0, 0, 0, false, nullptr};
   if (p.which == MLUOP_EXT_GROUPED_BACKWARD_FILTER) {
     a.slice_rows = planFilter(p, cu_count).slice_rows;
     a.blocks = p.groups + (a.slice_rows > 0 ? p.rows / a.slice_rows : 0);

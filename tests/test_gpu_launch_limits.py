@@ -81,3 +81,21 @@ def test_gradient_of_more_rows_than_a_launch(handle, rows, tokens):
         want.index_add_(0, t[at:at + (1 << 27)], grad[at:at + (1 << 27), 0].float())
     same = torch.equal(got[:, 0], want.to(torch.bfloat16))
     assert same
+
+
+def test_products_of_more_rows_than_a_launch(handle):
+    """64 rows a workgroup: 2^30 of them"""
+    import torch
+    import mluop_hip
+    room_for(16)
+    rows = (1 << 30) + 5000
+    x = torch.ones(rows, 1, dtype=torch.float16, device="cuda")
+    x[1::2] = 3.0
+    cut = (1 << 30) - 777
+    starts = torch.tensor([0, cut, rows - 9], dtype=torch.int32, device="cuda")
+    w = torch.tensor([2.0, -5.0], dtype=torch.float16, device="cuda").view(2, 1, 1)
+    for call in (mluop_hip.grouped_matmul_forward, mluop_hip.grouped_matmul_backward_data):
+        y = call(handle, x, w, starts)
+        for lo, hi, by in ((0, cut, 2), (cut, rows - 9, -5), (rows - 9, rows, 0)):
+            same = torch.equal(y[lo:hi], by * x[lo:hi])
+            assert same, (lo, hi)
