@@ -554,6 +554,7 @@ __global__ __launch_bounds__(kThreads) void groupNormGradApply(const T *__restri
 constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
 constexpr int kSmallRows = 4;         // of a thread
 constexpr int kSmallGradSamples = 4;  // taken one after the other
+constexpr int64_t kMostAlongY = 65535;  // workgroups of a grid
 
 // Sum over the lanes, in lane 63.
 __device__ __forceinline__ float waveSumAtLast(float v) {
@@ -617,11 +618,11 @@ __device__ __forceinline__ void smallOutside(const SmallLanes<V> &l, const Shape
 
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kSmallThreads) void groupNormSmall(const T *__restrict__ x, Shape s, Params p, float eps,
-                                                                int columns, float *__restrict__ mean,
+                                                                int columns, int first_sample, float *__restrict__ mean,
                                                                 float *__restrict__ rstd, T *__restrict__ out) {
   __shared__ float s_sum[kSmallWaves * V], s_mean[kSmallWaves * V], s_rstd[kSmallWaves * V];
   const SmallLanes<V> l(columns);
-  const int sample = blockIdx.y, per_group = s.channels / s.groups, slab = columns * V;
+  const int sample = first_sample + blockIdx.y, per_group = s.channels / s.groups, slab = columns * V;
   int first, rows;
   segmentRows(s.starts, s.rows, sample, &first, &rows);
   const int64_t at = (int64_t)first * s.channels + l.channel;
@@ -805,15 +806,19 @@ int smallColumns(const Shape &s, int v) {
   return s.rows <= kSmallRows * (kSmallThreads / columns) ? columns : 0;
 }
 
+constexpr int64_t kMostPairs = 15 << 20;
+
 mluOpStatus_t checkShape(const char *api, int64_t rows, int64_t channels, int64_t groups, int64_t samples) {
   PARAM_CHECK(api, rows >= 0);
   PARAM_CHECK(api, channels > 0);
   PARAM_CHECK(api, groups > 0);
   PARAM_CHECK(api, channels % groups == 0);
   PARAM_CHECK(api, samples > 0);
-  if (rows > INT32_MAX - 4096 || channels > (1 << 20) || samples > (1 << 20) || samples * groups > (1 << 28) ||
+  // (a pair, and four channels, have a workgroup each, in one launch)
+  static_assert(kMostPairs + (1 << 20) / kChannels <= mostBlocks(kThreads), "a grid's threads");
+  if (rows > INT32_MAX - 4096 || channels > (1 << 20) || samples > (1 << 20) || samples * groups > kMostPairs ||
       rows * channels > ((int64_t)1 << 46)) {
-    MLUOP_LOG(ERROR) << api << " At most 2^31 - 4097 rows, 2^20 channels, 2^20 samples, 2^28 pairs of a sample and a "
+    MLUOP_LOG(ERROR) << api << " At most 2^31 - 4097 rows, 2^20 channels, 2^20 samples, 15 * 2^20 pairs of a sample and a "
                      << "group and 2^46 values are supported.";
     return MLUOP_STATUS_NOT_SUPPORTED;
   }
@@ -920,11 +925,13 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGroupNormForward(mluOpHandle_t handle, mluOp
     const int columns = smallColumns(s, W);
     if (columns > 0) {
       byActivation(activation, [&](auto act) {
-        lc.begin("groupNormSmall");
-        groupNormSmall<T, W, decltype(act)::value><<<dim3(s.channels / (columns * W), (unsigned)samples), kSmallThreads, 0,
-                                                     lc.stream>>>(static_cast<const T *>(features), s, p, eps, columns,
-                                                                  mean, rstd, static_cast<T *>(out));
-        lc.end();
+        for (int64_t first = 0; first < samples; first += kMostAlongY) {
+          const unsigned count = (unsigned)std::min(samples - first, kMostAlongY);
+          lc.begin("groupNormSmall");
+          groupNormSmall<T, W, decltype(act)::value><<<dim3(s.channels / (columns * W), count), kSmallThreads, 0, lc.stream>>>(
+              static_cast<const T *>(features), s, p, eps, columns, (int)first, mean, rstd, static_cast<T *>(out));
+          lc.end();
+        }
       });
       return;
     }

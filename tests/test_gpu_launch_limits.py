@@ -30,6 +30,34 @@ def handle(gpu_handle):
         torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("groups,channels,act", [(2, 8, "none"), (1, 3, "silu")])
+def test_group_norm_of_very_many_samples(gpu_handle, groups, channels, act):
+    """few rows in more samples than a grid has workgroups along y; most samples are empty"""
+    import torch
+    import mluop_hip
+    rows, samples = 1000, 70_001
+    g = torch.Generator(device="cuda").manual_seed(channels)
+    x = torch.randn(rows, channels, device="cuda", generator=g)
+    dy = torch.randn(rows, channels, device="cuda", generator=g)
+    w = 1 + 0.3 * torch.randn(channels, device="cuda", generator=g)
+    b = 0.3 * torch.randn(channels, device="cuda", generator=g)
+    cuts = torch.randint(0, rows // 4, (samples - 1,), device="cuda", generator=g).sort().values * 4
+    starts = torch.cat([torch.zeros_like(cuts[:1]), cuts, torch.full_like(cuts[:1], rows)]).to(torch.int32)
+    filled = starts[1:] > starts[:-1]
+    assert bool((starts[1:] - starts[:-1]).max() >= 4) and int(filled.sum()) > 100
+    own = torch.cat([starts[:-1][filled], starts[-1:]])   # the same without samples of no rows
+    out, mean, rstd = mluop_hip.group_norm_forward(gpu_handle, x, w, b, groups, starts, 1e-5, act)
+    ref, ref_mean, ref_rstd = mluop_hip.group_norm_forward(gpu_handle, x, w, b, groups, own, 1e-5, act)
+    # (few rows and samples, and what they are with many, may be added up by different kernels)
+    assert torch.allclose(out, ref, atol=1e-4) and torch.allclose(mean[filled], ref_mean, atol=1e-5)
+    assert torch.allclose(rstd[filled], ref_rstd, rtol=1e-4) and not bool(mean[~filled].any())
+    assert torch.allclose(rstd[~filled], torch.tensor(1e-5 ** -0.5, device="cuda"))
+    got = mluop_hip.group_norm_backward(gpu_handle, dy, x, w, b, mean, rstd, groups, starts, act)
+    want = mluop_hip.group_norm_backward(gpu_handle, dy, x, w, b, ref_mean, ref_rstd, groups, own, act)
+    for a, c in zip(got, want):
+        assert torch.allclose(a, c, rtol=1e-3, atol=1e-3 * float(c.abs().max()))
+
+
 def test_adamw_of_a_tensor_longer_than_a_launch(handle):
     """2^24 workgroups of 2048 elements, behind a small tensor; the gradient is the parameter itself, which is read first"""
     import torch
