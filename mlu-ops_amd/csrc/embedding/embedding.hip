@@ -490,8 +490,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingBackward(mluOpHandle_t handle, mluO
   const mluop::LaunchCtx lc = handle->launchCtx();
   const Tokens names(tokens, token_type, rows);
   bool in_second = false, started = false;
-  if (num_tokens > 0) lc.begin("embeddingSort");
   if (num_tokens > rankedTokens((p.bits + p.pass_bits - 1) / p.pass_bits)) {
+    lc.begin("embeddingSort");
     const bool few = device_sort::tilesFor(num_tokens) <= device_sort::kFewTiles;
     const int digits = device_sort::sortDigits(p.pass_bits);
     const uint32_t mask = (1u << p.pass_bits) - 1u;
@@ -509,11 +509,13 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingBackward(mluOpHandle_t handle, mluO
       HIP_CHECK_RETURN(api, pass(items));
       in_second = !in_second;
     }
+    lc.end();
   } else if (num_tokens > 0) {
+    lc.begin("embeddingRankWords");
     embeddingRankWords<<<(unsigned)((num_tokens + kRanked - 1) / kRanked), kThreads, 0, lc.stream>>>(names, (uint32_t)num_tokens,
                                                                                                      words[0]);
+    lc.end();
   }
-  if (num_tokens > 0) lc.end();
   Sorted s = {words[in_second ? 1 : 0], starts, (uint32_t)num_tokens, (uint32_t)rows, (uint32_t)p.piece, 0,
               (size_t)rows * channels * elementBytes(type) >= kStreamedBytes};
   if (!started) {
