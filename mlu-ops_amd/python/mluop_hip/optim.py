@@ -30,6 +30,10 @@ class AdamW(torch.optim.Optimizer):
                                       min_8bit_size=int(min_8bit_size)))
         self._plans = {}
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plans = {}   # (of what a copy was made from; torch copies groups and states only)
+
     def _state_of(self, p, group):
         state = self.state[p]
         if not state:

@@ -1,0 +1,94 @@
+"""The AdamW optimizer over its life: copied and pickled, parameters that miss gradients, calls that are refused, parameters whose
+memory is laid out anew, gradients that are not finite, roots below the smallest normal number, and autograd's view of what a
+step has changed."""
+import copy
+import io
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+HYPER = dict(lr=1e-2, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.03)
+
+
+def parameters(seed=0, dtype=None, sizes=(10, 9000, 300)):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.nn.Parameter(torch.randn(n, device="cuda", generator=g).to(dtype or torch.float32)) for n in sizes]
+
+
+def give_gradients(params, seed, missing=()):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    for i, p in enumerate(params):
+        grad = torch.randn(p.shape, device="cuda", generator=g).to(p.dtype)
+        p.grad = None if i in missing else grad
+
+
+@pytest.mark.parametrize("way", ["deepcopy", "pickle"])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_copy_goes_on(way, bits):
+    import torch
+    from mluop_hip.optim import AdamW
+    a = parameters()
+    opt = AdamW(a, state_bits=bits, **HYPER)
+    give_gradients(a, 1)
+    opt.step()
+    if way == "deepcopy":
+        b, twin = copy.deepcopy((a, opt))
+    else:
+        buffer = io.BytesIO()
+        torch.save((a, opt), buffer)
+        buffer.seek(0)
+        b, twin = torch.load(buffer, weights_only=False)   # (written above)
+    for params, o in ((a, opt), (b, twin)):
+        give_gradients(params, 2)
+        o.step()
+    assert twin.param_groups[0]["params"][0] is b[0]
+    for p, q in zip(a, b):
+        assert p is not q and torch.equal(p, q)
+
+
+class Counted:
+    """the class of checked tensors, counting how many are made"""
+
+    def __init__(self, real):
+        self.real, self.made = real, 0
+
+    def __call__(self, *args):
+        self.made += 1
+        return self.real(*args)
+
+
+@pytest.mark.parametrize("bits,master,most", [(32, False, 106), (32, True, 87), (8, False, 74), (8, True, 65)])
+@pytest.mark.parametrize("count", ["below", "full", "above", "twice"])
+def test_tensors_around_a_launch(gpu_handle, bits, master, most, count):
+    """every tensor gets the step it gets alone, however many launches they fill"""
+    import torch
+    import mluop_hip
+    tensors = {"below": most - 1, "full": most, "above": most + 1, "twice": 2 * most + 3}[count]
+    g = torch.Generator(device="cuda").manual_seed(tensors)
+    sizes = [(37 * i) % 700 + 1 if i % 9 else 2048 * (i // 9 % 3) + 2047 for i in range(tensors)]
+    dtype = torch.bfloat16 if master else torch.float32
+    params = [torch.randn(n, device="cuda", generator=g).to(dtype) for n in sizes]
+    grads = [torch.randn(n, device="cuda", generator=g).to(dtype) for n in sizes]
+
+    def lists(params):
+        states = [[torch.zeros(p.numel(), device="cuda") if bits == 32 else
+                   torch.zeros(p.numel(), dtype=torch.uint8, device="cuda") for p in params] for _ in range(2)]
+        scales = [[torch.zeros(-(-p.numel() // 256), device="cuda") for p in params] for _ in range(2)]
+        return (params, *states, [p.float() for p in params] if master else None, *(scales if bits == 8 else (None, None)))
+    together, alone = lists([p.clone() for p in params]), lists([p.clone() for p in params])
+    plan = mluop_hip.AdamWTensors(*together)
+    gpu_handle.set_kernel_timing(True)
+    try:
+        plan.step(gpu_handle, grads, 1, **HYPER)
+        names = [name for name, _ in gpu_handle.kernel_timings()]
+    finally:
+        gpu_handle.set_kernel_timing(False)
+    assert names == ["adamwStep"] * (1 if tensors <= most else 2 if tensors <= 2 * most else 3)
+    for i in range(tensors):
+        mluop_hip.AdamWTensors(*[None if x is None else x[i:i + 1] for x in alone]).step(gpu_handle, grads[i:i + 1], 1, **HYPER)
+    for a, b in zip(together, alone):
+        if a is not None:
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
