@@ -60,6 +60,34 @@ class Counted:
         return self.real(*args)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_that_miss_gradients_keep_their_plans(bits, monkeypatch):
+    """step counts of one group fall apart, and a step checks no tensor anew for that"""
+    import torch
+    from mluop_hip import optim
+    counted = Counted(optim.AdamWTensors)
+    monkeypatch.setattr(optim, "AdamWTensors", counted)
+    missing = {2: (0,), 3: (1,), 5: (0, 2), 7: (0, 1, 2)}
+    a = parameters()
+    opt = optim.AdamW(a, state_bits=bits, **HYPER)
+    b = parameters()
+    each = [optim.AdamW([p], state_bits=bits, **HYPER) for p in b]
+    for k in range(10):
+        give_gradients(a, k, missing.get(k, ()))
+        give_gradients(b, k, missing.get(k, ()))
+        if k == 1:
+            counted.made = 0
+        opt.step()
+        if k >= 1:
+            assert counted.made == 0, k
+        for o in each:
+            o.step()
+        counted.made = 0
+    assert [opt.state[p]["step"] for p in a] == [7, 8, 8]
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
+
+
 @pytest.mark.parametrize("bits,master,most", [(32, False, 106), (32, True, 87), (8, False, 74), (8, True, 65)])
 @pytest.mark.parametrize("count", ["below", "full", "above", "twice"])
 def test_tensors_around_a_launch(gpu_handle, bits, master, most, count):
