@@ -88,8 +88,7 @@ class AdamW(torch.optim.Optimizer):
                 counts = {}
                 for place, p in enumerate(params):
                     if p.grad is not None:
-                        self.state[p]["step"] += 1
-                        counts.setdefault(self.state[p]["step"], []).append(place)
+                        counts.setdefault(self.state[p]["step"] + 1, []).append(place)
                 if not counts:
                     continue
                 with torch.cuda.device(device):
@@ -100,6 +99,8 @@ class AdamW(torch.optim.Optimizer):
                             grads[place] = params[place].grad
                         plan.step(_handle(), grads, step, group["lr"], group["betas"], group["eps"], group["weight_decay"],
                                   grad_scale)
+                        for place in places:   # (a step that was refused does not count)
+                            self.state[params[place]]["step"] = step
         return loss
 
     def _plan(self, number, params, eight, masters):

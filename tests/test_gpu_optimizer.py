@@ -88,6 +88,26 @@ def test_parameters_that_miss_gradients_keep_their_plans(bits, monkeypatch):
         assert torch.equal(p, q)
 
 
+def test_a_refused_step_is_not_counted():
+    import torch
+    import mluop_hip
+    from mluop_hip.optim import AdamW
+    a, b = parameters(), parameters()
+    opt, ref = AdamW(a, **HYPER), AdamW(b, **HYPER)
+    for params, o in ((a, opt), (b, ref)):
+        give_gradients(params, 1)
+        o.step()
+    opt.param_groups[0]["lr"] = float("nan")
+    with pytest.raises(mluop_hip.MluOpError):
+        opt.step()
+    opt.param_groups[0]["lr"] = HYPER["lr"]
+    assert [opt.state[p]["step"] for p in a] == [1, 1, 1]
+    opt.step()
+    ref.step()
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
+
+
 @pytest.mark.parametrize("bits,master,most", [(32, False, 106), (32, True, 87), (8, False, 74), (8, True, 65)])
 @pytest.mark.parametrize("count", ["below", "full", "above", "twice"])
 def test_tensors_around_a_launch(gpu_handle, bits, master, most, count):
