@@ -108,6 +108,23 @@ def test_a_refused_step_is_not_counted():
         assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("change", ["transposed", "shorter"])
+def test_parameters_laid_out_anew_on_the_same_memory(change):
+    """the states lie as the parameter did: a step that would mix them up is refused"""
+    import torch
+    from mluop_hip.optim import AdamW
+    p = torch.nn.Parameter(torch.randn(64, 64, device="cuda"))
+    opt = AdamW([p], **HYPER)
+    p.grad = torch.randn(64, 64, device="cuda")
+    opt.step()
+    p.data = p.data.t() if change == "transposed" else p.data[:32]
+    p.grad = torch.randn(p.shape, device="cuda")
+    was = p.detach().clone()
+    with pytest.raises(ValueError):
+        opt.step()
+    assert torch.equal(p, was)
+
+
 @pytest.mark.parametrize("bits,master,most", [(32, False, 106), (32, True, 87), (8, False, 74), (8, True, 65)])
 @pytest.mark.parametrize("count", ["below", "full", "above", "twice"])
 def test_tensors_around_a_launch(gpu_handle, bits, master, most, count):
