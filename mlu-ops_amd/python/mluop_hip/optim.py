@@ -107,8 +107,10 @@ class AdamW(torch.optim.Optimizer):
         """The checked tensors of a call, kept while parameters and states stay where they were and as they lay there."""
         states = [self.state[p] for p in params]
         names = ["exp_avg", "exp_avg_sq"] + ["master"] * masters + ["exp_avg_scale", "exp_avg_sq_scale"] * eight
+        # (a state follows its parameter's layout; looking at its own too took 270 us of the host in place of 165 for 200
+        # parameters with 8-bit states)
         where = ([(p.data_ptr(), p.shape, p.stride()) for p in params] +
-                 [(s[n].data_ptr(), s[n].stride()) for s in states for n in names])
+                 [s[n].data_ptr() for s in states for n in names])
         key = (number, params[0].dtype, params[0].device, eight, masters)
         kept = self._plans.get(key)
         if kept is None or kept[0] != where:
