@@ -125,6 +125,30 @@ def test_parameters_laid_out_anew_on_the_same_memory(change):
     assert torch.equal(p, was)
 
 
+def test_autograd_notices_a_step():
+    """a value that a backward pass needs was changed by a step in between"""
+    import torch
+    from mluop_hip.optim import AdamW
+    a = parameters(sizes=(40, 5000))
+    idle = torch.nn.Parameter(torch.ones(3, device="cuda"))
+    opt = AdamW(a + [idle], state_bits=8, **HYPER)
+    give_gradients(a, 1)
+    opt.step()
+    x = torch.randn(40, device="cuda", requires_grad=True)
+    y = (x * a[0]).sum()
+    versions = [p._version for p in a + [idle]]
+    opt.step()
+    assert all(p._version > v for p, v in zip(a, versions)) and idle._version == versions[-1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    # what is made without a record of versions can be stepped too
+    with torch.inference_mode():
+        q = torch.nn.Parameter(torch.ones(5, device="cuda"), requires_grad=False)
+        q.grad = torch.ones(5, device="cuda")
+        AdamW([q], **HYPER).step()
+    assert bool((q < 1).all())
+
+
 @pytest.mark.parametrize("bits,master,most", [(32, False, 106), (32, True, 87), (8, False, 74), (8, True, 65)])
 @pytest.mark.parametrize("count", ["below", "full", "above", "twice"])
 def test_tensors_around_a_launch(gpu_handle, bits, master, most, count):
