@@ -276,7 +276,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGroupNormBackward(mluOpHandle_t handle, mluO
 
 /* Rows of a table by their numbers: out[t, :] = scale * table[tokens[t], :], for num_tokens tokens (token_type INT32 or
  * INT64) of a table [rows, channels] whose rows lie row_stride elements apart (at least channels); out [num_tokens,
- * channels].  A token outside [0, rows) names no row: its result is zero.
+ * channels].  A token outside [0, rows) names no row: its result is zero.  A table may have no rows where there are no tokens.
  * The gradient of the table: grad_table[v, :] = scale * sum of output_grad[t, :] over the tokens that name v, added up in
  * an order that the tokens alone decide; zero for a row that none names.  The tokens are sorted in the workspace.  rows, num_tokens below 2^31. */
 mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingForward(mluOpHandle_t handle, mluOpDataType_t type, const void *table,

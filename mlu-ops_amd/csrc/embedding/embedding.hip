@@ -365,7 +365,7 @@ Plan planOf(int64_t n, int64_t rows, int64_t channels) {
 
 mluOpStatus_t checkTable(const char *api, int64_t n, int64_t rows, int64_t channels) {
   PARAM_CHECK(api, n >= 0);
-  PARAM_CHECK(api, rows > 0);
+  PARAM_CHECK(api, rows > 0 || (rows == 0 && n == 0));
   PARAM_CHECK(api, channels > 0);
   if (n > INT32_MAX - 4096 || rows > INT32_MAX - 4096 || channels > (1 << 20) || n * channels > ((int64_t)1 << 46) ||
       rows * channels > ((int64_t)1 << 46)) {
@@ -421,8 +421,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingForward(mluOpHandle_t handle, mluOp
   const mluOpStatus_t status = checkTable(api, num_tokens, rows, channels);
   if (status != MLUOP_STATUS_SUCCESS) return status;
   PARAM_CHECK(api, row_stride >= channels);
-  PARAM_CHECK(api, row_stride <= ((int64_t)1 << 46) / rows);
-  PARAM_CHECK(api, table != NULL);
+  PARAM_CHECK(api, rows == 0 || row_stride <= ((int64_t)1 << 46) / rows);
+  PARAM_CHECK(api, rows == 0 || table != NULL);
   PARAM_CHECK(api, num_tokens == 0 || (tokens != NULL && out != NULL));
   DEVICE_HANDLE_CHECK(api, handle);
   if (num_tokens == 0) return MLUOP_STATUS_SUCCESS;
@@ -470,11 +470,12 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingBackward(mluOpHandle_t handle, mluO
   PARAM_CHECK(api, num_tokens == 0 || row_stride >= channels);
   PARAM_CHECK(api, num_tokens == 0 || row_stride <= ((int64_t)1 << 46) / num_tokens);
   PARAM_CHECK(api, num_tokens == 0 || (output_grad != NULL && tokens != NULL));
-  PARAM_CHECK(api, grad_table != NULL);
+  PARAM_CHECK(api, rows == 0 || grad_table != NULL);
   PARAM_CHECK(api, workspace != NULL);
   const Plan p = planOf(num_tokens, rows, channels);
   PARAM_CHECK(api, workspace_size >= p.all());
   DEVICE_HANDLE_CHECK(api, handle);
+  if (rows == 0) return MLUOP_STATUS_SUCCESS;
   HIP_CHECK_RETURN(api, hipSetDevice(handle->device));
   if (handle->hasNotes()) {
     handle->forgetNotesIn(grad_table, (size_t)rows * channels * elementBytes(type));
