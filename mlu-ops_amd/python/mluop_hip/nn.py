@@ -373,7 +373,7 @@ def expert_order(experts_of_rows, experts):
     places begin, int32 [experts + 1]; and the place of every row's choices, int32 [rows, choices].
     `embedding(features, rows)` puts rows into that order, and its gradient adds the copies of a row up again;
     `embedding(results, places)` brings the results back."""
-    flat = experts_of_rows.reshape(experts_of_rows.shape[0], -1)
+    flat = experts_of_rows.reshape(experts_of_rows.shape[0], math.prod(experts_of_rows.shape[1:]))
     ordered, order = torch.sort(flat.reshape(-1), stable=True)
     starts = torch.searchsorted(ordered, torch.arange(experts + 1, device=flat.device, dtype=ordered.dtype), out_int32=True)
     places = torch.empty_like(order, dtype=torch.int32)

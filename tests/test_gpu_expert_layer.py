@@ -17,3 +17,30 @@ def test_lookups_in_a_table_without_rows(gpu_handle):
         assert grad.shape == (0, 24) and grad.dtype == dtype
         with pytest.raises(mluop_hip.MluOpError):
             mluop_hip.embedding_forward(gpu_handle, table, torch.zeros(1, dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_no_rows(dtype):
+    import torch
+    from mluop_hip import nn as spnn
+    dtype = getattr(torch, dtype)
+    layer = spnn.ExpertMLP(24, 40, experts=5, choices=2).cuda()
+    x = torch.zeros(0, 24, device="cuda", dtype=dtype, requires_grad=True)
+    out = layer(x)
+    assert out.shape == (0, 24) and out.dtype == dtype
+    grads = torch.autograd.grad(out, [x] + list(layer.parameters()), torch.zeros_like(out))
+    assert grads[0].shape == (0, 24)
+    for g, p in zip(grads[1:], layer.parameters()):
+        assert g.shape == p.shape and not bool(g.any())
+
+
+def test_order_of_no_rows():
+    import torch
+    from mluop_hip import nn as spnn
+    for shape in ((0, 2), (0,), (0, 0), (3, 0)):
+        chosen = torch.zeros(shape, dtype=torch.int64, device="cuda")
+        rows, starts, places = spnn.expert_order(chosen, 4)
+        assert rows.shape == (0,) and rows.dtype == torch.int32 and starts.tolist() == [0] * 5
+        assert places.shape[0] == shape[0] and places.numel() == 0
+    rows, starts, places = spnn.expert_order(torch.tensor([2, 0, 2], device="cuda"), 3)
+    assert rows.tolist() == [1, 0, 2] and starts.tolist() == [0, 1, 1, 3] and places.tolist() == [[1], [0], [2]]
