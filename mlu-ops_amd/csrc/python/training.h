@@ -108,20 +108,14 @@ class AdamWTensors {
     run(own, own.empty() ? MLUOP_DTYPE_FLOAT : dtypeCode(type_));
     run(wide, MLUOP_DTYPE_FLOAT);
     // Autograd's record of what has been written: a backward pass that needs a value from before the step says so.
-    for (size_t i = 0; i < raw_.size(); ++i) {
-      if (!grads[i] || !grads[i]->defined()) continue;
-      written(params_[i]);
-      for (size_t k = i; k < kept_.size(); k += raw_.size()) written(kept_[k]);
-    }
+    // (A tensor that was made without a record has none; states are no part of a graph.)
+    for (size_t i = 0; i < raw_.size(); ++i)
+      if (grads[i] && grads[i]->defined() && !params_[i].is_inference()) params_[i].unsafeGetTensorImpl()->bump_version();
   }
 
  private:
-  // (a tensor that was made without a record has none)
-  static void written(const at::Tensor &t) {
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-  }
   std::vector<mluOpExtAdamWTensor_t> raw_;
-  Tensors params_, kept_;  // kept_: list after list of the states, masters and scales
+  Tensors params_, kept_;
   at::ScalarType type_ = at::kFloat;
   at::Device device_ = at::kCPU;
   bool eight_ = false;
