@@ -201,7 +201,9 @@ __global__ __launch_bounds__(kThreads) void adamwStep(Tensors<MASTER, EIGHT> t, 
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
       m[i] = m[i] * by_m;
-      r[i] = r[i] > 0.f ? fmaxf(r[i] * by_r, kLeastCode) : 0.f;
+      const float root = r[i] * by_r;
+      // (a NaN stays one)
+      r[i] = r[i] == 0.f ? 0.f : (root < kLeastCode ? kLeastCode : root);
     }
     storeCodes(static_cast<uint8_t *>(m_at), at, n, whole, encode(m));
     storeCodes(static_cast<uint8_t *>(v_at), at, n, whole, encode(r));

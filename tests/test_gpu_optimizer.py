@@ -149,6 +149,46 @@ def test_autograd_notices_a_step():
     assert bool((q < 1).all())
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_gradients_that_are_not_finite(gpu_handle, bits, bad):
+    """a NaN poisons its own element and no other; an infinite one, with 8-bit states, its block of 256, whose scale it is"""
+    import torch
+    import mluop_hip
+    n, at = 1000, 300
+    start = parameters(4, sizes=(n,))[0].detach()
+    grad = parameters(5, sizes=(n,))[0].detach()
+    grad[at] = 0.0
+    spoilt = grad.clone()
+    spoilt[at] = bad
+    got = []
+    for g in (grad, spoilt):
+        p = start.clone()
+        states = [torch.zeros(n, device="cuda") if bits == 32 else torch.zeros(n, dtype=torch.uint8, device="cuda") for _ in range(2)]
+        scales = [[torch.zeros(4, device="cuda")] for _ in range(2)] if bits == 8 else [None, None]
+        plan = mluop_hip.AdamWTensors([p], states[:1], states[1:], None, *scales)
+        plan.step(gpu_handle, [g], 1, **HYPER)
+        one = p.clone()
+        held = [s.view(torch.float8_e4m3fn).float() if bits == 8 else s.clone() for s in states]
+        plan.step(gpu_handle, [grad], 2, **HYPER)
+        got.append((one, p, held))
+    clean, dirty = got
+    block = torch.zeros(n, dtype=torch.bool, device="cuda")
+    block[at] = True
+    assert torch.equal(dirty[0][~block], clean[0][~block]) and not bool(torch.isfinite(dirty[0][at]))
+    for held in dirty[2]:
+        assert not bool(torch.isfinite(held[at]))
+        if bad != bad:
+            assert bool(torch.isnan(held[at]))
+    if bits == 8 and bad == bad:
+        block[256:512] = True
+    # (and so after a step whose gradients are all finite)
+    assert not bool(torch.isfinite(dirty[1][at]))
+    assert torch.equal(dirty[1][~block], clean[1][~block])
+    for a, b in zip(dirty[2], clean[2]):
+        assert torch.equal(a[~block], b[~block])
+
+
 @pytest.mark.parametrize("bits,master,most", [(32, False, 106), (32, True, 87), (8, False, 74), (8, True, 65)])
 @pytest.mark.parametrize("count", ["below", "full", "above", "twice"])
 def test_tensors_around_a_launch(gpu_handle, bits, master, most, count):
