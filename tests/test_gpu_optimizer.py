@@ -189,6 +189,36 @@ def test_gradients_that_are_not_finite(gpu_handle, bits, bad):
         assert torch.equal(a[~block], b[~block])
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("size", [1e-18, 1e-19, 1e-20])
+def test_roots_of_numbers_below_the_smallest_normal(gpu_handle, bits, size):
+    """eps = 0: the first step is lr whatever the gradients' size, also where their squares have few bits left"""
+    import torch
+    import mluop_hip
+    n = 512
+    sign = torch.where(torch.arange(n, device="cuda") % 3 == 0, -1.0, 1.0)
+    p = torch.zeros(n, device="cuda")
+    states = [torch.zeros(n, device="cuda") if bits == 32 else torch.zeros(n, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    scales = [[torch.zeros(2, device="cuda")] for _ in range(2)] if bits == 8 else [None, None]
+    mluop_hip.AdamWTensors([p], states[:1], states[1:], None, *scales).step(
+        gpu_handle, [sign * size], 1, lr=0.5, betas=(0.9, 0.5), eps=0.0, weight_decay=0.0)
+    # v = size^2 / 2, a multiple of 2^-149: off by half of that, and its root by half as much relatively
+    room = 2.0 ** -149 / size ** 2 + 2.0 ** -20
+    assert float((p / (-0.5 * sign) - 1).abs().max()) <= room
+
+
+def test_an_eps_below_the_smallest_normal(gpu_handle):
+    """parameters without gradients so far do not move"""
+    import torch
+    import mluop_hip
+    p = torch.ones(300, device="cuda")
+    m, v = torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda")
+    mluop_hip.AdamWTensors([p], [m], [v]).step(gpu_handle, [torch.zeros(300, device="cuda")], 1, lr=0.5, betas=(0.9, 0.5),
+                                              eps=1e-40, weight_decay=0.0)
+    assert bool((p == 1).all())
+
+
+# Tensors of a launch: what 4 KB of addresses hold.
 @pytest.mark.parametrize("bits,master,most", [(32, False, 106), (32, True, 87), (8, False, 74), (8, True, 65)])
 @pytest.mark.parametrize("count", ["below", "full", "above", "twice"])
 def test_tensors_around_a_launch(gpu_handle, bits, master, most, count):
