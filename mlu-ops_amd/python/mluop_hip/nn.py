@@ -399,7 +399,9 @@ class ExpertMLP(torch.nn.Module):
         rows, starts, places = expert_order(chosen, self.experts)
         hidden = torch.nn.functional.silu(self.up(embedding(features, rows), starts))
         results = embedding(self.down(hidden, starts), places)
-        return (results * torch.softmax(scores, dim=1).to(results.dtype).unsqueeze(2)).sum(dim=1)
+        # (weights, products and sums in 32 bits whatever the rows' type, and one rounding)
+        weights = torch.softmax(scores.float(), dim=1)
+        return (results * weights.unsqueeze(2)).sum(dim=1).to(results.dtype)
 
 
 def group_norm(features, weight, bias, groups, row_starts=None, eps=1e-5, activation="none"):

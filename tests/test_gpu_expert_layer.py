@@ -44,3 +44,27 @@ def test_order_of_no_rows():
         assert places.shape[0] == shape[0] and places.numel() == 0
     rows, starts, places = spnn.expert_order(torch.tensor([2, 0, 2], device="cuda"), 3)
     assert rows.tolist() == [1, 0, 2] and starts.tolist() == [0, 1, 1, 3] and places.tolist() == [[1], [0], [2]]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("choices", [1, 2, 6])
+def test_results_are_weighed_and_added_in_32_bits(dtype, choices):
+    """the second layer's rows are given, so that what is left is sum of weight * row and one rounding"""
+    import torch
+    from mluop_hip import nn as spnn
+    dtype = getattr(torch, dtype)
+    torch.manual_seed(choices)
+    layer = spnn.ExpertMLP(32, 16, experts=8, choices=choices).cuda()
+    x = torch.randn(500, 32, device="cuda").to(dtype)
+    rows = {}
+    layer.down.register_forward_hook(lambda module, args, out: rows.setdefault("out", out))
+    out = layer(x)
+    assert out.dtype == dtype
+    scores, chosen = torch.topk(layer.gate(x.float()), choices, dim=1)
+    places = spnn.expert_order(chosen, 8)[2].long()
+    terms = rows["out"].double()[places] * torch.softmax(scores.double(), dim=1).unsqueeze(2)
+    want, size = terms.sum(dim=1), terms.abs().sum(dim=1)
+    last = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
+    # scores and softmax in fp32 (a score of a few units: its exponential is off by some units in the last place), products and sums
+    room = (choices + 32) * 2.0 ** -23 * size + last * want.abs() + 2.0 ** -25
+    assert bool(((out.double() - want).abs() <= room).all())
