@@ -31,7 +31,7 @@ class Net(torch.nn.Module):
         self.head = torch.nn.Linear(CHANNELS, CLASSES)
 
     def forward(self, categories, indices, dtype):
-        x = spnn.SparseTensor(self.embed(categories).to(dtype), indices, SPACE, BATCH, distinct=True)
+        x = spnn.SparseTensor(self.embed(categories).to(dtype), indices, SPACE, BATCH, distinct=True, ordered=True)
         features = self.encoder(x).features
         features = features + self.experts(features)
         return self.head(features.float())

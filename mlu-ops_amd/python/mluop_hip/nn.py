@@ -60,7 +60,8 @@ class Rulebook:
     asked for), out_indices, num_act_out."""
 
     def __init__(self, pairs, out_indices, indice_num_host, num_act_out, filter_space, sub_m, out_space,
-                 in_indices=None, in_space=None, distinct=False, built_on=None, tails=True, single=False):
+                 in_indices=None, in_space=None, distinct=False, built_on=None, tails=True, single=False, in_ordered=None,
+                 out_ordered=None):
         # the input coordinates were distinct: no offset names a result row twice, and the
         # operators may skip their check for such pairs (mluOpExtSetDistinctPairsPromise)
         self.distinct = distinct
@@ -68,6 +69,8 @@ class Rulebook:
         # layer's input, and its inverse, multiply full tiles of pairs: mluOpExtSetSinglePairsPromise)
         self.single = single
         self.in_indices = in_indices  # what an inverse convolution over this rulebook gives back
+        # whether their rows, and those of out_indices, lie sample after sample (None: nobody knows)
+        self.in_ordered, self.out_ordered = in_ordered, out_ordered
         self.in_space = None if in_space is None else tuple(in_space)
         self._pairs = pairs
         self._tails = tails
@@ -125,12 +128,20 @@ class Rulebook:
         return {} if self._for_operators is None else dict.fromkeys(self._for_operators.row_maps(), True)
 
 
+def _in_sample_order(samples):
+    return samples.shape[0] < 2 or bool((samples[1:] >= samples[:-1]).all())
+
+
 class SparseTensor:
     """`distinct=True` is the caller's word that no coordinate occurs twice (the output of a
     voxelizer, or of a strided layer, never repeats one); the convolution operators then skip
-    their check for pairs of one offset that share a result row."""
+    their check for pairs of one offset that share a result row.
 
-    def __init__(self, features, indices, spatial_shape, batch_size, rulebooks=None, distinct=False):
+    `ordered=True` is the caller's word that rows lie sample after sample (a strided layer's do, whatever its input's).  With
+    None the first layer that takes statistics by sample looks, once for all layers on these coordinates, and waits for the
+    answer; rows in no order are put into one for it."""
+
+    def __init__(self, features, indices, spatial_shape, batch_size, rulebooks=None, distinct=False, ordered=None):
         assert indices.dtype == torch.int32 and indices.dim() == 2 and indices.shape[1] == 4
         assert features.shape[0] == indices.shape[0]
         self.features = features
@@ -139,22 +150,43 @@ class SparseTensor:
         self.batch_size = int(batch_size)
         self.rulebooks = {} if rulebooks is None else rulebooks
         self.distinct = bool(distinct)
+        self.ordered = ordered
 
     def replace_features(self, features):
         return SparseTensor(features, self.indices, self.spatial_shape, self.batch_size, self.rulebooks,
-                            self.distinct)
+                            self.distinct, self.ordered)
+
+    def _rows_of_samples(self):
+        """(order, places, starts), None for one sample: the rows sample after sample and the place of every row among them (int32,
+        None where they lie so), and where every sample's begin (int32 [batch_size + 1]).  Kept with the rulebooks."""
+        if self.batch_size == 1:
+            return None, None, None
+        kept = self.rulebooks.get(("samples", id(self.indices)))
+        if kept is not None and kept[0] is self.indices:
+            return kept[1:]
+        if _capturing() and not self.ordered:
+            raise RuntimeError("whether a SparseTensor's rows are ordered by sample cannot be waited for while a graph is "
+                               "captured: say so (ordered=True), or run a layer on it before")
+        with torch.no_grad(), torch.inference_mode(False):
+            samples, order, places = self.indices[:, 0].contiguous(), None, None
+            if not self.ordered and not (self.ordered is None and _in_sample_order(samples)):
+                samples, order = torch.sort(samples, stable=True)
+                places = torch.empty_like(order, dtype=torch.int32)
+                places[order] = torch.arange(order.shape[0], device=order.device, dtype=torch.int32)
+                order = order.to(torch.int32)
+            numbers = torch.arange(self.batch_size + 1, device=samples.device, dtype=torch.int32)
+            starts = torch.searchsorted(samples, numbers, out_int32=True)
+        if not _capturing():   # (what is captured has not run)
+            self.rulebooks[("samples", id(self.indices))] = (self.indices, order, places, starts)
+        return order, places, starts
 
     def row_starts(self):
-        """int32 [batch_size + 1]: where every sample's rows begin, for rows that are ordered by sample; None for one
-        sample.  Kept with the rulebooks while the coordinates are these."""
-        if self.batch_size == 1:
-            return None
-        kept = self.rulebooks.get("row_starts")
-        if kept is None or kept[0] is not self.indices:
-            samples = torch.arange(self.batch_size + 1, device=self.indices.device, dtype=torch.int32)
-            kept = (self.indices, torch.searchsorted(self.indices[:, 0].contiguous(), samples, out_int32=True))
-            self.rulebooks["row_starts"] = kept
-        return kept[1]
+        """int32 [batch_size + 1]: where every sample's rows begin; None for one sample.  Of rows that are ordered by sample
+        only: others raise a ValueError."""
+        order, _, starts = self._rows_of_samples()
+        if order is not None:
+            raise ValueError("the rows are not ordered by sample")
+        return starts
 
     def dense(self):
         """[N, C, D, H, W] dense tensor (for inspection and tests)."""
@@ -217,7 +249,9 @@ class _ConvBase(torch.nn.Module):
             self.stride, self.dilation, self.sub_m, for_layer=True, tails=False, wait_counts=wait_counts)
         rb = Rulebook(pairs, out_indices, num, n_out, self.kernel_size, self.sub_m,
                       out_space, in_indices=x.indices, in_space=x.spatial_shape, distinct=x.distinct,
-                      built_on=handle, tails=False,
+                      built_on=handle, tails=False, in_ordered=x.ordered,
+                      # (a regular rulebook numbers its output cells in their linear order)
+                      out_ordered=x.ordered if self.sub_m else True,
                       single=not self.sub_m and all((k - 1) * d < s for k, d, s in
                                                     zip(self.kernel_size, self.dilation, self.stride)))
         if self.indice_key is not None:
@@ -238,13 +272,17 @@ class _ConvBase(torch.nn.Module):
             return rb.in_indices, rb.in_space, rb.distinct
         return rb.out_indices.contiguous(), rb.out_space, True
 
+    def _order_after(self, x, rb):
+        """What is known about the order of this layer's result on `x`, by sample."""
+        return x.ordered if self.sub_m else getattr(rb, "in_ordered" if self.inverse else "out_ordered", None)
+
     def _result(self, x, rb, feats):
         if self.sub_m:
             return x.replace_features(feats)
         # the cache travels on, so that an inverse layer downstream finds this rulebook by its key;
         # the active output cells of a regular convolution are distinct by construction
         return SparseTensor(feats, rb.out_indices.contiguous(), rb.out_space, x.batch_size, x.rulebooks,
-                            distinct=True)
+                            distinct=True, ordered=self._order_after(x, rb))
 
     def forward(self, x):
         return self._convolve(x)
@@ -297,7 +335,8 @@ class SparseInverseConv3d(_ConvBase):
         return rb
 
     def _result(self, x, rb, feats):
-        return SparseTensor(feats, rb.in_indices, rb.in_space, x.batch_size, x.rulebooks, distinct=rb.distinct)
+        return SparseTensor(feats, rb.in_indices, rb.in_space, x.batch_size, x.rulebooks, distinct=rb.distinct,
+                            ordered=self._order_after(x, rb))
 
 
 def _unwatched():
@@ -414,8 +453,8 @@ def group_norm(features, weight, bias, groups, row_starts=None, eps=1e-5, activa
 class GroupNormAct(torch.nn.Module):
     """Group norm over the channels of every sample, with an activation ("none", "relu", "silu") in the same pass.
 
-    Takes a SparseTensor, whose rows have to be ordered by sample (as voxelizers, `sparse_tensor_from_voxels` and strided
-    layers give them; the statistics are those of each sample's rows), or a tensor [rows, channels] with `row_starts`.
+    Takes a SparseTensor (the statistics are those of each sample's rows; rows that are not ordered by sample are put into
+    that order and back, two passes more), or a tensor [rows, channels] with `row_starts`.
     The parameters may be float32 whatever the features are."""
 
     def __init__(self, groups, channels, eps=1e-5, activation="none", affine=True):
@@ -431,8 +470,10 @@ class GroupNormAct(torch.nn.Module):
     def forward(self, x, row_starts=None):
         if not isinstance(x, SparseTensor):
             return group_norm(x, self.weight, self.bias, self.groups, row_starts, self.eps, self.activation)
-        return x.replace_features(group_norm(x.features, self.weight, self.bias, self.groups, x.row_starts(), self.eps,
-                                             self.activation))
+        order, places, starts = x._rows_of_samples()
+        rows = x.features if order is None else embedding(x.features, order)
+        rows = group_norm(rows, self.weight, self.bias, self.groups, starts, self.eps, self.activation)
+        return x.replace_features(rows if order is None else embedding(rows, places))
 
 
 class SparseSequential(torch.nn.Sequential):
@@ -479,7 +520,10 @@ class SparseSequential(torch.nn.Sequential):
                 if indices is not cells.indices:
                     # (features are not looked at while planning: a view of the right height)
                     cells = SparseTensor(indices.new_empty((indices.shape[0], 0)), indices, space,
-                                         cells.batch_size, cells.rulebooks, distinct)
+                                         cells.batch_size, cells.rulebooks, distinct, m._order_after(cells, rb))
+            elif isinstance(m, GroupNormAct) and type(m).forward is GroupNormAct.forward:
+                # (what is waited for is waited for here, too)
+                cells._rows_of_samples()
         return cells
 
     def forward(self, x):
@@ -583,7 +627,7 @@ def sparse_tensor_from_voxels(features, coors, spatial_shape, batch_index=0, bat
     if order_by_cell and _ordered_by_library(coors, spatial_shape, batch_index):
         order, indices = native().order_voxels(_guarded(), coors.contiguous(), [int(v) for v in spatial_shape],
                                                int(batch_index))
-        return SparseTensor(features[order], indices, spatial_shape, batch_size, distinct=True)
+        return SparseTensor(features[order], indices, spatial_shape, batch_size, distinct=True, ordered=True)
     if order_by_cell and coors.shape[0] > 1:
         d, h, w = (int(v) for v in spatial_shape)
         key = (coors[:, 0].to(torch.int64) * h + coors[:, 1].to(torch.int64)) * w + coors[:, 2].to(torch.int64)
@@ -593,4 +637,4 @@ def sparse_tensor_from_voxels(features, coors, spatial_shape, batch_index=0, bat
     n = torch.full((coors.shape[0], 1), int(batch_index), dtype=torch.int32, device=coors.device)
     # a voxelizer emits every voxel once
     return SparseTensor(features, torch.cat([n, coors], dim=1).contiguous(), spatial_shape, batch_size,
-                        distinct=True)
+                        distinct=True, ordered=True)
