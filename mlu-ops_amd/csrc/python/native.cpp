@@ -14,7 +14,9 @@
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <algorithm>
 #include <atomic>
 #include <map>
 #include <mutex>

@@ -237,6 +237,20 @@ StreamHandle &handleFor(const at::Tensor &t) {
   return streamHandle();
 }
 
+// A node's gradients, which are made outside of autograd: where they depend on a tensor that it follows, a derivative of
+// them is an error, and not left out.
+torch::autograd::variable_list differentiableOnce(torch::autograd::variable_list grads, at::TensorList depend_on) {
+  const bool followed = std::any_of(depend_on.begin(), depend_on.end(),
+                                    [](const at::Tensor &t) { return t.defined() && t.requires_grad(); });
+  if (!at::GradMode::is_enabled() || !followed) return grads;
+  for (at::Tensor &g : grads)
+    if (g.defined()) g = g.detach().set_requires_grad(true);
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      "this operator's gradient cannot be differentiated: it is differentiable once, not twice",
+      static_cast<int64_t>(grads.size()));
+  return (*error)(std::move(grads));
+}
+
 struct GroupNorm : torch::autograd::Function<GroupNorm> {
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &features, const at::Tensor &weight,
                             const at::Tensor &bias, int64_t groups, const MaybeTensor &row_starts, double eps,
@@ -264,11 +278,9 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     if (ctx->needs_input_grad(0)) out[0] = r[0];
     if (saved[1].defined() && ctx->needs_input_grad(1)) out[1] = r[1];
     if (saved[2].defined() && ctx->needs_input_grad(2)) out[2] = r[2];
-    return out;
+    return differentiableOnce(std::move(out), {grads[0], saved[0], saved[1], saved[2]});
   }
 };
-
-
 
 // ---- embedding -----------------------------------------------------------------------------
 
@@ -346,7 +358,7 @@ struct EmbeddingRows : torch::autograd::Function<EmbeddingRows> {
     const OperatorLock lock(h);
     out[0] = embeddingBackward(h.handle, ctx->saved_data["guarded"].toBool(), grads[0], saved[0],
                                ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble());
-    return out;
+    return differentiableOnce(std::move(out), {grads[0]});
   }
 };
 
@@ -436,7 +448,7 @@ struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
     const OperatorLock lock(h);
     if (ctx->needs_input_grad(0)) out[0] = groupedRows(h.handle, guarded, grads[0], saved[1], saved[2], false);
     if (ctx->needs_input_grad(1)) out[1] = groupedFilter(h.handle, guarded, saved[0], grads[0], saved[2]);
-    return out;
+    return differentiableOnce(std::move(out), {grads[0], saved[0], saved[1]});
   }
 };
 
