@@ -227,7 +227,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtIndiceConvolutionBackwardFilterNoAlloc(
  * for all tensors or for none.  state_type FLOAT: exp_avg (m) and exp_avg_sq (v) are fp32 [count], the scales are not looked
  * at.  UINT8: they are OCP e4m3 codes [count] of m and of sqrt(v), and every block of MLUOP_EXT_ADAMW_BLOCK consecutive
  * elements has an fp32 scale [ceil(count / block)] that its codes' values are multiplied by (largest magnitude / 448).
- * step counts from 1; 0 <= beta1, beta2 < 1; eps >= 0.  Tensors of no elements are passed over. */
+ * step counts from 1; 0 <= beta1, beta2 < 1; eps >= 0.  Tensors of no elements are passed over.  A NaN or an infinity in a
+ * gradient stays in its element, but for an infinity with 8-bit states, which is its block's scale. */
 #define MLUOP_EXT_ADAMW_BLOCK 256
 typedef struct {
   void *param;
@@ -251,7 +252,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtAdamWStep(mluOpHandle_t handle, const mluOpE
  * weight and bias [channels] of param_type, FLOAT or `type`; NULL: one and zero.  mean and rstd fp32 [samples, groups] are
  * results that the backward pass takes (0 and 1 / sqrt(eps) for a sample without rows).  Rows of no sample are zero in
  * every result.  Backward: input_grad [rows, channels], weight_grad and bias_grad [channels] of param_type (NULL where not
- * wanted).  One workspace size serves both. */
+ * wanted).  One workspace size serves both.  At most 2^20 channels and samples, and 15 * 2^20 pairs of a sample and a group. */
 typedef enum {
   MLUOP_EXT_ACTIVATION_NONE = 0,
   MLUOP_EXT_ACTIVATION_RELU = 1,
@@ -278,7 +279,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGroupNormBackward(mluOpHandle_t handle, mluO
  * INT64) of a table [rows, channels] whose rows lie row_stride elements apart (at least channels); out [num_tokens,
  * channels].  A token outside [0, rows) names no row: its result is zero.  A table may have no rows where there are no tokens.
  * The gradient of the table: grad_table[v, :] = scale * sum of output_grad[t, :] over the tokens that name v, added up in
- * an order that the tokens alone decide; zero for a row that none names.  The tokens are sorted in the workspace.  rows, num_tokens below 2^31. */
+ * an order that the tokens alone decide; zero for a row that none names.  The tokens are sorted in the workspace.  rows,
+ * num_tokens below 2^31. */
 mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingForward(mluOpHandle_t handle, mluOpDataType_t type, const void *table,
                                                      int64_t rows, int64_t channels, int64_t row_stride,
                                                      mluOpDataType_t token_type, const void *tokens, int64_t num_tokens,

@@ -126,9 +126,9 @@ __device__ __forceinline__ float blockMost(float v) {
 // caches (nobody reads a state before the next step): 130 M bf16 parameters with masters 757 -> 676 us (5.4 TB/s, where
 // a copy has 5.1), 250 M with 8-bit states 472 -> 450 us (5.6 TB/s), 33 fp32 tensors of 1.9 M elements in all 12.3 -> 10.8.
 // TINY: a root below the smallest normal number counts.  The hardware's own root and reciprocal take such numbers for zero: that
-// root is below 2^-63, and corrected it is lost beside an eps of 2^25 times that.  With a smaller eps (1.1e-10 in the first step with
-// beta2 = 0.999, 3.6e-12 later on) root and quotient are those that are defined.  us without / with: 250 M bf16 parameters with
-// 8-bit states 455 / 482, 33 fp32 tensors of 1.9 M elements in all 9.4 / 10.3, 130 M with masters 675 / 678.
+// root is below 2^-63, and corrected it is lost beside an eps of 2^25 times that.  With a smaller eps (1.1e-10 in the first
+// step with beta2 = 0.999, 3.6e-12 later on) root and quotient are those that are defined.  us without / with: 250 M bf16
+// parameters with 8-bit states 455 / 482, 33 fp32 tensors of 1.9 M elements in all 9.4 / 10.3, 130 M with masters 675 / 678.
 template <typename P, typename G, bool MASTER, bool EIGHT, bool TINY>
 __global__ __launch_bounds__(kThreads) void adamwStep(Tensors<MASTER, EIGHT> t, Hyper h) {
   typedef Tensors<MASTER, EIGHT> Table;
@@ -183,8 +183,8 @@ __global__ __launch_bounds__(kThreads) void adamwStep(Tensors<MASTER, EIGHT> t, 
     const float gi = g[i] * h.grad_scale;
     m[i] = m[i] * h.beta1 + gi * h.one_minus_beta1;
     v[i] = (EIGHT ? r[i] * r[i] : r[i]) * h.beta2 + gi * gi * h.one_minus_beta2;
-    // (the hardware's own reciprocal, one unit in the last place; and its own root too, but where codes are made of it: half a code
-    // on from there a unit decides between two of them, and the next step starts from it)
+    // (the hardware's own reciprocal, one unit in the last place; and its own root too, but where codes are made of it: half a
+    // code on from there a unit decides between two of them, and the next step starts from it)
     r[i] = EIGHT || TINY ? sqrtf(v[i]) : __builtin_amdgcn_sqrtf(v[i]);
     const float below = r[i] * h.inv_root2 + h.eps;
     p[i] = p[i] * h.decay - h.step_size * (TINY ? m[i] / below : m[i] * __builtin_amdgcn_rcpf(below));

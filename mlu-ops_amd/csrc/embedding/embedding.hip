@@ -26,8 +26,8 @@ struct Tokens {
   int step, high;  // words of a token, and where its upper half is (32 bits: the token again, of which nothing counts)
   uint32_t upper;
   Tokens(const void *tokens, mluOpDataType_t type, int64_t table_rows)
-      : at(static_cast<const uint32_t *>(tokens)), rows((uint32_t)table_rows), step(type == MLUOP_DTYPE_INT64 ? 2 : 1), high(step - 1),
-        upper(high != 0 ? ~0u : 0u) {}
+      : at(static_cast<const uint32_t *>(tokens)), rows((uint32_t)table_rows), step(type == MLUOP_DTYPE_INT64 ? 2 : 1),
+        high(step - 1), upper(high != 0 ? ~0u : 0u) {}
   // The row that token i names; `rows` where it names none.
   __device__ __forceinline__ uint32_t row(int64_t i) const {
     const uint32_t *word = at + i * step;
@@ -401,8 +401,9 @@ void byType(mluOpDataType_t type, int64_t channels, int64_t row_stride, uintptr_
 }
 
 // Rows of the table that a row of threads owns, of `turns` it would own one at a time: several of a large table, most of
-// whose rows nobody names, and a workgroup for each would mostly start and end; one of a small table.  us of a gradient with one /
-// with four: 131 072 x 2048 bf16 from 65 536 tokens 202 / 186, 600 000 x 64 from 30 000 55 / 52; 500 x 512 from 4000 18 / 23.
+// whose rows nobody names, and a workgroup for each would mostly start and end; one of a small table.  us of a gradient with
+// one / with four: 131 072 x 2048 bf16 from 65 536 tokens 202 / 186, 600 000 x 64 from 30 000 55 / 52; 500 x 512 from 4000 18 /
+// 23.
 int tableRows(int64_t turns) { return turns >= 16384 ? 4 : 1; }
 
 int rowsAtOnce(int64_t vectors) { return vectors >= kThreads ? 1 : (int)(kThreads / vectors); }
@@ -430,7 +431,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtEmbeddingForward(mluOpHandle_t handle, mluOp
   handle->forgetNotesIn(out, (size_t)num_tokens * channels * elementBytes(type));
   const Tokens t(tokens, token_type, rows);
   const mluop::LaunchCtx lc = handle->launchCtx();
-  byType(type, channels, row_stride, reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(out), [&](auto zero, auto v) {
+  const uintptr_t addresses = reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(out);
+  byType(type, channels, row_stride, addresses, [&](auto zero, auto v) {
     typedef decltype(zero) T;
     constexpr int V = decltype(v)::value;
     // (the last slab has fewer channels and more rows at once: its surplus workgroups find nothing)

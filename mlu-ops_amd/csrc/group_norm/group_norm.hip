@@ -548,8 +548,8 @@ __global__ __launch_bounds__(kThreads) void groupNormGradApply(const T *__restri
 // One launch, in which a workgroup keeps a sample's rows of `columns` * V channels, whole groups, in registers: it reads them
 // once, takes the mean, then the squares of the differences from it, and writes the results.  All lanes of a wave have
 // the same V channels of rows of their own.  Bound by what a launch and a few barriers take.  us in two or three launches /
-// in one, forward and gradients: 1000 x 64 fp16 in 16 groups 11.1 / 6.6 and 12.8 / 7.9, 4096 rows 11.2 / 9.5 and 13.1 / 12.7, 1000 x 16
-// fp32 in one group 11.2 / 6.5 and 12.2 / 11.0.  From the rows on that no longer fit there is nothing to choose.
+// in one, forward and gradients: 1000 x 64 fp16 in 16 groups 11.1 / 6.6 and 12.8 / 7.9, 4096 rows 11.2 / 9.5 and 13.1 / 12.7,
+// 1000 x 16 fp32 in one group 11.2 / 6.5 and 12.2 / 11.0.  From the rows on that no longer fit there is nothing to choose.
 
 constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
 constexpr int kSmallRows = 4;         // of a thread
@@ -792,7 +792,8 @@ size_t partialBytes(int64_t rows, int64_t channels, int64_t samples) {
 }
 
 // Whether the pass that applies joins the moments itself: each of its workgroups then reads those of a sample's tiles, of
-// no more than a few KB.  us in three launches / in two: 20 000 x 16 fp32 in two samples 11.2 / 10.0, 20 000 x 32 bf16 in 16 12.5 / 10.7.
+// no more than a few KB.  us in three launches / in two: 20 000 x 16 fp32 in two samples 11.2 / 10.0, 20 000 x 32 bf16 in 16
+// 12.5 / 10.7.
 bool joinedByApply(const Shape &s) {
   return s.rows > 0 && s.samples <= 64 && s.groups <= kThreads && (int64_t)s.most_tiles * s.channels <= 4096;
 }

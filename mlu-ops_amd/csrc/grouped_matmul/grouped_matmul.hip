@@ -1,10 +1,10 @@
-// Kernels of the products grouped by expert: y_r = x_r W_g, dx_r = dy_r W_g^T and dW_g = sum over the rows r of a group of x_r^T dy_r,
-// on matrix cores with fp32 sums and one rounding.  A tile of rows never crosses a group's end.
+// Kernels of the products grouped by expert: y_r = x_r W_g, dx_r = dy_r W_g^T and dW_g = sum over the rows r of a group of
+// x_r^T dy_r, on matrix cores with fp32 sums and one rounding.  A tile of rows never crosses a group's end.
 //   groupedTiles  rows in whole 16-byte pieces; bound by the matrix cores and, long and large, by the power they draw (the same
 //                 product of zeros is faster).  32 768 rows, 8 x 2048 x 8192 bf16: forward 1.00 ms (1.10 PFLOP/s), backward data
 //                 0.95 (1.16), filter gradient 0.87 (1.26), where a large library product has 1.24.
-//   groupedFew    the same with few rows a group or few tiles; bound by the filters' way from memory: 12 rows of ten of 32 experts,
-//                 1024 x 2048 bf16 (42 MB) 9.6 us, 4.4 TB/s with what a launch costs.
+//   groupedFew    the same with few rows a group or few tiles; bound by the filters' way from memory: 12 rows of ten of 32
+//                 experts, 1024 x 2048 bf16 (42 MB) 9.6 us, 4.4 TB/s with what a launch costs.
 //   groupedAny    any shape and stride; bound by the step from load to LDS to multiply, some 2 us of 64.
 #include <hip/hip_runtime.h>
 
@@ -308,8 +308,8 @@ __global__ __launch_bounds__(kAnyThreads) void groupedAny(const T *__restrict__ 
 // [result][step], and a fragment is one 16-byte read.  One that memory has along the results lies as [step][results]:
 // 2-byte elements are transposed by `ds_read_b64_tr_b16` (within 16 lanes, lane i gives the address of four results of the
 // reduction's part i / 4, and lane j receives result j of the four parts), fp32 ones are read one by one.  Either way rows are a
-// multiple of the banks apart, and their 16-byte pieces are permuted by row so that the lanes of a read meet all banks; the loads permute, since a
-// lane's place in LDS is fixed.
+// multiple of the banks apart, and their 16-byte pieces are permuted by row so that the lanes of a read meet all banks; the
+// loads permute, since a lane's place in LDS is fixed.
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short v4i16 __attribute__((ext_vector_type(4)));
@@ -480,8 +480,8 @@ __device__ __forceinline__ RaggedTile tileOfRows(const RowTiles &all, int xcd, i
 // In which order a workgroup takes its works (in LDS; NULL: by number).
 struct Order {
   const uint16_t *longest;  // blocks (groups, or slices of their rows) by falling length
-  const uint16_t *taken;    // or NULL: this workgroup's share of what does not fill a round of its XCD, pairs of a place in `longest`
-                            // and a tile of the XCD's
+  const uint16_t *taken;    // or NULL: this workgroup's share of what does not fill a round of its XCD, pairs of a place in
+                            // `longest` and a tile of the XCD's
   int whole;                // rounds that an XCD's tiles of every block make
   int blocks;               // that there are
 };
@@ -607,8 +607,8 @@ __device__ __forceinline__ void storeResults(u32x4 v, __amdgpu_buffer_rsrc_t to,
     __builtin_amdgcn_raw_buffer_store_b128(v, to, at, 0, 0);
 }
 
-// A workgroup has one tile and its two steps in LDS (256 x 256: 128 KB, one a CU): operands are read once for 256 results a side, which
-// leaves L2 at 10 TB/s in all; 128 x 128 tiles of the same product need twice that and reach 0.8 of the rate.
+// A workgroup has one tile and its two steps in LDS (256 x 256: 128 KB, one a CU): operands are read once for 256 results a
+// side, which leaves L2 at 10 TB/s in all; 128 x 128 tiles of the same product need twice that and reach 0.8 of the rate.
 // Workgroups stay: each takes the works blockIdx.x, blockIdx.x + gridDim.x, ... (or those of its order).  The first loads of
 // the next are under way while the results of this one are stored.
 template <typename T, int MODE, int BM, int BN, int WM, int WN>
@@ -817,8 +817,8 @@ __global__ __launch_bounds__(WM *WN * 64) void groupedTiles(const T *__restrict_
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// One tile a workgroup, and STAGES steps of both sides on their way: for few rows or tiles, where the filters are what is read, and
-// for the last round that 256 x 256 tiles leave (REST: a quarter of such a tile each).  The kernel above has one step under
+// One tile a workgroup, and STAGES steps of both sides on their way: for few rows or tiles, where the filters are what is read,
+// and for the last round that 256 x 256 tiles leave (REST: a quarter of such a tile each).  The kernel above has one step under
 // way, which a product that takes less than a way from memory for a step waits for again and again: 48 tiles of 64 steps left
 // over took 60 us in tiles of 128 x 128 of its own.
 constexpr int kRestStages = 4, kFewWaves = 4;
@@ -917,7 +917,8 @@ __global__ __launch_bounds__(256) void groupedSumSlices(Args a, T *__restrict__ 
   for (int base = 0; base < group; base += 64) {
     int other_first, other_rows = 0;
     if (base + lane < group) segmentRows(a.starts, a.rows, base + lane, &other_first, &other_rows);
-    first += __builtin_amdgcn_readlane(waveInclusiveScan(other_rows <= a.slice_rows ? 0 : slicesOf(other_rows, a.slice_rows)), 63);
+    const int slots = other_rows <= a.slice_rows ? 0 : slicesOf(other_rows, a.slice_rows);
+    first += __builtin_amdgcn_readlane(waveInclusiveScan(slots), 63);
   }
   // (inside the slots, whatever the starts hold)
   first = first < 0 || first > a.slots ? a.slots : first;
@@ -1024,25 +1025,25 @@ struct Tile {
   double few, full, end;
   double forward, data;  // TB/s at which filters come in, forward and for backward data
 };
-// The first two are groupedTiles, the others groupedFew; filter gradients take the first three, all of them groupedTiles.  Measured (fp16
-// forward of a 2048 x 2048 filter, us in this order): 16 rows 39 / 18 / 15 / 12 / 12 / 8.7 / 8.5, 500 rows 42 / 19 / 17 / 12.5 / 13 /
-// 15 / 24, 1000 rows 43 / 22 / 17.6 / 18.5 / 22 / 27 / 42, 4000 rows 50 / 38 / 51 / 68 / 70 / 89 / 148; bf16 40 000 rows 288 / 365 / 524
-// / - / - / 895 / 1480.
+// The first two are groupedTiles, the others groupedFew; filter gradients take the first three, all of them groupedTiles.
+// Measured (fp16 forward of a 2048 x 2048 filter, us in this order): 16 rows 39 / 18 / 15 / 12 / 12 / 8.7 / 8.5, 500 rows 42 /
+// 19 / 17 / 12.5 / 13 / 15 / 24, 1000 rows 43 / 22 / 17.6 / 18.5 / 22 / 27 / 42, 4000 rows 50 / 38 / 51 / 68 / 70 / 89 / 148;
+// bf16 40 000 rows 288 / 365 / 524 / - / - / 895 / 1480.
 constexpr int kTileKinds = 3;
-// Steps of the reduction from which on a last round that 256 x 256 tiles fill to a quarter or less is left for 128 x 128 ones.  Its
-// tiles take a whole round's time otherwise; an empty launch takes 2 us.  2048 columns of fp16, us of 33 / 40 / 48 tiles an XCD
-// (32 workgroups) without and with this: 8 steps 37 / 36 / 38 either way, 16 steps 58 / 57 / 59 and 52 / 54 / 58, 64 steps
+// Steps of the reduction from which on a last round that 256 x 256 tiles fill to a quarter or less is left for 128 x 128 ones.
+// Its tiles take a whole round's time otherwise; an empty launch takes 2 us.  2048 columns of fp16, us of 33 / 40 / 48 tiles an
+// XCD (32 workgroups) without and with this: 8 steps 37 / 36 / 38 either way, 16 steps 58 / 57 / 59 and 52 / 54 / 58, 64 steps
 // 180 / 180 / 182 and 153 / 156 / 183.
 constexpr int kRestSteps = 16;
-// Bytes of results from which on 256 x 256 tiles are stored past the caches, which then keep the operands: 82 MB 177 -> 158 us, 134 MB
-// 268 -> 250; 31 MB 34 -> 38.
+// Bytes of results from which on 256 x 256 tiles are stored past the caches, which then keep the operands: 82 MB 177 -> 158 us,
+// 134 MB 268 -> 250; 31 MB 34 -> 38.
 constexpr double kStreamedResults = 64e6;
-// Padded copies, us without and with them: 25 973 rows of 2048 x 100 fp16 112 / 35, 229 rows of 64 x 2048 x 100 99 / 32; one row of
-// 16 x 1024 x 100 32 / 12, where the filter is all there is to copy; twelve rows of 32 x 100 x 2048 stay at 6.6, which two launches take.
-// Bytes a us of padded copies, and a launch of them.
+// Padded copies, us without and with them: 25 973 rows of 2048 x 100 fp16 112 / 35, 229 rows of 64 x 2048 x 100 99 / 32; one
+// row of 16 x 1024 x 100 32 / 12, where the filter is all there is to copy; twelve rows of 32 x 100 x 2048 stay at 6.6, which
+// two launches take.  Bytes a us of padded copies, and a launch of them:
 constexpr double kCopied = 3.0e6, kCopyLaunch = 4.0;
-// 64 filters of 2048 x 2048 for a row each: 122 / 95 / 100 / 122 / 103 / 119 / 119, and backward data, which reads their rows, 136 /
-// 125 / 116 / 111 / 104 / 102 / 101.
+// 64 filters of 2048 x 2048 for a row each: 122 / 95 / 100 / 122 / 103 / 119 / 119, and backward data, which reads their rows,
+// 136 / 125 / 116 / 111 / 104 / 102 / 101.
 constexpr Tile kTiles[] = {{"groupedTiles256", 256, 256, 1, 1.25, 1.65, 5.0, 4.4, 3.9},
                            {"groupedTiles128", 128, 128, 2, 0.59, 1.06, 2.5, 5.6, 4.3},
                            {"groupedTiles64", 64, 128, 2, 0.43, 0.76, 2.0, 5.4, 4.6},
@@ -1050,10 +1051,10 @@ constexpr Tile kTiles[] = {{"groupedTiles256", 256, 256, 1, 1.25, 1.65, 5.0, 4.4
                            {"groupedFew32x128", 32, 128, 2, 0.28, 0.64, 1.5, 5.2, 5.1},
                            {"groupedFew32", 32, 64, 2, 0.25, 0.40, 1.5, 4.5, 5.25},
                            {"groupedFew16", 16, 64, 2, 0.22, 0.36, 1.5, 4.5, 5.3}};
-// fp32, whose steps are 32 deep: bound by the multiplies.  Forward of 2048 x 2048, us as above: 16 rows 460 / 149 / 74 / 45 / 44 / 27 /
-// 19, 1000 rows 461 / 149 / 81 / 79 / 78 / 83 / 103, 4000 rows 469 / 269 / 271 / 289 / 293 / 320 / 403; 16 000 rows 949 in the first
-// (141 TFLOP/s; a large library product has 154), 1077 in the second.  64 filters for a row each 931 / 527 / 277 / 295 / 207 / 233 / 216,
-// backward data 927 / 519 / 269 / 285 / 220 / 239 / 216.
+// fp32, whose steps are 32 deep: bound by the multiplies.  Forward of 2048 x 2048, us as above: 16 rows 460 / 149 / 74 / 45 /
+// 44 / 27 / 19, 1000 rows 461 / 149 / 81 / 79 / 78 / 83 / 103, 4000 rows 469 / 269 / 271 / 289 / 293 / 320 / 403; 16 000 rows
+// 949 in the first (141 TFLOP/s; a large library product has 154), 1077 in the second.  64 filters for a row each 931 / 527 /
+// 277 / 295 / 207 / 233 / 216, backward data 927 / 519 / 269 / 285 / 220 / 239 / 216.
 constexpr Tile kFloatTiles[] = {{"groupedTiles256", 256, 256, 1, 7.2, 7.0, 5.0, 4.4, 3.9},
                                 {"groupedTiles128", 128, 128, 2, 2.3, 4.3, 2.5, 5.6, 4.3},
                                 {"groupedTiles64", 64, 128, 2, 1.17, 2.1, 2.0, 5.4, 4.6},
@@ -1108,8 +1109,8 @@ int planRows(const Problem &p, const Tile *tiles, int kinds, int cu_count, doubl
 int64_t mostSlots(const Problem &p, int64_t slice_rows) { return 2 * (int64_t)p.rows / slice_rows; }
 
 // Tile and slices of the backward filter.  How long the groups are is not known here, but as a rule some are several times as
-// long as the mean: a group of kLongest times that is counted with, whose tiles the end waits for.  Shorter slices take less time, and
-// the sums of groups of several a way to memory and back.
+// long as the mean: a group of kLongest times that is counted with, whose tiles the end waits for.  Shorter slices take less
+// time, and the sums of groups of several a way to memory and back.
 double planSlices(const Problem &p, const Tile &t, int cu_count, int *slice_rows) {
   constexpr double kLongest = 3.0;
   const double tiles = (double)tilesOf(p.ci, t.m) * tilesOf(p.co, t.n), filter = (double)p.ci * p.co;
@@ -1215,7 +1216,8 @@ template <typename T, int MODE, int TILE, int WM, int WN>
 hipError_t launchTiles(const LaunchCtx &lc, const Problem &p, Args a, int cu_count) {
   constexpr int BM = kTiles[TILE].m, BN = kTiles[TILE].n;
   constexpr size_t kLds = (size_t)2 * (BM + BN) * 128;
-  static_assert((kLds + kStartsInLds * 4 + kRanked * 6 + kSharedBlocks * 4 + 4) * kTiles[TILE].per_cu <= 160 * 1024, "LDS of a CU");
+  static_assert((kLds + kStartsInLds * 4 + kRanked * 6 + kSharedBlocks * 4 + 4) * kTiles[TILE].per_cu <= 160 * 1024,
+                "LDS of a CU");
   auto kernel = groupedTiles<T, MODE, BM, BN, WM, WN>;
   const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
@@ -1333,7 +1335,8 @@ Padded padded(const Problem &p, int cu_count) {
   const bool ci = d.q.ci != p.ci, co = d.q.co != p.co;
   if (wholeSizes(p) || !wholeSizes(d.q) || p.rows == 0) return d;
   const bool filter = p.which == MLUOP_EXT_GROUPED_BACKWARD_FILTER, forward = p.which == MLUOP_EXT_GROUPED_FORWARD;
-  const size_t x = (size_t)p.rows * d.q.ci * size, y = (size_t)p.rows * d.q.co * size, w = (size_t)p.groups * d.q.ci * d.q.co * size;
+  const size_t x = (size_t)p.rows * d.q.ci * size, y = (size_t)p.rows * d.q.co * size,
+               w = (size_t)p.groups * d.q.ci * d.q.co * size;
   auto bytes = [](bool there, size_t n) { return there ? (n + 255) / 256 * 256 : 0; };
   d.left = filter || forward ? ci : co;
   d.right = filter ? co : true;
@@ -1359,8 +1362,8 @@ Padded padded(const Problem &p, int cu_count) {
 }
 
 // `blocks` blocks of rows x width elements at `at` and their padded copy.
-Copy copyOf(const void *at, void *copy, int64_t stride, int64_t blocks, int rows, int padded_rows, int width, int padded_width, int size,
-            bool of_groups) {
+Copy copyOf(const void *at, void *copy, int64_t stride, int64_t blocks, int rows, int padded_rows, int width,
+            int padded_width, int size, bool of_groups) {
   Copy c = {};
   c.from = static_cast<const char *>(at);
   c.to = static_cast<char *>(copy);
@@ -1396,7 +1399,8 @@ hipError_t launchPadded(const LaunchCtx &lc, const Problem &p, Padded d, int cu_
     const bool x = filter || forward;
     q.left = workspace;
     q.left_stride = x ? q.ci : q.co;
-    copies[count++] = copyOf(p.left, workspace, p.left_stride, 1, p.rows, p.rows, x ? p.ci : p.co, (int)q.left_stride, kSize, false);
+    copies[count++] = copyOf(p.left, workspace, p.left_stride, 1, p.rows, p.rows, x ? p.ci : p.co, (int)q.left_stride, kSize,
+                             false);
     workspace += d.left_bytes;
   }
   if (d.right) {

@@ -157,8 +157,8 @@ class SparseTensor:
                             self.distinct, self.ordered)
 
     def _rows_of_samples(self):
-        """(order, places, starts), None for one sample: the rows sample after sample and the place of every row among them (int32,
-        None where they lie so), and where every sample's begin (int32 [batch_size + 1]).  Kept with the rulebooks."""
+        """(order, places, starts), None for one sample: the rows sample after sample and the place of every row among them
+        (int32, None where they lie so), and where every sample's begin (int32 [batch_size + 1]).  Kept with the rulebooks."""
         if self.batch_size == 1:
             return None, None, None
         kept = self.rulebooks.get(("samples", id(self.indices)))

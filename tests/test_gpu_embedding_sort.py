@@ -72,7 +72,7 @@ def test_rows_around_the_pieces_in_use(gpu_handle, channels, shared, piece, case
     import mluop_hip
     lengths = lengths_around(piece)[case]
     print("embedding pieces", channels, shared, piece, case, flush=True)
-    tokens = torch.repeat_interleave(torch.arange(len(lengths), device="cuda"), torch.tensor(lengths, device="cuda")).to(torch.int32)
+    tokens = torch.arange(len(lengths), device="cuda").repeat_interleave(torch.tensor(lengths, device="cuda")).to(torch.int32)
     n = tokens.numel()
     rows = len(lengths) if shared else max(len(lengths) + 3, n // 24 + 1)
     if shared and n < 24 * rows:   # (rows of one word: more words of the last row)

@@ -65,6 +65,7 @@ def test_results_are_weighed_and_added_in_32_bits(dtype, choices):
     terms = rows["out"].double()[places] * torch.softmax(scores.double(), dim=1).unsqueeze(2)
     want, size = terms.sum(dim=1), terms.abs().sum(dim=1)
     last = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
-    # scores and softmax in fp32 (a score of a few units: its exponential is off by some units in the last place), products and sums
+    # scores and softmax in fp32 (a score of a few units: its exponential is off by some units in the last place), products
+    # and sums
     room = (choices + 32) * 2.0 ** -23 * size + last * want.abs() + 2.0 ** -25
     assert bool(((out.double() - want).abs() <= room).all())

@@ -37,7 +37,8 @@ def test_starts_that_make_no_sense_stay_in_bounds(gpu_handle, rows, channels, jo
 
 
 # (groups narrower than a vector, as wide, and wider)
-@pytest.mark.parametrize("dtype,channels,groups", [("float16", 48, 16), ("bfloat16", 32, 8), ("float32", 24, 2), ("float16", 33, 3)])
+@pytest.mark.parametrize("dtype,channels,groups", [("float16", 48, 16), ("bfloat16", 32, 8), ("float32", 24, 2),
+                                                   ("float16", 33, 3)])
 def test_results_past_the_caches(gpu_handle, dtype, channels, groups):
     """32 MB of results or more, samples of several tiles, of one row and of none, rows of no sample"""
     import torch

@@ -164,7 +164,7 @@ def test_gradients_that_are_not_finite(gpu_handle, bits, bad):
     got = []
     for g in (grad, spoilt):
         p = start.clone()
-        states = [torch.zeros(n, device="cuda") if bits == 32 else torch.zeros(n, dtype=torch.uint8, device="cuda") for _ in range(2)]
+        states = [torch.zeros(n, dtype=torch.float32 if bits == 32 else torch.uint8, device="cuda") for _ in range(2)]
         scales = [[torch.zeros(4, device="cuda")] for _ in range(2)] if bits == 8 else [None, None]
         plan = mluop_hip.AdamWTensors([p], states[:1], states[1:], None, *scales)
         plan.step(gpu_handle, [g], 1, **HYPER)
@@ -198,7 +198,7 @@ def test_roots_of_numbers_below_the_smallest_normal(gpu_handle, bits, size):
     n = 512
     sign = torch.where(torch.arange(n, device="cuda") % 3 == 0, -1.0, 1.0)
     p = torch.zeros(n, device="cuda")
-    states = [torch.zeros(n, device="cuda") if bits == 32 else torch.zeros(n, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    states = [torch.zeros(n, dtype=torch.float32 if bits == 32 else torch.uint8, device="cuda") for _ in range(2)]
     scales = [[torch.zeros(2, device="cuda")] for _ in range(2)] if bits == 8 else [None, None]
     mluop_hip.AdamWTensors([p], states[:1], states[1:], None, *scales).step(
         gpu_handle, [sign * size], 1, lr=0.5, betas=(0.9, 0.5), eps=0.0, weight_decay=0.0)
