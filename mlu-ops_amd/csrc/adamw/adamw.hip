@@ -128,7 +128,7 @@ __device__ __forceinline__ float blockMost(float v) {
 // TINY: a root below the smallest normal number counts.  The hardware's own root and reciprocal take such numbers for zero: that
 // root is below 2^-63, and corrected it is lost beside an eps of 2^25 times that.  With a smaller eps (1.1e-10 in the first
 // step with beta2 = 0.999, 3.6e-12 later on) root and quotient are those that are defined.  us without / with: 250 M bf16
-// parameters with 8-bit states 455 / 482, 33 fp32 tensors of 1.9 M elements in all 9.4 / 10.3, 130 M with masters 675 / 678.
+// parameters with 8-bit states 454 / 467, 33 fp32 tensors of 1.9 M elements in all 9.7 / 10.2, 130 M with masters 676 / 679.
 template <typename P, typename G, bool MASTER, bool EIGHT, bool TINY>
 __global__ __launch_bounds__(kThreads) void adamwStep(Tensors<MASTER, EIGHT> t, Hyper h) {
   typedef Tensors<MASTER, EIGHT> Table;

@@ -108,7 +108,9 @@ template <int V>
 using Lanes = RowLanes<V, kThreads>;
 
 __device__ __forceinline__ float sigmoid(float z) {
-  // (an exponential beyond the range is infinite, and its reciprocal zero)
+  // (An exponential beyond the range is infinite, and its reciprocal zero.  The exponential's argument is rounded once more: SiLU is
+  // off by up to 1.3 (1 + |z|) units of 2^-24 of itself below -5, where z's own rounding moves it by |z| / 2, and by 6 units
+  // around zero; expf and a division have 3.)
   return __builtin_amdgcn_rcpf(1.f + __expf(-z));
 }
 

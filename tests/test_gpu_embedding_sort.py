@@ -3,17 +3,9 @@ pass with few tiles or many, sorts of two and three passes), and rows whose word
 use: small whole numbers, so that every sum is exact in fp32."""
 import pytest
 
+from launches import launched
+
 pytestmark = pytest.mark.gpu
-
-
-def launched(handle, call):
-    """(the call's result, the names of the kernels it launched)"""
-    handle.set_kernel_timing(True)
-    try:
-        out = call()
-        return out, [name for name, _ in handle.kernel_timings()]
-    finally:
-        handle.set_kernel_timing(False)
 
 
 def expected(grad, tokens, rows, scale):

@@ -2,16 +2,9 @@
 no place in LDS (small whole numbers: sums are exact)."""
 import pytest
 
+from launches import launched
+
 pytestmark = pytest.mark.gpu
-
-
-def launched(handle, call):
-    handle.set_kernel_timing(True)
-    try:
-        out = call()
-        return out, [name for name, _ in handle.kernel_timings()]
-    finally:
-        handle.set_kernel_timing(False)
 
 
 @pytest.mark.parametrize("groups,rows,ci,co,kernel", [

@@ -2,16 +2,9 @@
 pass that applies them and by their own launch, and results that go past the caches."""
 import pytest
 
+from launches import launched
+
 pytestmark = pytest.mark.gpu
-
-
-def launched(handle, call):
-    handle.set_kernel_timing(True)
-    try:
-        out = call()
-        return out, [name for name, _ in handle.kernel_timings()]
-    finally:
-        handle.set_kernel_timing(False)
 
 
 @pytest.mark.parametrize("rows,channels,joined", [(5000, 16, False), (9000, 8, False), (60_000, 64, True), (30_000, 20, None)])

@@ -6,6 +6,8 @@ import io
 
 import pytest
 
+from launches import launched
+
 pytestmark = pytest.mark.gpu
 
 HYPER = dict(lr=1e-2, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.03)
@@ -239,12 +241,7 @@ def test_tensors_around_a_launch(gpu_handle, bits, master, most, count):
         return (params, *states, [p.float() for p in params] if master else None, *(scales if bits == 8 else (None, None)))
     together, alone = lists([p.clone() for p in params]), lists([p.clone() for p in params])
     plan = mluop_hip.AdamWTensors(*together)
-    gpu_handle.set_kernel_timing(True)
-    try:
-        plan.step(gpu_handle, grads, 1, **HYPER)
-        names = [name for name, _ in gpu_handle.kernel_timings()]
-    finally:
-        gpu_handle.set_kernel_timing(False)
+    _, names = launched(gpu_handle, lambda: plan.step(gpu_handle, grads, 1, **HYPER))
     assert names == ["adamwStep"] * (1 if tensors <= most else 2 if tensors <= 2 * most else 3)
     for i in range(tensors):
         mluop_hip.AdamWTensors(*[None if x is None else x[i:i + 1] for x in alone]).step(gpu_handle, grads[i:i + 1], 1, **HYPER)
