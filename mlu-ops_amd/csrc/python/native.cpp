@@ -618,6 +618,20 @@ struct LayerRulebook : torch::CustomClassHolder {
 };
 using LayerRulebookPtr = c10::intrusive_ptr<LayerRulebook>;
 
+// A node's gradients, which are made outside of autograd: where they depend on a tensor that it follows, a derivative of
+// them is an error, and not left out.
+torch::autograd::variable_list differentiableOnce(torch::autograd::variable_list grads, at::TensorList depend_on) {
+  const bool followed = std::any_of(depend_on.begin(), depend_on.end(),
+                                    [](const at::Tensor &t) { return t.defined() && t.requires_grad(); });
+  if (!at::GradMode::is_enabled() || !followed) return grads;
+  for (at::Tensor &g : grads)
+    if (g.defined()) g = g.detach().set_requires_grad(true);
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      "this operator's gradient cannot be differentiated: it is differentiable once, not twice",
+      static_cast<int64_t>(grads.size()));
+  return (*error)(std::move(grads));
+}
+
 struct IndiceConv : torch::autograd::Function<IndiceConv> {
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &features,
                             const at::Tensor &weight, const LayerRulebookPtr &rb, bool inverse, bool share_row_maps,
@@ -679,7 +693,7 @@ struct IndiceConv : torch::autograd::Function<IndiceConv> {
     if (ctx->needs_input_grad(1))
       out[1] = convBackwardFilter(h.handle, buffers, x, dy, rb->pairs, rb->counts(h.handle), rb->filter_space, sub_m,
                                   inverse, true, MLUOP_LAYOUT_ARRAY);
-    return out;
+    return differentiableOnce(std::move(out), {grads[0], x, w});
   }
 };
 

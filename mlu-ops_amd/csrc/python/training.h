@@ -237,20 +237,6 @@ StreamHandle &handleFor(const at::Tensor &t) {
   return streamHandle();
 }
 
-// A node's gradients, which are made outside of autograd: where they depend on a tensor that it follows, a derivative of
-// them is an error, and not left out.
-torch::autograd::variable_list differentiableOnce(torch::autograd::variable_list grads, at::TensorList depend_on) {
-  const bool followed = std::any_of(depend_on.begin(), depend_on.end(),
-                                    [](const at::Tensor &t) { return t.defined() && t.requires_grad(); });
-  if (!at::GradMode::is_enabled() || !followed) return grads;
-  for (at::Tensor &g : grads)
-    if (g.defined()) g = g.detach().set_requires_grad(true);
-  const auto error = std::make_shared<torch::autograd::DelayedError>(
-      "this operator's gradient cannot be differentiated: it is differentiable once, not twice",
-      static_cast<int64_t>(grads.size()));
-  return (*error)(std::move(grads));
-}
-
 struct GroupNorm : torch::autograd::Function<GroupNorm> {
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &features, const at::Tensor &weight,
                             const at::Tensor &bias, int64_t groups, const MaybeTensor &row_starts, double eps,

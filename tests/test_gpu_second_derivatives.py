@@ -1,4 +1,4 @@
-"""The training operators' nodes are differentiable once: a derivative of their gradients is refused, never left out of a sum."""
+"""The library's nodes are differentiable once: a derivative of their gradients is refused, never left out of a sum."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -16,14 +16,17 @@ def operators():
     starts = torch.tensor([0, 7, 20], dtype=torch.int32, device="cuda")
     x, w = randn(20, 8), randn(2, 8, 6)
     weight, bias = randn(8), randn(8)
+    cells = torch.tensor([[0, 0, i // 5, i % 5] for i in range(20)], dtype=torch.int32, device="cuda")
+    conv = spnn.SubMConv3d(8, 4, 3).cuda()
     return [("embedding", lambda t: spnn.embedding(t, tokens, 0.5), randn(9, 5)),
             ("rows", lambda t: spnn.grouped_matmul(t, w.clone().requires_grad_(), starts), x),
             ("filters", lambda t: spnn.grouped_matmul(x, t, starts), w),
             ("norm", lambda t: spnn.group_norm(t, weight, bias, 2, starts, activation="silu"), x),
-            ("norm's weight", lambda t: spnn.group_norm(x, t, bias, 2, starts, activation="silu"), weight)]
+            ("norm's weight", lambda t: spnn.group_norm(x, t, bias, 2, starts, activation="silu"), weight),
+            ("convolution", lambda t: conv(spnn.SparseTensor(t, cells, (1, 5, 5), 1, distinct=True)).features, x)]
 
 
-@pytest.mark.parametrize("which", range(5))
+@pytest.mark.parametrize("which", range(6))
 def test_a_second_derivative_is_refused(which):
     import torch
     name, f, t = operators()[which]
