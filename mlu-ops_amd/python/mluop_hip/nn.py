@@ -139,7 +139,7 @@ class SparseTensor:
 
     `ordered=True` is the caller's word that rows lie sample after sample (a strided layer's do, whatever its input's).  With
     None the first layer that takes statistics by sample looks, once for all layers on these coordinates, and waits for the
-    answer; rows in no order are put into one for it."""
+    answer; rows in no order are put into one for it.  (Behind guard bands the word is checked.)"""
 
     def __init__(self, features, indices, spatial_shape, batch_size, rulebooks=None, distinct=False, ordered=None):
         assert indices.dtype == torch.int32 and indices.dim() == 2 and indices.shape[1] == 4
@@ -169,6 +169,8 @@ class SparseTensor:
                                "captured: say so (ordered=True), or run a layer on it before")
         with torch.no_grad(), torch.inference_mode(False):
             samples, order, places = self.indices[:, 0].contiguous(), None, None
+            if self.ordered and _guarded() and not _capturing() and not _in_sample_order(samples):
+                raise ValueError("a SparseTensor's rows were said to be ordered by sample, and are not")
             if not self.ordered and not (self.ordered is None and _in_sample_order(samples)):
                 samples, order = torch.sort(samples, stable=True)
                 places = torch.empty_like(order, dtype=torch.int32)

@@ -108,6 +108,8 @@ def test_indice_keys_of_any_name(key):
 def test_the_order_is_looked_at_once_and_not_where_it_is_given(monkeypatch):
     import torch
     from mluop_hip import nn as spnn
+    import mluop_hip
+    monkeypatch.setattr(mluop_hip, "GUARD_BYTES", 0)
     looked = []
     real = spnn._in_sample_order
     monkeypatch.setattr(spnn, "_in_sample_order", lambda samples: looked.append(1) or real(samples))
@@ -125,6 +127,14 @@ def test_the_order_is_looked_at_once_and_not_where_it_is_given(monkeypatch):
     one, _ = tensor(True, samples=1)
     norm(one)
     assert not looked
+
+
+def test_a_word_that_is_not_true_is_refused_behind_guard_bands(gpu_handle):
+    from mluop_hip import nn as spnn
+    norm = spnn.GroupNormAct(4, 16).cuda()
+    norm(tensor(False, ordered=True)[0])
+    with pytest.raises(ValueError, match="ordered"):
+        norm(tensor(True, ordered=True)[0])
 
 
 def test_captured():
