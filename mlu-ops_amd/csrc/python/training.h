@@ -237,15 +237,18 @@ StreamHandle &handleFor(const at::Tensor &t) {
   return streamHandle();
 }
 
+inline at::Tensor orNone(const MaybeTensor &t) { return t ? *t : at::Tensor(); }
+
+// (tensors that may be missing are handed to a node as optional ones: one that is missing has no place among its inputs)
 struct GroupNorm : torch::autograd::Function<GroupNorm> {
-  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &features, const at::Tensor &weight,
-                            const at::Tensor &bias, int64_t groups, const MaybeTensor &row_starts, double eps,
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &features, const MaybeTensor &weight,
+                            const MaybeTensor &bias, int64_t groups, const MaybeTensor &row_starts, double eps,
                             int64_t activation, bool guarded) {
     StreamHandle &h = handleFor(features);
     const OperatorLock lock(h);
     const std::vector<at::Tensor> r = groupNormForward(h.handle, guarded, features, weight, bias, groups, row_starts, eps,
                                                        static_cast<int>(activation));
-    ctx->save_for_backward({features, weight, bias, row_starts ? *row_starts : at::Tensor(), r[1], r[2]});
+    ctx->save_for_backward({features, orNone(weight), orNone(bias), orNone(row_starts), r[1], r[2]});
     ctx->saved_data["groups"] = groups;
     ctx->saved_data["activation"] = activation;
     ctx->saved_data["guarded"] = guarded;
@@ -263,7 +266,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
         ctx->saved_data["groups"].toInt(), saved[3], static_cast<int>(ctx->saved_data["activation"].toInt()));
     if (ctx->needs_input_grad(0)) out[0] = r[0];
     if (saved[1].defined() && ctx->needs_input_grad(1)) out[1] = r[1];
-    if (saved[2].defined() && ctx->needs_input_grad(2)) out[2] = r[2];
+    if (saved[2].defined() && ctx->needs_input_grad(saved[1].defined() ? 2 : 1)) out[2] = r[2];
     return differentiableOnce(std::move(out), {grads[0], saved[0], saved[1], saved[2]});
   }
 };
@@ -478,8 +481,7 @@ void defineTraining(py::module_ &m) {
   m.def("group_norm", [](const at::Tensor &features, const MaybeTensor &weight, const MaybeTensor &bias, int64_t groups,
                          const MaybeTensor &row_starts, double eps, int64_t activation, bool guarded) {
     NoGil released;
-    return GroupNorm::apply(features, weight ? *weight : at::Tensor(), bias ? *bias : at::Tensor(), groups, row_starts,
-                            eps, activation, guarded);
+    return GroupNorm::apply(features, weight, bias, groups, row_starts, eps, activation, guarded);
   });
   m.def("embedding_forward", [](uintptr_t handle, bool guarded, const at::Tensor &table, const at::Tensor &tokens,
                                 double scale) {
