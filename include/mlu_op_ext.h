@@ -326,6 +326,100 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGroupedMatmulBackwardFilter(mluOpHandle_t ha
                                                                 int64_t groups, int64_t ci, int64_t co, void *workspace,
                                                                 size_t workspace_size, void *filters_grad);
 
+/* Layer norm: every row [channels] of features [rows, channels] (features_stride elements from row to row) by itself:
+ *   out = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(variance + eps),  variance of the population.
+ * weight and bias [channels] of param_type, FLOAT or `type`; NULL: one and zero.  mean and rstd fp32 [rows] are results that the
+ * backward pass takes.  Backward: input_grad [rows, channels], weight_grad and bias_grad [channels] of param_type (NULL where
+ * not wanted; zero where there are no rows).  At most 2^15 channels. */
+mluOpStatus_t MLUOP_WIN_API mluOpExtLayerNormForward(mluOpHandle_t handle, mluOpDataType_t type, const void *features,
+                                                     int64_t features_stride, int64_t rows, int64_t channels,
+                                                     mluOpDataType_t param_type, const void *weight, const void *bias,
+                                                     float eps, void *out, float *mean, float *rstd);
+mluOpStatus_t MLUOP_WIN_API mluOpExtGetLayerNormBackwardWorkspaceSize(int64_t rows, int64_t channels, size_t *size);
+mluOpStatus_t MLUOP_WIN_API mluOpExtLayerNormBackward(mluOpHandle_t handle, mluOpDataType_t type, const void *output_grad,
+                                                      int64_t output_grad_stride, const void *features,
+                                                      int64_t features_stride, int64_t rows, int64_t channels,
+                                                      mluOpDataType_t param_type, const void *weight, const float *mean,
+                                                      const float *rstd, void *workspace, size_t workspace_size,
+                                                      void *input_grad, void *weight_grad, void *bias_grad);
+
+/* A gated linear recurrence along the rows of every sample, each channel by itself:
+ *   SIGMOID  h_t = a h_(t-1) + (1 - a) x_t,  a = 1 / (1 + exp(-gate_t))
+ *   EXP      h_t = a h_(t-1) + x_t,          a = exp(gate_t)
+ * features and gates [rows, channels]; samples and row_starts as for the group norm; `initial` fp32 [samples, channels] (NULL:
+ * zero) is the state in front of a sample's first row, `final` fp32 [samples, channels] that behind its last (the initial one of a
+ * sample without rows).  reverse: from the last row of a sample to its first.  out [rows, channels]; rows of no sample are not
+ * read, and zero in every result.  carries fp32 [carries of the sizes query, channels] is a result that the backward pass takes,
+ * with the same row_starts, kind and direction.  Backward: final_grad fp32 [samples, channels] (NULL: zero), features_grad and
+ * gates_grad [rows, channels], initial_grad fp32 [samples, channels] (NULL where not wanted).  One workspace size serves
+ * both.  Rows are joined by composing their steps: a value that is not finite is one in the rows behind it (an infinity may be a
+ * NaN there), and in no row in front of it.  At most 2^20 channels and samples. */
+typedef enum {
+  MLUOP_EXT_GATE_SIGMOID = 0,
+  MLUOP_EXT_GATE_EXP = 1
+} mluOpExtGate_t;
+mluOpStatus_t MLUOP_WIN_API mluOpExtGetGatedScanSizes(int64_t rows, int64_t channels, int64_t samples, size_t *carries,
+                                                      size_t *workspace_size);
+mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanForward(mluOpHandle_t handle, mluOpDataType_t type, const void *features,
+                                                     int64_t features_stride, const void *gates, int64_t gates_stride,
+                                                     int64_t rows, int64_t channels, const int32_t *row_starts,
+                                                     int64_t samples, const float *initial, mluOpExtGate_t kind,
+                                                     int reverse, void *workspace, size_t workspace_size, void *out,
+                                                     float *final, float *carries);
+mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanBackward(mluOpHandle_t handle, mluOpDataType_t type, const void *output_grad,
+                                                      int64_t output_grad_stride, const float *final_grad,
+                                                      const void *features, int64_t features_stride, const void *gates,
+                                                      int64_t gates_stride, int64_t rows, int64_t channels,
+                                                      const int32_t *row_starts, int64_t samples, const float *carries,
+                                                      mluOpExtGate_t kind, int reverse, void *workspace,
+                                                      size_t workspace_size, void *features_grad, void *gates_grad,
+                                                      float *initial_grad);
+
+/* Rows into the order of the experts they are sent to, for the grouped products, and the results back.
+ * Order: experts_of_rows [rows, choices] (index_type INT32 or INT64; a number outside [0, experts) is no expert) gives, with the
+ * choices ordered by expert and equal experts by row and choice: ordered_rows int32 [rows * choices], the row at every place
+ * (-1 behind the last expert's); group_starts int32 [experts + 1], where every expert's places begin; places int32 [rows,
+ * choices], the place of every choice (-1 of one without an expert).  At most 2047 experts.
+ * Dispatch: out[places[r, k], :] = features[r, :], out [rows * choices, channels]; places from group_starts[experts] on are zero.
+ * `places` names every place in front of it once, as the order does; an entry outside of out is passed over.
+ * Combine: out[r, :] = sum over k of weights[r, k] * results[places[r, k], :] in the choices' order, nothing for an entry outside
+ * [0, rows * choices); weights [rows, choices] of weight_type, FLOAT or `type`; NULL: one.  Without weights it is the gradient
+ * of the dispatched rows.
+ * Its gradients: results_grad [rows * choices, channels], zero behind the experts' places, and weights_grad [rows, choices] of
+ * weight_type (NULL where not wanted; results are read for it only). */
+mluOpStatus_t MLUOP_WIN_API mluOpExtGetExpertOrderWorkspaceSize(int64_t rows, int64_t choices, int64_t experts,
+                                                                size_t *size);
+mluOpStatus_t MLUOP_WIN_API mluOpExtExpertOrder(mluOpHandle_t handle, mluOpDataType_t index_type,
+                                                const void *experts_of_rows, int64_t rows, int64_t choices,
+                                                int64_t experts, void *workspace, size_t workspace_size,
+                                                int32_t *ordered_rows, int32_t *group_starts, int32_t *places);
+mluOpStatus_t MLUOP_WIN_API mluOpExtExpertDispatch(mluOpHandle_t handle, mluOpDataType_t type, const void *features,
+                                                   int64_t features_stride, int64_t rows, int64_t channels,
+                                                   int64_t choices, const int32_t *places, const int32_t *group_starts,
+                                                   int64_t experts, void *out);
+mluOpStatus_t MLUOP_WIN_API mluOpExtExpertCombine(mluOpHandle_t handle, mluOpDataType_t type, const void *results,
+                                                  int64_t results_stride, int64_t rows, int64_t channels, int64_t choices,
+                                                  const int32_t *places, mluOpDataType_t weight_type, const void *weights,
+                                                  void *out);
+mluOpStatus_t MLUOP_WIN_API mluOpExtExpertCombineBackward(mluOpHandle_t handle, mluOpDataType_t type,
+                                                          const void *output_grad, int64_t output_grad_stride,
+                                                          const void *results, int64_t results_stride, int64_t rows,
+                                                          int64_t channels, int64_t choices, const int32_t *places,
+                                                          const int32_t *group_starts, int64_t experts,
+                                                          mluOpDataType_t weight_type, const void *weights,
+                                                          void *results_grad, void *weights_grad);
+
+/* Dropout onto a residual: out = residual + (kept ? scale * features : 0), `count` values that lie one after the other (residual
+ * NULL: none).  Its gradient for the features is the same call on the output's gradient without a residual.  The probability
+ * of dropping is p in [0, 1], rounded to a multiple of 2^-16, and scale is 1 / (1 - that) (at 1 nothing is kept).  state int64
+ * [2], on the device: the seed and the number of the call.  Eight elements share the four 32-bit words of Philox4x32-10 with
+ * the counter (element / 8 in 64 bits, number of the call in 64 bits) and the seed as key: element 8 g + i has the lower half of
+ * word i / 2 for an even i, the upper for an odd one, and is kept where that is not below p * 2^16.  A value that is dropped does
+ * not count, whatever it is. */
+mluOpStatus_t MLUOP_WIN_API mluOpExtDropoutAdd(mluOpHandle_t handle, mluOpDataType_t type, const void *features,
+                                               const void *residual, int64_t count, double p, const int64_t *state,
+                                               void *out);
+
 #if defined(__cplusplus)
 }
 #endif

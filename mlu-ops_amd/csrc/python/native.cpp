@@ -89,7 +89,19 @@ namespace {
   X(mluOpExtGetGroupedMatmulWorkspaceSize)                 \
   X(mluOpExtGroupedMatmulForward)                          \
   X(mluOpExtGroupedMatmulBackwardData)                     \
-  X(mluOpExtGroupedMatmulBackwardFilter)
+  X(mluOpExtGroupedMatmulBackwardFilter)                   \
+  X(mluOpExtLayerNormForward)                              \
+  X(mluOpExtGetLayerNormBackwardWorkspaceSize)             \
+  X(mluOpExtLayerNormBackward)                             \
+  X(mluOpExtGetGatedScanSizes)                             \
+  X(mluOpExtGatedScanForward)                              \
+  X(mluOpExtGatedScanBackward)                             \
+  X(mluOpExtGetExpertOrderWorkspaceSize)                   \
+  X(mluOpExtExpertOrder)                                   \
+  X(mluOpExtExpertDispatch)                                \
+  X(mluOpExtExpertCombine)                                 \
+  X(mluOpExtExpertCombineBackward)                         \
+  X(mluOpExtDropoutAdd)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -636,6 +648,8 @@ struct IndiceConv : torch::autograd::Function<IndiceConv> {
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &features,
                             const at::Tensor &weight, const LayerRulebookPtr &rb, bool inverse, bool share_row_maps,
                             bool guarded, bool relu) {
+    // (a layer that was not moved to its input's device would have its kernels read host memory)
+    if (weight.device() != features.device()) throw py::value_error("a layer's weight lies on its features' device");
     const at::Tensor x = features.contiguous(), w = weight.contiguous();
     ctx->saved_data["rulebook"] = c10::IValue::make_capsule(rb);
     ctx->saved_data["inverse"] = inverse;
@@ -840,6 +854,7 @@ at::Tensor scatterBackward(mluOpHandle_t handle, const Buffers &buffers, const a
 inline mluOpHandle_t asHandle(uintptr_t h) { return reinterpret_cast<mluOpHandle_t>(h); }
 
 #include "python/training.h"
+#include "python/block.h"
 
 }  // namespace
 
@@ -963,6 +978,7 @@ PYBIND11_MODULE(_native, m) {
         });
 
   defineTraining(m);
+  defineBlock(m);
 
   py::class_<LayerRulebook, LayerRulebookPtr>(m, "LayerRulebook")
       .def(py::init([](const at::Tensor &pairs, std::optional<Counts> counts, int64_t num_act_out, Counts filter_space,

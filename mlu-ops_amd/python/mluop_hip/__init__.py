@@ -626,8 +626,9 @@ def dynamic_point_to_voxel_backward(handle, grad_voxel_feats, feats, voxel_feats
                                                     _REDUCE_MODES[reduce_type])
 
 # the rest of a training step (mlu_op_ext.h)
-from . import training  # noqa: E402
+from . import block, training  # noqa: E402
 
-SIGNATURES.update(training.SIGNATURES)
-for _name in training.__all__:
-    globals()[_name] = getattr(training, _name)
+for _operators in (training, block):
+    SIGNATURES.update(_operators.SIGNATURES)
+    for _name in _operators.__all__:
+        globals()[_name] = getattr(_operators, _name)

@@ -17,6 +17,7 @@ import math
 import torch
 
 from . import Handle, _capturing, _guarded, get_indice_pairs, native, regular_output_space, rulebook_counts
+from .block import GATES
 from .training import ACTIVATIONS
 
 _handles = {}
@@ -408,19 +409,44 @@ class ExpertLinear(torch.nn.Module):
         return grouped_matmul(features, self.weight.to(features.dtype), group_starts)
 
 
+_MOST_EXPERTS = 2047  # that the library orders
+
+
 def expert_order(experts_of_rows, experts):
-    """(rows, group_starts, places) of a routing [rows, choices] of integers in [0, experts): the source row of every place
-    when all choices are ordered by expert (equal experts by row), int32 [rows * choices]; where each expert's
-    places begin, int32 [experts + 1]; and the place of every row's choices, int32 [rows, choices].
-    `embedding(features, rows)` puts rows into that order, and its gradient adds the copies of a row up again;
-    `embedding(results, places)` brings the results back."""
-    flat = experts_of_rows.reshape(experts_of_rows.shape[0], math.prod(experts_of_rows.shape[1:]))
+    """(rows, group_starts, places) of a routing [rows, choices] of integers: the source row of every place when all choices are
+    ordered by expert (equal experts by row), int32 [rows * choices]; where each expert's places begin, int32 [experts + 1]; and
+    the place of every row's choices, int32 [rows, choices].  A number outside [0, experts) is no expert: its choice has place -1,
+    and the places behind the last expert's have row -1.
+    `expert_dispatch(features, places, group_starts)` puts rows into that order, and `expert_combine(results, places,
+    group_starts, weights)` brings the results back."""
+    choices = math.prod(experts_of_rows.shape[1:])
+    if (experts_of_rows.is_cuda and experts_of_rows.dtype in (torch.int32, torch.int64) and choices > 0 and
+            0 < experts <= _MOST_EXPERTS and experts_of_rows.device.index == torch.cuda.current_device() and _unwatched()):
+        flat = experts_of_rows.detach().reshape(experts_of_rows.shape[0], choices)
+        return native().expert_order(native().stream_handle(), _guarded(), flat, experts)
+    flat = experts_of_rows.reshape(experts_of_rows.shape[0], choices)
+    flat = torch.where((flat >= 0) & (flat < experts), flat.long(), experts)
     ordered, order = torch.sort(flat.reshape(-1), stable=True)
     starts = torch.searchsorted(ordered, torch.arange(experts + 1, device=flat.device, dtype=ordered.dtype), out_int32=True)
     places = torch.empty_like(order, dtype=torch.int32)
     places[order] = torch.arange(order.shape[0], device=flat.device, dtype=torch.int32)
     rows = torch.div(order, max(flat.shape[1], 1), rounding_mode="floor").to(torch.int32)
-    return rows, starts, places.view(flat.shape)
+    return (torch.where(ordered < experts, rows, -1), starts,
+            torch.where(flat < experts, places.view(flat.shape), -1))
+
+
+def expert_dispatch(features, places, group_starts):
+    """Rows of `features` [rows, channels] at the places of their choices (`expert_order`), on the current device, with
+    autograd: [rows * choices, channels], zeros behind the last expert's places.  A row is read once, and the gradients of its
+    copies are added up in 32 bits, in the choices' order."""
+    return native().expert_dispatch(features, places, group_starts, _guarded())
+
+
+def expert_combine(results, places, group_starts, weights=None):
+    """Results [rows * choices, channels] of rows in expert order back at their rows, times `weights` [rows, choices] of their
+    type or float32 (None: one) and added up in 32 bits with one rounding: [rows, channels], with autograd for both.  A choice
+    without a place adds nothing."""
+    return native().expert_combine(results, weights, places, group_starts, _guarded())
 
 
 class ExpertMLP(torch.nn.Module):
@@ -437,12 +463,10 @@ class ExpertMLP(torch.nn.Module):
 
     def forward(self, features):
         scores, chosen = torch.topk(self.gate(features.to(self.gate.weight.dtype)), self.choices, dim=1)
-        rows, starts, places = expert_order(chosen, self.experts)
-        hidden = torch.nn.functional.silu(self.up(embedding(features, rows), starts))
-        results = embedding(self.down(hidden, starts), places)
+        _, starts, places = expert_order(chosen, self.experts)
+        hidden = torch.nn.functional.silu(self.up(expert_dispatch(features, places, starts), starts))
         # (weights, products and sums in 32 bits whatever the rows' type, and one rounding)
-        weights = torch.softmax(scores.float(), dim=1)
-        return (results * weights.unsqueeze(2)).sum(dim=1).to(results.dtype)
+        return expert_combine(self.down(hidden, starts), places, starts, torch.softmax(scores.float(), dim=1))
 
 
 def group_norm(features, weight, bias, groups, row_starts=None, eps=1e-5, activation="none"):
@@ -476,6 +500,106 @@ class GroupNormAct(torch.nn.Module):
         rows = x.features if order is None else embedding(x.features, order)
         rows = group_norm(rows, self.weight, self.bias, self.groups, starts, self.eps, self.activation)
         return x.replace_features(rows if order is None else embedding(rows, places))
+
+
+def layer_norm(features, weight, bias, eps=1e-5):
+    """Layer norm over the last dimension of `features` on the current device, with autograd.  `weight` and `bias` [channels] are
+    of the features' type or float32, or None."""
+    rows = features.reshape(math.prod(features.shape[:-1]), features.shape[-1])
+    return native().layer_norm(rows, weight, bias, eps, _guarded()).view(features.shape)
+
+
+class LayerNorm(torch.nn.Module):
+    """Layer norm over the channels of every row.  Takes a SparseTensor, or a tensor whose last dimension is the channels; the
+    parameters may be float32 whatever the features are."""
+
+    def __init__(self, channels, eps=1e-5, affine=True):
+        super().__init__()
+        self.channels, self.eps = int(channels), float(eps)
+        self.weight = torch.nn.Parameter(torch.ones(channels)) if affine else None
+        self.bias = torch.nn.Parameter(torch.zeros(channels)) if affine else None
+
+    def forward(self, x):
+        if isinstance(x, SparseTensor):
+            return x.replace_features(layer_norm(x.features, self.weight, self.bias, self.eps))
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+
+def gated_scan(features, gates, row_starts=None, initial=None, kind="sigmoid", reverse=False):
+    """(out, final): h_t = a h_(t-1) + (1 - a) x_t with a = sigmoid(gate_t), or ("exp") h_t = a h_(t-1) + x_t with a = exp(gate_t),
+    along the rows of every sample of `features` and `gates` [rows, channels] on the current device, with autograd.  Rows
+    row_starts[s] to row_starts[s + 1] - 1 are sample s (int32 on the device; None: one sample of all rows); `reverse` takes them
+    from the last to the first.  `initial` and `final` are float32 [samples, channels], the states in front of a sample and
+    behind it: with them, and one row a sample, it is the step of a program that answers."""
+    return native().gated_scan(features, gates, row_starts, initial, GATES[kind], reverse, _guarded())
+
+
+class GatedScan(torch.nn.Module):
+    """Mixes the rows of every sample along their order: features and gates of `hidden` channels by a learned linear map, the gated
+    recurrence over them, and a linear map back.
+
+    Takes a SparseTensor (rows that are not ordered by sample are put into that order and back; within a sample they are taken
+    as they lie), or a tensor [rows, channels] with `row_starts`.  `forward(rows, row_starts, initial, states=True)` also
+    returns the states behind each sample."""
+
+    def __init__(self, channels, hidden=None, kind="sigmoid", reverse=False):
+        super().__init__()
+        hidden = int(channels if hidden is None else hidden)
+        self.kind, self.reverse = kind, bool(reverse)
+        GATES[kind]
+        self.into = torch.nn.Linear(channels, 2 * hidden)
+        self.back = torch.nn.Linear(hidden, channels)
+        with torch.no_grad():   # memories of a few rows to begin with
+            self.into.bias[hidden:].fill_(1.0 if kind == "sigmoid" else 0.0)
+
+    def forward(self, x, row_starts=None, initial=None, states=False):
+        if isinstance(x, SparseTensor):
+            order, places, starts = x._rows_of_samples()
+            rows = x.features if order is None else embedding(x.features, order)
+            rows = self.forward(rows, starts)
+            return x.replace_features(rows if order is None else embedding(rows, places))
+        into, back = self.into, self.back
+        both = torch.nn.functional.linear(x, into.weight.to(x.dtype), into.bias.to(x.dtype))
+        features, gates = both.chunk(2, dim=1)
+        if self.kind == "exp":   # (a decay is below one)
+            gates = -torch.nn.functional.softplus(-gates)
+        out, final = gated_scan(features, gates, row_starts, initial, self.kind, self.reverse)
+        out = torch.nn.functional.linear(out, back.weight.to(x.dtype), back.bias.to(x.dtype))
+        return (out, final) if states else out
+
+
+def dropout_add(features, residual, p, state):
+    """residual + dropout of `features` on the current device, with autograd (`residual` may be None).  An element is dropped with
+    probability p, taken to a multiple of 2^-16, and divided by 1 - p otherwise.  `state` int64 [2] on the device, a seed and the
+    number of the call, decides together with an element's number: the backward pass computes the mask again, so that the
+    tensor may not be changed in between."""
+    return native().dropout_add(features, residual, p, state, _guarded())
+
+
+class DropoutAdd(torch.nn.Module):
+    """Dropout of features onto a residual, `forward(features, residual=None)`, tensors or SparseTensors.  Every call in training
+    mode has a number of its own, which is counted on the device: a captured graph drops other elements at every replay.  The seed
+    is drawn from torch's generator where none is given; it and the count are saved with the module's state."""
+
+    def __init__(self, p, seed=None):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError("p lies in [0, 1]")
+        self.p = float(p)
+        seed = int(torch.randint(0, 2 ** 62, ())) if seed is None else int(seed)
+        self.register_buffer("state", torch.tensor([seed, 0], dtype=torch.int64))
+        self.register_buffer("_next", torch.tensor([0, 1], dtype=torch.int64), persistent=False)
+
+    def forward(self, features, residual=None):
+        if isinstance(features, SparseTensor):
+            return features.replace_features(
+                self.forward(features.features, residual.features if isinstance(residual, SparseTensor) else residual))
+        if not self.training or self.p == 0.0:
+            return features if residual is None else residual + features
+        with torch.no_grad():
+            state = self.state.clone()
+            self.state.add_(self._next)
+        return dropout_add(features, residual, self.p, state)
 
 
 class SparseSequential(torch.nn.Sequential):
@@ -523,7 +647,7 @@ class SparseSequential(torch.nn.Sequential):
                     # (features are not looked at while planning: a view of the right height)
                     cells = SparseTensor(indices.new_empty((indices.shape[0], 0)), indices, space,
                                          cells.batch_size, cells.rulebooks, distinct, m._order_after(cells, rb))
-            elif isinstance(m, GroupNormAct) and type(m).forward is GroupNormAct.forward:
+            elif isinstance(m, (GroupNormAct, GatedScan)) and type(m).forward in (GroupNormAct.forward, GatedScan.forward):
                 # (what is waited for is waited for here, too)
                 cells._rows_of_samples()
         return cells
@@ -551,7 +675,7 @@ class SparseSequential(torch.nn.Sequential):
                 # a launch and a pass over the result less each: voxelizer and 11-layer encoder 1085 -> 1007 us,
                 # the encoder's training step 3231 -> 3095 us
                 x, stored = m._convolve(x, relu=True), following
-            elif isinstance(m, (_ConvBase, SparseSequential, GroupNormAct)):
+            elif isinstance(m, (_ConvBase, SparseSequential, GroupNormAct, GatedScan)):
                 x = m(x)
             else:
                 x = x.replace_features(m(x.features))
