@@ -28,17 +28,22 @@ using namespace mluop;
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kAcross = 16, kTeams = 64 / kAcross;  // lanes side by side, and teams of them behind one another
-constexpr int kRows = 8;                            // of a thread in a step
-// Rows that a wave takes at a time.  The states in front of every step are what the backward pass takes: the same for all types
-// and alignments.
-constexpr int kStepRows = kTeams * kRows;
-constexpr int kTileSteps = 4, kTileRows = kTileSteps * kStepRows;  // of a wave
-constexpr int kOutsideBlocks = 16;  // workgroups for the rows of no sample
+constexpr int kPiece = 8;                           // rows of a thread that are read together
+constexpr int kTileRows = 2 * kPiece * kTeams;      // of a wave
+// Rows that a thread, and a wave, applies at a time.  The states in front of every step are what the backward pass takes: the same
+// for all types and alignments.  (Eight rows have an a and a u each in registers, and leave two or three waves a SIMD: 248 636 x
+// 128 fp16 44 us to apply, four rows 39; gradients of 65 536 x 1024 bf16 135 and 120.)
+constexpr int kRows = 4, kStepRows = kTeams * kRows;
+constexpr int kOutsideBlocks = 8;  // workgroups of every slab for the rows of no sample
+
+// Who works out the states in front of the tiles: nobody (a wave has a whole sample), every wave for itself, a launch of its own.
+enum Joining { kWhole, kFolded, kJoined };
 
 struct Shape {
   int rows, channels, samples;
   int64_t x_stride, g_stride, dh_stride;  // elements from row to row; results lie row by row
-  int most_tiles, slabs;
+  int most_tiles;
+  int side_by_side;  // waves of a workgroup that have slabs of the same rows
   const int32_t *starts;
   bool reverse;
   bool streamed;  // results go past the caches
@@ -58,38 +63,47 @@ struct Work {
   static constexpr int kChannels = kAcross * V;
   int64_t first, tile_slot, step_slot;
   int step, rows, sample;  // sample -1: nothing
+  int in_sample, tiles;    // the tile's number in its sample, and how many that has
   int team, channel;
   bool there;              // this lane has channels; one that has none reads what the slab's first has
 
-  __device__ Work(int64_t unit, const Shape &s) : sample(-1) {
-    const int lane = (int)threadIdx.x % kAcross;
+  // Slabs lie along x, and as many of a workgroup's waves as can be have slabs side by side, so that it reads what lies together
+  // (four tiles of one slab: 35 us to read 248 636 x 128 fp16 in place of 31); tiles, or samples, along y.  FROM_LAST: the launch
+  // before had them in order, and what it had last comes first.
+  __device__ Work(const Shape &s, int64_t block, int64_t blocks, bool from_last) : sample(-1) {
+    const int lane = (int)threadIdx.x % kAcross, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
     team = (int)threadIdx.x / kAcross % kTeams;
-    const int64_t of = unit / s.slabs;
-    channel = (int)(unit - of * s.slabs) * kChannels + lane * V;
-    there = channel < s.channels;
-    if (!there) channel -= lane * V;
-    int segment_first, segment_rows, in_segment = 0;
+    channel = ((int)blockIdx.x * s.side_by_side + wave % s.side_by_side) * kChannels;
+    if (channel >= s.channels) return;
+    there = channel + lane * V < s.channels;
+    if (there) channel += lane * V;
+    const int of = (int)(from_last ? blocks - 1 - block : block) * (kWaves / s.side_by_side) + wave / s.side_by_side;
+    int segment_first, segment_rows;
+    in_sample = 0;
     if (WHOLE) {
       if (of >= s.samples) return;
-      sample = (int)of;
+      sample = of;
       segmentRows(s.starts, s.rows, sample, &segment_first, &segment_rows);
       rows = segment_rows;
     } else {
       if (of >= s.most_tiles) return;
-      const RaggedTile t = findRaggedTile<false>(s.starts, s.rows, s.samples, kTileRows, (int)of);
+      const RaggedTile t = findRaggedTile<false>(s.starts, s.rows, s.samples, kTileRows, of);
       if (t.segment < 0) return;
       sample = t.segment;
       segment_first = t.segment_first;
       segment_rows = t.segment_rows;
-      in_segment = t.in_segment;
+      in_sample = t.in_segment;
       rows = t.rows;
     }
+    const int from = in_sample * kTileRows;
+    tiles = (segment_rows + kTileRows - 1) / kTileRows;
     step = s.reverse ? -1 : 1;
-    first = s.reverse ? (int64_t)segment_first + segment_rows - 1 - (int64_t)in_segment * kTileRows
-                      : (int64_t)segment_first + (int64_t)in_segment * kTileRows;
-    tile_slot = firstSlot<kTileRows>(sample, segment_first) + in_segment;
-    step_slot = firstSlot<kStepRows>(sample, segment_first) + (int64_t)in_segment * kTileSteps;
+    first = s.reverse ? (int64_t)segment_first + segment_rows - 1 - from : (int64_t)segment_first + from;
+    tile_slot = firstSlot<kTileRows>(sample, segment_first) + in_sample;
+    step_slot = firstSlot<kStepRows>(sample, segment_first) + from / kStepRows;
   }
+  __device__ __forceinline__ bool begins() const { return in_sample == 0; }
+  __device__ __forceinline__ bool ends() const { return WHOLE || in_sample == tiles - 1; }
   __device__ __forceinline__ int steps() const { return (rows + kStepRows - 1) / kStepRows; }
 };
 
@@ -114,18 +128,6 @@ struct Lines {
   }
 };
 constexpr int64_t kMostStride = (int64_t)1 << 23;  // elements from row to row: offsets stay within 32 bits
-
-// The wave's unit of work.  Workgroups go round the 8 XCDs one by one.  FROM_LAST: what the launch before had last comes first, on
-// the XCDs whose caches have it.
-constexpr int kXcds = 8;
-__device__ __forceinline__ int64_t unitOf(int64_t block, int64_t blocks, bool from_last) {
-  if (from_last) block = (blocks / kXcds - 1 - block / kXcds) * kXcds + block % kXcds;
-  return block * kWaves + __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
-}
-int64_t blocksOf(int64_t units, int slabs) {
-  const int64_t blocks = (units * slabs + kWaves - 1) / kWaves;
-  return (blocks + kXcds - 1) / kXcds * kXcds;
-}
 
 // a and u of a gate: a row's step is h -> a h + u x.  Half of what these kernels compute is here.  What has to be exact is an a
 // close to one, whose error all steps of a long memory repeat: it is what a small u leaves of one.  An exponential beyond the
@@ -153,23 +155,23 @@ struct Word<4> { typedef uint32_t type; };
 template <>
 struct Word<2> { typedef uint16_t type; };
 
-template <typename T, int V>
+template <typename T, int V, int R>
 struct Rows {
   typedef typename Word<sizeof(T) * V>::type W;
-  W at[kRows];
+  W at[R];
   template <int TEAM_ROWS, typename WORK>
   __device__ __forceinline__ void load(const T *from, int64_t stride, const WORK &w, int first, float none) {
     const Lines<T, TEAM_ROWS> lines(from, stride, w, first);
-    if (first + (kTeams - 1) * TEAM_ROWS + kRows <= w.rows) {
+    if (first + (kTeams - 1) * TEAM_ROWS + R <= w.rows) {
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) at[r] = *reinterpret_cast<const W *>(lines.row(r));
+      for (int r = 0; r < R; ++r) at[r] = *reinterpret_cast<const W *>(lines.row(r));
       return;
     }
     Vector<T, V> empty;
 #pragma unroll
     for (int i = 0; i < V; ++i) empty.v[i] = (T)none;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
+    for (int r = 0; r < R; ++r) {
       at[r] = __builtin_bit_cast(W, empty);
       if (first + w.team * TEAM_ROWS + r < w.rows) at[r] = *reinterpret_cast<const W *>(lines.row(r));
     }
@@ -236,32 +238,32 @@ __device__ __forceinline__ void composeTeams(int team, float &a, float &b, float
 // ---- forward -------------------------------------------------------------------------------
 
 // What a tile does to the state that comes into it, to tiles[slot][channel].  GRAD: to the gradient that comes into it from behind.
-// A team has 32 rows of the tile here, and the teams are composed once.
+// A team has 16 rows of a tile here, and the teams are composed once.
 template <typename T, int V, int KIND, bool GRAD>
 __global__ __launch_bounds__(kThreads) void gatedScanTiles(const T *__restrict__ x, const T *__restrict__ g, Shape s,
-                                                           int64_t first_block, int64_t blocks, float2 *__restrict__ tiles) {
-  const Work<V, false> w(unitOf(first_block + blockIdx.x, blocks, false), s);
+                                                           int64_t first_block, float2 *__restrict__ tiles) {
+  const Work<V, false> w(s, first_block + blockIdx.y, 0, false);
   if (w.sample < 0) return;
   const int64_t x_stride = GRAD ? s.dh_stride : s.x_stride;
+  constexpr int kPieces = kTileRows / kTeams / kPiece;
   float a[V], b[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     a[i] = 1.f;
     b[i] = 0.f;
   }
-  // (8 rows of it are on their way while 8 others are composed)
   struct Piece {
-    Rows<T, V> x, g;
+    Rows<T, V, kPiece> x, g;
   } one, other;
   auto load = [&](Piece &p, int k) {
-    const int first = (GRAD ? kTileSteps - 1 - k : k) * kRows;
-    p.g.template load<kTileSteps * kRows>(g, s.g_stride, w, first, idle<KIND>());
-    p.x.template load<kTileSteps * kRows>(x, x_stride, w, first, 0.f);
+    const int first = (GRAD ? kPieces - 1 - k : k) * kPiece;
+    p.g.template load<kTileRows / kTeams>(g, s.g_stride, w, first, idle<KIND>());
+    p.x.template load<kTileRows / kTeams>(x, x_stride, w, first, 0.f);
   };
   auto compose = [&](const Piece &p) {
 #pragma unroll
-    for (int q = 0; q < kRows; ++q) {
-      const int r = GRAD ? kRows - 1 - q : q;
+    for (int q = 0; q < kPiece; ++q) {
+      const int r = GRAD ? kPiece - 1 - q : q;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         float ga, u;
@@ -272,12 +274,14 @@ __global__ __launch_bounds__(kThreads) void gatedScanTiles(const T *__restrict__
       }
     }
   };
+  // (a loop whatever the number of pieces: in a straight line the compiler mixes what it computes of two, and their loads are waited
+  // for together: 38 us in place of 31)
   load(one, 0);
 #pragma unroll 1
-  for (int k = 0; k < kTileSteps; k += 2) {
+  for (int k = 0; k < kPieces; k += 2) {
     load(other, k + 1);
     compose(one);
-    if (k + 2 < kTileSteps) load(one, k + 2);
+    if (k + 2 < kPieces) load(one, k + 2);
     compose(other);
   }
 #pragma unroll
@@ -288,100 +292,177 @@ __global__ __launch_bounds__(kThreads) void gatedScanTiles(const T *__restrict__
   }
 }
 
-// The state at every tile's beginning (from that of its sample, zero where there is none), to carries[slot][channel], and behind
-// the last tile.  FROM_LAST: tiles from a sample's last to its first.  kJoinChannels channels of a sample a workgroup; its tiles
-// are cut into runs, one for each of the threads that share a channel.  A run of up to kJoinAhead is read once.
-constexpr int kJoinThreads = 512, kJoinChannels = 8, kJoinRuns = kJoinThreads / kJoinChannels, kJoinAhead = 8;
+// The state in front of every tile (from that of its sample, zero where there is none), to states[slot][channel], and behind the
+// last.  FROM_LAST: tiles from a sample's last to its first.  kJoinChannels channels of a sample a workgroup; its tiles are cut
+// into runs of kJoinRun, one for each of the threads that share a channel, and are read once: kJoinTiles at a time.
+constexpr int kJoinThreads = 512, kJoinChannels = 8, kJoinRun = 16;
+constexpr int kJoinTiles = kJoinThreads / kJoinChannels * kJoinRun;
 template <bool FROM_LAST>
 __global__ __launch_bounds__(kJoinThreads) void gatedScanJoin(const float2 *__restrict__ tiles, Shape s, int first_sample,
                                                               const float *__restrict__ initial,
-                                                              float *__restrict__ carries, float *__restrict__ final) {
-  __shared__ float s_a[kJoinRuns][kJoinChannels], s_b[kJoinRuns][kJoinChannels];
+                                                              float *__restrict__ states, float *__restrict__ final) {
+  constexpr int kJoinWaves = kJoinThreads / 64;
+  __shared__ float2 s_wave[kJoinWaves][kJoinChannels];
   const int sample = first_sample + (int)blockIdx.y;
   int first, rows;
   segmentRows(s.starts, s.rows, sample, &first, &rows);
   const int count = (rows + kTileRows - 1) / kTileRows;
-  const int lane = threadIdx.x % kJoinChannels, run = threadIdx.x / kJoinChannels;
+  const int lane = threadIdx.x % kJoinChannels, run = threadIdx.x / kJoinChannels, wave = threadIdx.x / 64;
   const int channel = (int)blockIdx.x * kJoinChannels + lane;
   const bool there = channel < s.channels;
-  const int per = (count + kJoinRuns - 1) / kJoinRuns, lo = min(run * per, count), hi = there ? min(lo + per, count) : lo;
   const int64_t slot = firstSlot<kTileRows>(sample, first);
-  auto at = [&](int tile) { return (slot + (FROM_LAST ? count - 1 - tile : tile)) * s.channels + channel; };
-  float h = initial == nullptr || !there ? 0.f : initial[(int64_t)sample * s.channels + channel];
-  float a = 1.f, b = 0.f;
-  float2 v[kJoinAhead];
-  for (int t0 = lo; t0 < hi; t0 += kJoinAhead) {
+  auto at = [&](int tile) { return (slot + (FROM_LAST ? count - 1 - tile : tile)) * s.channels + (there ? channel : 0); };
+  float h0 = initial == nullptr || !there ? 0.f : initial[(int64_t)sample * s.channels + channel];
+  for (int t0 = 0; t0 < count; t0 += kJoinTiles) {
+    // (runs of one length as short as they can be)
+    const int here = min(count - t0, kJoinTiles), per = (here + kJoinTiles / kJoinRun - 1) / (kJoinTiles / kJoinRun);
+    const int lo = t0 + run * per, left = min(per, t0 + here - lo);
+    float2 v[kJoinRun];
 #pragma unroll
-    for (int j = 0; j < kJoinAhead; ++j) v[j] = tiles[at(min(t0 + j, hi - 1))];
+    for (int j = 0; j < kJoinRun; ++j) {
+      v[j] = make_float2(1.f, 0.f);
+      if (j < left) v[j] = tiles[at(lo + j)];
+    }
+    float a = 1.f, b = 0.f;
 #pragma unroll
-    for (int j = 0; j < kJoinAhead; ++j) {
-      if (t0 + j >= hi) break;
+    for (int j = 0; j < kJoinRun; ++j) {
       b = fmaf(v[j].x, b, v[j].y);
       a *= v[j].x;
     }
-  }
-  s_a[run][lane] = a;
-  s_b[run][lane] = b;
-  __syncthreads();
-  if (!there) return;
-  for (int q = 0; q < run; ++q) h = fmaf(s_a[q][lane], h, s_b[q][lane]);
-  for (int t0 = lo; t0 < hi; t0 += kJoinAhead) {
-    if (per > kJoinAhead) {
+    // the runs in front: of this wave, then of those before
 #pragma unroll
-      for (int j = 0; j < kJoinAhead; ++j) v[j] = tiles[at(min(t0 + j, hi - 1))];
+    for (int d = kJoinChannels; d < 64; d <<= 1) {
+      const float fa = __shfl_up(a, d, 64), fb = __shfl_up(b, d, 64);
+      const bool has = (int)(threadIdx.x & 63) >= d;
+      b = has ? fmaf(a, fb, b) : b;
+      a = has ? a * fa : a;
     }
+    __syncthreads();
+    if ((threadIdx.x & 63) >= 64 - kJoinChannels) s_wave[wave][lane] = make_float2(a, b);
+    float ea = __shfl_up(a, kJoinChannels, 64), eb = __shfl_up(b, kJoinChannels, 64);
+    if ((threadIdx.x & 63) < kJoinChannels) {
+      ea = 1.f;
+      eb = 0.f;
+    }
+    __syncthreads();
+    float h = h0;
 #pragma unroll
-    for (int j = 0; j < kJoinAhead; ++j) {
-      if (t0 + j >= hi) break;
-      carries[at(t0 + j)] = h;
+    for (int q = 0; q < kJoinWaves; ++q) {
+      const float2 m = s_wave[q][lane];
+      h0 = fmaf(m.x, h0, m.y);
+      h = q + 1 == wave ? h0 : h;
+    }
+    h = fmaf(ea, h, eb);
+#pragma unroll
+    for (int j = 0; j < kJoinRun; ++j) {
+      if (j < left && there) states[at(lo + j)] = h;
       h = fmaf(v[j].x, h, v[j].y);
     }
   }
-  if (run == kJoinRuns - 1 && final != nullptr) final[(int64_t)sample * s.channels + channel] = h;
+  if (run == 0 && there && final != nullptr) final[(int64_t)sample * s.channels + channel] = h0;
 }
 
-// The rows of no sample, which are zero in every result: by workgroup `block` of kOutsideBlocks.
+// The state that comes into a wave's rows: from the one in front of its tile (JOINED), or of its sample through the tiles in front.
+// FROM_LAST: the gradient that comes in from behind.  `states` are those of the tiles or the samples (null: zero).
+template <int V, Joining JOINING, bool FROM_LAST, typename WORK>
+__device__ __forceinline__ void incoming(const WORK &w, const Shape &s, const float *states, const float2 *tiles,
+                                         float (&h)[V]) {
+  const int64_t from = (JOINING == kJoined ? w.tile_slot : (int64_t)w.sample) * s.channels + w.channel;
+#pragma unroll
+  for (int i = 0; i < V; ++i) h[i] = states == nullptr ? 0.f : states[from + i];
+  if (JOINING != kFolded) return;
+  // a quarter of the tiles by each team
+  const int count = FROM_LAST ? w.tiles - 1 - w.in_sample : w.in_sample;
+  const int per = (count + kTeams - 1) / kTeams, lo = min(w.team * per, count), hi = min(lo + per, count);
+  const int64_t slot = w.tile_slot - w.in_sample;
+  float a[V], b[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    a[i] = 1.f;
+    b[i] = 0.f;
+  }
+  constexpr int kFoldAhead = 4;
+  for (int t0 = lo; t0 < hi; t0 += kFoldAhead) {
+    float2 v[kFoldAhead][V];
+#pragma unroll
+    for (int j = 0; j < kFoldAhead; ++j) {
+      const int t = min(t0 + j, hi - 1);
+      const float2 *at = tiles + (slot + (FROM_LAST ? w.tiles - 1 - t : t)) * s.channels + w.channel;
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[j][i] = at[i];
+    }
+#pragma unroll
+    for (int j = 0; j < kFoldAhead; ++j) {
+      if (t0 + j >= hi) break;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        b[i] = fmaf(v[j][i].x, b[i], v[j][i].y);
+        a[i] *= v[j][i].x;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float all_a, all_b;
+    composeTeams<false>(w.team, a[i], b[i], &all_a, &all_b);
+    h[i] = fmaf(all_a, h[i], all_b);
+  }
+}
+
+// The rows of no sample, which are zero in every result, and (`final` not null) what a sample without rows hands on: by workgroup
+// `block` of kOutsideBlocks of every slab.
 template <typename T, int V>
-__device__ void zeroOutside(const Shape &s, int block, T *out, T *out2) {
+__device__ void outside(const Shape &s, int block, const float *initial, float *final, T *out, T *out2) {
   const float zero[V] = {};
   const int vectors = s.channels / V;
+  block = block * (int)gridDim.x + (int)blockIdx.x;
+  const int blocks = kOutsideBlocks * (int)gridDim.x;
   for (int side = 0; side < 2; ++side) {
     int first, rows;
     segmentOrOutside(s.starts, s.rows, s.samples, side == 0 ? 0 : s.samples + 1, &first, &rows);
     const int64_t end = (int64_t)rows * vectors;
-    for (int64_t at = (int64_t)block * kThreads + threadIdx.x; at < end; at += kOutsideBlocks * kThreads) {
+    for (int64_t at = (int64_t)block * kThreads + threadIdx.x; at < end; at += (int64_t)blocks * kThreads) {
       storeFloats<T, V>(out + (int64_t)first * s.channels + at * V, zero);
       if (out2 != nullptr) storeFloats<T, V>(out2 + (int64_t)first * s.channels + at * V, zero);
     }
   }
+  if (final == nullptr) return;
+  for (int sample = block; sample < s.samples; sample += blocks) {
+    int first, rows;
+    segmentRows(s.starts, s.rows, sample, &first, &rows);
+    if (rows > 0) continue;
+    for (int64_t c = threadIdx.x; c < s.channels; c += kThreads) {
+      const int64_t at = (int64_t)sample * s.channels + c;
+      final[at] = initial == nullptr ? 0.f : initial[at];
+    }
+  }
 }
 
-// The states of a tile's rows, step by step, from the one at its beginning; the states in front of every step to step_states.
-// WHOLE: a wave has a sample, and nothing has run in front: `carries` are the samples' initial states, and it writes `final`.
-template <typename T, int V, int KIND, bool WHOLE>
-__global__ __launch_bounds__(kThreads) void gatedScanApply(const T *__restrict__ x, const T *__restrict__ g, Shape s,
+// The states of a tile's rows, step by step, and the states in front of every step to step_states.  But with JOINED it writes
+// `final` too.
+template <typename T, int V, int KIND, Joining JOINING>
+__global__ __launch_bounds__(kThreads, 5) void gatedScanApply(const T *__restrict__ x, const T *__restrict__ g, Shape s,
                                                            int64_t first_block, int64_t blocks,
-                                                           const float *__restrict__ carries,
+                                                           const float *__restrict__ states,
+                                                           const float2 *__restrict__ tiles,
                                                            float *__restrict__ step_states, float *__restrict__ final,
                                                            T *__restrict__ out) {
-  const int64_t block = first_block + blockIdx.x;
+  const int64_t block = first_block + blockIdx.y;
   if (block >= blocks) {
-    zeroOutside<T, V>(s, (int)(block - blocks), out, static_cast<T *>(nullptr));
+    outside<T, V>(s, (int)(block - blocks), states, JOINING == kJoined ? nullptr : final, out, static_cast<T *>(nullptr));
     return;
   }
-  const Work<V, WHOLE> w(unitOf(block, blocks, !WHOLE), s);
-  if (w.sample < 0) return;
-  const int64_t from = (WHOLE ? w.sample : w.tile_slot) * s.channels + w.channel;
+  const Work<V, JOINING == kWhole> w(s, block, blocks, JOINING != kWhole);
+  if (w.sample < 0 || w.rows == 0) return;
   float h0[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) h0[i] = carries == nullptr || !w.there ? 0.f : carries[from + i];
   const int steps = w.steps();
-  Rows<T, V> xs, gs;
+  Rows<T, V, kRows> xs, gs;
   auto load = [&](int k) {
     gs.template load<kRows>(g, s.g_stride, w, k * kStepRows, idle<KIND>());
     xs.template load<kRows>(x, s.x_stride, w, k * kStepRows, 0.f);
   };
   load(0);
+  incoming<V, JOINING, false>(w, s, states, tiles, h0);
   for (int k = 0; k < steps; ++k) {
     float ra[kRows][V], rb[kRows][V], a[V], b[V];
 #pragma unroll
@@ -420,36 +501,34 @@ __global__ __launch_bounds__(kThreads) void gatedScanApply(const T *__restrict__
       if (r < mine) storeRow<T, V>(lines.row(r), h, s.streamed);
     }
   }
-  if (WHOLE && w.there && w.team == 0) {
+  if (JOINING != kJoined && w.ends() && w.there && w.team == 0) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) final[from + i] = h0[i];
+    for (int i = 0; i < V; ++i) final[(int64_t)w.sample * s.channels + w.channel + i] = h0[i];
   }
 }
 
 // ---- backward ------------------------------------------------------------------------------
 
 // The gradients of a tile's rows, from the last step to the first: a step's states again from the one in front of it, and the
-// gradient that comes in from behind.  WHOLE: as above, `grad_carries` are the gradients of the final states.
-template <typename T, int V, int KIND, bool WHOLE>
-__global__ __launch_bounds__(kThreads, 3) void gatedScanGrad(const T *__restrict__ dh, const T *__restrict__ x,
+// gradient that comes in from behind.  But with JOINED it writes the initial states' too.
+template <typename T, int V, int KIND, Joining JOINING>
+__global__ __launch_bounds__(kThreads, 4) void gatedScanGrad(const T *__restrict__ dh, const T *__restrict__ x,
                                                           const T *__restrict__ g, Shape s, int64_t first_block,
                                                           int64_t blocks, const float *__restrict__ step_states,
-                                                          const float *__restrict__ grad_carries,
+                                                          const float *__restrict__ grads, const float2 *__restrict__ tiles,
                                                           float *__restrict__ initial_grad, T *__restrict__ dx,
                                                           T *__restrict__ dg) {
-  const int64_t block = first_block + blockIdx.x;
+  const int64_t block = first_block + blockIdx.y;
   if (block >= blocks) {
-    zeroOutside<T, V>(s, (int)(block - blocks), dx, dg);
+    outside<T, V>(s, (int)(block - blocks), grads, JOINING == kJoined ? nullptr : initial_grad, dx, dg);
     return;
   }
-  const Work<V, WHOLE> w(unitOf(block, blocks, !WHOLE), s);
-  if (w.sample < 0) return;
-  const int64_t from = (WHOLE ? w.sample : w.tile_slot) * s.channels + w.channel;
+  const Work<V, JOINING == kWhole> w(s, block, blocks, JOINING != kWhole);
+  if (w.sample < 0 || w.rows == 0) return;
   float l0[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) l0[i] = grad_carries == nullptr || !w.there ? 0.f : grad_carries[from + i];
+  incoming<V, JOINING, true>(w, s, grads, tiles, l0);
   for (int k = w.steps() - 1; k >= 0; --k) {
-    Rows<T, V> xs, gs, ds;
+    Rows<T, V, kRows> xs, gs, ds;
     gs.template load<kRows>(g, s.g_stride, w, k * kStepRows, idle<KIND>());
     xs.template load<kRows>(x, s.x_stride, w, k * kStepRows, 0.f);
     ds.template load<kRows>(dh, s.dh_stride, w, k * kStepRows, 0.f);
@@ -481,14 +560,15 @@ __global__ __launch_bounds__(kThreads, 3) void gatedScanGrad(const T *__restrict
       l[i] = fmaf(behind, l0[i], c[i]);
       l0[i] = fmaf(all_a, l0[i], all_b);
     }
-    // states in front of every row
-    float before[kRows][V];
+    // the states again, and what a row's gradient is multiplied with for its gate's
+    float slope[kRows][V];
 #pragma unroll
     for (int r = 0; r < kRows; ++r)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        before[r][i] = h[i];
-        h[i] = fmaf(ra[r][i], h[i], ru[r][i] * xs.value(r, i));
+        const float v = xs.value(r, i);
+        slope[r][i] = KIND == MLUOP_EXT_GATE_SIGMOID ? ru[r][i] * (h[i] - v) : h[i];
+        h[i] = fmaf(ra[r][i], h[i], ru[r][i] * v);
       }
     const Lines<T, kRows> to_x(dx, s.channels, w, k * kStepRows), to_g(dg, s.channels, w, k * kStepRows);
     const int mine = w.there ? w.rows - k * kStepRows - w.team * kRows : 0;
@@ -500,16 +580,16 @@ __global__ __launch_bounds__(kThreads, 3) void gatedScanGrad(const T *__restrict
         const float all = ds.value(r, i) + l[i];
         l[i] = ra[r][i] * all;
         gx[i] = ru[r][i] * all;
-        gg[i] = KIND == MLUOP_EXT_GATE_SIGMOID ? ru[r][i] * l[i] * (before[r][i] - xs.value(r, i)) : l[i] * before[r][i];
+        gg[i] = l[i] * slope[r][i];
       }
       if (r >= mine) continue;
       storeRow<T, V>(to_x.row(r), gx, s.streamed);
       storeRow<T, V>(to_g.row(r), gg, s.streamed);
     }
   }
-  if (WHOLE && w.there && w.team == 0 && initial_grad != nullptr) {
+  if (JOINING != kJoined && w.begins() && w.there && w.team == 0 && initial_grad != nullptr) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) initial_grad[from + i] = l0[i];
+    for (int i = 0; i < V; ++i) initial_grad[(int64_t)w.sample * s.channels + w.channel + i] = l0[i];
   }
 }
 
@@ -568,26 +648,44 @@ size_t workspaceBytes(int64_t rows, int64_t channels, int64_t samples) {
 }
 struct Workspace {
   float2 *tiles;
-  float *carries;
+  float *states;
   Workspace(void *workspace, int64_t rows, int64_t channels, int64_t samples) {
     tiles = reinterpret_cast<float2 *>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~(uintptr_t)15);
-    carries = reinterpret_cast<float *>(tiles + mostSlots<kTileRows>(rows, samples) * channels);
+    states = reinterpret_cast<float *>(tiles + mostSlots<kTileRows>(rows, samples) * channels);
   }
 };
 
-// A wave for a whole sample, and one launch in place of three: where there are few rows, or about one a sample, as in a step of many
-// sequences.  (At worst one sample has them all, in 128 steps of a microsecond.)
-bool wholeSamples(int64_t rows, int64_t samples) { return rows <= std::max<int64_t>(512, std::min<int64_t>(2 * samples, 4096)); }
+// A wave for a whole sample, and one launch in place of two or three: where there are few rows, or about one a sample, as in a step of
+// many sequences.  (At worst one sample has them all, in 256 steps of a microsecond.)  Every wave folds the tiles in front of its own where
+// these are few, at most 16 for a team.
+Joining joiningOf(int64_t rows, int64_t samples) {
+  if (rows <= std::max<int64_t>(512, std::min<int64_t>(2 * samples, 4096))) return kWhole;
+  return rows <= 64 * kTileRows ? kFolded : kJoined;
+}
+template <typename F>
+void byJoining(Joining joining, F f) {
+  if (joining == kWhole)
+    f(std::integral_constant<Joining, kWhole>());
+  else if (joining == kFolded)
+    f(std::integral_constant<Joining, kFolded>());
+  else
+    f(std::integral_constant<Joining, kJoined>());
+}
 
-constexpr int64_t kMostAlongY = 65535;  // workgroups of a grid
+// Workgroups along y in as many launches as they need.
+constexpr int64_t kMostAlongY = 65535;
+template <typename F>
+void alongY(int64_t blocks, F f) {
+  for (int64_t first = 0; first < blocks; first += kMostAlongY) f(first, (unsigned)std::min(blocks - first, kMostAlongY));
+}
 
 template <bool FROM_LAST>
-void join(const mluop::LaunchCtx &lc, const float2 *tiles, const Shape &s, const float *initial, float *carries, float *final) {
+void join(const mluop::LaunchCtx &lc, const float2 *tiles, const Shape &s, const float *initial, float *states, float *final) {
   for (int64_t first = 0; first < s.samples; first += kMostAlongY) {
     lc.begin("gatedScanJoin");
     gatedScanJoin<FROM_LAST><<<dim3((unsigned)((s.channels + kJoinChannels - 1) / kJoinChannels),
                                     (unsigned)std::min<int64_t>(s.samples - first, kMostAlongY)),
-                               kJoinThreads, 0, lc.stream>>>(tiles, s, (int)first, initial, carries, final);
+                               kJoinThreads, 0, lc.stream>>>(tiles, s, (int)first, initial, states, final);
     lc.end();
   }
 }
@@ -628,13 +726,14 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanForward(mluOpHandle_t handle, mluOp
   HIP_CHECK_RETURN(api, hipSetDevice(handle->device));
   const size_t bytes = (size_t)rows * channels * elementBytes(type);
   const int64_t most = mostRaggedTiles(rows, samples, kTileRows);
+  const Joining joining = joiningOf(rows, samples);
   if (handle->hasNotes()) {
     handle->forgetNotesIn(out, bytes);
     handle->forgetNotesIn(final, (size_t)samples * channels * sizeof(float));
     handle->forgetNotesIn(carries, (size_t)mostSlots<kStepRows>(rows, samples) * channels * sizeof(float));
     handle->forgetNotesIn(workspace, workspace_size);
   }
-  Shape s = {(int)rows,  (int)channels, (int)samples, features_stride, gates_stride, 0, (int)most, 0,
+  Shape s = {(int)rows,  (int)channels, (int)samples, features_stride, gates_stride, 0, (int)most, 1,
              row_starts, reverse != 0,  bytes >= kStreamedBytes};
   const Workspace w(workspace, rows, channels, samples);
   const mluop::LaunchCtx lc = handle->launchCtx();
@@ -645,23 +744,27 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanForward(mluOpHandle_t handle, mluOp
       typedef decltype(zero) T;
       constexpr int V = decltype(v)::value, KIND = decltype(of_kind)::value;
       const T *x = static_cast<const T *>(features), *g = static_cast<const T *>(gates);
-      s.slabs = (int)((channels + kAcross * V - 1) / (kAcross * V));
-      const bool whole = wholeSamples(rows, samples);
-      const int64_t blocks = blocksOf(whole ? samples : most, s.slabs);
-      if (!whole) {
-        inLaunches(blocks, kThreads, [&](int64_t first, unsigned count) {
+      const int64_t all = (channels + kAcross * V - 1) / (kAcross * V);
+      s.side_by_side = all >= 3 ? 4 : (int)all;
+      const unsigned slabs = (unsigned)((all + s.side_by_side - 1) / s.side_by_side);
+      const int64_t in_block = kWaves / s.side_by_side, blocks = ((joining == kWhole ? samples : most) + in_block - 1) / in_block;
+      if (joining != kWhole) {
+        alongY(blocks, [&](int64_t first, unsigned count) {
           lc.begin("gatedScanTiles");
-          gatedScanTiles<T, V, KIND, false><<<count, kThreads, 0, lc.stream>>>(x, g, s, first, blocks, w.tiles);
+          gatedScanTiles<T, V, KIND, false><<<dim3(slabs, count), kThreads, 0, lc.stream>>>(x, g, s, first, w.tiles);
           lc.end();
         });
-        join<false>(lc, w.tiles, s, initial, w.carries, final);
       }
-      auto kernel = whole ? gatedScanApply<T, V, KIND, true> : gatedScanApply<T, V, KIND, false>;
-      inLaunches(blocks + kOutsideBlocks, kThreads, [&](int64_t first, unsigned count) {
-        lc.begin("gatedScanApply");
-        kernel<<<count, kThreads, 0, lc.stream>>>(x, g, s, first, blocks, whole ? initial : w.carries, carries, final,
-                                                  static_cast<T *>(out));
-        lc.end();
+      if (joining == kJoined) join<false>(lc, w.tiles, s, initial, w.states, final);
+      byJoining(joining, [&](auto how) {
+        constexpr Joining JOINING = decltype(how)::value;
+        alongY(blocks + kOutsideBlocks, [&](int64_t first, unsigned count) {
+          lc.begin("gatedScanApply");
+          gatedScanApply<T, V, KIND, JOINING><<<dim3(slabs, count), kThreads, 0, lc.stream>>>(
+              x, g, s, first, blocks, JOINING == kJoined ? w.states : initial, w.tiles, carries, final,
+              static_cast<T *>(out));
+          lc.end();
+        });
       });
     });
   });
@@ -694,13 +797,14 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanBackward(mluOpHandle_t handle, mluO
   HIP_CHECK_RETURN(api, hipSetDevice(handle->device));
   const size_t bytes = (size_t)rows * channels * elementBytes(type);
   const int64_t most = mostRaggedTiles(rows, samples, kTileRows);
+  const Joining joining = joiningOf(rows, samples);
   if (handle->hasNotes()) {
     handle->forgetNotesIn(features_grad, bytes);
     handle->forgetNotesIn(gates_grad, bytes);
     if (initial_grad) handle->forgetNotesIn(initial_grad, (size_t)samples * channels * sizeof(float));
     handle->forgetNotesIn(workspace, workspace_size);
   }
-  Shape s = {(int)rows,  (int)channels, (int)samples, features_stride, gates_stride, output_grad_stride, (int)most, 0,
+  Shape s = {(int)rows,  (int)channels, (int)samples, features_stride, gates_stride, output_grad_stride, (int)most, 1,
              row_starts, reverse != 0,  bytes >= kStreamedBytes};
   const Workspace w(workspace, rows, channels, samples);
   const mluop::LaunchCtx lc = handle->launchCtx();
@@ -713,23 +817,27 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanBackward(mluOpHandle_t handle, mluO
       constexpr int V = decltype(v)::value, KIND = decltype(of_kind)::value;
       const T *dh = static_cast<const T *>(output_grad), *x = static_cast<const T *>(features);
       const T *g = static_cast<const T *>(gates);
-      s.slabs = (int)((channels + kAcross * V - 1) / (kAcross * V));
-      const bool whole = wholeSamples(rows, samples);
-      const int64_t blocks = blocksOf(whole ? samples : most, s.slabs);
-      if (!whole) {
-        inLaunches(blocks, kThreads, [&](int64_t first, unsigned count) {
+      const int64_t all = (channels + kAcross * V - 1) / (kAcross * V);
+      s.side_by_side = all >= 3 ? 4 : (int)all;
+      const unsigned slabs = (unsigned)((all + s.side_by_side - 1) / s.side_by_side);
+      const int64_t in_block = kWaves / s.side_by_side, blocks = ((joining == kWhole ? samples : most) + in_block - 1) / in_block;
+      if (joining != kWhole) {
+        alongY(blocks, [&](int64_t first, unsigned count) {
           lc.begin("gatedScanTiles");
-          gatedScanTiles<T, V, KIND, true><<<count, kThreads, 0, lc.stream>>>(dh, g, s, first, blocks, w.tiles);
+          gatedScanTiles<T, V, KIND, true><<<dim3(slabs, count), kThreads, 0, lc.stream>>>(dh, g, s, first, w.tiles);
           lc.end();
         });
-        join<true>(lc, w.tiles, s, final_grad, w.carries, initial_grad);
       }
-      auto kernel = whole ? gatedScanGrad<T, V, KIND, true> : gatedScanGrad<T, V, KIND, false>;
-      inLaunches(blocks + kOutsideBlocks, kThreads, [&](int64_t first, unsigned count) {
-        lc.begin("gatedScanGrad");
-        kernel<<<count, kThreads, 0, lc.stream>>>(dh, x, g, s, first, blocks, carries, whole ? final_grad : w.carries,
-                                                  initial_grad, static_cast<T *>(features_grad), static_cast<T *>(gates_grad));
-        lc.end();
+      if (joining == kJoined) join<true>(lc, w.tiles, s, final_grad, w.states, initial_grad);
+      byJoining(joining, [&](auto how) {
+        constexpr Joining JOINING = decltype(how)::value;
+        alongY(blocks + kOutsideBlocks, [&](int64_t first, unsigned count) {
+          lc.begin("gatedScanGrad");
+          gatedScanGrad<T, V, KIND, JOINING><<<dim3(slabs, count), kThreads, 0, lc.stream>>>(
+              dh, x, g, s, first, blocks, carries, JOINING == kJoined ? w.states : final_grad, w.tiles, initial_grad,
+              static_cast<T *>(features_grad), static_cast<T *>(gates_grad));
+          lc.end();
+        });
       });
     });
   });
