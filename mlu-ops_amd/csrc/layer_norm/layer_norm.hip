@@ -43,18 +43,18 @@ struct Team {
     for (int i = 0; i < COUNT; ++i) v[i] = sumOverLanes<(LANES < 64 ? LANES : 64)>(v[i]);
     if constexpr (LANES > 64) {
       constexpr int kWaves = LANES / 64;
-      __shared__ float s_wave[kWaves][COUNT];
+      __shared__ float s_wave[kTeams][kWaves][COUNT];
       __syncthreads();
       if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-        for (int i = 0; i < COUNT; ++i) s_wave[threadIdx.x >> 6][i] = v[i];
+        for (int i = 0; i < COUNT; ++i) s_wave[team][lane >> 6][i] = v[i];
       }
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < COUNT; ++i) {
         v[i] = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) v[i] += s_wave[w][i];
+        for (int w = 0; w < kWaves; ++w) v[i] += s_wave[team][w][i];
       }
     }
   }
@@ -63,8 +63,9 @@ struct Team {
 // ---- forward -------------------------------------------------------------------------------
 
 // y = (x - mean) * rstd * weight + bias.  The mean is the sum's, put right by the mean of the differences from it, so that rows far
-// off zero lose nothing; the variance is that of the differences.  R rows of a team are on their way together.
-template <typename T, int V, int LANES, int N, int R>
+// off zero lose nothing; the variance is that of the differences.  Weight and bias stay in registers.  Bound by memory: 248 636 x
+// 128 fp16 (127 MB) 23.7 us, 5.4 TB/s; 32 768 x 2048 bf16 (268 MB) 52 us, 5.2 TB/s.
+template <typename T, int V, int LANES, int N>
 __global__ __launch_bounds__((Team<V, LANES, N>::kWorkgroup)) void layerNormRows(const T *__restrict__ x, Shape s,
                                                                                 ChannelParams p, float eps,
                                                                                 T *__restrict__ out,
@@ -82,67 +83,48 @@ __global__ __launch_bounds__((Team<V, LANES, N>::kWorkgroup)) void layerNormRows
     }
   }
   const float by = 1.f / (float)s.channels;
-  const int64_t step = (int64_t)gridDim.x * Lanes::kTeams;
   // (all teams of a workgroup take as many turns: sums are taken by whole waves)
-  for (int64_t first = (int64_t)blockIdx.x * Lanes::kTeams; first < s.rows; first += R * step) {
-    Vector<T, V> v[R][N];
+  for (int64_t first = (int64_t)blockIdx.x * Lanes::kTeams; first < s.rows; first += (int64_t)gridDim.x * Lanes::kTeams) {
+    const int64_t r = first + l.team;
+    const bool row = r < s.rows;
+    Vector<T, V> v[N];
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-      const int64_t r = first + l.team + j * step;
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        v[j][n] = {};
-        if (r < s.rows && l.channel(n) < s.channels)
-          v[j][n] = *reinterpret_cast<const Vector<T, V> *>(x + r * s.x_stride + l.channel(n));
-      }
+    for (int n = 0; n < N; ++n) {
+      v[n] = {};
+      if (row && l.channel(n) < s.channels) v[n] = *reinterpret_cast<const Vector<T, V> *>(x + r * s.x_stride + l.channel(n));
     }
-    float m[R], moments[2 * R];
+    float m[1] = {0.f}, moments[2] = {0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-      m[j] = 0.f;
+    for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int i = 0; i < V; ++i) m[j] += (float)v[j][n].v[i];
-    }
+      for (int i = 0; i < V; ++i) m[0] += (float)v[n].v[i];
     l.sum(m);
+    m[0] *= by;
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-      m[j] *= by;
-      float sum = 0.f, squares = 0.f;
+    for (int n = 0; n < N; ++n) {
+      const bool there = l.channel(n) < s.channels;
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const bool there = l.channel(n) < s.channels;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = there ? (float)v[j][n].v[i] - m[j] : 0.f;
-          sum += d;
-          squares = fmaf(d, d, squares);
-        }
+      for (int i = 0; i < V; ++i) {
+        const float d = there ? (float)v[n].v[i] - m[0] : 0.f;
+        moments[0] += d;
+        moments[1] = fmaf(d, d, moments[1]);
       }
-      moments[2 * j] = sum;
-      moments[2 * j + 1] = squares;
     }
     l.sum(moments);
+    const float off = moments[0] * by, variance = fmaf(-off, off, moments[1] * by);
+    const float inv = 1.f / sqrtf((variance < 0.f ? 0.f : variance) + eps);  // (NaN stays NaN)
+    if (!row) continue;
+    if (l.lane == 0) {
+      mean[r] = m[0] + off;
+      rstd[r] = inv;
+    }
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-      const int64_t r = first + l.team + j * step;
-      const float off = moments[2 * j] * by;
-      const float variance = fmaf(-off, off, moments[2 * j + 1] * by);
-      const float inv = 1.f / sqrtf((variance < 0.f ? 0.f : variance) + eps);  // (NaN stays NaN)
-      if (r >= s.rows) continue;
-      if (l.lane == 0) {
-        mean[r] = m[j] + off;
-        rstd[r] = inv;
-      }
+    for (int n = 0; n < N; ++n) {
+      if (l.channel(n) >= s.channels) continue;
+      float y[V];
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        if (l.channel(n) >= s.channels) continue;
-        float y[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = fmaf(((float)v[j][n].v[i] - m[j] - off) * inv, w[n][i], b[n][i]);
-        storeFloats<T, V>(out + r * s.channels + l.channel(n), y, s.streamed);
-      }
+      for (int i = 0; i < V; ++i) y[i] = fmaf(((float)v[n].v[i] - m[0] - off) * inv, w[n][i], b[n][i]);
+      storeFloats<T, V>(out + r * s.channels + l.channel(n), y, s.streamed);
     }
   }
 }
@@ -151,8 +133,8 @@ __global__ __launch_bounds__((Team<V, LANES, N>::kWorkgroup)) void layerNormRows
 
 // dx = rstd (d - mean of d - normed * mean of d normed) with d = dy * weight, and with SUMS a workgroup's sums of dy * normed
 // and dy of every channel over its rows, to partial[workgroup][2][channels].  A team's lanes have the same channels in
-// every row, so that these stay in registers until the last row.
-template <typename T, int V, int LANES, int N, int R, bool SUMS>
+// every row, so that these stay in registers until the last row.  Bound by memory: 32 768 x 2048 bf16 (403 MB) 77 us, 5.2 TB/s.
+template <typename T, int V, int LANES, int N, bool SUMS>
 __global__ __launch_bounds__((Team<V, LANES, N>::kWorkgroup)) void layerNormGrad(const T *__restrict__ dy,
                                                                                 const T *__restrict__ x, Shape s,
                                                                                 ChannelParams p,
@@ -167,64 +149,46 @@ __global__ __launch_bounds__((Team<V, LANES, N>::kWorkgroup)) void layerNormGrad
   for (int n = 0; n < N; ++n)
     if (l.channel(n) < s.channels) p.weights<V>(l.channel(n), w[n]);
   const float by = 1.f / (float)s.channels;
-  const int64_t step = (int64_t)gridDim.x * Lanes::kTeams;
-  for (int64_t first = (int64_t)blockIdx.x * Lanes::kTeams; first < s.rows; first += R * step) {
-    Vector<T, V> dys[R][N], xs[R][N];
-    float m[R], inv[R], sums[2 * R];
+  for (int64_t first = (int64_t)blockIdx.x * Lanes::kTeams; first < s.rows; first += (int64_t)gridDim.x * Lanes::kTeams) {
+    const int64_t r = first + l.team;
+    const bool row = r < s.rows;
+    Vector<T, V> dys[N], xs[N];
+    const float m = row ? mean[r] : 0.f, inv = row ? rstd[r] : 0.f;
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-      const int64_t r = first + l.team + j * step;
-      m[j] = inv[j] = 0.f;
-      if (r < s.rows) {
-        m[j] = mean[r];
-        inv[j] = rstd[r];
-      }
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        dys[j][n] = xs[j][n] = {};
-        if (r < s.rows && l.channel(n) < s.channels) {
-          dys[j][n] = *reinterpret_cast<const Vector<T, V> *>(dy + r * s.dy_stride + l.channel(n));
-          xs[j][n] = *reinterpret_cast<const Vector<T, V> *>(x + r * s.x_stride + l.channel(n));
-        }
+    for (int n = 0; n < N; ++n) {
+      dys[n] = xs[n] = {};
+      if (row && l.channel(n) < s.channels) {
+        dys[n] = *reinterpret_cast<const Vector<T, V> *>(dy + r * s.dy_stride + l.channel(n));
+        xs[n] = *reinterpret_cast<const Vector<T, V> *>(x + r * s.x_stride + l.channel(n));
       }
     }
+    float sums[2] = {0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-      const bool row = first + l.team + j * step < s.rows;
-      float a = 0.f, b = 0.f;
+    for (int n = 0; n < N; ++n) {
+      if (!row || l.channel(n) >= s.channels) continue;
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        if (!row || l.channel(n) >= s.channels) continue;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float g = (float)dys[j][n].v[i], normed = ((float)xs[j][n].v[i] - m[j]) * inv[j], d = g * w[n][i];
-          a += d;
-          b = fmaf(d, normed, b);
-          if constexpr (SUMS) {
-            dw[n][i] = fmaf(g, normed, dw[n][i]);
-            db[n][i] += g;
-          }
+      for (int i = 0; i < V; ++i) {
+        const float g = (float)dys[n].v[i], normed = ((float)xs[n].v[i] - m) * inv, d = g * w[n][i];
+        sums[0] += d;
+        sums[1] = fmaf(d, normed, sums[1]);
+        if constexpr (SUMS) {
+          dw[n][i] = fmaf(g, normed, dw[n][i]);
+          db[n][i] += g;
         }
       }
-      sums[2 * j] = a;
-      sums[2 * j + 1] = b;
     }
     l.sum(sums);
+    const float a = sums[0] * by, b = sums[1] * by;
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-      const int64_t r = first + l.team + j * step;
-      const float a = sums[2 * j] * by, b = sums[2 * j + 1] * by;
+    for (int n = 0; n < N; ++n) {
+      if (!row || l.channel(n) >= s.channels) continue;
+      float d[V];
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        if (r >= s.rows || l.channel(n) >= s.channels) continue;
-        float d[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float normed = ((float)xs[j][n].v[i] - m[j]) * inv[j];
-          d[i] = inv[j] * (fmaf((float)dys[j][n].v[i], w[n][i], -a) - normed * b);
-        }
-        storeFloats<T, V>(dx + r * s.channels + l.channel(n), d, s.streamed);
+      for (int i = 0; i < V; ++i) {
+        const float normed = ((float)xs[n].v[i] - m) * inv;
+        d[i] = inv * (fmaf((float)dys[n].v[i], w[n][i], -a) - normed * b);
       }
+      storeFloats<T, V>(dx + r * s.channels + l.channel(n), d, s.streamed);
     }
   }
   if constexpr (SUMS) {
@@ -277,11 +241,10 @@ __global__ __launch_bounds__(kThreads) void layerNormColumnSums(const T *__restr
   to[s.channels + c] = db;
 }
 
-// partial[parts][2][channels] added up: kChannels sums a workgroup, each by kThreads / kChannels threads.
-constexpr int kChannels = 16, kAhead = 4;
-__global__ __launch_bounds__(kThreads) void layerNormJoinSums(const float *__restrict__ partial, int parts, int channels,
-                                                              ChannelParams p, void *weight_grad, void *bias_grad) {
-  constexpr int kShares = kThreads / kChannels;
+// partial[parts][2][channels] added up: kChannels sums a workgroup, each by kShares threads.
+constexpr int kJoinThreads = 1024, kChannels = 16, kShares = kJoinThreads / kChannels, kAhead = 8;
+__global__ __launch_bounds__(kJoinThreads) void layerNormJoinSums(const float *__restrict__ partial, int parts, int channels,
+                                                                  ChannelParams p, void *weight_grad, void *bias_grad) {
   __shared__ float s_sum[kShares][kChannels];
   const int lane = threadIdx.x % kChannels, share = threadIdx.x / kChannels;
   const int at = (int)blockIdx.x * kChannels + lane;
@@ -317,6 +280,8 @@ void byType(mluOpDataType_t type, int64_t channels, int64_t strides, uintptr_t a
   auto sixteen = [&](auto zero) {
     if (fits(8))
       f(zero, std::integral_constant<int, 8>());
+    else if (fits(4))
+      f(zero, std::integral_constant<int, 4>());
     else if (fits(2))
       f(zero, std::integral_constant<int, 2>());
     else
@@ -333,29 +298,40 @@ void byType(mluOpDataType_t type, int64_t channels, int64_t strides, uintptr_t a
   }
 }
 
-// Calls f(LANES, N): the smallest team that holds a row of `vectors` vectors.
+// Vectors of a thread: 16 bytes, whatever their width.  (More, and no barrier between the waves of a wide row, leaves few waves a
+// SIMD: 32 768 x 2048 bf16, 64 bytes a thread 106 us forward and 117 backward, 16 bytes 53 and 77.  Less has a wave add up few
+// values: 200 000 x 33 bf16, 2 bytes a thread 35 us forward, 16 bytes 17.)
+template <typename T, int V>
+constexpr int kVectors = 16 / (int)sizeof(T) / V;
+
+// Calls f(LANES): the smallest team that holds a row whose threads' 16 bytes are `pieces`.
 template <typename F>
-void byTeam(int64_t vectors, F f) {
-  auto one = std::integral_constant<int, 1>();
-  if (vectors <= 8)
-    f(std::integral_constant<int, 8>(), one);
-  else if (vectors <= 16)
-    f(std::integral_constant<int, 16>(), one);
-  else if (vectors <= 32)
-    f(std::integral_constant<int, 32>(), one);
-  else if (vectors <= 64)
-    f(std::integral_constant<int, 64>(), one);
-  else if (vectors <= 128)
-    f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
-  else if (vectors <= 256)
-    f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+void byTeam(int64_t pieces, F f) {
+  if (pieces <= 8)
+    f(std::integral_constant<int, 8>());
+  else if (pieces <= 16)
+    f(std::integral_constant<int, 16>());
+  else if (pieces <= 32)
+    f(std::integral_constant<int, 32>());
+  else if (pieces <= 64)
+    f(std::integral_constant<int, 64>());
+  else if (pieces <= 128)
+    f(std::integral_constant<int, 128>());
+  else if (pieces <= 256)
+    f(std::integral_constant<int, 256>());
+  else if (pieces <= 512)
+    f(std::integral_constant<int, 512>());
   else
-    f(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
+    f(std::integral_constant<int, 1024>());
 }
-constexpr int kTeamVectors = 1024;  // that byTeam's largest holds
+constexpr int kTeamPieces = 1024;   // that byTeam's largest holds
 constexpr int kWideThreads = 1024;  // of a workgroup that holds a row of up to kMostChannels
 
-constexpr int kSumParts = 512;      // most rows of partial sums
+constexpr int kBlocks = 4096;       // most workgroups of 256 threads
+
+// Most rows of partial sums: as many workgroups as the CUs hold together, as long as the sums themselves stay few (32 768 x 2048 bf16:
+// 512 workgroups 95 us and 5 to add up, 1024 77 and 7; 16 384 x 8192: 149 and 12, 154 and 22; 60 000 x 250: 31 and 5, 2048 22 and 6).
+int64_t sumParts(int64_t channels) { return channels <= 512 ? 2048 : channels <= 2048 ? 1024 : 512; }
 
 mluOpStatus_t checkShape(const char *api, int64_t rows, int64_t channels) {
   PARAM_CHECK(api, rows >= 0);
@@ -371,7 +347,7 @@ bool strideFits(int64_t rows, int64_t channels, int64_t stride) {
   return stride >= channels && (rows == 0 || stride <= ((int64_t)1 << 46) / rows);
 }
 
-size_t workspaceBytes(int64_t channels) { return 16 + (size_t)kSumParts * 2 * channels * sizeof(float); }
+size_t workspaceBytes(int64_t channels) { return 16 + (size_t)sumParts(channels) * 2 * channels * sizeof(float); }
 
 }  // namespace
 
@@ -407,17 +383,16 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtLayerNormForward(mluOpHandle_t handle, mluOp
     auto launch = [&](auto lanes, auto vectors) {
       constexpr int LANES = decltype(lanes)::value, N = decltype(vectors)::value;
       typedef Team<V, LANES, N> L;
-      constexpr int R = LANES > 64 ? 1 : 4 / N;
-      // (weight and bias stay in registers: workgroups for all CUs to hold, and rows for each)
-      const int64_t blocks = (rows + L::kTeams * R - 1) / (L::kTeams * R);
-      const unsigned grid = (unsigned)std::min<int64_t>(blocks, LANES > kThreads ? 512 : 2048);
+      const unsigned grid = (unsigned)std::min<int64_t>((rows + L::kTeams - 1) / L::kTeams, kBlocks * kThreads / L::kWorkgroup);
       lc.begin("layerNormRows");
-      layerNormRows<T, V, LANES, N, R><<<grid, L::kWorkgroup, 0, lc.stream>>>(
+      layerNormRows<T, V, LANES, N><<<grid, L::kWorkgroup, 0, lc.stream>>>(
           static_cast<const T *>(features), s, p, eps, static_cast<T *>(out), mean, rstd);
       lc.end();
     };
-    if (channels / V <= kTeamVectors)
-      byTeam(channels / V, launch);
+    constexpr int kN = kVectors<T, V>;
+    const int64_t pieces = (channels + V * kN - 1) / (V * kN);
+    if (pieces <= kTeamPieces)
+      byTeam(pieces, [&](auto lanes) { launch(lanes, std::integral_constant<int, kN>()); });
     else
       launch(std::integral_constant<int, kWideThreads>(), std::integral_constant<int, kMostChannels / kWideThreads / V>());
   });
@@ -475,26 +450,27 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtLayerNormBackward(mluOpHandle_t handle, mluO
       constexpr int V = decltype(v)::value;
       const T *dy = static_cast<const T *>(output_grad), *x = static_cast<const T *>(features);
       T *dx = static_cast<T *>(input_grad);
-      if (channels / V <= kTeamVectors) {
-        byTeam(channels / V, [&](auto lanes, auto vectors) {
-          constexpr int LANES = decltype(lanes)::value, N = decltype(vectors)::value;
+      constexpr int kN = kVectors<T, V>;
+      const int64_t pieces = (channels + V * kN - 1) / (V * kN);
+      if (pieces <= kTeamPieces) {
+        byTeam(pieces, [&](auto lanes) {
+          constexpr int LANES = decltype(lanes)::value, N = kN;
           typedef Team<V, LANES, N> L;
-          constexpr int R = LANES > 64 || N > 1 ? 1 : 2;
-          const int64_t blocks = (rows + L::kTeams * R - 1) / (L::kTeams * R);
-          parts = (int)std::min<int64_t>(blocks, kSumParts);
+          const int64_t blocks = (rows + L::kTeams - 1) / L::kTeams;
+          parts = (int)std::min<int64_t>(blocks, sumParts(channels));
           lc.begin("layerNormGrad");
           if (sums)
-            layerNormGrad<T, V, LANES, N, R, true><<<(unsigned)parts, L::kWorkgroup, 0, lc.stream>>>(dy, x, s, p, mean, rstd,
+            layerNormGrad<T, V, LANES, N, true><<<(unsigned)parts, L::kWorkgroup, 0, lc.stream>>>(dy, x, s, p, mean, rstd,
                                                                                                      dx, partial);
           else
-            layerNormGrad<T, V, LANES, N, R, false><<<(unsigned)std::min<int64_t>(blocks, 2048), L::kWorkgroup, 0, lc.stream>>>(
+            layerNormGrad<T, V, LANES, N, false><<<(unsigned)std::min<int64_t>(blocks, kBlocks * kThreads / L::kWorkgroup), L::kWorkgroup, 0, lc.stream>>>(
                 dy, x, s, p, mean, rstd, dx, nullptr);
           lc.end();
         });
       } else {
         constexpr int N = kMostChannels / kWideThreads / V;
         lc.begin("layerNormGrad");
-        layerNormGrad<T, V, kWideThreads, N, 1, false><<<(unsigned)std::min<int64_t>(rows, 512), kWideThreads, 0, lc.stream>>>(
+        layerNormGrad<T, V, kWideThreads, N, false><<<(unsigned)std::min<int64_t>(rows, 512), kWideThreads, 0, lc.stream>>>(
             dy, x, s, p, mean, rstd, dx, nullptr);
         lc.end();
         if (sums) {
@@ -509,7 +485,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtLayerNormBackward(mluOpHandle_t handle, mluO
   }
   if (sums) {
     lc.begin("layerNormJoinSums");
-    layerNormJoinSums<<<(unsigned)((2 * channels + kChannels - 1) / kChannels), kThreads, 0, lc.stream>>>(
+    layerNormJoinSums<<<(unsigned)((2 * channels + kChannels - 1) / kChannels), kJoinThreads, 0, lc.stream>>>(
         partial, parts, (int)channels, p, weight_grad, bias_grad);
     lc.end();
   }
