@@ -41,6 +41,131 @@ struct Choices {
   }
 };
 
+// Tiles of kOrderTile choices, a workgroup each: one launch where one holds them all, else one that counts and one that places.
+// A wave has 64 * kTurns consecutive choices, 64 at a time in order; choices of one expert find each other with a ballot for each bit
+// of its number.  A choice's place is behind those of lower experts, of its expert in earlier tiles, in earlier waves, in earlier
+// turns of its wave, and in lower lanes.  us of the general partition / of these: 24 choices of 32 experts 7.8 / XX,
+// 65 536 of 64 16 / XX, 240 000 of 8 27 / XX.
+constexpr int kOrderThreads = 512, kOrderWaves = kOrderThreads / 64, kTurns = 4, kOrderTile = kOrderThreads * kTurns;
+constexpr int kMostDigits = device_sort::kMaxDigits;
+
+__global__ __launch_bounds__(kOrderThreads) void expertCounts(Choices items, int64_t n, int digits,
+                                                              uint32_t *__restrict__ hist) {
+  __shared__ uint32_t s_count[kMostDigits];
+  const int64_t base = (int64_t)blockIdx.x * kOrderTile + threadIdx.x;
+  Choices::Item item[kTurns];
+#pragma unroll
+  for (int j = 0; j < kTurns; ++j) item[j] = items.load(min(base + j * kOrderThreads, n - 1));
+  for (int d = threadIdx.x; d < digits; d += kOrderThreads) s_count[d] = 0;
+  __syncthreads();
+  // (integer adds in LDS: the order they land in does not matter for a count)
+#pragma unroll
+  for (int j = 0; j < kTurns; ++j)
+    if (base + j * kOrderThreads < n) atomicAdd(&s_count[item[j].expert], 1u);
+  __syncthreads();
+  for (int d = threadIdx.x; d < digits; d += kOrderThreads) hist[(size_t)blockIdx.x * digits + d] = s_count[d];
+}
+
+// Choices of every digit in all tiles, and in those in front of this workgroup's, to s_total and s_before: as many threads a digit
+// as there are, `across` (a power of two) digits side by side.
+__device__ __forceinline__ void countsOfTiles(const uint32_t *__restrict__ hist, int tiles, int digits, int across,
+                                              uint32_t *s_total, uint32_t *s_before) {
+  constexpr int kAtOnce = 8;
+  for (int d = threadIdx.x; d < digits; d += kOrderThreads) s_total[d] = s_before[d] = 0;
+  __syncthreads();
+  const int shares = kOrderThreads / across, share = (int)threadIdx.x / across;
+  for (int d = (int)threadIdx.x % across; d < digits; d += across) {
+    uint32_t total = 0, before = 0;
+    for (int t0 = share; t0 < tiles; t0 += kAtOnce * shares) {
+      uint32_t v[kAtOnce];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) v[j] = hist[(size_t)min(t0 + j * shares, tiles - 1) * digits + d];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int t = t0 + j * shares;
+        total += t < tiles ? v[j] : 0u;
+        before += t < tiles && t < (int)blockIdx.x ? v[j] : 0u;
+      }
+    }
+    atomicAdd(&s_total[d], total);
+    atomicAdd(&s_before[d], before);
+  }
+  __syncthreads();
+}
+
+// ALONE: one workgroup has all choices.
+template <bool ALONE>
+__global__ __launch_bounds__(kOrderThreads) void expertPlaces(Choices items, int64_t n, int digits, int digit_bits, int across,
+                                                              const uint32_t *__restrict__ hist,
+                                                              int32_t *__restrict__ starts) {
+  __shared__ uint16_t s_count[kOrderWaves][kMostDigits];
+  __shared__ uint32_t s_first[kMostDigits], s_before[ALONE ? 1 : kMostDigits], s_wave[kOrderWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned long long below = (1ull << lane) - 1ull;
+  const int64_t base = (int64_t)blockIdx.x * kOrderTile + wave * 64 * kTurns + lane;
+  Choices::Item item[kTurns];
+#pragma unroll
+  for (int j = 0; j < kTurns; ++j) item[j] = items.load(min(base + j * 64, n - 1));
+  for (int d = threadIdx.x; d < digits; d += kOrderThreads)
+#pragma unroll
+    for (int w = 0; w < kOrderWaves; ++w) s_count[w][d] = 0;
+  __syncthreads();
+  volatile uint16_t *mine = s_count[wave];
+  uint32_t place[kTurns];
+#pragma unroll
+  for (int j = 0; j < kTurns; ++j) {
+    const bool valid = base + j * 64 < n;
+    const uint32_t digit = item[j].expert;
+    unsigned long long peers = __ballot(valid);
+    for (int b = 0; b < digit_bits; ++b) {
+      const bool bit = (digit >> b) & 1u;
+      const unsigned long long with = __ballot(bit);
+      peers &= bit ? with : ~with;
+    }
+    const int leader = valid ? __ffsll((long long)peers) - 1 : lane;
+    uint32_t before = 0;
+    if (valid && lane == leader) {
+      before = mine[digit];
+      mine[digit] = (uint16_t)(before + (uint32_t)__popcll(peers));
+    }
+    before = __shfl(before, leader, 64);
+    place[j] = before + (uint32_t)__popcll(peers & below);
+  }
+  __syncthreads();
+  // counts of a digit become those of the waves in front, and its total; a run of digits for each thread
+  const int per = (digits + kOrderThreads - 1) / kOrderThreads, d0 = (int)threadIdx.x * per;
+  for (int d = d0; d < min(d0 + per, digits); ++d) {
+    uint32_t run = 0;
+#pragma unroll
+    for (int w = 0; w < kOrderWaves; ++w) {
+      const uint32_t c = s_count[w][d];
+      s_count[w][d] = (uint16_t)run;
+      run += c;
+    }
+    if (ALONE) s_first[d] = run;
+  }
+  if (!ALONE) countsOfTiles(hist, (int)gridDim.x, digits, across, s_first, s_before);
+  // totals become starts
+  uint32_t sum = 0;
+  for (int d = d0; d < min(d0 + per, digits); ++d) sum += s_first[d];
+  const uint32_t upto = device_sort::waveInclusiveSum(sum);
+  if (lane == 63) s_wave[wave] = upto;
+  __syncthreads();
+  uint32_t run = upto - sum;
+  for (int w = 0; w < wave; ++w) run += s_wave[w];
+  for (int d = d0; d < min(d0 + per, digits); ++d) {
+    const uint32_t total = s_first[d];
+    if (blockIdx.x == 0) starts[d] = (int32_t)run;
+    s_first[d] = ALONE ? run : run + s_before[d];
+    run += total;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kTurns; ++j)
+    if (base + j * 64 < n)
+      items.store((size_t)s_first[item[j].expert] + s_count[wave][item[j].expert] + place[j], item[j], base + j * 64);
+}
+
 __global__ __launch_bounds__(kThreads) void expertStarts(const uint32_t *__restrict__ from, int count,
                                                          int32_t *__restrict__ to) {
   const int i = (int)blockIdx.x * kThreads + (int)threadIdx.x;
@@ -49,44 +174,50 @@ __global__ __launch_bounds__(kThreads) void expertStarts(const uint32_t *__restr
 
 // ---- rows to their places and back ---------------------------------------------------------
 
-// What a row's choices have in common: threads of V channels each over rows, as many rows at once as fit.
-template <int V>
-using Lanes = RowLanes<V, kThreads>;
+// LANES threads have a row, 16 bytes each whatever the vectors' width, as often as the row needs.  (A vector each: 60 000 rows of 250
+// bf16 from two places 60 us, 16 bytes 30.)
+template <typename T, int V>
+constexpr int kVectors = 16 / (int)sizeof(T) / V;
 
 constexpr int kTailBlocks = 64;  // workgroups for the places behind the last expert's, which are zero
 
 template <typename T, int V>
-__device__ void zeroTail(const Lanes<V> &l, const int32_t *starts, int experts, int64_t n, int channels, int block, T *out) {
-  const int64_t first = starts[experts];
+__device__ void zeroTail(const int32_t *starts, int experts, int64_t n, int channels, int block, T *out) {
+  const int64_t first = starts[experts], from = first < 0 ? 0 : first, vectors = channels / V;
   const float zero[V] = {};
-  for (int64_t p = (first < 0 ? 0 : first) + (int64_t)block * l.rows_at_once + l.row; p < n;
-       p += (int64_t)kTailBlocks * l.rows_at_once)
-    storeFloats<T, V>(out + p * channels + l.channel, zero);
+  for (int64_t at = from * vectors + (int64_t)block * kThreads + threadIdx.x; at < n * vectors;
+       at += (int64_t)kTailBlocks * kThreads)
+    storeFloats<T, V>(out + at * V, zero);
 }
 
-// out[place of (r, k)] = x[r] for every choice k: a row is read once and written as often as it is sent.
-template <typename T, int V>
+// out[place of (r, k)] = x[r] for every choice k: a row is read once and written as often as it is sent.  Bound by memory: 32 768 x 2
+// x 2048 bf16 (403 MB) 70 us, 5.7 TB/s.
+template <typename T, int V, int LANES>
 __global__ __launch_bounds__(kThreads) void expertDispatch(const T *__restrict__ x, int64_t x_stride, int64_t rows,
                                                            int channels, int choices, const int32_t *__restrict__ places,
                                                            const int32_t *__restrict__ starts, int experts,
                                                            int64_t first_block, int64_t row_blocks, bool streamed,
                                                            T *__restrict__ out) {
-  const Lanes<V> l(channels);
-  if (l.row < 0) return;
+  constexpr int N = kVectors<T, V>;
   const int64_t n = rows * choices, block = first_block + blockIdx.x;
   if (block >= row_blocks) {
-    zeroTail<T, V>(l, starts, experts, n, channels, (int)(block - row_blocks), out);
+    zeroTail<T, V>(starts, experts, n, channels, (int)(block - row_blocks), out);
     return;
   }
-  const int64_t r = block * l.rows_at_once + l.row;
+  const int64_t r = block * (kThreads / LANES) + (int)threadIdx.x / LANES;
   if (r >= rows) return;
-  const Vector<T, V> v = *reinterpret_cast<const Vector<T, V> *>(x + r * x_stride + l.channel);
-  float f[V];
+  for (int c = (int)threadIdx.x % LANES * V; c < channels; c += LANES * V * N) {
+    float v[N][V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = (float)v.v[i];
-  for (int k = 0; k < choices; ++k) {
-    const int64_t p = places[r * choices + k];
-    if (p >= 0 && p < n) storeFloats<T, V>(out + p * channels + l.channel, f, streamed);
+    for (int j = 0; j < N; ++j)
+      if (c + j * LANES * V < channels) loadFloats<T, V>(x + r * x_stride + c + j * LANES * V, v[j]);
+    for (int k = 0; k < choices; ++k) {
+      const int64_t p = places[r * choices + k];
+      if (p < 0 || p >= n) continue;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (c + j * LANES * V < channels) storeFloats<T, V>(out + p * channels + c + j * LANES * V, v[j], streamed);
+    }
   }
 }
 
@@ -113,50 +244,67 @@ struct Weights {
 constexpr int kAhead = 4;  // choices whose rows are on their way together
 
 // out[r] = sum over k of weight (r, k) * y[place of (r, k)], in the choices' order; a choice without a place adds nothing.
-template <typename T, int V>
+// Bound by memory, which it reads in places all over: 32 768 x 2 x 2048 bf16 (403 MB) 79 us, 5.1 TB/s.
+template <typename T, int V, int LANES>
 __global__ __launch_bounds__(kThreads) void expertCombine(const T *__restrict__ y, int64_t y_stride, int64_t rows,
                                                           int channels, int choices, const int32_t *__restrict__ places,
                                                           Weights weights, int64_t first_block, bool streamed,
                                                           T *__restrict__ out) {
-  const Lanes<V> l(channels);
-  if (l.row < 0) return;
-  const int64_t n = rows * choices, r = (first_block + blockIdx.x) * l.rows_at_once + l.row;
+  constexpr int N = kVectors<T, V>;
+  const int64_t n = rows * choices, r = (first_block + blockIdx.x) * (kThreads / LANES) + (int)threadIdx.x / LANES;
   if (r >= rows) return;
-  float sum[V] = {};
-  for (int k0 = 0; k0 < choices; k0 += kAhead) {
-    Vector<T, V> v[kAhead];
-    float w[kAhead];
-    bool there[kAhead];
+  for (int c = (int)threadIdx.x % LANES * V; c < channels; c += LANES * V * N) {
+    float sum[N][V] = {};
+    for (int k0 = 0; k0 < choices; k0 += kAhead) {
+      Vector<T, V> v[kAhead][N];
+      float w[kAhead];
+      bool there[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int64_t at = r * choices + (k0 + j < choices ? k0 + j : k0);
-      const int64_t p = places[at];
-      there[j] = k0 + j < choices && p >= 0 && p < n;
-      w[j] = weights.load(at);
-      v[j] = *reinterpret_cast<const Vector<T, V> *>(y + (there[j] ? p : 0) * y_stride + l.channel);
+      for (int j = 0; j < kAhead; ++j) {
+        const int64_t at = r * choices + (k0 + j < choices ? k0 + j : k0);
+        const int64_t p = places[at];
+        there[j] = k0 + j < choices && p >= 0 && p < n;
+        w[j] = weights.load(at);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int at_c = c + i * LANES * V;
+          v[j][i] = *reinterpret_cast<const Vector<T, V> *>(y + (there[j] ? p : 0) * y_stride + (at_c < channels ? at_c : c));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (!there[j]) continue;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int e = 0; e < V; ++e) sum[i][e] = fmaf(w[j], (float)v[j][i].v[e], sum[i][e]);
+      }
     }
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      if (!there[j]) continue;
-#pragma unroll
-      for (int i = 0; i < V; ++i) sum[i] = fmaf(w[j], (float)v[j].v[i], sum[i]);
-    }
+    for (int i = 0; i < N; ++i)
+      if (c + i * LANES * V < channels) storeFloats<T, V>(out + r * channels + c + i * LANES * V, sum[i], streamed);
   }
-  storeFloats<T, V>(out + r * channels + l.channel, sum, streamed);
 }
 
-// The gradients of the weighted sum: dy_r goes to the places times its weights, and the weights' gradients are products with what
-// lies there.  LANES lanes of a wave a row.
+// The gradients of the weighted sum: dout_r goes to the places times its weights, and the weights' gradients are products with what
+// lies there.  Up to 64 lanes, one wave's, a row.  Bound by memory: 16 384 x 4 x 1024 fp16 (302 MB) 54 us, 5.6 TB/s.  (Stores past the
+// caches, which serve the others: 32 768 x 2 x 2048 bf16 144 us in place of 126.)
 template <typename T, int V, int LANES>
 __global__ __launch_bounds__(kThreads) void expertCombineGrad(const T *__restrict__ dout, int64_t dout_stride,
                                                               const T *__restrict__ y, int64_t y_stride, int64_t rows,
                                                               int channels, int choices,
-                                                              const int32_t *__restrict__ places, Weights weights,
-                                                              int64_t first_block, bool streamed, T *__restrict__ dy,
-                                                              void *__restrict__ dweights) {
-  constexpr int kRows = kThreads / LANES;
+                                                              const int32_t *__restrict__ places,
+                                                              const int32_t *__restrict__ starts, int experts,
+                                                              Weights weights, int64_t first_block, int64_t row_blocks,
+                                                              T *__restrict__ dy, void *__restrict__ dweights) {
+  constexpr int N = kVectors<T, V>;
   const int lane = (int)threadIdx.x % LANES;
-  const int64_t n = rows * choices, r = (first_block + blockIdx.x) * kRows + (int)threadIdx.x / LANES;
+  const int64_t n = rows * choices, block = first_block + blockIdx.x;
+  if (block >= row_blocks) {
+    zeroTail<T, V>(starts, experts, n, channels, (int)(block - row_blocks), dy);
+    return;
+  }
+  const int64_t r = block * (kThreads / LANES) + (int)threadIdx.x / LANES;
   const bool row = r < rows;
   for (int k0 = 0; k0 < choices; k0 += kAhead) {
     int64_t p[kAhead];
@@ -172,25 +320,33 @@ __global__ __launch_bounds__(kThreads) void expertCombineGrad(const T *__restric
       }
     }
     if (row) {
-      for (int c = lane * V; c < channels; c += LANES * V) {
-        float g[V];
-        loadFloats<T, V>(dout + r * dout_stride + c, g);
-        Vector<T, V> v[kAhead];
+      for (int c = lane * V; c < channels; c += LANES * V * N) {
+        float g[N][V] = {};
+        Vector<T, V> v[kAhead][N];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-          v[j] = {};
-          if (p[j] >= 0 && dweights != nullptr) v[j] = *reinterpret_cast<const Vector<T, V> *>(y + p[j] * y_stride + c);
+        for (int i = 0; i < N; ++i) {
+          const int at = c + i * LANES * V;
+          if (at < channels) loadFloats<T, V>(dout + r * dout_stride + at, g[i]);
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j) {
+            v[j][i] = {};
+            if (p[j] >= 0 && dweights != nullptr && at < channels)
+              v[j][i] = *reinterpret_cast<const Vector<T, V> *>(y + p[j] * y_stride + at);
+          }
         }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
           if (p[j] < 0) continue;
-          float d[V];
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            d[i] = w[j] * g[i];
-            along[j] = fmaf(g[i], (float)v[j].v[i], along[j]);
+          for (int i = 0; i < N; ++i) {
+            float d[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              d[e] = w[j] * g[i][e];
+              along[j] = fmaf(g[i][e], (float)v[j][i].v[e], along[j]);
+            }
+            if (c + i * LANES * V < channels) storeFloats<T, V>(dy + p[j] * channels + c + i * LANES * V, d);
           }
-          storeFloats<T, V>(dy + p[j] * channels + c, d, streamed);
         }
       }
     }
@@ -203,17 +359,10 @@ __global__ __launch_bounds__(kThreads) void expertCombineGrad(const T *__restric
   }
 }
 
-template <typename T, int V>
-__global__ __launch_bounds__(kThreads) void expertZeroTail(const int32_t *__restrict__ starts, int experts, int64_t n,
-                                                           int channels, T *__restrict__ out) {
-  const Lanes<V> l(channels);
-  if (l.row >= 0) zeroTail<T, V>(l, starts, experts, n, channels, (int)blockIdx.x, out);
-}
-
 // ---- host side -----------------------------------------------------------------------------
 
 constexpr int kMostExperts = device_sort::kMaxDigits - 1;
-constexpr int kCounterWords = 16 * device_sort::kMaxDigits;  // that a workgroup of the order's second launch reads by itself
+constexpr int kCounterWords = 16 * device_sort::kMaxDigits;  // that every workgroup of the second launch adds up by itself
 
 struct Plan {
   int tiles, digits, digit_bits;
@@ -224,13 +373,15 @@ struct Plan {
 
 Plan planOf(int64_t n, int64_t experts) {
   Plan p;
-  p.tiles = device_sort::tilesFor(n);
-  p.few = device_sort::roundsFor(n) == 1 && p.tiles * (experts + 1) <= kCounterWords;
+  const int64_t tiles = (n + kOrderTile - 1) / kOrderTile;
+  p.few = tiles * (experts + 1) <= kCounterWords;
+  p.tiles = (int)tiles;
   p.digits = (int)(p.few ? experts + 1
                          : (experts + device_sort::kColumns) / device_sort::kColumns * device_sort::kColumns);
   p.digit_bits = 1;
   while (((int64_t)1 << p.digit_bits) < experts + 1) ++p.digit_bits;
-  p.counters = (device_sort::counterWords(n, p.digits) * sizeof(uint32_t) + 255) & ~(size_t)255;
+  const size_t words = p.few ? (size_t)tiles * p.digits : device_sort::counterWords(n, p.digits);
+  p.counters = (words * sizeof(uint32_t) + 255) & ~(size_t)255;
   p.starts = (size_t)p.digits * sizeof(uint32_t);
   return p;
 }
@@ -271,6 +422,8 @@ void byType(mluOpDataType_t type, int64_t channels, int64_t strides, uintptr_t a
   auto sixteen = [&](auto zero) {
     if (fits(8))
       f(zero, std::integral_constant<int, 8>());
+    else if (fits(4))
+      f(zero, std::integral_constant<int, 4>());
     else if (fits(2))
       f(zero, std::integral_constant<int, 2>());
     else
@@ -287,8 +440,24 @@ void byType(mluOpDataType_t type, int64_t channels, int64_t strides, uintptr_t a
   }
 }
 
-int rowsAtOnce(int64_t vectors) { return vectors >= kThreads ? 1 : (int)(kThreads / vectors); }
-unsigned slabsOf(int64_t vectors) { return (unsigned)((vectors + kThreads - 1) / kThreads); }
+// Calls f(LANES): threads for a row of so many pieces of 16 bytes, at most MOST.
+template <int MOST, typename F>
+void byLanes(int64_t pieces, F f) {
+  if (pieces <= 8)
+    f(std::integral_constant<int, 8>());
+  else if (pieces <= 16)
+    f(std::integral_constant<int, 16>());
+  else if (pieces <= 32)
+    f(std::integral_constant<int, 32>());
+  else if (pieces <= 64 || MOST <= 64)
+    f(std::integral_constant<int, 64>());
+  else if (pieces <= 128)
+    f(std::integral_constant<int, (MOST < 128 ? MOST : 128)>());
+  else
+    f(std::integral_constant<int, MOST>());
+}
+template <typename T>
+int64_t piecesOf(int64_t channels) { return (channels * (int64_t)sizeof(T) + 15) / 16; }
 
 }  // namespace
 
@@ -335,11 +504,14 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtExpertOrder(mluOpHandle_t handle, mluOpDataT
   lc.begin("expertOrder");
   if (n == 0) {
     expertStarts<<<(unsigned)(experts / kThreads + 1), kThreads, 0, lc.stream>>>(nullptr, (int)experts + 1, group_starts);
+  } else if (n <= kOrderTile) {
+    expertPlaces<true><<<1, kOrderThreads, 0, lc.stream>>>(items, n, (int)experts + 1, p.digit_bits, 0, nullptr, group_starts);
   } else if (p.few) {
-    uint32_t *hist = counters + device_sort::kMaxDigits;
-    device_sort::countTiles<Choices><<<p.tiles, device_sort::kTileThreads, 0, lc.stream>>>(items, n, p.digits, 1, hist);
-    device_sort::partitionTiles<Choices, false><<<p.tiles, device_sort::kTileThreads, 0, lc.stream>>>(
-        items, n, p.digits, p.digit_bits, 1, hist, nullptr, reinterpret_cast<uint32_t *>(group_starts));
+    int across = 1;
+    while (across < experts + 1 && across < kOrderThreads) across <<= 1;
+    expertCounts<<<p.tiles, kOrderThreads, 0, lc.stream>>>(items, n, p.digits, counters);
+    expertPlaces<false><<<p.tiles, kOrderThreads, 0, lc.stream>>>(items, n, p.digits, p.digit_bits, across, counters,
+                                                                  group_starts);
   } else {
     HIP_CHECK_RETURN(api, device_sort::partition(lc.stream, items, n, p.digits, p.digit_bits, counters, starts));
     expertStarts<<<(unsigned)(experts / kThreads + 1), kThreads, 0, lc.stream>>>(starts, (int)experts + 1, group_starts);
@@ -372,13 +544,16 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtExpertDispatch(mluOpHandle_t handle, mluOpDa
   byType(type, channels, features_stride, addresses, [&](auto zero, auto v) {
     typedef decltype(zero) T;
     constexpr int V = decltype(v)::value;
-    const int64_t at_once = rowsAtOnce(channels / V), blocks = (rows + at_once - 1) / at_once;
-    inLaunches(blocks + kTailBlocks, kThreads, [&](int64_t first, unsigned count) {
-      lc.begin("expertDispatch");
-      expertDispatch<T, V><<<dim3(count, slabsOf(channels / V)), kThreads, 0, lc.stream>>>(
-          static_cast<const T *>(features), features_stride, rows, (int)channels, (int)choices, places, group_starts,
-          (int)experts, first, blocks, bytes >= kStreamedBytes, static_cast<T *>(out));
-      lc.end();
+    byLanes<256>(piecesOf<T>(channels), [&](auto lanes) {
+      constexpr int LANES = decltype(lanes)::value;
+      const int64_t blocks = (rows + kThreads / LANES - 1) / (kThreads / LANES);
+      inLaunches(blocks + kTailBlocks, kThreads, [&](int64_t first, unsigned count) {
+        lc.begin("expertDispatch");
+        expertDispatch<T, V, LANES><<<count, kThreads, 0, lc.stream>>>(
+            static_cast<const T *>(features), features_stride, rows, (int)channels, (int)choices, places, group_starts,
+            (int)experts, first, blocks, bytes >= kStreamedBytes, static_cast<T *>(out));
+        lc.end();
+      });
     });
   });
   HIP_CHECK_RETURN(api, hipGetLastError());
@@ -407,13 +582,15 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtExpertCombine(mluOpHandle_t handle, mluOpDat
   byType(type, channels, results_stride, addresses, [&](auto zero, auto v) {
     typedef decltype(zero) T;
     constexpr int V = decltype(v)::value;
-    const int64_t at_once = rowsAtOnce(channels / V);
-    inLaunches((rows + at_once - 1) / at_once, kThreads, [&](int64_t first, unsigned count) {
-      lc.begin("expertCombine");
-      expertCombine<T, V><<<dim3(count, slabsOf(channels / V)), kThreads, 0, lc.stream>>>(
-          static_cast<const T *>(results), results_stride, rows, (int)channels, (int)choices, places,
-          Weights{weights, weight_type}, first, bytes >= kStreamedBytes, static_cast<T *>(out));
-      lc.end();
+    byLanes<256>(piecesOf<T>(channels), [&](auto lanes) {
+      constexpr int LANES = decltype(lanes)::value;
+      inLaunches((rows + kThreads / LANES - 1) / (kThreads / LANES), kThreads, [&](int64_t first, unsigned count) {
+        lc.begin("expertCombine");
+        expertCombine<T, V, LANES><<<count, kThreads, 0, lc.stream>>>(
+            static_cast<const T *>(results), results_stride, rows, (int)channels, (int)choices, places,
+            Weights{weights, weight_type}, first, bytes >= kStreamedBytes, static_cast<T *>(out));
+        lc.end();
+      });
     });
   });
   HIP_CHECK_RETURN(api, hipGetLastError());
@@ -455,25 +632,17 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtExpertCombineBackward(mluOpHandle_t handle, 
     T *dy = static_cast<T *>(results_grad);
     auto launch = [&](auto lanes) {
       constexpr int LANES = decltype(lanes)::value;
-      inLaunches((rows + kThreads / LANES - 1) / (kThreads / LANES), kThreads, [&](int64_t first, unsigned count) {
+      const int64_t blocks = (rows + kThreads / LANES - 1) / (kThreads / LANES);
+      inLaunches(blocks + kTailBlocks, kThreads, [&](int64_t first, unsigned count) {
         lc.begin("expertCombineGrad");
         expertCombineGrad<T, V, LANES><<<count, kThreads, 0, lc.stream>>>(
             static_cast<const T *>(output_grad), output_grad_stride, static_cast<const T *>(results), results_stride, rows,
-            (int)channels, (int)choices, places, Weights{weights, weight_type}, first, bytes >= kStreamedBytes, dy,
+            (int)channels, (int)choices, places, group_starts, (int)experts, Weights{weights, weight_type}, first, blocks, dy,
             weights_grad);
         lc.end();
       });
     };
-    if (channels / V <= 8)
-      launch(std::integral_constant<int, 8>());
-    else if (channels / V <= 16)
-      launch(std::integral_constant<int, 16>());
-    else
-      launch(std::integral_constant<int, 64>());
-    lc.begin("expertZeroTail");
-    expertZeroTail<T, V><<<dim3(kTailBlocks, slabsOf(channels / V)), kThreads, 0, lc.stream>>>(
-        group_starts, (int)experts, rows * choices, (int)channels, dy);
-    lc.end();
+    byLanes<64>(piecesOf<T>(channels), launch);
   });
   HIP_CHECK_RETURN(api, hipGetLastError());
   return MLUOP_STATUS_SUCCESS;
