@@ -44,8 +44,8 @@ struct Choices {
 // Tiles of kOrderTile choices, a workgroup each: one launch where one holds them all, else one that counts and one that places.
 // A wave has 64 * kTurns consecutive choices, 64 at a time in order; choices of one expert find each other with a ballot for each bit
 // of its number.  A choice's place is behind those of lower experts, of its expert in earlier tiles, in earlier waves, in earlier
-// turns of its wave, and in lower lanes.  us of the general partition / of these: 24 choices of 32 experts 7.8 / XX,
-// 65 536 of 64 16 / XX, 240 000 of 8 27 / XX.
+// turns of its wave, and in lower lanes.  us of the general partition / of these: 24 choices of 32 experts 7.8 /
+// 3.6, 65 536 of 64 15 / 10, 240 000 of 8 26 / 9.
 constexpr int kOrderThreads = 512, kOrderWaves = kOrderThreads / 64, kTurns = 4, kOrderTile = kOrderThreads * kTurns;
 constexpr int kMostDigits = device_sort::kMaxDigits;
 

@@ -127,7 +127,9 @@ struct Lines {
     return reinterpret_cast<T *>(base + (uintptr_t)(r * row_bytes) + (uintptr_t)offset);
   }
 };
-constexpr int64_t kMostStride = (int64_t)1 << 23;  // elements from row to row: offsets stay within 32 bits
+// (96 rows of fp32 that far apart: offsets stay within 32 bits)
+constexpr int64_t kMostStride = MLUOP_EXT_GATED_SCAN_MOST_STRIDE;
+static_assert((uint64_t)(kTileRows + 1) * kMostStride * sizeof(float) < (uint64_t)1 << 32, "32-bit offsets");
 
 // a and u of a gate: a row's step is h -> a h + u x.  Half of what these kernels compute is here.  What has to be exact is an a
 // close to one, whose error all steps of a long memory repeat: it is what a small u leaves of one.  An exponential beyond the

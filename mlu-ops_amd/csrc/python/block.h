@@ -126,8 +126,8 @@ struct ScanArguments {
 
   ScanArguments(const at::Tensor &features, const at::Tensor &g, const MaybeTensor &row_starts, int kind_code)
       : kind(static_cast<mluOpExtGate_t>(kind_code)) {
-    x = floatRows(features, "features are [rows, channels] of float32, float16 or bfloat16 on the GPU");
-    gates = floatRowsLike(g, x, "gates have the features' shape and type, on their GPU");
+    x = near(floatRows(features, "features are [rows, channels] of float32, float16 or bfloat16 on the GPU"));
+    gates = near(floatRowsLike(g, x, "gates have the features' shape and type, on their GPU"));
     rows = x.size(0);
     channels = x.size(1);
     samples = 1;
@@ -138,6 +138,8 @@ struct ScanArguments {
     type = dtypeCode(x.scalar_type());
     check(api.mluOpExtGetGatedScanSizes(rows, channels, samples, &carries, &workspace), "mluOpExtGetGatedScanSizes");
   }
+  // (rows that lie further apart than the operator takes are laid out anew)
+  static at::Tensor near(const at::Tensor &t) { return rowStride(t) > MLUOP_EXT_GATED_SCAN_MOST_STRIDE ? t.contiguous() : t; }
   // States [samples, channels], or nothing.
   at::Tensor states(const MaybeTensor &t, const char *what) const {
     if (!t || !t->defined()) return at::Tensor();
@@ -172,7 +174,7 @@ std::vector<at::Tensor> gatedScanBackward(mluOpHandle_t handle, bool guarded, co
                                           const at::Tensor &carries, const MaybeTensor &row_starts, int kind, bool reverse,
                                           bool want_initial) {
   const ScanArguments a(features, gates, row_starts, kind);
-  const at::Tensor dh = floatRowsLike(output_grad, a.x, "output_grad has the features' shape and type, on their GPU");
+  const at::Tensor dh = a.near(floatRowsLike(output_grad, a.x, "output_grad has the features' shape and type, on their GPU"));
   const at::Tensor df = a.states(final_grad, "final_grad is float32 [samples, channels] on the features' GPU");
   require(carries.device() == a.x.device() && carries.scalar_type() == at::kFloat && carries.dim() == 2 &&
               carries.size(0) == static_cast<int64_t>(a.carries) && carries.size(1) == a.channels && carries.is_contiguous(),

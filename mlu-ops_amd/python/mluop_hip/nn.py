@@ -554,6 +554,8 @@ class GatedScan(torch.nn.Module):
 
     def forward(self, x, row_starts=None, initial=None, states=False):
         if isinstance(x, SparseTensor):
+            if row_starts is not None or initial is not None or states:
+                raise ValueError("row_starts and states go with a tensor of rows")
             order, places, starts = x._rows_of_samples()
             rows = x.features if order is None else embedding(x.features, order)
             rows = self.forward(rows, starts)
