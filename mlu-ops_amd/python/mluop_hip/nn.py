@@ -438,7 +438,8 @@ def expert_order(experts_of_rows, experts):
 def expert_dispatch(features, places, group_starts):
     """Rows of `features` [rows, channels] at the places of their choices (`expert_order`), on the current device, with
     autograd: [rows * choices, channels], zeros behind the last expert's places.  A row is read once, and the gradients of its
-    copies are added up in 32 bits, in the choices' order."""
+    copies are added up in 32 bits, in the choices' order.  A choice is left out by a routing that gives it no expert; a place that
+    is taken out afterwards would leave its row, and the row of its gradient, as memory had them."""
     return native().expert_dispatch(features, places, group_starts, _guarded())
 
 
@@ -581,7 +582,11 @@ def dropout_add(features, residual, p, state):
 class DropoutAdd(torch.nn.Module):
     """Dropout of features onto a residual, `forward(features, residual=None)`, tensors or SparseTensors.  Every call in training
     mode has a number of its own, which is counted on the device: a captured graph drops other elements at every replay.  The seed
-    is drawn from torch's generator where none is given; it and the count are saved with the module's state."""
+    is drawn from torch's generator where none is given; it and the count are saved with the module's state.
+
+    Processes that train together drop the same elements where their seeds are the same (a wrapper that broadcasts buffers makes
+    them the same).  A forward pass that is run again inside of a backward pass, as activation checkpoints do, would have another
+    number and is refused: `dropout_add` with a state from outside of the checkpoint gives the same elements both times."""
 
     def __init__(self, p, seed=None):
         super().__init__()
@@ -598,6 +603,8 @@ class DropoutAdd(torch.nn.Module):
                 self.forward(features.features, residual.features if isinstance(residual, SparseTensor) else residual))
         if not self.training or self.p == 0.0:
             return features if residual is None else residual + features
+        if torch._C._current_graph_task_id() >= 0:
+            raise RuntimeError("a DropoutAdd inside of a backward pass would drop other elements than its forward pass did")
         with torch.no_grad():
             state = self.state.clone()
             self.state.add_(self._next)
