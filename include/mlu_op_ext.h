@@ -353,7 +353,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtLayerNormBackward(mluOpHandle_t handle, mluO
  * with the same row_starts, kind and direction.  Backward: final_grad fp32 [samples, channels] (NULL: zero), features_grad and
  * gates_grad [rows, channels], initial_grad fp32 [samples, channels] (NULL where not wanted).  One workspace size serves
  * both.  Rows are joined by composing their steps: a value that is not finite is one in the rows behind it (an infinity may be a
- * NaN there), and in no row in front of it.  At most 2^20 channels and samples, and MLUOP_EXT_GATED_SCAN_MOST_STRIDE elements from
+ * NaN there), and in no row in front of it; and with EXP gates above zero, products of a along a sample that leave fp32's range may
+ * make NaNs of states that are finite.  At most 2^20 channels and samples, and MLUOP_EXT_GATED_SCAN_MOST_STRIDE elements from
  * row to row. */
 #define MLUOP_EXT_GATED_SCAN_MOST_STRIDE (1 << 23)
 typedef enum {

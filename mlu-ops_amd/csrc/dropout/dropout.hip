@@ -1,5 +1,5 @@
-// mluOpExtDropoutAdd (no counterpart in the reference): elements dropped at random, the others scaled and added to a residual.  The
-// mask is never stored: it is computed again wherever it is needed, from the seed, the call and the element's number.
+// mluOpExtDropoutAdd (no counterpart in the reference): elements dropped at random, the others scaled and added to a residual.
+// The mask is never stored: it is computed again wherever it is needed, from the seed, the call and the element's number.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -42,8 +42,9 @@ __device__ __forceinline__ void randomWords(uint64_t low, uint64_t high, uint64_
 }
 
 // Bound by memory: 65 536 x 2048 bf16 onto a residual (805 MB) 141 us, 5.7 TB/s; 248 636 x 128 fp32 (382 MB) 68 us, its gradient
-// (255 MB) 46.  Ten rounds are some 60 operations for each of 8 elements' numbers and hide behind the loads; a number of 32 bits for
-// each element would be twice that.  ADD: onto the residual.  WIDE: addresses are multiples of 16 bytes.  Elements that are dropped are zero whatever they hold.
+// (255 MB) 46.  Ten rounds are some 60 operations for each of 8 elements' numbers and hide behind the loads; a number of 32 bits
+// for each element would be twice that.  ADD: onto the residual.  WIDE: addresses are multiples of 16 bytes.  Elements that are
+// dropped are zero whatever they hold.
 template <typename T, bool ADD, bool WIDE>
 __global__ __launch_bounds__(kThreads) void dropoutAdd(const T *__restrict__ x, const T *__restrict__ residual, int64_t n,
                                                        uint32_t threshold, float scale, const uint64_t *__restrict__ state,

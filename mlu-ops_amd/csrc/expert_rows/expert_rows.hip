@@ -42,10 +42,10 @@ struct Choices {
 };
 
 // Tiles of kOrderTile choices, a workgroup each: one launch where one holds them all, else one that counts and one that places.
-// A wave has 64 * kTurns consecutive choices, 64 at a time in order; choices of one expert find each other with a ballot for each bit
-// of its number.  A choice's place is behind those of lower experts, of its expert in earlier tiles, in earlier waves, in earlier
-// turns of its wave, and in lower lanes.  us of the general partition / of these: 24 choices of 32 experts 7.8 /
-// 3.6, 65 536 of 64 15 / 10, 240 000 of 8 26 / 9.
+// A wave has 64 * kTurns consecutive choices, 64 at a time in order; choices of one expert find each other with a ballot for each
+// bit of its number.  A choice's place is behind those of lower experts, of its expert in earlier tiles, in earlier waves, in
+// earlier turns of its wave, and in lower lanes.  us of the general partition / of these: 24 choices of 32 experts 7.8 / 3.6,
+// 65 536 of 64 15 / 10, 240 000 of 8 26 / 9.
 constexpr int kOrderThreads = 512, kOrderWaves = kOrderThreads / 64, kTurns = 4, kOrderTile = kOrderThreads * kTurns;
 constexpr int kMostDigits = device_sort::kMaxDigits;
 
@@ -66,8 +66,8 @@ __global__ __launch_bounds__(kOrderThreads) void expertCounts(Choices items, int
   for (int d = threadIdx.x; d < digits; d += kOrderThreads) hist[(size_t)blockIdx.x * digits + d] = s_count[d];
 }
 
-// Choices of every digit in all tiles, and in those in front of this workgroup's, to s_total and s_before: as many threads a digit
-// as there are, `across` (a power of two) digits side by side.
+// Choices of every digit in all tiles, and in those in front of this workgroup's, to s_total and s_before: as many threads a
+// digit as there are, `across` (a power of two) digits side by side.
 __device__ __forceinline__ void countsOfTiles(const uint32_t *__restrict__ hist, int tiles, int digits, int across,
                                               uint32_t *s_total, uint32_t *s_before) {
   constexpr int kAtOnce = 8;
@@ -174,8 +174,8 @@ __global__ __launch_bounds__(kThreads) void expertStarts(const uint32_t *__restr
 
 // ---- rows to their places and back ---------------------------------------------------------
 
-// LANES threads have a row, 16 bytes each whatever the vectors' width, as often as the row needs.  (A vector each: 60 000 rows of 250
-// bf16 from two places 60 us, 16 bytes 30.)
+// LANES threads have a row, 16 bytes each whatever the vectors' width, as often as the row needs.  (A vector each: 60 000 rows of
+// 250 bf16 from two places 60 us, 16 bytes 30.)
 template <typename T, int V>
 constexpr int kVectors = 16 / (int)sizeof(T) / V;
 
@@ -190,8 +190,8 @@ __device__ void zeroTail(const int32_t *starts, int experts, int64_t n, int chan
     storeFloats<T, V>(out + at * V, zero);
 }
 
-// out[place of (r, k)] = x[r] for every choice k: a row is read once and written as often as it is sent.  Bound by memory: 32 768 x 2
-// x 2048 bf16 (403 MB) 70 us, 5.7 TB/s.
+// out[place of (r, k)] = x[r] for every choice k: a row is read once and written as often as it is sent.  Bound by memory: 32 768
+// x 2 x 2048 bf16 (403 MB) 70 us, 5.7 TB/s.
 template <typename T, int V, int LANES>
 __global__ __launch_bounds__(kThreads) void expertDispatch(const T *__restrict__ x, int64_t x_stride, int64_t rows,
                                                            int channels, int choices, const int32_t *__restrict__ places,
@@ -286,9 +286,9 @@ __global__ __launch_bounds__(kThreads) void expertCombine(const T *__restrict__ 
   }
 }
 
-// The gradients of the weighted sum: dout_r goes to the places times its weights, and the weights' gradients are products with what
-// lies there.  Up to 64 lanes, one wave's, a row.  Bound by memory: 16 384 x 4 x 1024 fp16 (302 MB) 54 us, 5.6 TB/s.  (Stores past the
-// caches, which serve the others: 32 768 x 2 x 2048 bf16 144 us in place of 126.)
+// The gradients of the weighted sum: dout_r goes to the places times its weights, and the weights' gradients are products with
+// what lies there.  Up to 64 lanes, one wave's, a row.  Bound by memory: 16 384 x 4 x 1024 fp16 (302 MB) 54 us, 5.6 TB/s.
+// (Stores past the caches, which serve the others: 32 768 x 2 x 2048 bf16 144 us in place of 126.)
 template <typename T, int V, int LANES>
 __global__ __launch_bounds__(kThreads) void expertCombineGrad(const T *__restrict__ dout, int64_t dout_stride,
                                                               const T *__restrict__ y, int64_t y_stride, int64_t rows,

@@ -9,9 +9,9 @@
 // Maps, states and sums are fp32.
 //
 // Everything is done by single waves, which wait for no other: 16 lanes hold 8 bytes of a row each, a line of 128, and four
-// teams of 16 lanes have 8 rows each, one behind the other.  (Workgroups that composed 256 rows through LDS had 152 to 256
-// registers a thread and three waves or fewer a SIMD, which all waited together: 248 636 x 128 fp16, 48 us to read and 54 to
-// apply.)
+// teams of 16 lanes have rows one behind the other, 16 each where a tile is read, 4 each of a step.  (Workgroups that composed
+// 256 rows through LDS had 152 to 256 registers a thread and three waves or fewer a SIMD, which all waited together: 248 636 x
+// 128 fp16, 48 us to read and 54 to apply.)
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -30,9 +30,9 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kAcross = 16, kTeams = 64 / kAcross;  // lanes side by side, and teams of them behind one another
 constexpr int kPiece = 8;                           // rows of a thread that are read together
 constexpr int kTileRows = 2 * kPiece * kTeams;      // of a wave
-// Rows that a thread, and a wave, applies at a time.  The states in front of every step are what the backward pass takes: the same
-// for all types and alignments.  (Eight rows have an a and a u each in registers, and leave two or three waves a SIMD: 248 636 x
-// 128 fp16 44 us to apply, four rows 39; gradients of 65 536 x 1024 bf16 135 and 120.)
+// Rows that a thread, and a wave, applies at a time.  The states in front of every step are what the backward pass takes: the
+// same for all types and alignments.  (Eight rows have an a and a u each in registers, and leave two or three waves a SIMD:
+// 248 636 x 128 fp16 44 us to apply, four rows 39; gradients of 65 536 x 1024 bf16 135 and 120.)
 constexpr int kRows = 4, kStepRows = kTeams * kRows;
 constexpr int kOutsideBlocks = 8;  // workgroups of every slab for the rows of no sample
 
@@ -56,8 +56,8 @@ __device__ __forceinline__ int64_t firstSlot(int sample, int first_row) { return
 template <int ROWS>
 int64_t mostSlots(int64_t rows, int64_t samples) { return rows / ROWS + samples; }
 
-// What a wave has: a tile's rows in the order in which they are taken (row i of it is at `first + i * step`), or with WHOLE those of
-// a sample, and a slab of channels.
+// What a wave has: a tile's rows in the order in which they are taken (row i of it is at `first + i * step`), or with WHOLE those
+// of a sample, and a slab of channels.
 template <int V, bool WHOLE>
 struct Work {
   static constexpr int kChannels = kAcross * V;
@@ -107,8 +107,8 @@ struct Work {
   __device__ __forceinline__ int steps() const { return (rows + kStepRows - 1) / kStepRows; }
 };
 
-// Where the threads of a wave have TEAM_ROWS rows each of a tensor, row `at` and the following of the first team: a scalar address
-// for every row and one 32-bit offset for every thread (addresses of their own took most of the registers).
+// Where the threads of a wave have TEAM_ROWS rows each of a tensor, row `at` and the following of the first team: a scalar
+// address for every row and one 32-bit offset for every thread (addresses of their own took most of the registers).
 template <typename T, int TEAM_ROWS>
 struct Lines {
   uintptr_t base;
@@ -127,7 +127,7 @@ struct Lines {
     return reinterpret_cast<T *>(base + (uintptr_t)(r * row_bytes) + (uintptr_t)offset);
   }
 };
-// (96 rows of fp32 that far apart: offsets stay within 32 bits)
+// (a tile's rows of fp32 that far apart: offsets stay within 32 bits)
 constexpr int64_t kMostStride = MLUOP_EXT_GATED_SCAN_MOST_STRIDE;
 static_assert((uint64_t)(kTileRows + 1) * kMostStride * sizeof(float) < (uint64_t)1 << 32, "32-bit offsets");
 
@@ -233,14 +233,15 @@ __device__ __forceinline__ void composeTeams(int team, float &a, float &b, float
   const bool second = ((team & 1) != 0) != FROM_LAST, behind = (team >= 2) != FROM_LAST;
   a = second ? a1 : 1.f;
   b = second ? b1 : 0.f;
-  b = fmaf(a, behind ? pb1 : 0.f, b);
-  a *= behind ? pa1 : 1.f;
+  // (selected, not multiplied with zero: `a` may be infinite)
+  b = behind ? fmaf(a, pb1, b) : b;
+  a = behind ? a * pa1 : a;
 }
 
 // ---- forward -------------------------------------------------------------------------------
 
-// What a tile does to the state that comes into it, to tiles[slot][channel].  GRAD: to the gradient that comes into it from behind.
-// A team has 16 rows of a tile here, and the teams are composed once.
+// What a tile does to the state that comes into it, to tiles[slot][channel].  GRAD: to the gradient that comes into it from
+// behind.  A team has 16 rows of a tile here, and the teams are composed once.
 template <typename T, int V, int KIND, bool GRAD>
 __global__ __launch_bounds__(kThreads) void gatedScanTiles(const T *__restrict__ x, const T *__restrict__ g, Shape s,
                                                            int64_t first_block, float2 *__restrict__ tiles) {
@@ -276,8 +277,8 @@ __global__ __launch_bounds__(kThreads) void gatedScanTiles(const T *__restrict__
       }
     }
   };
-  // (a loop whatever the number of pieces: in a straight line the compiler mixes what it computes of two, and their loads are waited
-  // for together: 38 us in place of 31)
+  // (a loop whatever the number of pieces: in a straight line the compiler mixes what it computes of two, and their loads are
+  // waited for together: 38 us in place of 31)
   load(one, 0);
 #pragma unroll 1
   for (int k = 0; k < kPieces; k += 2) {
@@ -364,8 +365,8 @@ __global__ __launch_bounds__(kJoinThreads) void gatedScanJoin(const float2 *__re
   if (run == 0 && there && final != nullptr) final[(int64_t)sample * s.channels + channel] = h0;
 }
 
-// The state that comes into a wave's rows: from the one in front of its tile (JOINED), or of its sample through the tiles in front.
-// FROM_LAST: the gradient that comes in from behind.  `states` are those of the tiles or the samples (null: zero).
+// The state that comes into a wave's rows: from the one in front of its tile (JOINED), or of its sample through the tiles in
+// front.  FROM_LAST: the gradient that comes in from behind.  `states` are those of the tiles or the samples (null: zero).
 template <int V, Joining JOINING, bool FROM_LAST, typename WORK>
 __device__ __forceinline__ void incoming(const WORK &w, const Shape &s, const float *states, const float2 *tiles,
                                          float (&h)[V]) {
@@ -657,9 +658,9 @@ struct Workspace {
   }
 };
 
-// A wave for a whole sample, and one launch in place of two or three: where there are few rows, or about one a sample, as in a step of
-// many sequences.  (At worst one sample has them all, in 256 steps of a microsecond.)  Every wave folds the tiles in front of its own where
-// these are few, at most 16 for a team.
+// A wave for a whole sample, and one launch in place of two or three: where there are few rows, or about one a sample, as in a
+// step of many sequences.  (At worst one sample has them all, in 256 steps of a microsecond.)  Every wave folds the tiles in
+// front of its own where these are few, at most 16 for a team.
 Joining joiningOf(int64_t rows, int64_t samples) {
   if (rows <= std::max<int64_t>(512, std::min<int64_t>(2 * samples, 4096))) return kWhole;
   return rows <= 64 * kTileRows ? kFolded : kJoined;

@@ -62,9 +62,9 @@ struct Team {
 
 // ---- forward -------------------------------------------------------------------------------
 
-// y = (x - mean) * rstd * weight + bias.  The mean is the sum's, put right by the mean of the differences from it, so that rows far
-// off zero lose nothing; the variance is that of the differences.  Weight and bias stay in registers.  Bound by memory: 248 636 x
-// 128 fp16 (127 MB) 23.7 us, 5.4 TB/s; 32 768 x 2048 bf16 (268 MB) 52 us, 5.2 TB/s.
+// y = (x - mean) * rstd * weight + bias.  The mean is the sum's, put right by the mean of the differences from it, so that rows
+// far off zero lose nothing; the variance is that of the differences.  Weight and bias stay in registers.  Bound by memory:
+// 248 636 x 128 fp16 (127 MB) 23.7 us, 5.4 TB/s; 32 768 x 2048 bf16 (268 MB) 52 us, 5.2 TB/s.
 template <typename T, int V, int LANES, int N>
 __global__ __launch_bounds__((Team<V, LANES, N>::kWorkgroup)) void layerNormRows(const T *__restrict__ x, Shape s,
                                                                                 ChannelParams p, float eps,
@@ -329,8 +329,9 @@ constexpr int kWideThreads = 1024;  // of a workgroup that holds a row of up to 
 
 constexpr int kBlocks = 4096;       // most workgroups of 256 threads
 
-// Most rows of partial sums: as many workgroups as the CUs hold together, as long as the sums themselves stay few (32 768 x 2048 bf16:
-// 512 workgroups 95 us and 5 to add up, 1024 77 and 7; 16 384 x 8192: 149 and 12, 154 and 22; 60 000 x 250: 31 and 5, 2048 22 and 6).
+// Most rows of partial sums: as many workgroups as the CUs hold together, as long as the sums themselves stay few (32 768 x 2048
+// bf16: 512 workgroups 95 us and 5 to add up, 1024 77 and 7; 16 384 x 8192: 149 and 12, 154 and 22; 60 000 x 250: 31 and 5, 2048
+// 22 and 6).
 int64_t sumParts(int64_t channels) { return channels <= 512 ? 2048 : channels <= 2048 ? 1024 : 512; }
 
 mluOpStatus_t checkShape(const char *api, int64_t rows, int64_t channels) {
@@ -459,12 +460,13 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtLayerNormBackward(mluOpHandle_t handle, mluO
           const int64_t blocks = (rows + L::kTeams - 1) / L::kTeams;
           parts = (int)std::min<int64_t>(blocks, sumParts(channels));
           lc.begin("layerNormGrad");
-          if (sums)
-            layerNormGrad<T, V, LANES, N, true><<<(unsigned)parts, L::kWorkgroup, 0, lc.stream>>>(dy, x, s, p, mean, rstd,
-                                                                                                     dx, partial);
-          else
-            layerNormGrad<T, V, LANES, N, false><<<(unsigned)std::min<int64_t>(blocks, kBlocks * kThreads / L::kWorkgroup), L::kWorkgroup, 0, lc.stream>>>(
-                dy, x, s, p, mean, rstd, dx, nullptr);
+          if (sums) {
+            layerNormGrad<T, V, LANES, N, true><<<(unsigned)parts, L::kWorkgroup, 0, lc.stream>>>(dy, x, s, p, mean, rstd, dx,
+                                                                                                  partial);
+          } else {
+            const unsigned grid = (unsigned)std::min<int64_t>(blocks, kBlocks * kThreads / L::kWorkgroup);
+            layerNormGrad<T, V, LANES, N, false><<<grid, L::kWorkgroup, 0, lc.stream>>>(dy, x, s, p, mean, rstd, dx, nullptr);
+          }
           lc.end();
         });
       } else {

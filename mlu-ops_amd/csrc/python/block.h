@@ -314,8 +314,8 @@ std::vector<at::Tensor> expertCombineBackward(mluOpHandle_t handle, bool guarded
   const at::Tensor w = weightsOn(weights, y, from, &weight_type);
   const Buffers buffers(guarded, y.device());
   const at::Tensor dy = buffers.output({y.size(0), y.size(1)}, y.scalar_type(), "results_grad");
-  const at::Tensor dw = want_weights && w.defined() ? buffers.output({from.size(0), from.size(1)}, w.scalar_type(), "weights_grad")
-                                                    : at::Tensor();
+  const at::Tensor dw =
+      want_weights && w.defined() ? buffers.output({from.size(0), from.size(1)}, w.scalar_type(), "weights_grad") : at::Tensor();
   check(api.mluOpExtExpertCombineBackward(handle, dtypeCode(y.scalar_type()), dout.data_ptr(), rowStride(dout), y.data_ptr(),
                                           rowStride(y), from.size(0), y.size(1), from.size(1),
                                           addressOf<const int32_t>(from), addressOf<const int32_t>(starts),

@@ -1,5 +1,5 @@
-"""Operators of a residual block over ragged rows (mlu_op_ext.h): layer norm, a gated recurrence along the rows of every sample, rows
-by expert and back, dropout onto a residual.  Each function makes one call of the C API on a `Handle` and returns new tensors; all
+"""Operators of a residual block over ragged rows (mlu_op_ext.h): layer norm, a gated recurrence along the rows of every sample,
+rows by expert and back, dropout onto a residual.  Each function makes one call of the C API on a `Handle` and returns new tensors; all
 are names of the package itself."""
 import ctypes
 
