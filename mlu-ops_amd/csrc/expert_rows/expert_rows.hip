@@ -175,9 +175,20 @@ __global__ __launch_bounds__(kThreads) void expertStarts(const uint32_t *__restr
 // ---- rows to their places and back ---------------------------------------------------------
 
 // LANES threads have a row, 16 bytes each whatever the vectors' width, as often as the row needs.  (A vector each: 60 000 rows of
-// 250 bf16 from two places 60 us, 16 bytes 30.)
+// 250 bf16 from two places 60 us, 16 bytes 30.  Eight threads or more, where two hold a row: 1 875 000 rows of 16 bf16 back 92 us,
+// two 47.)
 template <typename T, int V>
 constexpr int kVectors = 16 / (int)sizeof(T) / V;
+
+// Rows that are not whole lines of 128 bytes share lines with their neighbours.  Workgroups go to the eight XCDs in turn: with runs
+// of rows for each, what shares a line in front and behind mostly meets in one L2, and results stay in the caches, where a line is
+// filled before it goes to memory (sent past them 1 875 000 rows of 16 bf16 take 54 us, else 37, in runs 30; 227 272 x 4 x 33 bf16
+// 49 and in runs 39, their gradients 81 and 66).  Whole lines are better off in turn (32 768 x 2 x 2048 bf16 76 and in runs 80).
+__device__ __forceinline__ int64_t inRuns(int64_t block, int64_t blocks) {
+  const int64_t run = blocks / 8;
+  return block < run * 8 ? block % 8 * run + block / 8 : block;
+}
+inline bool wholeLines(int64_t channels, mluOpDataType_t type) { return channels * elementBytes(type) % 128 == 0; }
 
 constexpr int kTailBlocks = 64;  // workgroups for the places behind the last expert's, which are zero
 
@@ -196,15 +207,15 @@ template <typename T, int V, int LANES>
 __global__ __launch_bounds__(kThreads) void expertDispatch(const T *__restrict__ x, int64_t x_stride, int64_t rows,
                                                            int channels, int choices, const int32_t *__restrict__ places,
                                                            const int32_t *__restrict__ starts, int experts,
-                                                           int64_t first_block, int64_t row_blocks, bool streamed,
-                                                           T *__restrict__ out) {
+                                                           int64_t first_block, int64_t row_blocks, bool lines,
+                                                           bool streamed, T *__restrict__ out) {
   constexpr int N = kVectors<T, V>;
   const int64_t n = rows * choices, block = first_block + blockIdx.x;
   if (block >= row_blocks) {
     zeroTail<T, V>(starts, experts, n, channels, (int)(block - row_blocks), out);
     return;
   }
-  const int64_t r = block * (kThreads / LANES) + (int)threadIdx.x / LANES;
+  const int64_t r = (lines ? block : inRuns(block, row_blocks)) * (kThreads / LANES) + (int)threadIdx.x / LANES;
   if (r >= rows) return;
   for (int c = (int)threadIdx.x % LANES * V; c < channels; c += LANES * V * N) {
     float v[N][V];
@@ -244,14 +255,16 @@ struct Weights {
 constexpr int kAhead = 4;  // choices whose rows are on their way together
 
 // out[r] = sum over k of weight (r, k) * y[place of (r, k)], in the choices' order; a choice without a place adds nothing.
-// Bound by memory, which it reads in places all over: 32 768 x 2 x 2048 bf16 (403 MB) 79 us, 5.1 TB/s.
+// Bound by memory, which it reads in places all over: 32 768 x 2 x 2048 bf16 (403 MB) 70 us, 5.7 TB/s.  (Choices that a row has
+// not read as its first: 79.)
 template <typename T, int V, int LANES>
 __global__ __launch_bounds__(kThreads) void expertCombine(const T *__restrict__ y, int64_t y_stride, int64_t rows,
                                                           int channels, int choices, const int32_t *__restrict__ places,
-                                                          Weights weights, int64_t first_block, bool streamed,
-                                                          T *__restrict__ out) {
+                                                          Weights weights, int64_t first_block, int64_t row_blocks,
+                                                          bool lines, bool streamed, T *__restrict__ out) {
   constexpr int N = kVectors<T, V>;
-  const int64_t n = rows * choices, r = (first_block + blockIdx.x) * (kThreads / LANES) + (int)threadIdx.x / LANES;
+  const int64_t n = rows * choices, block = first_block + blockIdx.x;
+  const int64_t r = (lines ? block : inRuns(block, row_blocks)) * (kThreads / LANES) + (int)threadIdx.x / LANES;
   if (r >= rows) return;
   for (int c = (int)threadIdx.x % LANES * V; c < channels; c += LANES * V * N) {
     float sum[N][V] = {};
@@ -261,9 +274,10 @@ __global__ __launch_bounds__(kThreads) void expertCombine(const T *__restrict__ 
       bool there[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const int64_t at = r * choices + (k0 + j < choices ? k0 + j : k0);
-        const int64_t p = places[at];
-        there[j] = k0 + j < choices && p >= 0 && p < n;
+        there[j] = false;
+        if (k0 + j >= choices) continue;
+        const int64_t at = r * choices + k0 + j, p = places[at];
+        there[j] = p >= 0 && p < n;
         w[j] = weights.load(at);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -296,7 +310,8 @@ __global__ __launch_bounds__(kThreads) void expertCombineGrad(const T *__restric
                                                               const int32_t *__restrict__ places,
                                                               const int32_t *__restrict__ starts, int experts,
                                                               Weights weights, int64_t first_block, int64_t row_blocks,
-                                                              T *__restrict__ dy, void *__restrict__ dweights) {
+                                                              bool lines, T *__restrict__ dy,
+                                                              void *__restrict__ dweights) {
   constexpr int N = kVectors<T, V>;
   const int lane = (int)threadIdx.x % LANES;
   const int64_t n = rows * choices, block = first_block + blockIdx.x;
@@ -304,7 +319,7 @@ __global__ __launch_bounds__(kThreads) void expertCombineGrad(const T *__restric
     zeroTail<T, V>(starts, experts, n, channels, (int)(block - row_blocks), dy);
     return;
   }
-  const int64_t r = block * (kThreads / LANES) + (int)threadIdx.x / LANES;
+  const int64_t r = (lines ? block : inRuns(block, row_blocks)) * (kThreads / LANES) + (int)threadIdx.x / LANES;
   const bool row = r < rows;
   for (int k0 = 0; k0 < choices; k0 += kAhead) {
     int64_t p[kAhead];
@@ -443,7 +458,11 @@ void byType(mluOpDataType_t type, int64_t channels, int64_t strides, uintptr_t a
 // Calls f(LANES): threads for a row of so many pieces of 16 bytes, at most MOST.
 template <int MOST, typename F>
 void byLanes(int64_t pieces, F f) {
-  if (pieces <= 8)
+  if (pieces <= 2)
+    f(std::integral_constant<int, 2>());
+  else if (pieces <= 4)
+    f(std::integral_constant<int, 4>());
+  else if (pieces <= 8)
     f(std::integral_constant<int, 8>());
   else if (pieces <= 16)
     f(std::integral_constant<int, 16>());
@@ -539,6 +558,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtExpertDispatch(mluOpHandle_t handle, mluOpDa
   HIP_CHECK_RETURN(api, hipSetDevice(handle->device));
   const size_t bytes = (size_t)rows * choices * channels * elementBytes(type);
   handle->forgetNotesIn(out, bytes);
+  const bool lines = wholeLines(channels, type);
   const mluop::LaunchCtx lc = handle->launchCtx();
   const uintptr_t addresses = reinterpret_cast<uintptr_t>(features) | reinterpret_cast<uintptr_t>(out);
   byType(type, channels, features_stride, addresses, [&](auto zero, auto v) {
@@ -551,7 +571,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtExpertDispatch(mluOpHandle_t handle, mluOpDa
         lc.begin("expertDispatch");
         expertDispatch<T, V, LANES><<<count, kThreads, 0, lc.stream>>>(
             static_cast<const T *>(features), features_stride, rows, (int)channels, (int)choices, places, group_starts,
-            (int)experts, first, blocks, bytes >= kStreamedBytes, static_cast<T *>(out));
+            (int)experts, first, blocks, lines, lines && bytes >= kStreamedBytes, static_cast<T *>(out));
         lc.end();
       });
     });
@@ -577,6 +597,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtExpertCombine(mluOpHandle_t handle, mluOpDat
   HIP_CHECK_RETURN(api, hipSetDevice(handle->device));
   const size_t bytes = (size_t)rows * channels * elementBytes(type);
   handle->forgetNotesIn(out, bytes);
+  const bool lines = wholeLines(channels, type);
   const mluop::LaunchCtx lc = handle->launchCtx();
   const uintptr_t addresses = reinterpret_cast<uintptr_t>(results) | reinterpret_cast<uintptr_t>(out);
   byType(type, channels, results_stride, addresses, [&](auto zero, auto v) {
@@ -584,11 +605,12 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtExpertCombine(mluOpHandle_t handle, mluOpDat
     constexpr int V = decltype(v)::value;
     byLanes<256>(piecesOf<T>(channels), [&](auto lanes) {
       constexpr int LANES = decltype(lanes)::value;
-      inLaunches((rows + kThreads / LANES - 1) / (kThreads / LANES), kThreads, [&](int64_t first, unsigned count) {
+      const int64_t blocks = (rows + kThreads / LANES - 1) / (kThreads / LANES);
+      inLaunches(blocks, kThreads, [&](int64_t first, unsigned count) {
         lc.begin("expertCombine");
         expertCombine<T, V, LANES><<<count, kThreads, 0, lc.stream>>>(
             static_cast<const T *>(results), results_stride, rows, (int)channels, (int)choices, places,
-            Weights{weights, weight_type}, first, bytes >= kStreamedBytes, static_cast<T *>(out));
+            Weights{weights, weight_type}, first, blocks, lines, bytes >= kStreamedBytes, static_cast<T *>(out));
         lc.end();
       });
     });
@@ -623,6 +645,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtExpertCombineBackward(mluOpHandle_t handle, 
     handle->forgetNotesIn(results_grad, bytes);
     if (weights_grad) handle->forgetNotesIn(weights_grad, (size_t)rows * choices * elementBytes(weight_type));
   }
+  const bool lines = wholeLines(channels, type);
   const mluop::LaunchCtx lc = handle->launchCtx();
   const uintptr_t addresses = reinterpret_cast<uintptr_t>(output_grad) | reinterpret_cast<uintptr_t>(results) |
                               reinterpret_cast<uintptr_t>(results_grad);
@@ -637,8 +660,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtExpertCombineBackward(mluOpHandle_t handle, 
         lc.begin("expertCombineGrad");
         expertCombineGrad<T, V, LANES><<<count, kThreads, 0, lc.stream>>>(
             static_cast<const T *>(output_grad), output_grad_stride, static_cast<const T *>(results), results_stride, rows,
-            (int)channels, (int)choices, places, group_starts, (int)experts, Weights{weights, weight_type}, first, blocks, dy,
-            weights_grad);
+            (int)channels, (int)choices, places, group_starts, (int)experts, Weights{weights, weight_type}, first, blocks,
+            lines, dy, weights_grad);
         lc.end();
       });
     };
