@@ -1,0 +1,60 @@
+"""Rows of few channels through the operators of a residual block: threads that share a row are fewer, and rows share lines."""
+import pytest
+
+from test_gpu_expert_rows import LAST, LEAST, routing, taken
+
+pytestmark = pytest.mark.gpu
+
+CHANNELS = [1, 2, 4, 7, 8, 12, 16, 24, 31, 32, 33, 48]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("channels", CHANNELS)
+def test_norm(gpu_handle, dtype, channels):
+    import torch
+    import mluop_hip
+    rows = 4099
+    g = torch.Generator(device="cuda").manual_seed(channels)
+    x, dy = (torch.randn(rows, channels, device="cuda", generator=g).to(getattr(torch, dtype)) for _ in range(2))
+    w, b = 1 + 0.2 * torch.randn(channels, device="cuda", generator=g), torch.randn(channels, device="cuda", generator=g)
+    # (an eps of the spread's size: the root of a row of two values that are almost one hides no error)
+    out, mean, rstd = mluop_hip.layer_norm_forward(gpu_handle, x, w, b, 0.1)
+    leaves = [t.double().requires_grad_() for t in (x, w, b)]
+    want = torch.nn.functional.layer_norm(leaves[0], (channels,), leaves[1], leaves[2], 0.1)
+    grads = torch.autograd.grad(want, leaves, dy.double())
+    # a row's sums have at most 48 terms of 2^-24 each, its gradient three such sums of values below 2^6
+    row = 160 * 2.0 ** -24
+    assert bool(((out.double() - want).abs() <= LAST[dtype] * want.abs() + row * 8).all())
+    got = mluop_hip.layer_norm_backward(gpu_handle, dy, x, w, b, mean, rstd)
+    assert bool(((got[0].double() - grads[0]).abs() <= LAST[dtype] * grads[0].abs() + row * 64).all())
+    # a column: up to 256 teams one after the other, some tens of workgroups, 64 shares, of values below 2^5
+    normed = (leaves[0].detach() - mean.double()[:, None]) * rstd.double()[:, None]
+    for a, c, terms in ((got[1], grads[1], dy.double() * normed), (got[2], grads[2], dy.double())):
+        assert bool(((a.double() - c).abs() <= 512 * 2.0 ** -24 * terms.abs().sum(0) + rows * row).all())
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("channels", CHANNELS)
+@pytest.mark.parametrize("choices", [1, 2, 5])
+def test_rows_by_expert(gpu_handle, dtype, channels, choices):
+    import torch
+    import mluop_hip
+    rows, experts = 3001, 11
+    chosen, g = routing(rows, choices, experts, channels)
+    x, y, dy = (torch.randn(n, channels, device="cuda", generator=g).to(getattr(torch, dtype))
+                for n in (rows, rows * choices, rows))
+    w = torch.rand(rows, choices, device="cuda", generator=g)
+    named, starts, places = mluop_hip.expert_order(gpu_handle, chosen, experts)
+    assert torch.equal(mluop_hip.expert_dispatch(gpu_handle, x, places, starts),
+                       mluop_hip.embedding_forward(gpu_handle, x, named))
+
+    def near(got, want, size, units, last):
+        assert bool(((got.double() - want).abs() <= LAST[last] * want.abs() + units * 2.0 ** -24 * size + LEAST).all())
+    terms = taken(y, places) * w.double().unsqueeze(2)
+    near(mluop_hip.expert_combine(gpu_handle, y, places, w), terms.sum(dim=1), terms.abs().sum(dim=1), choices + 1, dtype)
+    dr, dw = mluop_hip.expert_combine_backward(gpu_handle, dy, y, places, w, starts)
+    want, there = torch.zeros(rows * choices, channels, device="cuda", dtype=torch.float64), places >= 0
+    want[places[there].long()] = (dy.double().unsqueeze(1) * w.double().unsqueeze(2))[there]
+    near(dr, want, want.abs(), 1, dtype)
+    terms = dy.double().unsqueeze(1) * taken(y, places)
+    near(dw, terms.sum(dim=2), terms.abs().sum(dim=2), channels + 8, "float32")
