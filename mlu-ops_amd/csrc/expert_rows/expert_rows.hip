@@ -175,15 +175,16 @@ __global__ __launch_bounds__(kThreads) void expertStarts(const uint32_t *__restr
 // ---- rows to their places and back ---------------------------------------------------------
 
 // LANES threads have a row, 16 bytes each whatever the vectors' width, as often as the row needs.  (A vector each: 60 000 rows of
-// 250 bf16 from two places 60 us, 16 bytes 30.  Eight threads or more, where two hold a row: 1 875 000 rows of 16 bf16 back 92 us,
-// two 47.)
+// 250 bf16 from two places 60 us, 16 bytes 30.  Eight threads or more, where two hold a row: 1 875 000 rows of 16 bf16 back 92
+// us, two 47.)
 template <typename T, int V>
 constexpr int kVectors = 16 / (int)sizeof(T) / V;
 
-// Rows that are not whole lines of 128 bytes share lines with their neighbours.  Workgroups go to the eight XCDs in turn: with runs
-// of rows for each, what shares a line in front and behind mostly meets in one L2, and results stay in the caches, where a line is
-// filled before it goes to memory (sent past them 1 875 000 rows of 16 bf16 take 54 us, else 37, in runs 30; 227 272 x 4 x 33 bf16
-// 49 and in runs 39, their gradients 81 and 66).  Whole lines are better off in turn (32 768 x 2 x 2048 bf16 76 and in runs 80).
+// Rows that are not whole lines of 128 bytes share lines with their neighbours.  Workgroups go to the eight XCDs in turn: with
+// runs of rows for each, what shares a line in front and behind mostly meets in one L2, and results stay in the caches, where a
+// line is filled before it goes to memory (sent past them 1 875 000 rows of 16 bf16 take 54 us, else 37, in runs 30; 227 272 x 4
+// x 33 bf16 49 and in runs 39, their gradients 81 and 66).  Whole lines are better off in turn (32 768 x 2 x 2048 bf16 76 and in
+// runs 80).
 __device__ __forceinline__ int64_t inRuns(int64_t block, int64_t blocks) {
   const int64_t run = blocks / 8;
   return block < run * 8 ? block % 8 * run + block / 8 : block;

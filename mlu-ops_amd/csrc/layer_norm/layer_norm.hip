@@ -304,8 +304,8 @@ void byType(mluOpDataType_t type, int64_t channels, int64_t strides, uintptr_t a
 template <typename T, int V>
 constexpr int kVectors = 16 / (int)sizeof(T) / V;
 
-// Calls f(LANES): the smallest team that holds a row whose threads' 16 bytes are `pieces`.  (Teams of eight for 1 875 000 rows of 16
-// bf16: 57 us forward and 61 backward, of two 24 and 40.)
+// Calls f(LANES): the smallest team that holds a row whose threads' 16 bytes are `pieces`.  (Teams of eight for 1 875 000 rows of
+// 16 bf16: 57 us forward and 61 backward, of two 24 and 40.)
 template <typename F>
 void byTeam(int64_t pieces, F f) {
   if (pieces <= 2)
