@@ -9,7 +9,8 @@
 // Maps, states and sums are fp32.
 //
 // Everything is done by single waves, which wait for no other: 16 lanes hold 8 bytes of a row each, a line of 128, and four
-// teams of 16 lanes have rows one behind the other, 16 each where a tile is read, 4 each of a step.  (Workgroups that composed
+// teams of 16 lanes have rows one behind the other, 16 each where a tile is read, 4 each of a step.  Narrow rows are held by 4 or
+// 8 lanes, and there are 16 or 8 teams.  (Workgroups that composed
 // 256 rows through LDS had 152 to 256 registers a thread and three waves or fewer a SIMD, which all waited together: 248 636 x
 // 128 fp16, 48 us to read and 54 to apply.)
 #include <hip/hip_runtime.h>
@@ -19,6 +20,7 @@
 
 #include "core/core.h"
 #include "core/elements.h"
+#include "core/lane_sum.h"
 #include "core/ragged.h"
 #include "mlu_op_ext.h"
 
@@ -27,13 +29,22 @@ namespace {
 using namespace mluop;
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kAcross = 16, kTeams = 64 / kAcross;  // lanes side by side, and teams of them behind one another
-constexpr int kPiece = 8;                           // rows of a thread that are read together
-constexpr int kTileRows = 2 * kPiece * kTeams;      // of a wave
-// Rows that a thread, and a wave, applies at a time.  The states in front of every step are what the backward pass takes: the
-// same for all types and alignments.  (Eight rows have an a and a u each in registers, and leave two or three waves a SIMD:
+constexpr int kPiece = 8;       // rows of a thread that are read together
+// Rows that a thread applies at a time.  (Eight rows have an a and a u each in registers, and leave two or three waves a SIMD:
 // 248 636 x 128 fp16 44 us to apply, four rows 39; gradients of 65 536 x 1024 bf16 135 and 120.)
-constexpr int kRows = 4, kStepRows = kTeams * kRows;
+constexpr int kRows = 4;
+constexpr int kStateRows = 16;  // from one of the states that the backward pass takes to the next, whatever lies how
+constexpr int kLeastTile = 64, kMostTile = 256;
+
+// ACROSS lanes side by side, and teams of them behind one another.  (1 875 000 x 16 bf16: by 16 lanes, of which four have
+// channels, 76 us to read and 94 to apply, by 4 31 and 43; its gradients 142 and 88.  937 500 x 32, by 16 and 8: 43 and 49, 30
+// and 38; 82 and 73.)
+template <int ACROSS>
+struct Layout {
+  static constexpr int kTeams = 64 / ACROSS;
+  static constexpr int kTileRows = 2 * kPiece * kTeams, kStepRows = kRows * kTeams;  // of a wave
+  static_assert(kTileRows >= kLeastTile && kTileRows <= kMostTile && kStepRows % kStateRows == 0, "");
+};
 constexpr int kOutsideBlocks = 8;  // workgroups of every slab for the rows of no sample
 
 // Who works out the states in front of the tiles: nobody (a wave has a whole sample), every wave for itself, a launch of its own.
@@ -58,10 +69,11 @@ int64_t mostSlots(int64_t rows, int64_t samples) { return rows / ROWS + samples;
 
 // What a wave has: a tile's rows in the order in which they are taken (row i of it is at `first + i * step`), or with WHOLE those
 // of a sample, and a slab of channels.
-template <int V, bool WHOLE>
-struct Work {
-  static constexpr int kChannels = kAcross * V;
-  int64_t first, tile_slot, step_slot;
+template <int V, int ACROSS, bool WHOLE>
+struct Work : Layout<ACROSS> {
+  using Layout<ACROSS>::kTeams, Layout<ACROSS>::kTileRows, Layout<ACROSS>::kStepRows;
+  static constexpr int kChannels = ACROSS * V;
+  int64_t first, tile_slot, state_slot;
   int step, rows, sample;  // sample -1: nothing
   int in_sample, tiles;    // the tile's number in its sample, and how many that has
   int team, channel;
@@ -71,8 +83,8 @@ struct Work {
   // (four tiles of one slab: 35 us to read 248 636 x 128 fp16 in place of 31); tiles, or samples, along y.  FROM_LAST: the launch
   // before had them in order, and what it had last comes first.
   __device__ Work(const Shape &s, int64_t block, int64_t blocks, bool from_last) : sample(-1) {
-    const int lane = (int)threadIdx.x % kAcross, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
-    team = (int)threadIdx.x / kAcross % kTeams;
+    const int lane = (int)threadIdx.x % ACROSS, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+    team = (int)threadIdx.x / ACROSS % kTeams;
     channel = ((int)blockIdx.x * s.side_by_side + wave % s.side_by_side) * kChannels;
     if (channel >= s.channels) return;
     there = channel + lane * V < s.channels;
@@ -100,7 +112,7 @@ struct Work {
     step = s.reverse ? -1 : 1;
     first = s.reverse ? (int64_t)segment_first + segment_rows - 1 - from : (int64_t)segment_first + from;
     tile_slot = firstSlot<kTileRows>(sample, segment_first) + in_sample;
-    step_slot = firstSlot<kStepRows>(sample, segment_first) + from / kStepRows;
+    state_slot = firstSlot<kStateRows>(sample, segment_first) + from / kStateRows;
   }
   __device__ __forceinline__ bool begins() const { return in_sample == 0; }
   __device__ __forceinline__ bool ends() const { return WHOLE || in_sample == tiles - 1; }
@@ -117,19 +129,20 @@ struct Lines {
   template <typename WORK>
   __device__ __forceinline__ Lines(const T *from, int64_t stride, const WORK &w, int at) {
     // (backwards the last team's rows lie first)
-    const int64_t row = w.first + (int64_t)w.step * at - (w.step < 0 ? (kTeams - 1) * TEAM_ROWS : 0);
+    const int64_t row = w.first + (int64_t)w.step * at - (w.step < 0 ? (WORK::kTeams - 1) * TEAM_ROWS : 0);
     base = reinterpret_cast<uintptr_t>(from) + (uintptr_t)(row * stride * (int64_t)sizeof(T));
     row_bytes = w.step * stride * (int64_t)sizeof(T);
-    offset = (uint32_t)(w.step < 0 ? kTeams - 1 - w.team : w.team) * (uint32_t)(TEAM_ROWS * stride * (int64_t)sizeof(T)) +
+    offset = (uint32_t)(w.step < 0 ? WORK::kTeams - 1 - w.team : w.team) * (uint32_t)(TEAM_ROWS * stride * (int64_t)sizeof(T)) +
              (uint32_t)w.channel * (uint32_t)sizeof(T);
   }
   __device__ __forceinline__ T *row(int r) const {
     return reinterpret_cast<T *>(base + (uintptr_t)(r * row_bytes) + (uintptr_t)offset);
   }
 };
-// (a tile's rows of fp32 that far apart: offsets stay within 32 bits)
-constexpr int64_t kMostStride = MLUOP_EXT_GATED_SCAN_MOST_STRIDE;
-static_assert((uint64_t)(kTileRows + 1) * kMostStride * sizeof(float) < (uint64_t)1 << 32, "32-bit offsets");
+// (a tile's rows of fp32 that far apart: offsets stay within 32 bits; longer tiles are for rows less far apart)
+constexpr int64_t kMostStride = MLUOP_EXT_GATED_SCAN_MOST_STRIDE, kNarrowStride = kMostStride * kLeastTile / kMostTile;
+static_assert((uint64_t)(kLeastTile + 1) * kMostStride * sizeof(float) < (uint64_t)1 << 32, "32-bit offsets");
+static_assert((uint64_t)(kMostTile + 1) * kNarrowStride * sizeof(float) < (uint64_t)1 << 32, "32-bit offsets");
 
 // a and u of a gate: a row's step is h -> a h + u x.  Half of what these kernels compute is here.  What has to be exact is an a
 // close to one, whose error all steps of a long memory repeat: it is what a small u leaves of one.  An exponential beyond the
@@ -164,7 +177,7 @@ struct Rows {
   template <int TEAM_ROWS, typename WORK>
   __device__ __forceinline__ void load(const T *from, int64_t stride, const WORK &w, int first, float none) {
     const Lines<T, TEAM_ROWS> lines(from, stride, w, first);
-    if (first + (kTeams - 1) * TEAM_ROWS + R <= w.rows) {
+    if (first + (WORK::kTeams - 1) * TEAM_ROWS + R <= w.rows) {
 #pragma unroll
       for (int r = 0; r < R; ++r) at[r] = *reinterpret_cast<const W *>(lines.row(r));
       return;
@@ -213,10 +226,33 @@ __device__ __forceinline__ void halves(float v, float *low, float *high) {
   *high = __uint_as_float(r[1]);
 }
 
-// The four teams' maps (a, b) composed, the first team's first, or with FROM_LAST the last's.  `a` and `b` become the composition
-// of the teams in front of this one; all_a, all_b that of all four.  By whole waves.
-template <bool FROM_LAST>
+// What the lane 4 or 8 away has, inside of a row of 16.
+template <int AWAY>
+__device__ __forceinline__ float exchanged(float v) {
+  static_assert(AWAY == 4 || AWAY == 8, "");
+  if constexpr (AWAY == 8) return lanesMoved<0x128>(v);  // turned by eight
+  return lanesMoved<0x1B>(lanesMoved<0x141>(v));         // eight mirrored, then every four
+}
+
+// The teams' maps (a, b) composed, the first team's first, or with FROM_LAST the last's.  `a` and `b` become the composition
+// of the teams in front of this one; all_a, all_b that of all.  By whole waves.
+template <int ACROSS, bool FROM_LAST>
 __device__ __forceinline__ void composeTeams(int team, float &a, float &b, float *all_a, float *all_b) {
+  // teams inside of a row of 16 lanes: what is in front of this one (pa, pb) there, and all of the row's in a and b
+  float pa = 1.f, pb = 0.f;
+  auto pairs = [&](auto away) {
+    constexpr int AWAY = decltype(away)::value;
+    const bool second = ((team & (AWAY / ACROSS)) != 0) != FROM_LAST;
+    const float oa = exchanged<AWAY>(a), ob = exchanged<AWAY>(b);
+    // (in front of what is in front so far: the other's)
+    pb = second ? fmaf(pa, ob, pb) : pb;
+    pa = second ? pa * oa : pa;
+    b = second ? fmaf(a, ob, b) : fmaf(oa, b, ob);
+    a *= oa;
+  };
+  if constexpr (ACROSS <= 4) pairs(std::integral_constant<int, 4>());
+  if constexpr (ACROSS <= 8) pairs(std::integral_constant<int, 8>());
+  // rows of 16 lanes
   float a_even, a_odd, b_even, b_odd;
   rowsOfPairs(a, &a_even, &a_odd);
   rowsOfPairs(b, &b_even, &b_odd);
@@ -230,25 +266,31 @@ __device__ __forceinline__ void composeTeams(int team, float &a, float &b, float
   const float pa2 = FROM_LAST ? pa_low : pa_high, pb2 = FROM_LAST ? pb_low : pb_high;
   *all_a = pa1 * pa2;
   *all_b = fmaf(pa2, pb1, pb2);
-  const bool second = ((team & 1) != 0) != FROM_LAST, behind = (team >= 2) != FROM_LAST;
+  const int row = team / (16 / ACROSS);
+  const bool second = ((row & 1) != 0) != FROM_LAST, behind = (row >= 2) != FROM_LAST;
+  // (selected, not multiplied with zero: `a` may be infinite)
   a = second ? a1 : 1.f;
   b = second ? b1 : 0.f;
-  // (selected, not multiplied with zero: `a` may be infinite)
   b = behind ? fmaf(a, pb1, b) : b;
   a = behind ? a * pa1 : a;
+  if constexpr (ACROSS < 16) {
+    b = fmaf(pa, b, pb);
+    a *= pa;
+  }
 }
 
 // ---- forward -------------------------------------------------------------------------------
 
 // What a tile does to the state that comes into it, to tiles[slot][channel].  GRAD: to the gradient that comes into it from
 // behind.  A team has 16 rows of a tile here, and the teams are composed once.
-template <typename T, int V, int KIND, bool GRAD>
+template <typename T, int V, int ACROSS, int KIND, bool GRAD>
 __global__ __launch_bounds__(kThreads) void gatedScanTiles(const T *__restrict__ x, const T *__restrict__ g, Shape s,
                                                            int64_t first_block, float2 *__restrict__ tiles) {
-  const Work<V, false> w(s, first_block + blockIdx.y, 0, false);
+  typedef Work<V, ACROSS, false> Waves;
+  const Waves w(s, first_block + blockIdx.y, 0, false);
   if (w.sample < 0) return;
   const int64_t x_stride = GRAD ? s.dh_stride : s.x_stride;
-  constexpr int kPieces = kTileRows / kTeams / kPiece;
+  constexpr int kTeamRows = Waves::kTileRows / Waves::kTeams, kPieces = kTeamRows / kPiece;
   float a[V], b[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -260,8 +302,8 @@ __global__ __launch_bounds__(kThreads) void gatedScanTiles(const T *__restrict__
   } one, other;
   auto load = [&](Piece &p, int k) {
     const int first = (GRAD ? kPieces - 1 - k : k) * kPiece;
-    p.g.template load<kTileRows / kTeams>(g, s.g_stride, w, first, idle<KIND>());
-    p.x.template load<kTileRows / kTeams>(x, x_stride, w, first, 0.f);
+    p.g.template load<kTeamRows>(g, s.g_stride, w, first, idle<KIND>());
+    p.x.template load<kTeamRows>(x, x_stride, w, first, 0.f);
   };
   auto compose = [&](const Piece &p) {
 #pragma unroll
@@ -290,17 +332,20 @@ __global__ __launch_bounds__(kThreads) void gatedScanTiles(const T *__restrict__
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     float all_a, all_b;
-    composeTeams<GRAD>(w.team, a[i], b[i], &all_a, &all_b);
+    composeTeams<ACROSS, GRAD>(w.team, a[i], b[i], &all_a, &all_b);
     if (w.there && w.team == 0) tiles[w.tile_slot * s.channels + w.channel + i] = make_float2(all_a, all_b);
   }
 }
 
-// The state in front of every tile (from that of its sample, zero where there is none), to states[slot][channel], and behind the
-// last.  FROM_LAST: tiles from a sample's last to its first.  kJoinChannels channels of a sample a workgroup; its tiles are cut
-// into runs of kJoinRun, one for each of the threads that share a channel, and are read once: kJoinTiles at a time.
+// The state in front of every tile of TILE rows (from that of its sample, zero where there is none), to states[slot][channel],
+// and behind the last.  FROM_LAST: tiles from a sample's last to its first.  kJoinChannels channels of a sample a workgroup; its
+// tiles are cut into runs of kJoinRun, one for each of the threads that share a channel, and are read once: kJoinTiles at a
+// time.  (One sample of 7325 tiles of 64 channels 25 us, 3 for each turn.  The next turn's tiles on their way meanwhile: no
+// less.  Four channels a workgroup, and turns twice as long: 22, but four samples of some 970 tiles of 128 channels 10 in place
+// of 9.)
 constexpr int kJoinThreads = 512, kJoinChannels = 8, kJoinRun = 16;
 constexpr int kJoinTiles = kJoinThreads / kJoinChannels * kJoinRun;
-template <bool FROM_LAST>
+template <int TILE, bool FROM_LAST>
 __global__ __launch_bounds__(kJoinThreads) void gatedScanJoin(const float2 *__restrict__ tiles, Shape s, int first_sample,
                                                               const float *__restrict__ initial,
                                                               float *__restrict__ states, float *__restrict__ final) {
@@ -309,11 +354,11 @@ __global__ __launch_bounds__(kJoinThreads) void gatedScanJoin(const float2 *__re
   const int sample = first_sample + (int)blockIdx.y;
   int first, rows;
   segmentRows(s.starts, s.rows, sample, &first, &rows);
-  const int count = (rows + kTileRows - 1) / kTileRows;
+  const int count = (rows + TILE - 1) / TILE;
   const int lane = threadIdx.x % kJoinChannels, run = threadIdx.x / kJoinChannels, wave = threadIdx.x / 64;
   const int channel = (int)blockIdx.x * kJoinChannels + lane;
   const bool there = channel < s.channels;
-  const int64_t slot = firstSlot<kTileRows>(sample, first);
+  const int64_t slot = firstSlot<TILE>(sample, first);
   auto at = [&](int tile) { return (slot + (FROM_LAST ? count - 1 - tile : tile)) * s.channels + (there ? channel : 0); };
   float h0 = initial == nullptr || !there ? 0.f : initial[(int64_t)sample * s.channels + channel];
   for (int t0 = 0; t0 < count; t0 += kJoinTiles) {
@@ -367,16 +412,16 @@ __global__ __launch_bounds__(kJoinThreads) void gatedScanJoin(const float2 *__re
 
 // The state that comes into a wave's rows: from the one in front of its tile (JOINED), or of its sample through the tiles in
 // front.  FROM_LAST: the gradient that comes in from behind.  `states` are those of the tiles or the samples (null: zero).
-template <int V, Joining JOINING, bool FROM_LAST, typename WORK>
+template <int V, int ACROSS, Joining JOINING, bool FROM_LAST, typename WORK>
 __device__ __forceinline__ void incoming(const WORK &w, const Shape &s, const float *states, const float2 *tiles,
                                          float (&h)[V]) {
   const int64_t from = (JOINING == kJoined ? w.tile_slot : (int64_t)w.sample) * s.channels + w.channel;
 #pragma unroll
   for (int i = 0; i < V; ++i) h[i] = states == nullptr ? 0.f : states[from + i];
   if (JOINING != kFolded) return;
-  // a quarter of the tiles by each team
+  // as many of the tiles by each team
   const int count = FROM_LAST ? w.tiles - 1 - w.in_sample : w.in_sample;
-  const int per = (count + kTeams - 1) / kTeams, lo = min(w.team * per, count), hi = min(lo + per, count);
+  const int per = (count + WORK::kTeams - 1) / WORK::kTeams, lo = min(w.team * per, count), hi = min(lo + per, count);
   const int64_t slot = w.tile_slot - w.in_sample;
   float a[V], b[V];
 #pragma unroll
@@ -407,7 +452,7 @@ __device__ __forceinline__ void incoming(const WORK &w, const Shape &s, const fl
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     float all_a, all_b;
-    composeTeams<false>(w.team, a[i], b[i], &all_a, &all_b);
+    composeTeams<ACROSS, false>(w.team, a[i], b[i], &all_a, &all_b);
     h[i] = fmaf(all_a, h[i], all_b);
   }
 }
@@ -441,21 +486,23 @@ __device__ void outside(const Shape &s, int block, const float *initial, float *
   }
 }
 
-// The states of a tile's rows, step by step, and the states in front of every step to step_states.  But with JOINED it writes
+// The states of a tile's rows, step by step, and the state in front of every kStateRows rows to kept.  But with JOINED it writes
 // `final` too.
-template <typename T, int V, int KIND, Joining JOINING>
+template <typename T, int V, int ACROSS, int KIND, Joining JOINING>
 __global__ __launch_bounds__(kThreads, 5) void gatedScanApply(const T *__restrict__ x, const T *__restrict__ g, Shape s,
                                                            int64_t first_block, int64_t blocks,
                                                            const float *__restrict__ states,
                                                            const float2 *__restrict__ tiles,
-                                                           float *__restrict__ step_states, float *__restrict__ final,
+                                                           float *__restrict__ kept, float *__restrict__ final,
                                                            T *__restrict__ out) {
   const int64_t block = first_block + blockIdx.y;
   if (block >= blocks) {
     outside<T, V>(s, (int)(block - blocks), states, JOINING == kJoined ? nullptr : final, out, static_cast<T *>(nullptr));
     return;
   }
-  const Work<V, JOINING == kWhole> w(s, block, blocks, JOINING != kWhole);
+  typedef Work<V, ACROSS, JOINING == kWhole> Waves;
+  constexpr int kStepRows = Waves::kStepRows, kStates = kStepRows / kStateRows;
+  const Waves w(s, block, blocks, JOINING != kWhole);
   if (w.sample < 0 || w.rows == 0) return;
   float h0[V];
   const int steps = w.steps();
@@ -465,7 +512,7 @@ __global__ __launch_bounds__(kThreads, 5) void gatedScanApply(const T *__restric
     xs.template load<kRows>(x, s.x_stride, w, k * kStepRows, 0.f);
   };
   load(0);
-  incoming<V, JOINING, false>(w, s, states, tiles, h0);
+  incoming<V, ACROSS, JOINING, false>(w, s, states, tiles, h0);
   for (int k = 0; k < steps; ++k) {
     float ra[kRows][V], rb[kRows][V], a[V], b[V];
 #pragma unroll
@@ -484,19 +531,23 @@ __global__ __launch_bounds__(kThreads, 5) void gatedScanApply(const T *__restric
         a[i] *= ra[r][i];
       }
     if (k + 1 < steps) load(k + 1);
-    if (w.there && w.team == 0)
+    if (kStates == 1 && w.there && w.team == 0)
 #pragma unroll
-      for (int i = 0; i < V; ++i) step_states[(w.step_slot + k) * s.channels + w.channel + i] = h0[i];
+      for (int i = 0; i < V; ++i) kept[(w.state_slot + k) * s.channels + w.channel + i] = h0[i];
     float h[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float all_a, all_b;
-      composeTeams<false>(w.team, a[i], b[i], &all_a, &all_b);
+      composeTeams<ACROSS, false>(w.team, a[i], b[i], &all_a, &all_b);
       h[i] = fmaf(a[i], h0[i], b[i]);
       h0[i] = fmaf(all_a, h0[i], all_b);
     }
     const Lines<T, kRows> lines(out, s.channels, w, k * kStepRows);
     const int mine = w.there ? w.rows - k * kStepRows - w.team * kRows : 0;
+    if (kStates > 1 && mine > 0 && w.team * kRows % kStateRows == 0)
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        kept[(w.state_slot + k * kStates + w.team * kRows / kStateRows) * s.channels + w.channel + i] = h[i];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
 #pragma unroll
@@ -514,10 +565,10 @@ __global__ __launch_bounds__(kThreads, 5) void gatedScanApply(const T *__restric
 
 // The gradients of a tile's rows, from the last step to the first: a step's states again from the one in front of it, and the
 // gradient that comes in from behind.  But with JOINED it writes the initial states' too.
-template <typename T, int V, int KIND, Joining JOINING>
+template <typename T, int V, int ACROSS, int KIND, Joining JOINING>
 __global__ __launch_bounds__(kThreads, 4) void gatedScanGrad(const T *__restrict__ dh, const T *__restrict__ x,
                                                           const T *__restrict__ g, Shape s, int64_t first_block,
-                                                          int64_t blocks, const float *__restrict__ step_states,
+                                                          int64_t blocks, const float *__restrict__ kept,
                                                           const float *__restrict__ grads, const float2 *__restrict__ tiles,
                                                           float *__restrict__ initial_grad, T *__restrict__ dx,
                                                           T *__restrict__ dg) {
@@ -526,10 +577,12 @@ __global__ __launch_bounds__(kThreads, 4) void gatedScanGrad(const T *__restrict
     outside<T, V>(s, (int)(block - blocks), grads, JOINING == kJoined ? nullptr : initial_grad, dx, dg);
     return;
   }
-  const Work<V, JOINING == kWhole> w(s, block, blocks, JOINING != kWhole);
+  typedef Work<V, ACROSS, JOINING == kWhole> Waves;
+  constexpr int kStepRows = Waves::kStepRows, kStates = kStepRows / kStateRows;
+  const Waves w(s, block, blocks, JOINING != kWhole);
   if (w.sample < 0 || w.rows == 0) return;
   float l0[V];
-  incoming<V, JOINING, true>(w, s, grads, tiles, l0);
+  incoming<V, ACROSS, JOINING, true>(w, s, grads, tiles, l0);
   for (int k = w.steps() - 1; k >= 0; --k) {
     Rows<T, V, kRows> xs, gs, ds;
     gs.template load<kRows>(g, s.g_stride, w, k * kStepRows, idle<KIND>());
@@ -537,7 +590,7 @@ __global__ __launch_bounds__(kThreads, 4) void gatedScanGrad(const T *__restrict
     ds.template load<kRows>(dh, s.dh_stride, w, k * kStepRows, 0.f);
     float h[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) h[i] = w.there ? step_states[(w.step_slot + k) * s.channels + w.channel + i] : 0.f;
+    for (int i = 0; i < V; ++i) h[i] = w.there ? kept[(w.state_slot + k * kStates) * s.channels + w.channel + i] : 0.f;
     float ra[kRows][V], ru[kRows][V], a[V], b[V], c[V], l[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -557,9 +610,9 @@ __global__ __launch_bounds__(kThreads, 4) void gatedScanGrad(const T *__restrict
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float all_a, all_b, behind = a[i];
-      composeTeams<false>(w.team, a[i], b[i], &all_a, &all_b);
+      composeTeams<ACROSS, false>(w.team, a[i], b[i], &all_a, &all_b);
       h[i] = fmaf(a[i], h[i], b[i]);
-      composeTeams<true>(w.team, behind, c[i], &all_a, &all_b);
+      composeTeams<ACROSS, true>(w.team, behind, c[i], &all_a, &all_b);
       l[i] = fmaf(behind, l0[i], c[i]);
       l0[i] = fmaf(all_a, l0[i], all_b);
     }
@@ -623,6 +676,17 @@ void byType(mluOpDataType_t type, int64_t channels, int64_t strides, uintptr_t a
   }
 }
 
+// Calls f(ACROSS): the lanes that hold a row, at least 4 and at most 16.
+template <typename F>
+void byAcross(int64_t vectors, int64_t most_stride, F f) {
+  if (vectors > 8 || most_stride > kNarrowStride)
+    f(std::integral_constant<int, 16>());
+  else if (vectors > 4)
+    f(std::integral_constant<int, 8>());
+  else
+    f(std::integral_constant<int, 4>());
+}
+
 template <typename F>
 void byKind(mluOpExtGate_t kind, F f) {
   if (kind == MLUOP_EXT_GATE_SIGMOID)
@@ -647,23 +711,24 @@ bool strideFits(int64_t channels, int64_t stride) { return stride >= channels &&
 
 // Maps of the tiles and states in front of them.  (The caller's memory need not be aligned.)
 size_t workspaceBytes(int64_t rows, int64_t channels, int64_t samples) {
-  return 16 + (size_t)mostSlots<kTileRows>(rows, samples) * channels * (sizeof(float2) + sizeof(float));
+  return 16 + (size_t)mostSlots<kLeastTile>(rows, samples) * channels * (sizeof(float2) + sizeof(float));
 }
 struct Workspace {
   float2 *tiles;
   float *states;
   Workspace(void *workspace, int64_t rows, int64_t channels, int64_t samples) {
     tiles = reinterpret_cast<float2 *>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~(uintptr_t)15);
-    states = reinterpret_cast<float *>(tiles + mostSlots<kTileRows>(rows, samples) * channels);
+    states = reinterpret_cast<float *>(tiles + mostSlots<kLeastTile>(rows, samples) * channels);
   }
 };
 
 // A wave for a whole sample, and one launch in place of two or three: where there are few rows, or about one a sample, as in a
 // step of many sequences.  (At worst one sample has them all, in 256 steps of a microsecond.)  Every wave folds the tiles in
 // front of its own where these are few, at most 16 for a team.
+constexpr int64_t kFoldedRows = 4096;
 Joining joiningOf(int64_t rows, int64_t samples) {
-  if (rows <= std::max<int64_t>(512, std::min<int64_t>(2 * samples, 4096))) return kWhole;
-  return rows <= 64 * kTileRows ? kFolded : kJoined;
+  if (rows <= std::max<int64_t>(512, std::min<int64_t>(2 * samples, kFoldedRows))) return kWhole;
+  return rows <= kFoldedRows ? kFolded : kJoined;
 }
 template <typename F>
 void byJoining(Joining joining, F f) {
@@ -675,6 +740,21 @@ void byJoining(Joining joining, F f) {
     f(std::integral_constant<Joining, kJoined>());
 }
 
+// Slabs of CHANNELS channels along x, as many of a workgroup's waves as can be with slabs side by side; tiles, or samples, along
+// y.
+struct Grid {
+  unsigned slabs;
+  int64_t blocks;
+};
+template <int CHANNELS>
+Grid gridOf(Shape *s, Joining joining, int tile) {
+  const int64_t all = (s->channels + CHANNELS - 1) / CHANNELS;
+  s->side_by_side = all >= 3 ? 4 : (int)all;
+  s->most_tiles = (int)mostRaggedTiles(s->rows, s->samples, tile);
+  const int64_t in_block = kWaves / s->side_by_side, items = joining == kWhole ? s->samples : s->most_tiles;
+  return {(unsigned)((all + s->side_by_side - 1) / s->side_by_side), (items + in_block - 1) / in_block};
+}
+
 // Workgroups along y in as many launches as they need.
 constexpr int64_t kMostAlongY = 65535;
 template <typename F>
@@ -682,11 +762,11 @@ void alongY(int64_t blocks, F f) {
   for (int64_t first = 0; first < blocks; first += kMostAlongY) f(first, (unsigned)std::min(blocks - first, kMostAlongY));
 }
 
-template <bool FROM_LAST>
+template <int TILE, bool FROM_LAST>
 void join(const mluop::LaunchCtx &lc, const float2 *tiles, const Shape &s, const float *initial, float *states, float *final) {
   for (int64_t first = 0; first < s.samples; first += kMostAlongY) {
     lc.begin("gatedScanJoin");
-    gatedScanJoin<FROM_LAST><<<dim3((unsigned)((s.channels + kJoinChannels - 1) / kJoinChannels),
+    gatedScanJoin<TILE, FROM_LAST><<<dim3((unsigned)((s.channels + kJoinChannels - 1) / kJoinChannels),
                                     (unsigned)std::min<int64_t>(s.samples - first, kMostAlongY)),
                                kJoinThreads, 0, lc.stream>>>(tiles, s, (int)first, initial, states, final);
     lc.end();
@@ -702,7 +782,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGetGatedScanSizes(int64_t rows, int64_t chan
   PARAM_CHECK(api, workspace_size != NULL);
   const mluOpStatus_t status = checkShape(api, rows, channels, samples);
   if (status != MLUOP_STATUS_SUCCESS) return status;
-  *carries = (size_t)mostSlots<kStepRows>(rows, samples);
+  *carries = (size_t)mostSlots<kStateRows>(rows, samples);
   *workspace_size = workspaceBytes(rows, channels, samples);
   return MLUOP_STATUS_SUCCESS;
 }
@@ -728,45 +808,45 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanForward(mluOpHandle_t handle, mluOp
   DEVICE_HANDLE_CHECK(api, handle);
   HIP_CHECK_RETURN(api, hipSetDevice(handle->device));
   const size_t bytes = (size_t)rows * channels * elementBytes(type);
-  const int64_t most = mostRaggedTiles(rows, samples, kTileRows);
   const Joining joining = joiningOf(rows, samples);
   if (handle->hasNotes()) {
     handle->forgetNotesIn(out, bytes);
     handle->forgetNotesIn(final, (size_t)samples * channels * sizeof(float));
-    handle->forgetNotesIn(carries, (size_t)mostSlots<kStepRows>(rows, samples) * channels * sizeof(float));
+    handle->forgetNotesIn(carries, (size_t)mostSlots<kStateRows>(rows, samples) * channels * sizeof(float));
     handle->forgetNotesIn(workspace, workspace_size);
   }
-  Shape s = {(int)rows,  (int)channels, (int)samples, features_stride, gates_stride, 0, (int)most, 1,
+  Shape s = {(int)rows,  (int)channels, (int)samples, features_stride, gates_stride, 0, 0, 1,
              row_starts, reverse != 0,  bytes >= kStreamedBytes};
   const Workspace w(workspace, rows, channels, samples);
   const mluop::LaunchCtx lc = handle->launchCtx();
   const uintptr_t addresses = reinterpret_cast<uintptr_t>(features) | reinterpret_cast<uintptr_t>(gates) |
                               reinterpret_cast<uintptr_t>(out);
   byType(type, channels, features_stride | gates_stride, addresses, [&](auto zero, auto v) {
-    byKind(kind, [&](auto of_kind) {
-      typedef decltype(zero) T;
-      constexpr int V = decltype(v)::value, KIND = decltype(of_kind)::value;
-      const T *x = static_cast<const T *>(features), *g = static_cast<const T *>(gates);
-      const int64_t all = (channels + kAcross * V - 1) / (kAcross * V);
-      s.side_by_side = all >= 3 ? 4 : (int)all;
-      const unsigned slabs = (unsigned)((all + s.side_by_side - 1) / s.side_by_side);
-      const int64_t in_block = kWaves / s.side_by_side, blocks = ((joining == kWhole ? samples : most) + in_block - 1) / in_block;
-      if (joining != kWhole) {
-        alongY(blocks, [&](int64_t first, unsigned count) {
-          lc.begin("gatedScanTiles");
-          gatedScanTiles<T, V, KIND, false><<<dim3(slabs, count), kThreads, 0, lc.stream>>>(x, g, s, first, w.tiles);
-          lc.end();
-        });
-      }
-      if (joining == kJoined) join<false>(lc, w.tiles, s, initial, w.states, final);
-      byJoining(joining, [&](auto how) {
-        constexpr Joining JOINING = decltype(how)::value;
-        alongY(blocks + kOutsideBlocks, [&](int64_t first, unsigned count) {
-          lc.begin("gatedScanApply");
-          gatedScanApply<T, V, KIND, JOINING><<<dim3(slabs, count), kThreads, 0, lc.stream>>>(
-              x, g, s, first, blocks, JOINING == kJoined ? w.states : initial, w.tiles, carries, final,
-              static_cast<T *>(out));
-          lc.end();
+    typedef decltype(zero) T;
+    constexpr int V = decltype(v)::value;
+    const T *x = static_cast<const T *>(features), *g = static_cast<const T *>(gates);
+    byAcross(channels / V, std::max(features_stride, gates_stride), [&](auto across) {
+      byKind(kind, [&](auto of_kind) {
+        constexpr int ACROSS = decltype(across)::value, KIND = decltype(of_kind)::value, TILE = Layout<ACROSS>::kTileRows;
+        const Grid grid = gridOf<ACROSS * V>(&s, joining, TILE);
+        if (joining != kWhole) {
+          alongY(grid.blocks, [&](int64_t first, unsigned count) {
+            lc.begin("gatedScanTiles");
+            gatedScanTiles<T, V, ACROSS, KIND, false><<<dim3(grid.slabs, count), kThreads, 0, lc.stream>>>(x, g, s, first,
+                                                                                                        w.tiles);
+            lc.end();
+          });
+        }
+        if (joining == kJoined) join<TILE, false>(lc, w.tiles, s, initial, w.states, final);
+        byJoining(joining, [&](auto how) {
+          constexpr Joining JOINING = decltype(how)::value;
+          alongY(grid.blocks + kOutsideBlocks, [&](int64_t first, unsigned count) {
+            lc.begin("gatedScanApply");
+            gatedScanApply<T, V, ACROSS, KIND, JOINING><<<dim3(grid.slabs, count), kThreads, 0, lc.stream>>>(
+                x, g, s, first, grid.blocks, JOINING == kJoined ? w.states : initial, w.tiles, carries, final,
+                static_cast<T *>(out));
+            lc.end();
+          });
         });
       });
     });
@@ -799,7 +879,6 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanBackward(mluOpHandle_t handle, mluO
   DEVICE_HANDLE_CHECK(api, handle);
   HIP_CHECK_RETURN(api, hipSetDevice(handle->device));
   const size_t bytes = (size_t)rows * channels * elementBytes(type);
-  const int64_t most = mostRaggedTiles(rows, samples, kTileRows);
   const Joining joining = joiningOf(rows, samples);
   if (handle->hasNotes()) {
     handle->forgetNotesIn(features_grad, bytes);
@@ -807,7 +886,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanBackward(mluOpHandle_t handle, mluO
     if (initial_grad) handle->forgetNotesIn(initial_grad, (size_t)samples * channels * sizeof(float));
     handle->forgetNotesIn(workspace, workspace_size);
   }
-  Shape s = {(int)rows,  (int)channels, (int)samples, features_stride, gates_stride, output_grad_stride, (int)most, 1,
+  Shape s = {(int)rows,  (int)channels, (int)samples, features_stride, gates_stride, output_grad_stride, 0, 1,
              row_starts, reverse != 0,  bytes >= kStreamedBytes};
   const Workspace w(workspace, rows, channels, samples);
   const mluop::LaunchCtx lc = handle->launchCtx();
@@ -815,31 +894,32 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanBackward(mluOpHandle_t handle, mluO
                               reinterpret_cast<uintptr_t>(output_grad) | reinterpret_cast<uintptr_t>(features_grad) |
                               reinterpret_cast<uintptr_t>(gates_grad);
   byType(type, channels, features_stride | gates_stride | output_grad_stride, addresses, [&](auto zero, auto v) {
-    byKind(kind, [&](auto of_kind) {
-      typedef decltype(zero) T;
-      constexpr int V = decltype(v)::value, KIND = decltype(of_kind)::value;
-      const T *dh = static_cast<const T *>(output_grad), *x = static_cast<const T *>(features);
-      const T *g = static_cast<const T *>(gates);
-      const int64_t all = (channels + kAcross * V - 1) / (kAcross * V);
-      s.side_by_side = all >= 3 ? 4 : (int)all;
-      const unsigned slabs = (unsigned)((all + s.side_by_side - 1) / s.side_by_side);
-      const int64_t in_block = kWaves / s.side_by_side, blocks = ((joining == kWhole ? samples : most) + in_block - 1) / in_block;
-      if (joining != kWhole) {
-        alongY(blocks, [&](int64_t first, unsigned count) {
-          lc.begin("gatedScanTiles");
-          gatedScanTiles<T, V, KIND, true><<<dim3(slabs, count), kThreads, 0, lc.stream>>>(dh, g, s, first, w.tiles);
-          lc.end();
-        });
-      }
-      if (joining == kJoined) join<true>(lc, w.tiles, s, final_grad, w.states, initial_grad);
-      byJoining(joining, [&](auto how) {
-        constexpr Joining JOINING = decltype(how)::value;
-        alongY(blocks + kOutsideBlocks, [&](int64_t first, unsigned count) {
-          lc.begin("gatedScanGrad");
-          gatedScanGrad<T, V, KIND, JOINING><<<dim3(slabs, count), kThreads, 0, lc.stream>>>(
-              dh, x, g, s, first, blocks, carries, JOINING == kJoined ? w.states : final_grad, w.tiles, initial_grad,
-              static_cast<T *>(features_grad), static_cast<T *>(gates_grad));
-          lc.end();
+    typedef decltype(zero) T;
+    constexpr int V = decltype(v)::value;
+    const T *dh = static_cast<const T *>(output_grad), *x = static_cast<const T *>(features);
+    const T *g = static_cast<const T *>(gates);
+    byAcross(channels / V, std::max({features_stride, gates_stride, output_grad_stride}), [&](auto across) {
+      byKind(kind, [&](auto of_kind) {
+        constexpr int ACROSS = decltype(across)::value, KIND = decltype(of_kind)::value, TILE = Layout<ACROSS>::kTileRows;
+        const Grid grid = gridOf<ACROSS * V>(&s, joining, TILE);
+        if (joining != kWhole) {
+          alongY(grid.blocks, [&](int64_t first, unsigned count) {
+            lc.begin("gatedScanTiles");
+            gatedScanTiles<T, V, ACROSS, KIND, true><<<dim3(grid.slabs, count), kThreads, 0, lc.stream>>>(dh, g, s, first,
+                                                                                                       w.tiles);
+            lc.end();
+          });
+        }
+        if (joining == kJoined) join<TILE, true>(lc, w.tiles, s, final_grad, w.states, initial_grad);
+        byJoining(joining, [&](auto how) {
+          constexpr Joining JOINING = decltype(how)::value;
+          alongY(grid.blocks + kOutsideBlocks, [&](int64_t first, unsigned count) {
+            lc.begin("gatedScanGrad");
+            gatedScanGrad<T, V, ACROSS, KIND, JOINING><<<dim3(grid.slabs, count), kThreads, 0, lc.stream>>>(
+                dh, x, g, s, first, grid.blocks, carries, JOINING == kJoined ? w.states : final_grad, w.tiles, initial_grad,
+                static_cast<T *>(features_grad), static_cast<T *>(gates_grad));
+            lc.end();
+          });
         });
       });
     });

@@ -58,3 +58,41 @@ def test_rows_by_expert(gpu_handle, dtype, channels, choices):
     near(dr, want, want.abs(), 1, dtype)
     terms = dy.double().unsqueeze(1) * taken(y, places)
     near(dw, terms.sum(dim=2), terms.abs().sum(dim=2), channels + 8, "float32")
+
+
+RAGGED = [3, 3, 4100, 4101, 8900]
+
+
+@pytest.mark.parametrize("dtype,kind,reverse", [("float32", "sigmoid", False), ("bfloat16", "exp", True),
+                                                ("bfloat16", "sigmoid", True), ("float16", "exp", False)])
+@pytest.mark.parametrize("rows,starts", [(100, None), (3000, None), (9001, None), (9001, RAGGED), (70, list(range(71)))])
+@pytest.mark.parametrize("channels", [1, 3, 8, 12, 16, 20, 32])
+def test_recurrence(gpu_handle, dtype, kind, reverse, rows, starts, channels):
+    """as whole samples, with tiles that every wave folds, and joined; 4, 8 or 16 lanes across"""
+    import torch
+    from test_gpu_gated_scan import check, inputs
+    samples = 1 if starts is None else len(starts) - 1
+    x, g, h0, dh, df = inputs(rows, channels, samples, getattr(torch, dtype), kind, rows + channels)
+    check(gpu_handle, x, g, starts, h0, dh, df, kind, reverse, dtype)
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("rows", [200, 9000])
+def test_recurrence_whose_gradients_lie_otherwise(gpu_handle, rows, reverse):
+    """a gradient whose rows lie apart at odd places is taken by more lanes than the forward pass's rows were"""
+    import torch
+    import mluop_hip
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x, gates = (torch.randn(rows, 16, device="cuda", generator=g).bfloat16() for _ in range(2))
+    wide = torch.randn(rows, 19, device="cuda", generator=g).bfloat16()
+    starts = torch.tensor([0, 5, rows - 3], dtype=torch.int32, device="cuda")
+    out, final, carries = mluop_hip.gated_scan_forward(gpu_handle, x, gates, starts, reverse=reverse)
+    near = mluop_hip.gated_scan_backward(gpu_handle, wide[:, 1:17].contiguous(), None, x, gates, carries, starts, reverse=reverse)
+    apart = mluop_hip.gated_scan_backward(gpu_handle, wide[:, 1:17], None, x, gates, carries, starts, reverse=reverse)
+    for a, b in zip(near, apart):
+        # (the same but for the order of compositions: a rounding to bfloat16 of each, and fp32 sums of values below 2^5)
+        assert torch.allclose(a.float(), b.float(), rtol=2.0 ** -7, atol=2.0 ** -14)
+    again = mluop_hip.gated_scan_forward(gpu_handle, wide[:, :16], gates, starts, reverse=reverse)
+    same = mluop_hip.gated_scan_forward(gpu_handle, wide[:, :16].contiguous(), gates, starts, reverse=reverse)
+    for a, b in zip(again[:2], same[:2]):   # (of the carries some rows belong to no sample)
+        assert torch.allclose(a.float(), b.float(), rtol=2.0 ** -7, atol=2.0 ** -14)
