@@ -255,3 +255,45 @@ def test_several_streams_of_one_thread():
                 assert all(torch.equal(a, b) for a, b in zip(got, want))
     finally:
         mluop_hip.GUARD_BYTES = guard
+
+
+@pytest.mark.parametrize("share", [0.03, 0.6, 1.0])
+def test_very_many_choices_of_no_expert(gpu_handle, share):
+    """their places are zero, in the order and in the gradients of a weighted sum"""
+    import torch
+    import mluop_hip
+    rows, choices, channels = 30_001, 3, 72
+    g = torch.Generator(device="cuda").manual_seed(int(100 * share))
+    chosen = torch.randint(0, 9, (rows, choices), device="cuda", generator=g)
+    chosen[torch.rand((rows, choices), device="cuda", generator=g) < share] = -1
+    x = torch.randn(rows, channels, device="cuda", generator=g).half()
+    ordered, starts, places = mluop_hip.expert_order(gpu_handle, chosen, 9)
+    sent = int(starts[-1])
+    assert sent == int((chosen >= 0).sum())
+    to = mluop_hip.expert_dispatch(gpu_handle, x, places, starts)
+    assert torch.equal(to[:sent], x[ordered[:sent].long()]) and not bool(to[sent:].any())
+    w = torch.rand(rows, choices, device="cuda", generator=g)
+    dy, dw = mluop_hip.expert_combine_backward(gpu_handle, x, to, places, w, starts)
+    assert not bool(dy[sent:].any()) and bool((dw[chosen < 0] == 0).all())
+    there = places >= 0
+    want = (x.float().unsqueeze(1) * w.unsqueeze(2))[there].half()
+    assert torch.equal(dy[places[there].long()], want)
+
+
+@pytest.mark.parametrize("starts", [[0, 1000, 100_000], [200_000, 200_000, 299_000], [7, 7]])
+def test_very_many_rows_of_no_sample(gpu_handle, starts):
+    """rows in front of the first sample and behind the last are zero in every result, whatever they hold"""
+    import torch
+    import mluop_hip
+    rows, channels = 300_001, 48
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x, gates, dh = (torch.randn(rows, channels, device="cuda", generator=g).bfloat16() for _ in range(3))
+    for t in (x, gates, dh):
+        t[:starts[0]] = float("nan")
+        t[starts[-1]:] = float("nan")
+    where = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    out, final, carries = mluop_hip.gated_scan_forward(gpu_handle, x, gates, where)
+    dx, dg, _ = mluop_hip.gated_scan_backward(gpu_handle, dh, None, x, gates, carries, where)
+    for t in (out, dx, dg):
+        assert not bool(t[:starts[0]].any()) and not bool(t[starts[-1]:].any()) and not bool(t.isnan().any())
+    assert not bool(final.isnan().any())
