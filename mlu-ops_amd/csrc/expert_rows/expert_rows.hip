@@ -192,8 +192,8 @@ __device__ __forceinline__ int64_t inRuns(int64_t block, int64_t blocks) {
 inline bool wholeLines(int64_t channels, mluOpDataType_t type) { return channels * elementBytes(type) % 128 == 0; }
 
 // The places behind the last expert's are zero: there is one for every choice without an expert, and the threads of row r have
-// every one that is r further on, and as many rows again.  (By 64 workgroups of their own: 157 us, where 30 % of 16 384 x 4 x 1024
-// fp16 are sent nowhere, and their gradients 162; so 34 and 56.)
+// every one that is r further on, and as many rows again.  (By 64 workgroups of their own: 157 us, where 30 % of 16 384 x 4 x
+// 1024 fp16 are sent nowhere, and their gradients 162; so 34 and 56.)
 template <typename T, int V, int LANES>
 __device__ __forceinline__ void zeroTail(int tail, int64_t r, int64_t rows, int64_t n, int channels, bool streamed, T *out) {
   const float zero[V] = {};

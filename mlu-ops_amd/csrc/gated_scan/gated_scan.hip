@@ -45,7 +45,6 @@ struct Layout {
   static constexpr int kTileRows = 2 * kPiece * kTeams, kStepRows = kRows * kTeams;  // of a wave
   static_assert(kTileRows >= kLeastTile && kTileRows <= kMostTile && kStepRows % kStateRows == 0, "");
 };
-constexpr int kOutsideBlocks = 8;  // workgroups of every slab for the rows of no sample
 
 // Who works out the states in front of the tiles: nobody (a wave has a whole sample), every wave for itself, a launch of its own.
 enum Joining { kWhole, kFolded, kJoined };
@@ -55,6 +54,7 @@ struct Shape {
   int64_t x_stride, g_stride, dh_stride;  // elements from row to row; results lie row by row
   int most_tiles;
   int side_by_side;  // waves of a workgroup that have slabs of the same rows
+  int outside;       // workgroups along y for the rows of no sample
   const int32_t *starts;
   bool reverse;
   bool streamed;  // results go past the caches
@@ -458,13 +458,13 @@ __device__ __forceinline__ void incoming(const WORK &w, const Shape &s, const fl
 }
 
 // The rows of no sample, which are zero in every result, and (`final` not null) what a sample without rows hands on: by workgroup
-// `block` of kOutsideBlocks of every slab.
+// `block` of those of every slab.
 template <typename T, int V>
 __device__ void outside(const Shape &s, int block, const float *initial, float *final, T *out, T *out2) {
   const float zero[V] = {};
   const int vectors = s.channels / V;
   block = block * (int)gridDim.x + (int)blockIdx.x;
-  const int blocks = kOutsideBlocks * (int)gridDim.x;
+  const int blocks = s.outside * (int)gridDim.x;
   for (int side = 0; side < 2; ++side) {
     int first, rows;
     segmentOrOutside(s.starts, s.rows, s.samples, side == 0 ? 0 : s.samples + 1, &first, &rows);
@@ -740,6 +740,11 @@ void byJoining(Joining joining, F f) {
     f(std::integral_constant<Joining, kJoined>());
 }
 
+// Workgroups for the rows of no sample: as many as would have so many values each, if all rows were such.  (8 of a slab: 60 us to
+// apply 248 636 x 128 fp16 where the last 98 636 rows are no sample's, 110 where all but 100 are; so 27 and 13, and 38 as before
+// where none are.)
+constexpr int64_t kOutsideValues = 16384, kMostOutside = 1024;
+
 // Slabs of CHANNELS channels along x, as many of a workgroup's waves as can be with slabs side by side; tiles, or samples, along
 // y.
 struct Grid {
@@ -752,7 +757,10 @@ Grid gridOf(Shape *s, Joining joining, int tile) {
   s->side_by_side = all >= 3 ? 4 : (int)all;
   s->most_tiles = (int)mostRaggedTiles(s->rows, s->samples, tile);
   const int64_t in_block = kWaves / s->side_by_side, items = joining == kWhole ? s->samples : s->most_tiles;
-  return {(unsigned)((all + s->side_by_side - 1) / s->side_by_side), (items + in_block - 1) / in_block};
+  const unsigned slabs = (unsigned)((all + s->side_by_side - 1) / s->side_by_side);
+  const int64_t pieces = (int64_t)s->rows * s->channels / kOutsideValues;
+  s->outside = (int)std::max<int64_t>(std::min<int64_t>(pieces, kMostOutside) / slabs, 8);
+  return {slabs, (items + in_block - 1) / in_block};
 }
 
 // Workgroups along y in as many launches as they need.
@@ -815,7 +823,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanForward(mluOpHandle_t handle, mluOp
     handle->forgetNotesIn(carries, (size_t)mostSlots<kStateRows>(rows, samples) * channels * sizeof(float));
     handle->forgetNotesIn(workspace, workspace_size);
   }
-  Shape s = {(int)rows,  (int)channels, (int)samples, features_stride, gates_stride, 0, 0, 1,
+  Shape s = {(int)rows,  (int)channels, (int)samples, features_stride, gates_stride, 0, 0, 1, 0,
              row_starts, reverse != 0,  bytes >= kStreamedBytes};
   const Workspace w(workspace, rows, channels, samples);
   const mluop::LaunchCtx lc = handle->launchCtx();
@@ -840,7 +848,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanForward(mluOpHandle_t handle, mluOp
         if (joining == kJoined) join<TILE, false>(lc, w.tiles, s, initial, w.states, final);
         byJoining(joining, [&](auto how) {
           constexpr Joining JOINING = decltype(how)::value;
-          alongY(grid.blocks + kOutsideBlocks, [&](int64_t first, unsigned count) {
+          alongY(grid.blocks + s.outside, [&](int64_t first, unsigned count) {
             lc.begin("gatedScanApply");
             gatedScanApply<T, V, ACROSS, KIND, JOINING><<<dim3(grid.slabs, count), kThreads, 0, lc.stream>>>(
                 x, g, s, first, grid.blocks, JOINING == kJoined ? w.states : initial, w.tiles, carries, final,
@@ -886,7 +894,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanBackward(mluOpHandle_t handle, mluO
     if (initial_grad) handle->forgetNotesIn(initial_grad, (size_t)samples * channels * sizeof(float));
     handle->forgetNotesIn(workspace, workspace_size);
   }
-  Shape s = {(int)rows,  (int)channels, (int)samples, features_stride, gates_stride, output_grad_stride, 0, 1,
+  Shape s = {(int)rows,  (int)channels, (int)samples, features_stride, gates_stride, output_grad_stride, 0, 1, 0,
              row_starts, reverse != 0,  bytes >= kStreamedBytes};
   const Workspace w(workspace, rows, channels, samples);
   const mluop::LaunchCtx lc = handle->launchCtx();
@@ -913,7 +921,7 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanBackward(mluOpHandle_t handle, mluO
         if (joining == kJoined) join<TILE, true>(lc, w.tiles, s, final_grad, w.states, initial_grad);
         byJoining(joining, [&](auto how) {
           constexpr Joining JOINING = decltype(how)::value;
-          alongY(grid.blocks + kOutsideBlocks, [&](int64_t first, unsigned count) {
+          alongY(grid.blocks + s.outside, [&](int64_t first, unsigned count) {
             lc.begin("gatedScanGrad");
             gatedScanGrad<T, V, ACROSS, KIND, JOINING><<<dim3(grid.slabs, count), kThreads, 0, lc.stream>>>(
                 dh, x, g, s, first, grid.blocks, carries, JOINING == kJoined ? w.states : final_grad, w.tiles, initial_grad,
