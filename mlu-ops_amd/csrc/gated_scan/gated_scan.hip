@@ -52,7 +52,7 @@ enum Joining { kWhole, kFolded, kJoined };
 struct Shape {
   int rows, channels, samples;
   int64_t x_stride, g_stride, dh_stride;  // elements from row to row; results lie row by row
-  int most_tiles;
+  int slots;         // for tiles
   int side_by_side;  // waves of a workgroup that have slabs of the same rows
   int outside;       // workgroups along y for the rows of no sample
   const int32_t *starts;
@@ -66,6 +66,25 @@ template <int ROWS>
 __device__ __forceinline__ int64_t firstSlot(int sample, int first_row) { return (int64_t)first_row / ROWS + sample; }
 template <int ROWS>
 int64_t mostSlots(int64_t rows, int64_t samples) { return rows / ROWS + samples; }
+
+// The last sample whose first slot is not behind `slot` (0 where there is none), in scalar registers: of 64 pieces of the samples
+// at a time, by whole waves.  (Slots rise with the samples.  One tile after the other, 64 samples at a time, 2001 rows in 1000
+// samples took 48 us to read, so 38.)
+template <int ROWS>
+__device__ __forceinline__ int sampleOfSlot(const Shape &s, int slot) {
+  const int lane = (int)threadIdx.x % 64;
+  int from = 0, count = s.samples;
+  while (count > 1) {
+    const int step = (count + 63) / 64, at = from + min(lane * step, count - 1);
+    int first, rows;
+    segmentRows(s.starts, s.rows, at, &first, &rows);
+    const uint64_t reached = __ballot(lane * step < count && firstSlot<ROWS>(at, first) <= slot);
+    const int piece = reached == 0 ? 0 : 63 - __builtin_clzll(reached);
+    from += piece * step;
+    count = min(step, count - piece * step);
+  }
+  return __builtin_amdgcn_readfirstlane(from);
+}
 
 // What a wave has: a tile's rows in the order in which they are taken (row i of it is at `first + i * step`), or with WHOLE those
 // of a sample, and a slab of channels.
@@ -98,14 +117,14 @@ struct Work : Layout<ACROSS> {
       segmentRows(s.starts, s.rows, sample, &segment_first, &segment_rows);
       rows = segment_rows;
     } else {
-      if (of >= s.most_tiles) return;
-      const RaggedTile t = findRaggedTile<false>(s.starts, s.rows, s.samples, kTileRows, of);
-      if (t.segment < 0) return;
-      sample = t.segment;
-      segment_first = t.segment_first;
-      segment_rows = t.segment_rows;
-      in_sample = t.in_segment;
-      rows = t.rows;
+      if (of >= s.slots) return;
+      const int found = sampleOfSlot<kTileRows>(s, of);
+      segmentRows(s.starts, s.rows, found, &segment_first, &segment_rows);
+      in_sample = (int)(of - firstSlot<kTileRows>(found, segment_first));
+      // (a sample without rows has a slot, too)
+      if (in_sample < 0 || (in_sample > 0 && in_sample * kTileRows >= segment_rows)) return;
+      sample = found;
+      rows = min(kTileRows, segment_rows - in_sample * kTileRows);
     }
     const int from = in_sample * kTileRows;
     tiles = (segment_rows + kTileRows - 1) / kTileRows;
@@ -288,7 +307,9 @@ __global__ __launch_bounds__(kThreads) void gatedScanTiles(const T *__restrict__
                                                            int64_t first_block, float2 *__restrict__ tiles) {
   typedef Work<V, ACROSS, false> Waves;
   const Waves w(s, first_block + blockIdx.y, 0, false);
-  if (w.sample < 0) return;
+  // (the tile that comes last makes no state that is kept, and samples of one tile are not read here at all: 2001 rows in 1000
+  // samples 38 us else, so 14)
+  if (w.sample < 0 || w.rows == 0 || (GRAD ? w.begins() : w.ends())) return;
   const int64_t x_stride = GRAD ? s.dh_stride : s.x_stride;
   constexpr int kTeamRows = Waves::kTileRows / Waves::kTeams, kPieces = kTeamRows / kPiece;
   float a[V], b[V];
@@ -337,33 +358,32 @@ __global__ __launch_bounds__(kThreads) void gatedScanTiles(const T *__restrict__
   }
 }
 
-// The state in front of every tile of TILE rows (from that of its sample, zero where there is none), to states[slot][channel],
-// and behind the last.  FROM_LAST: tiles from a sample's last to its first.  kJoinChannels channels of a sample a workgroup; its
-// tiles are cut into runs of kJoinRun, one for each of the threads that share a channel, and are read once: kJoinTiles at a
-// time.  (One sample of 7325 tiles of 64 channels 25 us, 3 for each turn.  The next turn's tiles on their way meanwhile: no
-// less.  Four channels a workgroup, and turns twice as long: 22, but four samples of some 970 tiles of 128 channels 10 in place
-// of 9.)
+// The state in front of every tile of TILE rows but a sample's first (from that in front of the sample, zero where there is
+// none), to states[slot][channel].  FROM_LAST: tiles from a sample's last to its first.  kJoinChannels channels of a sample a
+// workgroup; its tiles are cut into runs of kJoinRun, one for each of the threads that share a channel, and are read once:
+// kJoinTiles at a time.  (One sample of 7325 tiles of 64 channels 25 us, 3 for each turn.  The next turn's tiles on their way
+// meanwhile: no less.  Four channels a workgroup, and turns twice as long: 22, but four samples of some 970 tiles of 128 channels
+// 10 in place of 9.)  Samples of few tiles go by 64 at a time.  (A workgroup for each: 10 000 samples of 10 rows of 256 channels
+// 702 us, 1000 of 100 rows 72; so 13 and 14.)
 constexpr int kJoinThreads = 512, kJoinChannels = 8, kJoinRun = 16;
 constexpr int kJoinTiles = kJoinThreads / kJoinChannels * kJoinRun;
+constexpr int kJoinBlocks = 4096;  // most workgroups; each takes every so many samples
 template <int TILE, bool FROM_LAST>
-__global__ __launch_bounds__(kJoinThreads) void gatedScanJoin(const float2 *__restrict__ tiles, Shape s, int first_sample,
-                                                              const float *__restrict__ initial,
-                                                              float *__restrict__ states, float *__restrict__ final) {
+__device__ __forceinline__ void joinSample(const float2 *tiles, const Shape &s, int sample, const float *initial, float *states) {
   constexpr int kJoinWaves = kJoinThreads / 64;
   __shared__ float2 s_wave[kJoinWaves][kJoinChannels];
-  const int sample = first_sample + (int)blockIdx.y;
   int first, rows;
   segmentRows(s.starts, s.rows, sample, &first, &rows);
-  const int count = (rows + TILE - 1) / TILE;
+  const int count = (rows + TILE - 1) / TILE, maps = count - 1;
   const int lane = threadIdx.x % kJoinChannels, run = threadIdx.x / kJoinChannels, wave = threadIdx.x / 64;
   const int channel = (int)blockIdx.x * kJoinChannels + lane;
   const bool there = channel < s.channels;
   const int64_t slot = firstSlot<TILE>(sample, first);
   auto at = [&](int tile) { return (slot + (FROM_LAST ? count - 1 - tile : tile)) * s.channels + (there ? channel : 0); };
   float h0 = initial == nullptr || !there ? 0.f : initial[(int64_t)sample * s.channels + channel];
-  for (int t0 = 0; t0 < count; t0 += kJoinTiles) {
+  for (int t0 = 0; t0 < maps; t0 += kJoinTiles) {
     // (runs of one length as short as they can be)
-    const int here = min(count - t0, kJoinTiles), per = (here + kJoinTiles / kJoinRun - 1) / (kJoinTiles / kJoinRun);
+    const int here = min(maps - t0, kJoinTiles), per = (here + kJoinTiles / kJoinRun - 1) / (kJoinTiles / kJoinRun);
     const int lo = t0 + run * per, left = min(per, t0 + here - lo);
     float2 v[kJoinRun];
 #pragma unroll
@@ -403,21 +423,57 @@ __global__ __launch_bounds__(kJoinThreads) void gatedScanJoin(const float2 *__re
     h = fmaf(ea, h, eb);
 #pragma unroll
     for (int j = 0; j < kJoinRun; ++j) {
-      if (j < left && there) states[at(lo + j)] = h;
       h = fmaf(v[j].x, h, v[j].y);
+      if (j < left && there) states[at(lo + j + 1)] = h;
     }
   }
-  if (run == 0 && there && final != nullptr) final[(int64_t)sample * s.channels + channel] = h0;
+}
+template <int TILE, bool FROM_LAST>
+__global__ __launch_bounds__(kJoinThreads) void gatedScanJoin(const float2 *__restrict__ tiles, Shape s,
+                                                              const float *__restrict__ initial,
+                                                              float *__restrict__ states) {
+  constexpr int kAtOnce = kJoinThreads / kJoinChannels;
+  static_assert(kAtOnce == 64, "a ballot names the samples");
+  const int by = (int)gridDim.y, channel = (int)blockIdx.x * kJoinChannels + (int)threadIdx.x % kJoinChannels;
+  for (int64_t first = blockIdx.y; first < s.samples; first += (int64_t)kAtOnce * by) {
+    // 64 samples together: those of few tiles by a thread for every channel
+    const int64_t mine = first + (int64_t)(threadIdx.x / kJoinChannels) * by;
+    int begin = 0, rows = 0;
+    if (mine < s.samples) segmentRows(s.starts, s.rows, (int)mine, &begin, &rows);
+    const int maps = (rows + TILE - 1) / TILE - 1;
+    if (maps > 0 && maps <= kJoinRun && channel < s.channels) {
+      const int64_t slot = firstSlot<TILE>((int)mine, begin);
+      auto at = [&](int tile) { return (slot + (FROM_LAST ? maps - tile : tile)) * s.channels + channel; };
+      float h = initial == nullptr ? 0.f : initial[mine * s.channels + channel];
+      float2 v[kJoinRun];
+#pragma unroll
+      for (int j = 0; j < kJoinRun; ++j) v[j] = tiles[at(min(j, maps - 1))];
+      // (stores behind the last of the loads, which are waited for in one order with them: 100 samples of 16 tiles 33 us, so 13)
+#pragma unroll
+      for (int j = 0; j < kJoinRun; ++j) v[j].y = h = fmaf(v[j].x, h, v[j].y);
+#pragma unroll
+      for (int j = 0; j < kJoinRun; ++j)
+        if (j < maps) states[at(j + 1)] = v[j].y;
+    }
+    // then those of many, one after the other: the same ones for every wave
+    const int64_t looked_at = first + (int64_t)(threadIdx.x & 63) * by;
+    rows = 0;
+    if (looked_at < s.samples) segmentRows(s.starts, s.rows, (int)looked_at, &begin, &rows);
+    for (uint64_t some = __ballot(rows > TILE * (kJoinRun + 1)); some != 0; some &= some - 1)
+      joinSample<TILE, FROM_LAST>(tiles, s, (int)(first + (int64_t)__builtin_ctzll(some) * by), initial, states);
+  }
 }
 
 // The state that comes into a wave's rows: from the one in front of its tile (JOINED), or of its sample through the tiles in
-// front.  FROM_LAST: the gradient that comes in from behind.  `states` are those of the tiles or the samples (null: zero).
+// front.  FROM_LAST: the gradient that comes in from behind.  `initial` are those of the samples (null: zero).
 template <int V, int ACROSS, Joining JOINING, bool FROM_LAST, typename WORK>
-__device__ __forceinline__ void incoming(const WORK &w, const Shape &s, const float *states, const float2 *tiles,
-                                         float (&h)[V]) {
-  const int64_t from = (JOINING == kJoined ? w.tile_slot : (int64_t)w.sample) * s.channels + w.channel;
+__device__ __forceinline__ void incoming(const WORK &w, const Shape &s, const float *initial, const float2 *tiles,
+                                         const float *states, float (&h)[V]) {
+  const bool joined = JOINING == kJoined && !(FROM_LAST ? w.ends() : w.begins());
+  const float *from = joined ? states + w.tile_slot * s.channels
+                             : (initial == nullptr ? nullptr : initial + (int64_t)w.sample * s.channels);
 #pragma unroll
-  for (int i = 0; i < V; ++i) h[i] = states == nullptr ? 0.f : states[from + i];
+  for (int i = 0; i < V; ++i) h[i] = from == nullptr ? 0.f : from[w.channel + i];
   if (JOINING != kFolded) return;
   // as many of the tiles by each team
   const int count = FROM_LAST ? w.tiles - 1 - w.in_sample : w.in_sample;
@@ -457,10 +513,9 @@ __device__ __forceinline__ void incoming(const WORK &w, const Shape &s, const fl
   }
 }
 
-// The rows of no sample, which are zero in every result, and (`final` not null) what a sample without rows hands on: by workgroup
-// `block` of those of every slab.
+// The rows of no sample, which are zero in every result: by workgroup `block` of those of every slab.
 template <typename T, int V>
-__device__ void outside(const Shape &s, int block, const float *initial, float *final, T *out, T *out2) {
+__device__ void outside(const Shape &s, int block, T *out, T *out2) {
   const float zero[V] = {};
   const int vectors = s.channels / V;
   block = block * (int)gridDim.x + (int)blockIdx.x;
@@ -474,36 +529,38 @@ __device__ void outside(const Shape &s, int block, const float *initial, float *
       if (out2 != nullptr) storeFloats<T, V>(out2 + (int64_t)first * s.channels + at * V, zero);
     }
   }
-  if (final == nullptr) return;
-  for (int sample = block; sample < s.samples; sample += blocks) {
-    int first, rows;
-    segmentRows(s.starts, s.rows, sample, &first, &rows);
-    if (rows > 0) continue;
-    for (int64_t c = threadIdx.x; c < s.channels; c += kThreads) {
-      const int64_t at = (int64_t)sample * s.channels + c;
-      final[at] = initial == nullptr ? 0.f : initial[at];
-    }
-  }
 }
 
-// The states of a tile's rows, step by step, and the state in front of every kStateRows rows to kept.  But with JOINED it writes
-// `final` too.
+// What a sample without rows hands on, by the wave that has its slot.
+template <typename WORK, int V>
+__device__ __forceinline__ void handOn(const WORK &w, const Shape &s, const float *from, float *to) {
+  if (!w.there || w.team != 0) return;
+  const int64_t at = (int64_t)w.sample * s.channels + w.channel;
+#pragma unroll
+  for (int i = 0; i < V; ++i) to[at + i] = from == nullptr ? 0.f : from[at + i];
+}
+
+// The states of a tile's rows, step by step, and the state in front of every kStateRows rows to kept.
 template <typename T, int V, int ACROSS, int KIND, Joining JOINING>
 __global__ __launch_bounds__(kThreads, 5) void gatedScanApply(const T *__restrict__ x, const T *__restrict__ g, Shape s,
                                                            int64_t first_block, int64_t blocks,
-                                                           const float *__restrict__ states,
+                                                           const float *__restrict__ initial,
                                                            const float2 *__restrict__ tiles,
-                                                           float *__restrict__ kept, float *__restrict__ final,
-                                                           T *__restrict__ out) {
+                                                           const float *__restrict__ states, float *__restrict__ kept,
+                                                           float *__restrict__ final, T *__restrict__ out) {
   const int64_t block = first_block + blockIdx.y;
   if (block >= blocks) {
-    outside<T, V>(s, (int)(block - blocks), states, JOINING == kJoined ? nullptr : final, out, static_cast<T *>(nullptr));
+    outside<T, V>(s, (int)(block - blocks), out, static_cast<T *>(nullptr));
     return;
   }
   typedef Work<V, ACROSS, JOINING == kWhole> Waves;
   constexpr int kStepRows = Waves::kStepRows, kStates = kStepRows / kStateRows;
   const Waves w(s, block, blocks, JOINING != kWhole);
-  if (w.sample < 0 || w.rows == 0) return;
+  if (w.sample < 0) return;
+  if (w.rows == 0) {
+    handOn<Waves, V>(w, s, initial, final);
+    return;
+  }
   float h0[V];
   const int steps = w.steps();
   Rows<T, V, kRows> xs, gs;
@@ -512,7 +569,7 @@ __global__ __launch_bounds__(kThreads, 5) void gatedScanApply(const T *__restric
     xs.template load<kRows>(x, s.x_stride, w, k * kStepRows, 0.f);
   };
   load(0);
-  incoming<V, ACROSS, JOINING, false>(w, s, states, tiles, h0);
+  incoming<V, ACROSS, JOINING, false>(w, s, initial, tiles, states, h0);
   for (int k = 0; k < steps; ++k) {
     float ra[kRows][V], rb[kRows][V], a[V], b[V];
 #pragma unroll
@@ -555,7 +612,7 @@ __global__ __launch_bounds__(kThreads, 5) void gatedScanApply(const T *__restric
       if (r < mine) storeRow<T, V>(lines.row(r), h, s.streamed);
     }
   }
-  if (JOINING != kJoined && w.ends() && w.there && w.team == 0) {
+  if (w.ends() && w.there && w.team == 0) {
 #pragma unroll
     for (int i = 0; i < V; ++i) final[(int64_t)w.sample * s.channels + w.channel + i] = h0[i];
   }
@@ -564,25 +621,31 @@ __global__ __launch_bounds__(kThreads, 5) void gatedScanApply(const T *__restric
 // ---- backward ------------------------------------------------------------------------------
 
 // The gradients of a tile's rows, from the last step to the first: a step's states again from the one in front of it, and the
-// gradient that comes in from behind.  But with JOINED it writes the initial states' too.
+// gradient that comes in from behind.
 template <typename T, int V, int ACROSS, int KIND, Joining JOINING>
 __global__ __launch_bounds__(kThreads, 4) void gatedScanGrad(const T *__restrict__ dh, const T *__restrict__ x,
                                                           const T *__restrict__ g, Shape s, int64_t first_block,
                                                           int64_t blocks, const float *__restrict__ kept,
-                                                          const float *__restrict__ grads, const float2 *__restrict__ tiles,
+                                                          const float *__restrict__ final_grad,
+                                                          const float2 *__restrict__ tiles,
+                                                          const float *__restrict__ grads,
                                                           float *__restrict__ initial_grad, T *__restrict__ dx,
                                                           T *__restrict__ dg) {
   const int64_t block = first_block + blockIdx.y;
   if (block >= blocks) {
-    outside<T, V>(s, (int)(block - blocks), grads, JOINING == kJoined ? nullptr : initial_grad, dx, dg);
+    outside<T, V>(s, (int)(block - blocks), dx, dg);
     return;
   }
   typedef Work<V, ACROSS, JOINING == kWhole> Waves;
   constexpr int kStepRows = Waves::kStepRows, kStates = kStepRows / kStateRows;
   const Waves w(s, block, blocks, JOINING != kWhole);
-  if (w.sample < 0 || w.rows == 0) return;
+  if (w.sample < 0) return;
+  if (w.rows == 0) {
+    if (initial_grad != nullptr) handOn<Waves, V>(w, s, final_grad, initial_grad);
+    return;
+  }
   float l0[V];
-  incoming<V, ACROSS, JOINING, true>(w, s, grads, tiles, l0);
+  incoming<V, ACROSS, JOINING, true>(w, s, final_grad, tiles, grads, l0);
   for (int k = w.steps() - 1; k >= 0; --k) {
     Rows<T, V, kRows> xs, gs, ds;
     gs.template load<kRows>(g, s.g_stride, w, k * kStepRows, idle<KIND>());
@@ -643,7 +706,7 @@ __global__ __launch_bounds__(kThreads, 4) void gatedScanGrad(const T *__restrict
       storeRow<T, V>(to_g.row(r), gg, s.streamed);
     }
   }
-  if (JOINING != kJoined && w.begins() && w.there && w.team == 0 && initial_grad != nullptr) {
+  if (w.begins() && w.there && w.team == 0 && initial_grad != nullptr) {
 #pragma unroll
     for (int i = 0; i < V; ++i) initial_grad[(int64_t)w.sample * s.channels + w.channel + i] = l0[i];
   }
@@ -722,13 +785,15 @@ struct Workspace {
   }
 };
 
-// A wave for a whole sample, and one launch in place of two or three: where there are few rows, or about one a sample, as in a
-// step of many sequences.  (At worst one sample has them all, in 256 steps of a microsecond.)  Every wave folds the tiles in
-// front of its own where these are few, at most 16 for a team.
-constexpr int64_t kFoldedRows = 4096;
+// A wave for a whole sample, and one launch in place of two or three, where there are few rows more than samples, as in a step of
+// many sequences: it takes a microsecond for every 16 rows of the longest.  (us with a launch more / whole: one sample of 129
+// rows of 1024 12 / 9, of 257 12 / 18, of 501 13 / 33; 400 sequences of which one has 113 rows 24 / 14.  At worst one of as many
+// samples has all 4096 rows, in 256 such steps.)  Every wave folds the tiles in front of its own where these are few, at most 16
+// for a team.
+constexpr int64_t kFoldedRows = 4096, kWholeRows = 128;
 Joining joiningOf(int64_t rows, int64_t samples) {
-  if (rows <= std::max<int64_t>(512, std::min<int64_t>(2 * samples, kFoldedRows))) return kWhole;
-  return rows <= kFoldedRows ? kFolded : kJoined;
+  if (rows > kFoldedRows) return kJoined;
+  return rows <= samples + kWholeRows ? kWhole : kFolded;
 }
 template <typename F>
 void byJoining(Joining joining, F f) {
@@ -755,8 +820,8 @@ template <int CHANNELS>
 Grid gridOf(Shape *s, Joining joining, int tile) {
   const int64_t all = (s->channels + CHANNELS - 1) / CHANNELS;
   s->side_by_side = all >= 3 ? 4 : (int)all;
-  s->most_tiles = (int)mostRaggedTiles(s->rows, s->samples, tile);
-  const int64_t in_block = kWaves / s->side_by_side, items = joining == kWhole ? s->samples : s->most_tiles;
+  s->slots = s->rows / tile + s->samples;
+  const int64_t in_block = kWaves / s->side_by_side, items = joining == kWhole ? s->samples : s->slots;
   const unsigned slabs = (unsigned)((all + s->side_by_side - 1) / s->side_by_side);
   const int64_t pieces = (int64_t)s->rows * s->channels / kOutsideValues;
   s->outside = (int)std::max<int64_t>(std::min<int64_t>(pieces, kMostOutside) / slabs, 8);
@@ -771,14 +836,13 @@ void alongY(int64_t blocks, F f) {
 }
 
 template <int TILE, bool FROM_LAST>
-void join(const mluop::LaunchCtx &lc, const float2 *tiles, const Shape &s, const float *initial, float *states, float *final) {
-  for (int64_t first = 0; first < s.samples; first += kMostAlongY) {
-    lc.begin("gatedScanJoin");
-    gatedScanJoin<TILE, FROM_LAST><<<dim3((unsigned)((s.channels + kJoinChannels - 1) / kJoinChannels),
-                                    (unsigned)std::min<int64_t>(s.samples - first, kMostAlongY)),
-                               kJoinThreads, 0, lc.stream>>>(tiles, s, (int)first, initial, states, final);
-    lc.end();
-  }
+void join(const mluop::LaunchCtx &lc, const float2 *tiles, const Shape &s, const float *initial, float *states) {
+  lc.begin("gatedScanJoin");
+  const int slabs = (s.channels + kJoinChannels - 1) / kJoinChannels;
+  const int along_y = std::min(s.samples, std::max(kJoinBlocks / slabs, 1));
+  gatedScanJoin<TILE, FROM_LAST><<<dim3((unsigned)slabs, (unsigned)along_y), kJoinThreads, 0, lc.stream>>>(tiles, s, initial,
+                                                                                                         states);
+  lc.end();
 }
 
 }  // namespace
@@ -845,13 +909,13 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanForward(mluOpHandle_t handle, mluOp
             lc.end();
           });
         }
-        if (joining == kJoined) join<TILE, false>(lc, w.tiles, s, initial, w.states, final);
+        if (joining == kJoined) join<TILE, false>(lc, w.tiles, s, initial, w.states);
         byJoining(joining, [&](auto how) {
           constexpr Joining JOINING = decltype(how)::value;
           alongY(grid.blocks + s.outside, [&](int64_t first, unsigned count) {
             lc.begin("gatedScanApply");
             gatedScanApply<T, V, ACROSS, KIND, JOINING><<<dim3(grid.slabs, count), kThreads, 0, lc.stream>>>(
-                x, g, s, first, grid.blocks, JOINING == kJoined ? w.states : initial, w.tiles, carries, final,
+                x, g, s, first, grid.blocks, initial, w.tiles, w.states, carries, final,
                 static_cast<T *>(out));
             lc.end();
           });
@@ -918,13 +982,13 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGatedScanBackward(mluOpHandle_t handle, mluO
             lc.end();
           });
         }
-        if (joining == kJoined) join<TILE, true>(lc, w.tiles, s, final_grad, w.states, initial_grad);
+        if (joining == kJoined) join<TILE, true>(lc, w.tiles, s, final_grad, w.states);
         byJoining(joining, [&](auto how) {
           constexpr Joining JOINING = decltype(how)::value;
           alongY(grid.blocks + s.outside, [&](int64_t first, unsigned count) {
             lc.begin("gatedScanGrad");
             gatedScanGrad<T, V, ACROSS, KIND, JOINING><<<dim3(grid.slabs, count), kThreads, 0, lc.stream>>>(
-                dh, x, g, s, first, grid.blocks, carries, JOINING == kJoined ? w.states : final_grad, w.tiles, initial_grad,
+                dh, x, g, s, first, grid.blocks, carries, final_grad, w.tiles, w.states, initial_grad,
                 static_cast<T *>(features_grad), static_cast<T *>(gates_grad));
             lc.end();
           });

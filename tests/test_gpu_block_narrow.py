@@ -96,3 +96,32 @@ def test_recurrence_whose_gradients_lie_otherwise(gpu_handle, rows, reverse):
     same = mluop_hip.gated_scan_forward(gpu_handle, wide[:, :16].contiguous(), gates, starts, reverse=reverse)
     for a, b in zip(again[:2], same[:2]):   # (of the carries some rows belong to no sample)
         assert torch.allclose(a.float(), b.float(), rtol=2.0 ** -7, atol=2.0 ** -14)
+
+
+def lengths(which):
+    """of samples: long ones, some of several tiles, and many of few rows or none"""
+    import random
+    draw = random.Random(which)
+    if which == "joined":
+        some = [5000, 0, 2500, 700, 64, 65, 128, 129, 1, 256, 257, 300] + [draw.choice([0, 0, 1, 2, 7, 40]) for _ in range(190)]
+    elif which == "folded":
+        some = [400, 0, 200] + [draw.choice([0, 0, 1, 2, 3, 70]) for _ in range(130)]
+    else:
+        some = [90, 0] + [draw.choice([0, 0, 1, 1, 2]) for _ in range(170)]
+    draw.shuffle(some)
+    return some
+
+
+@pytest.mark.parametrize("dtype,kind,reverse", [("float32", "exp", False), ("bfloat16", "sigmoid", True),
+                                                ("float32", "sigmoid", True), ("float16", "exp", False)])
+@pytest.mark.parametrize("which", ["whole", "folded", "joined"])
+@pytest.mark.parametrize("channels", [5, 12, 72])
+def test_recurrence_of_samples_long_and_short(gpu_handle, dtype, kind, reverse, which, channels):
+    import torch
+    from itertools import accumulate
+    from test_gpu_gated_scan import check, inputs
+    some = lengths(which)
+    starts = [3] + [3 + n for n in accumulate(some)]
+    rows = starts[-1] + 2
+    x, g, h0, dh, df = inputs(rows, channels, len(some), getattr(torch, dtype), kind, rows + channels)
+    check(gpu_handle, x, g, starts, h0, dh, df, kind, reverse, dtype)
