@@ -577,8 +577,7 @@ __global__ __launch_bounds__(kThreads, 5) void gatedScanApply(const T *__restric
       a[i] = 1.f;
       b[i] = 0.f;
     }
-#pragma unroll
-    for (int r = 0; r < kRows; ++r)
+    auto row = [&](int r) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         float u;
@@ -587,6 +586,18 @@ __global__ __launch_bounds__(kThreads, 5) void gatedScanApply(const T *__restric
         b[i] = fmaf(ra[r][i], b[i], rb[r][i]);
         a[i] *= ra[r][i];
       }
+    };
+    row(0);
+    // (the one row of a sample, as in a step of many sequences, is the first team's first: of 2048 x 1024 bf16 38 us without this)
+    if (JOINING != kWhole || w.rows > 1) {
+#pragma unroll
+      for (int r = 1; r < kRows; ++r) row(r);
+    } else {
+#pragma unroll
+      for (int r = 1; r < kRows; ++r)
+#pragma unroll
+        for (int i = 0; i < V; ++i) ra[r][i] = rb[r][i] = 0.f;
+    }
     if (k + 1 < steps) load(k + 1);
     if (kStates == 1 && w.there && w.team == 0)
 #pragma unroll
