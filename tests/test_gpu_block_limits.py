@@ -41,7 +41,9 @@ def test_norm_of_more_elements_than_32_bits(handle):
     total = torch.zeros(channels, device="cuda", dtype=torch.float64)
     for first in range(0, rows, 1 << 18):
         at = slice(first, min(first + (1 << 18), rows))
-        total += ((x[at].float() - mean[at, None]) * rstd[at, None]).sum(0, dtype=torch.float64)
+        # (a product with ones: torch's sums of many rows by several workgroups have been off)
+        terms = ((x[at].float() - mean[at, None]) * rstd[at, None]).double()
+        total += (torch.ones(1, terms.shape[0], device="cuda", dtype=torch.float64) @ terms)[0]
     # (a sum of 2^22 numbers of about one, some 2^11 of them one after the other: its size stays below 2^14 or so, and 2^12
     # roundings of half a step of that are 4)
     assert bool(((dw.double() - total).abs() <= 4.0).all())
