@@ -585,17 +585,27 @@ class DropoutAdd(torch.nn.Module):
     is drawn from torch's generator where none is given; it and the count are saved with the module's state.
 
     Processes that train together drop the same elements where their seeds are the same (a wrapper that broadcasts buffers makes
-    them the same).  A forward pass that is run again inside of a backward pass, as activation checkpoints do, would have another
-    number and is refused: `dropout_add` with a state from outside of the checkpoint gives the same elements both times."""
+    them the same), and so do a module and its deep copy, which has its seed and its count.  `reset_parameters` begins anew, with
+    `seed` where one was given and with one drawn then where none was; a module made on the meta device needs it once it has
+    memory, unless a state is loaded.
+
+    A forward pass that is run again inside of a backward pass, as activation checkpoints do, would have another number and is
+    refused: `dropout_add` with a state from outside of the checkpoint gives the same elements both times."""
 
     def __init__(self, p, seed=None):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError("p lies in [0, 1]")
         self.p = float(p)
-        seed = int(torch.randint(0, 2 ** 62, ())) if seed is None else int(seed)
-        self.register_buffer("state", torch.tensor([seed, 0], dtype=torch.int64))
-        self.register_buffer("_next", torch.tensor([0, 1], dtype=torch.int64), persistent=False)
+        self.seed = None if seed is None else int(seed)
+        self.register_buffer("state", torch.zeros(2, dtype=torch.int64))
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        # (drawn on the host whatever torch's default device is)
+        seed = int(torch.randint(0, 2 ** 62, (), device="cpu")) if self.seed is None else self.seed
+        with torch.no_grad():
+            self.state.copy_(torch.tensor([seed, 0], dtype=torch.int64, device="cpu"))
 
     def forward(self, features, residual=None):
         if isinstance(features, SparseTensor):
@@ -607,7 +617,7 @@ class DropoutAdd(torch.nn.Module):
             raise RuntimeError("a DropoutAdd inside of a backward pass would drop other elements than its forward pass did")
         with torch.no_grad():
             state = self.state.clone()
-            self.state.add_(self._next)
+            self.state[1:].add_(1)
         return dropout_add(features, residual, self.p, state)
 
 
