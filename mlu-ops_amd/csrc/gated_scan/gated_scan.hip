@@ -163,12 +163,26 @@ constexpr int64_t kMostStride = MLUOP_EXT_GATED_SCAN_MOST_STRIDE, kNarrowStride 
 static_assert((uint64_t)(kLeastTile + 1) * kMostStride * sizeof(float) < (uint64_t)1 << 32, "32-bit offsets");
 static_assert((uint64_t)(kMostTile + 1) * kNarrowStride * sizeof(float) < (uint64_t)1 << 32, "32-bit offsets");
 
+// e^g of a gate of type T.  Its product with log2(e) is rounded, by which 2^p is off by up to 1.23 |g| units of 2^-24 of itself.
+// With fp32 rows that is put right: c = g - p ln(2) is what was lost, and e + e c has it again; where 2^p is infinite, zero or
+// no number it stays that (248 636 x 128 fp32 127 us in either way).  Rows of 16 bits, whose results are rounded to 2^13 such
+// units and more, do without (us without and with it: 248 636 x 128 fp16 75 and 80, 65 536 x 1024 bf16 forward and backward 328
+// and 336).
+template <typename T>
+__device__ __forceinline__ float exponential(float g) {
+  const float p = g * 1.44269504f, e = __builtin_amdgcn_exp2f(p);
+  if constexpr (!std::is_same_v<T, float>) return e;
+  const float c = fmaf(p, 1.9046542e-9f, fmaf(p, -0.693147182f, g));  // (ln(2) is 0.693147182 - 1.9046542e-9)
+  return fabsf(p) < 128.f ? fmaf(e, c, e) : e;
+}
+
 // a and u of a gate: a row's step is h -> a h + u x.  Half of what these kernels compute is here.  What has to be exact is an a
 // close to one, whose error all steps of a long memory repeat: it is what a small u leaves of one.  An exponential beyond the
-// range is infinite, its reciprocal zero.
-template <int KIND>
+// range is infinite, its reciprocal zero.  In units of 2^-24 of the result: the power is off by 2 and the step that puts it right
+// by 1, a sum or a product by 1, a reciprocal by 2; with fp32 rows together at most 7 for a and 6 for u, whatever the gate is.
+template <typename T, int KIND>
 __device__ __forceinline__ void gate(float g, float *a, float *u) {
-  const float e = __builtin_amdgcn_exp2f(g * 1.44269504f);
+  const float e = exponential<T>(g);
   if (KIND == MLUOP_EXT_GATE_SIGMOID) {
     *u = __builtin_amdgcn_rcpf(1.f + e);
     *a = g < 0.f ? e * *u : 1.f - *u;
@@ -333,7 +347,7 @@ __global__ __launch_bounds__(kThreads) void gatedScanTiles(const T *__restrict__
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         float ga, u;
-        gate<KIND>(p.g.value(r, i), &ga, &u);
+        gate<T, KIND>(p.g.value(r, i), &ga, &u);
         const float v = p.x.value(r, i);
         b[i] = GRAD ? ga * (b[i] + v) : fmaf(ga, b[i], u * v);
         a[i] *= ga;
@@ -581,7 +595,7 @@ __global__ __launch_bounds__(kThreads, 5) void gatedScanApply(const T *__restric
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         float u;
-        gate<KIND>(gs.value(r, i), &ra[r][i], &u);
+        gate<T, KIND>(gs.value(r, i), &ra[r][i], &u);
         rb[r][i] = u * xs.value(r, i);
         b[i] = fmaf(ra[r][i], b[i], rb[r][i]);
         a[i] *= ra[r][i];
@@ -675,7 +689,7 @@ __global__ __launch_bounds__(kThreads, 4) void gatedScanGrad(const T *__restrict
     for (int r = 0; r < kRows; ++r)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        gate<KIND>(gs.value(r, i), &ra[r][i], &ru[r][i]);
+        gate<T, KIND>(gs.value(r, i), &ra[r][i], &ru[r][i]);
         b[i] = fmaf(ra[r][i], b[i], ru[r][i] * xs.value(r, i));
         // (the gradient comes from behind: through this row first, then through those in front of it, composed so far)
         a[i] *= ra[r][i];
