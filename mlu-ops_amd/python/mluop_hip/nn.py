@@ -453,7 +453,7 @@ def expert_combine(results, places, group_starts, weights=None):
 class ExpertMLP(torch.nn.Module):
     """Two expert layers with SiLU in between; every row of features [rows, channels] goes to `choices` of `experts`, the
     largest of a learned linear map, and its results are added up with the softmax of their scores as weights.  One row (a
-    step of a program that answers) takes the same way as a batch."""
+    step of a program that answers) takes the same way as a batch.  Takes a SparseTensor or its features."""
 
     def __init__(self, channels, hidden, experts, choices):
         super().__init__()
@@ -463,6 +463,8 @@ class ExpertMLP(torch.nn.Module):
         self.down = ExpertLinear(experts, hidden, channels)
 
     def forward(self, features):
+        if isinstance(features, SparseTensor):
+            return features.replace_features(self.forward(features.features))
         scores, chosen = torch.topk(self.gate(features.to(self.gate.weight.dtype)), self.choices, dim=1)
         _, starts, places = expert_order(chosen, self.experts)
         hidden = torch.nn.functional.silu(self.up(expert_dispatch(features, places, starts), starts))
