@@ -330,7 +330,8 @@ mluOpStatus_t MLUOP_WIN_API mluOpExtGroupedMatmulBackwardFilter(mluOpHandle_t ha
  *   out = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(variance + eps),  variance of the population.
  * weight and bias [channels] of param_type, FLOAT or `type`; NULL: one and zero.  mean and rstd fp32 [rows] are results that the
  * backward pass takes.  Backward: input_grad [rows, channels], weight_grad and bias_grad [channels] of param_type (NULL where
- * not wanted; zero where there are no rows).  At most 2^15 channels. */
+ * not wanted; zero where there are no rows).  Statistics are fp32: where squares of differences from the mean leave its range,
+ * rstd is zero.  At most 2^15 channels. */
 mluOpStatus_t MLUOP_WIN_API mluOpExtLayerNormForward(mluOpHandle_t handle, mluOpDataType_t type, const void *features,
                                                      int64_t features_stride, int64_t rows, int64_t channels,
                                                      mluOpDataType_t param_type, const void *weight, const void *bias,
